@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define LA_ABI_VERSION 14
+#define LA_ABI_VERSION 15
 
 /* element types */
 enum {
@@ -663,6 +663,55 @@ typedef struct {
 
 size_t la_block_sparse_prefill_workspace(const la_prefill_args *a);
 int la_block_sparse_prefill(const la_prefill_args *a, void *stream);
+
+/*
+ * Dense causal attention with grouped heads over whole prompts, chunks or single
+ * tokens (dense_attention, core.py:148-181, for one pass over K and V).
+ *   lse[h][t] = log sum_s exp(scale q_t . k_s),  out[t] = sum_s exp(scale q_t . k_s - lse) v_s
+ * over the keys s a query sees: with causal != 0 the queries are the sequence's last
+ * Lq positions of its Lk keys, so query t sees s <= Lk - Lq + t; else all Lk.  A query
+ * that sees no key gets zeros and lse = -inf.  What a query does not see never reaches
+ * its row, infinities and NaN included.
+ *  - batched (cu_q null): q, out (B, Hq, Tq, D), k, v (B, Hkv, Tk, D); q_len / k_len
+ *    (optional, int32 [B]) give each sequence's Lq / Lk (clamped to [0, Tq] / [0, Tk]);
+ *    rows at or past Lq are zeros (lse -inf);
+ *  - packed: cu_q (int32 [B + 1], ascending) puts sequence b's queries at rows
+ *    cu_q[b] .. cu_q[b+1] - 1 of q and out, cu_k (null: cu_q) its keys at those rows of
+ *    k and v; Tq and Tk are the tensors' rows and the *_sb strides are unused.  Rows no
+ *    sequence holds are left as they were, or zeroed (zero_rest).
+ * Unit stride over D; every row 16-byte aligned.  D 64 or 128; dtype LA_F32, LA_BF16 or
+ * LA_F16, out_dtype that or LA_F32.  lse (optional, fp32) has strides l_sb, l_sh and 1.
+ * scale must be positive.  Workspace: la_dense_attention_workspace() bytes, 256-byte
+ * aligned (the parts of few rows over many keys, which several workgroups share).
+ */
+typedef struct {
+  const void *q;
+  const void *k;
+  const void *v;
+  void *out;
+  float *lse;
+  const int32_t *cu_q;
+  const int32_t *cu_k;
+  const int32_t *q_len;
+  const int32_t *k_len;
+  void *workspace;
+  int64_t ws_bytes;
+  int64_t B, Hq, Hkv, Tq, Tk, D;
+  int64_t q_sb, q_sh, q_st;
+  int64_t k_sb, k_sh, k_st;
+  int64_t v_sb, v_sh, v_st;
+  int64_t o_sb, o_sh, o_st;
+  int64_t l_sb, l_sh;
+  float scale;
+  int32_t causal;
+  int32_t dtype;
+  int32_t out_dtype;
+  int32_t zero_rest;
+  int32_t reserved;
+} la_dense_attn_args;
+
+size_t la_dense_attention_workspace(const la_dense_attn_args *a);
+int la_dense_attention(const la_dense_attn_args *a, void *stream);
 
 #ifdef __cplusplus
 }

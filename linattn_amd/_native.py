@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblinattn_hip.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 LIST_READS_PARTS = 256  # LA_LIST_READS_PARTS
 
 LA_F32, LA_BF16, LA_F16, LA_FP8_E4M3, LA_F64 = 0, 1, 2, 3, 4
@@ -48,6 +48,8 @@ EXPORTED = (
     "la_block_means",
     "la_xattn_select_workspace",
     "la_xattn_select",
+    "la_dense_attention_workspace",
+    "la_dense_attention",
     "la_device_status",
     "la_test_set_spin_limit",
 )
@@ -169,6 +171,17 @@ class LaPrefillArgs(ctypes.Structure):
                 ("reserved2", _i32)]
 
 
+class LaDenseAttnArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("lse", _vp), ("cu_q", _vp),
+                ("cu_k", _vp), ("q_len", _vp), ("k_len", _vp), ("workspace", _vp),
+                ("ws_bytes", _i64), ("B", _i64), ("Hq", _i64), ("Hkv", _i64), ("Tq", _i64),
+                ("Tk", _i64), ("D", _i64), ("q_sb", _i64), ("q_sh", _i64), ("q_st", _i64),
+                ("k_sb", _i64), ("k_sh", _i64), ("k_st", _i64), ("v_sb", _i64), ("v_sh", _i64),
+                ("v_st", _i64), ("o_sb", _i64), ("o_sh", _i64), ("o_st", _i64), ("l_sb", _i64),
+                ("l_sh", _i64), ("scale", ctypes.c_float), ("causal", _i32), ("dtype", _i32),
+                ("out_dtype", _i32), ("zero_rest", _i32), ("reserved", _i32)]
+
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -221,6 +234,9 @@ def load() -> ctypes.CDLL:
     L.la_xattn_select_workspace.restype = ctypes.c_size_t
     L.la_xattn_select.argtypes = [P(LaXattnSelectArgs), _vp]
     L.la_xattn_select.restype = ctypes.c_int
+    L.la_dense_attention_workspace.argtypes = [P(LaDenseAttnArgs)]
+    L.la_dense_attention_workspace.restype = ctypes.c_size_t
+    L.la_dense_attention.argtypes = [P(LaDenseAttnArgs), _vp]
     L.la_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), _i32, _vp]
     L.la_test_set_spin_limit.argtypes = [ctypes.c_uint32]
     for name in EXPORTED:

@@ -1,0 +1,181 @@
+// What the kernels of dense attention and of the key weights share: which rows a
+// workgroup takes, and how key rows reach LDS.
+#pragma once
+
+#include "common.h"
+
+namespace la {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int DA_BS = 64;  // keys of a staged tile
+
+// Element types on the matrix cores: 32 x 32 += (32 x 16) (16 x 32).
+struct DaBf16 {
+  typedef bf16x8 x8;
+  typedef __bf16 elem;
+  static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+struct DaF16 {
+  typedef f16x8 x8;
+  typedef _Float16 elem;
+  static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// 16-byte chunk swizzles of a staged row r.  A K read takes the same chunk of 32 rows in
+// passes of two 8-lane groups ({0,3}, {1,2}, ...): rows 8i.. and 8j.. with bit 4
+// different.  A transposed V read takes four consecutive chunks of four rows.
+template <int D>
+__device__ __forceinline__ int da_swz_k(int r) {
+  return D == 128 ? (2 * (r & 7)) ^ ((r >> 4) & 1) : ((r >> 1) & 3) | (((r >> 4) & 1) << 2);
+}
+template <int D>
+__device__ __forceinline__ int da_swz_v(int r) {
+  return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
+}
+
+// Sequences of a call, as the kernels read them.
+struct DaSeqs {
+  const int32_t *cu_q, *cu_k, *q_len, *k_len;
+  int64_t Tq, Tk;
+  int32_t B, G;
+};
+
+// The rows of a tile: rows r0 .. r0 + R - 1 of the lq * G (query, head of the group) pairs
+// of sequence b and one KV head, row r being query r / G of head r % G.
+struct DaTile {
+  int32_t b;       // -1: none, and r0 is the number of tiles there are
+  int32_t r0, lq, lk;
+  int64_t q0, k0;  // packed: first row of the sequence in q and in k
+};
+
+__device__ __forceinline__ int32_t da_cu(const int32_t *cu, int i, int64_t rows) {
+  return (int32_t)min(max((int64_t)cu[i], (int64_t)0), rows);
+}
+
+__device__ __forceinline__ int32_t da_wave_sum(int32_t x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+__device__ __forceinline__ int32_t da_wave_max(int32_t x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
+  return x;
+}
+
+__device__ __forceinline__ void da_seq(const DaSeqs &s, DaTile &t) {
+  if (s.cu_q) {
+    const int32_t a = da_cu(s.cu_q, t.b, s.Tq), e = da_cu(s.cu_q, t.b + 1, s.Tq);
+    t.q0 = a;
+    t.lq = max(e - a, 0);
+    const int32_t *ck = s.cu_k ? s.cu_k : s.cu_q;
+    const int32_t c = da_cu(ck, t.b, s.Tk), d = da_cu(ck, t.b + 1, s.Tk);
+    t.k0 = c;
+    t.lk = max(d - c, 0);
+  } else {
+    t.q0 = t.k0 = 0;
+    t.lq = (int32_t)(s.q_len ? min(max((int64_t)s.q_len[t.b], (int64_t)0), s.Tq) : s.Tq);
+    t.lk = (int32_t)(s.k_len ? min(max((int64_t)s.k_len[t.b], (int64_t)0), s.Tk) : s.Tk);
+  }
+}
+
+// Tile number i of R rows: the sequences' last tiles (the longest causal rows) first, so
+// that a launch does not end with its longest workgroups.  Packed sequences: of the tiles
+// ordered by their number within the sequence, descending, the i-th; every wave finds it
+// by counting, 64 sequences at a time.  Batched: every sequence has a tile of each number
+// (one past its length has no live rows).
+__device__ __forceinline__ DaTile da_tile(const DaSeqs &s, int32_t i, int32_t ntile, int R) {
+  DaTile t;
+  t.b = -1;
+  t.r0 = t.lq = t.lk = 0;
+  t.q0 = t.k0 = 0;
+  if (!s.cu_q) {
+    const int32_t per = ntile / s.B;
+    t.b = i % s.B;
+    t.r0 = (per - 1 - i / s.B) * R;
+    da_seq(s, t);
+    return t;
+  }
+  const int lane = threadIdx.x & 63;
+  auto tiles_of = [&](int b) -> int32_t {  // (b < B)
+    const int32_t n = max(da_cu(s.cu_q, b + 1, s.Tq) - da_cu(s.cu_q, b, s.Tq), 0);
+    return (int32_t)(((int64_t)n * s.G + R - 1) / R);
+  };
+  if (s.B == 1) {
+    const int32_t n = tiles_of(0);
+    if (i >= n) {
+      t.r0 = n;
+      return t;
+    }
+    t.b = 0;
+    t.r0 = (n - 1 - i) * R;
+    da_seq(s, t);
+    return t;
+  }
+  const int32_t mine = lane < s.B ? tiles_of(lane) : 0;  // (of the first 64)
+  auto above = [&](int32_t level) -> int32_t {  // tiles numbered `level` or more
+    int32_t c = max(mine - level, 0);
+    for (int b = 64 + lane; b < s.B; b += 64) c += max(tiles_of(b) - level, 0);
+    return da_wave_sum(c);
+  };
+  const int32_t all = above(0);
+  if (i >= all) {
+    t.r0 = all;
+    return t;
+  }
+  int32_t most = mine;
+  for (int b = 64 + lane; b < s.B; b += 64) most = max(most, tiles_of(b));
+  int32_t lo = 0, hi = da_wave_max(most);  // above(lo) > i >= above(hi)
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (above(mid) > i) lo = mid;
+    else hi = mid;
+  }
+  int32_t rank = i - above(hi);
+  for (int b0 = 0; b0 < s.B; b0 += 64) {
+    const int b = b0 + lane;
+    const uint64_t has = __ballot((b0 == 0 ? mine : b < s.B ? tiles_of(b) : 0) > lo);
+    const int32_t c = __popcll(has);
+    if (rank < c) {
+      const int before = __popcll(has & ((1ull << lane) - 1ull));
+      const uint64_t at = __ballot(((has >> lane) & 1) && before == rank);
+      t.b = b0 + __ffsll((unsigned long long)at) - 1;
+      break;
+    }
+    rank -= c;
+  }
+  t.b = __builtin_amdgcn_readfirstlane(t.b);
+  t.r0 = lo * R;
+  da_seq(s, t);
+  return t;
+}
+
+// Tiles of R rows that a call needs at most, for one KV head.
+inline int64_t da_tiles(bool packed, int64_t B, int64_t Tq, int64_t G, int64_t R) {
+  return packed ? Tq * G / R + B + 1 : B * ceil_div(Tq * G, R);
+}
+
+// Workgroup -> (KV head, tile).  Consecutive workgroups go to the 8 XCDs in turn: with a
+// multiple of 8 streams each XCD keeps the streams' keys in its own L2.
+__device__ __forceinline__ void da_stream(uint32_t wg, uint32_t ns, uint32_t nt, uint32_t &stream,
+                                          uint32_t &tix) {
+  if (ns % 8 == 0) {
+    stream = (wg & 7) + 8 * ((wg >> 3) / nt);
+    tix = (wg >> 3) % nt;
+  } else {
+    stream = wg % ns;
+    tix = wg / ns;
+  }
+}
+
+}  // namespace la

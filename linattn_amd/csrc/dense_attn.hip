@@ -1,0 +1,677 @@
+// Dense attention of prompts, chunks and single tokens with grouped heads, batched or
+// packed (la_dense_attention; dense_attention, core.py:148-181).
+//
+// A workgroup takes R rows of one KV head of one sequence: row r is query r / G of head
+// r % G of its group, so the heads of a group share every staged key, and a tile's rows
+// end at nearly the same key.  It walks the keys in tiles of 64 with the running
+// maximum and sum of a softmax: S^T = K Q^T, P = exp2(c S - m), O^T += V^T P^T.
+#include <algorithm>
+
+#include "dense_attn.h"
+
+namespace la {
+
+struct DaKP {
+  DaSeqs s;
+  const void *q, *k, *v;
+  void *out;
+  float *lse;
+  float *ws_ml, *ws_acc;  // parts: [row of q][head][split] (max, sum) and D values
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, o_sb, o_sh, o_st, l_sb, l_sh;
+  int32_t Hq, Hkv, ntile, splits, causal, out_dt, zero_rest;
+  float qscale, thr_gap;  // log2(e) scale; 8 / qscale
+};
+
+constexpr float DA_LN2 = 0.69314718055994530942f;
+
+__device__ __forceinline__ float da_ninf() { return __int_as_float(0xff800000); }
+
+// Four outputs of a row, 8- or 16-byte aligned.
+__device__ __forceinline__ void da_store4(void *out, int64_t at, int dt, float x0, float x1, float x2, float x3) {
+  if (dt == LA_F32) {
+    *(float4 *)((float *)out + at) = float4{x0, x1, x2, x3};
+  } else if (dt == LA_BF16) {
+    *(uint2 *)((uint16_t *)out + at) =
+        uint2{(uint32_t)f32_to_bf16_bits(x0) | ((uint32_t)f32_to_bf16_bits(x1) << 16),
+              (uint32_t)f32_to_bf16_bits(x2) | ((uint32_t)f32_to_bf16_bits(x3) << 16)};
+  } else {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    *(f16x4 *)((_Float16 *)out + at) = f16x4{(_Float16)x0, (_Float16)x1, (_Float16)x2, (_Float16)x3};
+  }
+}
+__device__ __forceinline__ void da_store1(void *out, int64_t at, int dt, float x) { store_from_f32(out, at, dt, x); }
+
+// Where row (query t, head h) of a tile's sequence lies.
+__device__ __forceinline__ int64_t da_out_at(const DaKP &p, const DaTile &tl, int64_t t, int h) {
+  return (p.s.cu_q ? (tl.q0 + t) * p.o_st : tl.b * p.o_sb + t * p.o_st) + h * p.o_sh;
+}
+__device__ __forceinline__ int64_t da_lse_at(const DaKP &p, const DaTile &tl, int64_t t, int h) {
+  return (p.s.cu_q ? tl.q0 + t : tl.b * p.l_sb + t) + h * p.l_sh;
+}
+__device__ __forceinline__ int64_t da_part_at(const DaKP &p, const DaTile &tl, int64_t t, int h, int split) {
+  return (((p.s.cu_q ? tl.q0 + t : tl.b * p.s.Tq + t) * p.Hq + h) * p.splits) + split;
+}
+
+// Rows that no sequence holds: a batched tile's rows past the sequence's last query
+// (first split), or, by the workgroups that got no tile, the packed rows outside of
+// cu_q[0] .. cu_q[B].
+template <int D>
+__device__ __forceinline__ void da_zero_row(const DaKP &p, int64_t o, int64_t l, int lane) {
+  for (int d = lane; d < D; d += 64) da_store1(p.out, o + d, p.out_dt, 0.f);
+  if (p.lse && lane == 0) p.lse[l] = da_ninf();
+}
+template <int D>
+__device__ void da_rest(const DaKP &p, const DaTile &tl, int R, int kvh, int split, int tix, int w, int nw) {
+  if (split != 0) return;
+  const int lane = threadIdx.x & 63, G = p.s.G;
+  if (!p.s.cu_q) {
+    const int64_t end = min((int64_t)tl.r0 + R, p.s.Tq * G);
+    for (int64_t r = max((int64_t)tl.r0, (int64_t)tl.lq * G) + w; r < end; r += nw)
+      da_zero_row<D>(p, da_out_at(p, tl, r / G, kvh * G + (int)(r % G)),
+                     da_lse_at(p, tl, r / G, kvh * G + (int)(r % G)), lane);
+    return;
+  }
+  if (!p.zero_rest || tl.b >= 0) return;
+  const int64_t first = da_cu(p.s.cu_q, 0, p.s.Tq);
+  const int64_t last = max(first, (int64_t)da_cu(p.s.cu_q, p.s.B, p.s.Tq));
+  const int64_t n = (first + p.s.Tq - last) * G;
+  for (int64_t r = (int64_t)(tix - tl.r0) * nw + w; r < n; r += (int64_t)(p.ntile - tl.r0) * nw) {
+    int64_t t = r / G;
+    if (t >= first) t += last - first;
+    const int h = kvh * G + (int)(r % G);
+    da_zero_row<D>(p, t * p.o_st + h * p.o_sh, t + h * p.l_sh, lane);
+  }
+}
+
+// One row over keys a .. e - 1, by a wave, key by key (m in log2 units; lane i holds dims
+// i D / 64 ..).  For rows of a tile whose matrix products met an infinity or a NaN of V
+// that the row does not see (0 * inf): it reads nothing else.
+template <class E, int D>
+__device__ __noinline__ void da_row(const E *q, const E *k, const E *v, int64_t k_st, int64_t v_st, int a,
+                                    int e, float qscale, float *m_out, float *l_out, float *acc) {
+  constexpr int N = D / 64;
+  const int lane = threadIdx.x & 63;
+  float m = da_ninf(), l = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int key0 = a; key0 < e; key0 += 64) {
+    const int key = min(key0 + lane, e - 1);
+    float s = 0.f;
+    for (int d = 0; d < D; ++d) s = __builtin_fmaf((float)q[d], (float)k[key * k_st + d], s);
+    s = key0 + lane < e ? s * qscale : da_ninf();
+    float mx = s;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    const float mn = fmaxf(m, mx);
+    const float alpha = m == da_ninf() ? 0.f : fast_exp2(m - mn);
+    const float pr = fast_exp2(s - (mn == da_ninf() ? 0.f : mn));
+    m = mn;
+    l = l * alpha + group_sum<64>(pr);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] *= alpha;
+    const int n = min(64, e - key0);
+    for (int j = 0; j < n; ++j) {
+      const float w = __shfl(pr, j, 64);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        acc[i] = __builtin_fmaf(w, (float)v[(int64_t)(key0 + j) * v_st + lane * N + i], acc[i]);
+    }
+  }
+  *m_out = m;
+  *l_out = l;
+}
+
+// Rows of a wave (row number r_first + i, i < NR) whose results are not finite, of which
+// bit i of `bad` says so: those with an infinity or NaN of V among what their tiles (keys
+// a .. end - 1) held and they do not see are done again; the others stand.  (What a tile
+// holds past the last key is that key again.)  Returns the bits of the rows done.
+template <class E, int D, int NR>
+__device__ __noinline__ uint32_t da_again(const DaKP &p, const DaTile &tl, int kvh, int split, int r_first,
+                                          uint32_t bad, int a, int end) {
+  const int lane = threadIdx.x & 63, G = p.s.G;
+  const E *kb = (const E *)p.k + (p.s.cu_q ? tl.k0 * p.k_st : tl.b * p.k_sb) + kvh * p.k_sh;
+  const E *vb = (const E *)p.v + (p.s.cu_q ? tl.k0 * p.v_st : tl.b * p.v_sb) + kvh * p.v_sh;
+  uint32_t done = 0;
+  for (int i = 0; i < NR; ++i) {
+    if (!((bad >> i) & 1u)) continue;
+    const int r = r_first + i, t = r / G, h = kvh * G + r % G;
+    const int lim = p.causal ? min(tl.lk - 1, tl.lk - tl.lq + t) : tl.lk - 1;
+    bool met = false;
+    for (int key = max(max(lim + 1, a), 0); key < end; ++key)
+      for (int d = lane; d < D; d += 64)
+        met = met || !(fabsf((float)vb[(int64_t)min(key, tl.lk - 1) * p.v_st + d]) < __int_as_float(0x7f800000));
+    if (__ballot(met) == 0) continue;
+    done |= 1u << i;
+    const E *q = (const E *)p.q + (p.s.cu_q ? (tl.q0 + t) * p.q_st : tl.b * p.q_sb + t * p.q_st) + h * p.q_sh;
+    float m, l, acc[D / 64];
+    da_row<E, D>(q, kb, vb, p.k_st, p.v_st, a, min(end, lim + 1), p.qscale, &m, &l, acc);
+    if (p.splits > 1) {
+      const int64_t pi = da_part_at(p, tl, t, h, split);
+      if (lane == 0) {
+        p.ws_ml[2 * pi] = m;
+        p.ws_ml[2 * pi + 1] = l;
+      }
+      for (int x = 0; x < D / 64; ++x) p.ws_acc[pi * D + lane * (D / 64) + x] = acc[x];
+      continue;
+    }
+    const int64_t o = da_out_at(p, tl, t, h);
+    for (int x = 0; x < D / 64; ++x)
+      da_store1(p.out, o + lane * (D / 64) + x, p.out_dt, l == 0.f ? 0.f : acc[x] / l);
+    if (p.lse && lane == 0) p.lse[da_lse_at(p, tl, t, h)] = l == 0.f ? da_ninf() : (m + __log2f(l)) * DA_LN2;
+  }
+  return done;
+}
+
+// bf16 / fp16 rows: NW waves of 32 rows.  K and V tiles go global -> LDS by LDS-DMA,
+// double buffered, one barrier a tile.  S^T by 32x32x16 products (A = K rows, B = q held
+// in registers) leaves a lane 16 scores of one row, so masks, maxima and sums are per
+// lane; O^T takes P from the same registers (the contraction index is mapped to the keys
+// a lane holds) and V^T by LDS transpose reads.  P is rounded to the inputs' type for
+// that product (to half a step, 2^-9 or 2^-12 of each weight, independently: as much as
+// the output's own rounding); its sum l, and with it lse, is of the fp32 values.
+template <class T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
+  constexpr int R = 32 * NW, BLK = DA_BS * D, CH = D / 8, RP = 64 / CH, NX = DA_BS / RP / NW;
+  constexpr int NS = D / 16, ND = D / 32;
+  typedef typename T::x8 x8;
+  typedef typename T::elem elem;
+  __shared__ __align__(16) uint16_t smem[4 * BLK];  // K slots 0, 1, then V slots 0, 1
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hf = lane >> 5, r32 = lane & 31;
+  uint32_t stream, tix;
+  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, p.ntile, stream, tix);
+  const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
+  const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R);
+  const int G = p.s.G;
+  if (tl.b < 0 || tl.r0 + R > tl.lq * G) da_rest<D>(p, tl, R, kvh, split, (int)tix, w, NW);
+  if (tl.b < 0 || tl.r0 >= tl.lq * G) return;
+
+  const int nrow = tl.lq * G, diag = tl.lk - tl.lq;
+  auto limit = [&](int t) { return p.causal ? diag + t : tl.lk - 1; };  // last key seen
+  const int r_first = tl.r0 + 32 * w;
+  const int r_mine = min(r_first + r32, nrow - 1);
+  const bool live = r_first + r32 < nrow, wave_live = r_first < nrow;
+  const int t = r_mine / G, h = kvh * G + r_mine % G;
+  const int lim = limit(t);
+  const int lim_lo = limit(min(r_first, nrow - 1) / G);
+  const int lim_hi = limit(min(r_first + 31, nrow - 1) / G);
+  const int lim_tile = limit((min(tl.r0 + R, nrow) - 1) / G);
+  const int n_all = lim_tile < 0 ? 0 : lim_tile / DA_BS + 1;
+  const int j0 = (int)((int64_t)n_all * split / p.splits), j1 = (int)((int64_t)n_all * (split + 1) / p.splits);
+
+  x8 qf[NS];  // B operand: dims 16 s + 8 hf ..
+  {
+    const elem *qp = (const elem *)p.q + (p.s.cu_q ? (tl.q0 + t) * p.q_st : tl.b * p.q_sb + t * p.q_st) +
+                     h * p.q_sh + 8 * hf;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = *(const x8 *)(qp + 16 * s);
+  }
+  const uint16_t *kbh = (const uint16_t *)p.k + (p.s.cu_q ? tl.k0 * p.k_st : tl.b * p.k_sb) + kvh * p.k_sh;
+  const uint16_t *vbh = (const uint16_t *)p.v + (p.s.cu_q ? tl.k0 * p.v_st : tl.b * p.v_sb) + kvh * p.v_sh;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
+  // LDS-DMA: instruction x of wave w fills rows RP (NW x + w) + lane / CH
+  auto dma = [&](int kb, int slot) {
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      const int u = NW * x + w, rr = RP * u + lane / CH;
+      const int64_t key = min(kb * DA_BS + rr, tl.lk - 1);  // (past the end: masked)
+      const uint32_t m0 = lds0 + 2 * (slot * BLK + u * 512);
+      asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(kbh + key * p.k_st + 8 * ((lane % CH) ^ da_swz_k<D>(rr))),
+                   "{m0}"(m0) : "memory");
+    }
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      const int u = NW * x + w, rr = RP * u + lane / CH;
+      const int64_t key = min(kb * DA_BS + rr, tl.lk - 1);
+      const uint32_t m0 = lds0 + 2 * ((2 + slot) * BLK + u * 512);
+      asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(vbh + key * p.v_st + 8 * ((lane % CH) ^ da_swz_v<D>(rr))),
+                   "{m0}"(m0) : "memory");
+    }
+  };
+
+  float m = da_ninf(), thr = da_ninf(), l = 0.f, nmu = 0.f;
+  f32x16 acc[ND];
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+
+  if (j0 < j1) dma(j0, 0);
+  for (int j = j0; j < j1; ++j) {
+    const int par = (j - j0) & 1;
+    wait_vmcnt<0>();
+    lds_barrier();  // tile j has landed for every wave, tile j - 1 is read
+    if (j + 1 < j1) dma(j + 1, par ^ 1);
+    if (!wave_live || j * DA_BS > lim_hi) continue;
+    const uint16_t *sk = smem + par * BLK, *sv = smem + (2 + par) * BLK;
+    f32x16 st[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
+      const int kr = 32 * kt + r32, sw = da_swz_k<D>(kr);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        st[kt] = T::mfma(*(const x8 *)&sk[kr * D + 8 * ((2 * s + hf) ^ sw)], qf[s], st[kt]);
+    }
+    // register i of a tile holds key 8 (i / 4) + 4 hf + i % 4
+    if (j * DA_BS + DA_BS - 1 > lim_lo) {
+      const int d = lim - j * DA_BS - 4 * hf;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          st[kt][i] = 32 * kt + 8 * (i >> 2) + (i & 3) <= d ? st[kt][i] : da_ninf();
+    }
+    float mx = st[0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, st[0][i]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[1][i]);
+    // the reference maximum is raised only past 2^8 of headroom (the weights stay below
+    // 256); both halves of a row keep the same one
+    if (__ballot(mx > thr) != 0) {
+      const float mn = fmaxf(m, pair32_max(mx));
+      const float alpha = m == da_ninf() ? 0.f : fast_exp2((m - mn) * p.qscale);
+      m = mn;
+      thr = mn + p.thr_gap;
+      nmu = mn == da_ninf() ? 0.f : -mn * p.qscale;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        st[kt][i] = fast_exp2(__builtin_fmaf(st[kt][i], p.qscale, nmu));
+        l += st[kt][i];
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        x8 pw;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pw[e] = (elem)st[kt][8 * ks + e];
+        // V^T: 16-lane group c of the wave points at rows k0 + i / 4 and reads
+        // columns 32 dt + 16 (c % 2) + (its lane) of four keys
+        const int vr = 32 * kt + 16 * ks + 4 * hf + ((lane & 15) >> 2);
+        const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), ve = 4 * (lane & 1);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          const int at = vr * D + 8 * ((4 * dt + vc) ^ da_swz_v<D>(vr)) + ve;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sv + at));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sv + at + 8 * D));
+          const x8 a = __builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          acc[dt] = T::mfma(a, pw, acc[dt]);
+        }
+      }
+    }
+  }
+  if (!wave_live) return;
+  l = pair32_sum(l);
+  // results that are not finite, and what their rows do not see
+  float sum = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[dt][i], 0.f, sum);
+  uint64_t bad = __ballot(sum != 0.f);  // (NaN)
+  uint32_t done = 0;
+  if (bad != 0)
+    done = da_again<elem, D, 32>(p, tl, kvh, split, r_first,
+                                 (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
+                                 j0 * DA_BS, min(j1, lim_hi / DA_BS + 1) * DA_BS);
+  if (!live || ((done >> r32) & 1u)) return;
+  // register i of dim tile dt holds dim 32 dt + 8 (i / 4) + 4 hf + i % 4
+  if (p.splits > 1) {
+    const int64_t pi = da_part_at(p, tl, t, h, split);
+    if (hf == 0) {
+      p.ws_ml[2 * pi] = m == da_ninf() ? m : m * p.qscale;
+      p.ws_ml[2 * pi + 1] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(float4 *)(p.ws_acc + pi * D + 32 * dt + 8 * i + 4 * hf) =
+            float4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
+    return;
+  }
+  const bool none = l == 0.f;  // no key seen
+  const float inv = none ? 0.f : 1.f / l;
+  const int64_t o = da_out_at(p, tl, t, h) + 4 * hf;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      da_store4(p.out, o + 32 * dt + 8 * i, p.out_dt, acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv,
+                acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv);
+  if (p.lse && hf == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (m * p.qscale + __log2f(l)) * DA_LN2;
+}
+
+// fp32 rows: four waves of 16 rows on 16x16x4 products, all of it fp32.  A staged tile is
+// 32 keys; lane (c, i) = (lane / 16, lane % 16) reads 16-byte chunk 4 s + c of K row i,
+// whose four values feed four products (dims 16 s + 4 c + e), and holds P of row i for
+// keys 4 c + e, which the product over V takes in that order.
+template <int D>
+__global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
+  constexpr int NW = 4, R = 16 * NW, BS = 32, BLK = BS * D, CH = D / 4, RP = 64 / CH, NX = BS / RP / NW;
+  constexpr int NS = D / 16;
+  __shared__ __align__(16) float smem[4 * BLK];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane >> 4, ri = lane & 15;
+  uint32_t stream, tix;
+  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, p.ntile, stream, tix);
+  const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
+  const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R);
+  const int G = p.s.G;
+  if (tl.b < 0 || tl.r0 + R > tl.lq * G) da_rest<D>(p, tl, R, kvh, split, (int)tix, w, NW);
+  if (tl.b < 0 || tl.r0 >= tl.lq * G) return;
+
+  const int nrow = tl.lq * G, diag = tl.lk - tl.lq;
+  auto limit = [&](int t) { return p.causal ? diag + t : tl.lk - 1; };
+  const int r_first = tl.r0 + 16 * w;
+  const int r_mine = min(r_first + ri, nrow - 1);
+  const bool live = r_first + ri < nrow, wave_live = r_first < nrow;
+  const int t = r_mine / G, h = kvh * G + r_mine % G;
+  const int lim = limit(t);
+  const int lim_lo = limit(min(r_first, nrow - 1) / G);
+  const int lim_hi = limit(min(r_first + 15, nrow - 1) / G);
+  const int lim_tile = limit((min(tl.r0 + R, nrow) - 1) / G);
+  const int n_all = lim_tile < 0 ? 0 : lim_tile / BS + 1;
+  const int j0 = (int)((int64_t)n_all * split / p.splits), j1 = (int)((int64_t)n_all * (split + 1) / p.splits);
+
+  f32x4 qf[NS];
+  {
+    const float *qp = (const float *)p.q + (p.s.cu_q ? (tl.q0 + t) * p.q_st : tl.b * p.q_sb + t * p.q_st) +
+                      h * p.q_sh + 4 * c;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = *(const f32x4 *)(qp + 16 * s);
+  }
+  const float *kbh = (const float *)p.k + (p.s.cu_q ? tl.k0 * p.k_st : tl.b * p.k_sb) + kvh * p.k_sh;
+  const float *vbh = (const float *)p.v + (p.s.cu_q ? tl.k0 * p.v_st : tl.b * p.v_sb) + kvh * p.v_sh;
+  auto swz_k = [](int r) { return 2 * (r & 7); };
+  auto swz_v = [](int r) { return 4 * ((r >> 2) & 3); };
+  auto dma = [&](int kb, int slot) {
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      const int u = NW * x + w, rr = RP * u + lane / CH;
+      const int64_t key = min(kb * BS + rr, tl.lk - 1);
+      dma16(kbh + key * p.k_st + 4 * ((lane % CH) ^ swz_k(rr)), smem + slot * BLK + u * 256);
+      dma16(vbh + key * p.v_st + 4 * ((lane % CH) ^ swz_v(rr)), smem + (2 + slot) * BLK + u * 256);
+    }
+  };
+
+  float m = da_ninf(), thr = da_ninf(), l = 0.f, nmu = 0.f;
+  f32x4 acc[NS];
+#pragma unroll
+  for (int dt = 0; dt < NS; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (j0 < j1) dma(j0, 0);
+  for (int j = j0; j < j1; ++j) {
+    const int par = (j - j0) & 1;
+    wait_vmcnt<0>();
+    lds_barrier();
+    if (j + 1 < j1) dma(j + 1, par ^ 1);
+    if (!wave_live || j * BS > lim_hi) continue;
+    const float *sk = smem + par * BLK, *sv = smem + (2 + par) * BLK;
+    f32x4 st[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      st[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int kr = 16 * kt + ri;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const f32x4 a = *(const f32x4 *)&sk[kr * D + 4 * ((4 * s + c) ^ swz_k(kr))];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], qf[s][e], st[kt], 0, 0, 0);
+      }
+    }
+    // register e of a tile holds key 4 c + e
+    if (j * BS + BS - 1 > lim_lo) {
+      const int d = lim - j * BS - 4 * c;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[kt][e] = 16 * kt + e <= d ? st[kt][e] : da_ninf();
+    }
+    float mx = da_ninf();
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, st[kt][e]);
+    if (__ballot(mx > thr) != 0) {
+      const float mn = fmaxf(m, pair32_max(pair16_max(mx)));
+      const float alpha = m == da_ninf() ? 0.f : fast_exp2((m - mn) * p.qscale);
+      m = mn;
+      thr = mn + p.thr_gap;
+      nmu = mn == da_ninf() ? 0.f : -mn * p.qscale;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NS; ++dt) acc[dt] *= alpha;
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float pr = fast_exp2(__builtin_fmaf(st[kt][e], p.qscale, nmu));
+        l += pr;
+        const int kr = 16 * kt + 4 * c + e;
+#pragma unroll
+        for (int dt = 0; dt < NS; ++dt)
+          acc[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+              sv[kr * D + 4 * ((4 * dt + (ri >> 2)) ^ swz_v(kr)) + (ri & 3)], pr, acc[dt], 0, 0, 0);
+      }
+  }
+  if (!wave_live) return;
+  l = pair32_sum(pair16_sum(l));
+  float sum = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < NS; ++dt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(acc[dt][e], 0.f, sum);
+  uint64_t bad = __ballot(sum != 0.f);
+  uint32_t done = 0;
+  if (bad != 0) {
+    bad |= bad >> 32;
+    done = da_again<float, D, 16>(p, tl, kvh, split, r_first,
+                                  (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
+                                  j0 * BS, min(j1, lim_hi / BS + 1) * BS);
+  }
+  if (!live || ((done >> ri) & 1u)) return;
+  // register e of dim tile dt holds dim 16 dt + 4 c + e
+  if (p.splits > 1) {
+    const int64_t pi = da_part_at(p, tl, t, h, split);
+    if (c == 0) {
+      p.ws_ml[2 * pi] = m == da_ninf() ? m : m * p.qscale;
+      p.ws_ml[2 * pi + 1] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < NS; ++dt)
+      *(float4 *)(p.ws_acc + pi * D + 16 * dt + 4 * c) = float4{acc[dt][0], acc[dt][1], acc[dt][2], acc[dt][3]};
+    return;
+  }
+  const bool none = l == 0.f;
+  const float inv = none ? 0.f : 1.f / l;
+  const int64_t o = da_out_at(p, tl, t, h) + 4 * c;
+#pragma unroll
+  for (int dt = 0; dt < NS; ++dt)
+    da_store4(p.out, o + 16 * dt, p.out_dt, acc[dt][0] * inv, acc[dt][1] * inv, acc[dt][2] * inv, acc[dt][3] * inv);
+  if (p.lse && c == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (m * p.qscale + __log2f(l)) * DA_LN2;
+}
+
+// Joins the parts of a row: a wave a row.
+template <int D>
+__global__ __launch_bounds__(256) void dense_combine_kernel(DaKP p, int64_t rows) {
+  constexpr int N = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int h = (int)(row % p.Hq);
+  const int64_t qr = row / p.Hq;
+  int64_t o, lo;
+  if (p.s.cu_q) {
+    if (qr < da_cu(p.s.cu_q, 0, p.s.Tq) || qr >= da_cu(p.s.cu_q, p.s.B, p.s.Tq)) return;
+    o = qr * p.o_st + h * p.o_sh;
+    lo = qr + h * p.l_sh;
+  } else {
+    const int64_t b = qr / p.s.Tq, t = qr % p.s.Tq;
+    if (p.s.q_len && t >= p.s.q_len[b]) return;  // (zeros, by the tiles)
+    o = b * p.o_sb + t * p.o_st + h * p.o_sh;
+    lo = b * p.l_sb + t + h * p.l_sh;
+  }
+  const float2 *ml = (const float2 *)p.ws_ml + row * p.splits;
+  float m = da_ninf();
+  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, ml[i].x);
+  float l = 0.f, acc[N];
+#pragma unroll
+  for (int x = 0; x < N; ++x) acc[x] = 0.f;
+  for (int i = 0; i < p.splits; ++i) {
+    const float2 part = ml[i];
+    if (part.x == da_ninf() && part.y == 0.f) continue;
+    const float f = fast_exp2(part.x - (m == da_ninf() ? 0.f : m));
+    l = __builtin_fmaf(part.y, f, l);
+    const float *a = p.ws_acc + (row * p.splits + i) * D + lane * N;
+#pragma unroll
+    for (int x = 0; x < N; ++x) acc[x] = __builtin_fmaf(a[x], f, acc[x]);
+  }
+  const bool none = l == 0.f;
+  const float inv = none ? 0.f : 1.f / l;
+#pragma unroll
+  for (int x = 0; x < N; ++x) da_store1(p.out, o + lane * N + x, p.out_dt, acc[x] * inv);
+  if (p.lse && lane == 0) p.lse[lo] = none ? da_ninf() : (m + __log2f(l)) * DA_LN2;
+}
+
+// ------------------------------------------------------------------ host ----
+struct DaPlan {
+  int nw = 4, rows = 128;  // waves and rows of a workgroup
+  int64_t ntile = 0, splits = 1;
+  size_t ml = 0, bytes = 0;
+};
+
+static DaPlan da_plan(const la_dense_attn_args *a) {
+  DaPlan pl;
+  const bool packed = a->cu_q != nullptr, f32 = a->dtype == LA_F32;
+  const int64_t G = a->Hq / a->Hkv;
+  auto tiles = [&](int64_t R) { return da_tiles(packed, a->B, a->Tq, G, R); };
+  if (f32) {
+    pl.nw = 4;
+    pl.rows = 64;
+  } else {
+    pl.nw = 4;
+    pl.rows = 128;
+  }
+  pl.ntile = tiles(pl.rows);
+  // parts of at least four staged tiles, two workgroups a CU
+  const int64_t wgs = pl.ntile * a->Hkv, keys = packed ? ceil_div(a->Tk, a->B) : a->Tk;
+  const int64_t want = (int64_t)2 * num_cus() / std::max<int64_t>(1, wgs);
+  pl.splits = std::max<int64_t>(1, std::min<int64_t>({want, keys / (4 * DA_BS), 64}));
+  if (pl.splits > 1) {
+    const int64_t parts = (packed ? 1 : a->B) * a->Tq * a->Hq * pl.splits;
+    pl.ml = ((size_t)parts * 2 * sizeof(float) + 255) / 256 * 256;
+    pl.bytes = pl.ml + (size_t)parts * a->D * sizeof(float);
+  }
+  return pl;
+}
+
+static int da_check(const la_dense_attn_args *a) {
+  LA_REQUIRE(a != nullptr, "la_dense_attention: null args");
+  LA_REQUIRE(a->B > 0 && a->Hq > 0 && a->Hkv > 0 && a->Tq >= 0 && a->Tk >= 0, "la_dense_attention: sizes must be positive");
+  LA_REQUIRE(a->Hq % a->Hkv == 0, "la_dense_attention: Hq must be a multiple of Hkv");
+  LA_REQUIRE(a->D == 64 || a->D == 128, "la_dense_attention: head_dim %lld (64 or 128)", (long long)a->D);
+  LA_REQUIRE(a->dtype == LA_F32 || a->dtype == LA_BF16 || a->dtype == LA_F16, "la_dense_attention: dtype");
+  LA_REQUIRE(a->out_dtype == a->dtype || a->out_dtype == LA_F32, "la_dense_attention: out_dtype is dtype or fp32");
+  LA_REQUIRE(a->scale > 0.f && a->scale < 1e30f, "la_dense_attention: scale must be positive");
+  LA_REQUIRE(a->B < ((int64_t)1 << 24) && a->Tk < ((int64_t)1 << 30) && a->Tq * (a->Hq / a->Hkv) < ((int64_t)1 << 30),
+             "la_dense_attention: sizes past 2^30 rows");
+  LA_REQUIRE(a->cu_q || !a->cu_k, "la_dense_attention: cu_k without cu_q");
+  LA_REQUIRE(!(a->cu_q && (a->q_len || a->k_len)), "la_dense_attention: lengths are for batched calls");
+  return LA_OK;
+}
+
+static int da_rows_ok(const char *what, const void *p, int64_t esz, int64_t sb, int64_t sh, int64_t st, int64_t heads,
+                      int64_t rows) {
+  const int64_t n = 16 / esz;
+  if (heads == 1) sh = 0;
+  if (rows == 1) st = 0;
+  LA_REQUIRE(p != nullptr, "la_dense_attention: null %s", what);
+  LA_REQUIRE((uintptr_t)p % 16 == 0 && sb % n == 0 && sh % n == 0 && st % n == 0,
+             "la_dense_attention: rows of %s must be 16-byte aligned", what);
+  return LA_OK;
+}
+
+template <class K>
+static int da_launch(K kernel, int64_t wgs, int threads, const DaKP &p, hipStream_t st) {
+  kernel<<<dim3((uint32_t)wgs), dim3(threads), 0, st>>>(p);
+  LA_LAUNCHED();
+  return LA_OK;
+}
+
+template <class T, int D>
+static int da_launch16(const DaPlan &pl, const DaKP &p, hipStream_t st) {
+  const int64_t wgs = pl.ntile * p.Hkv * pl.splits;
+  return da_launch(dense_attn_kernel<T, D, 4>, wgs, 256, p, st);
+}
+
+}  // namespace la
+
+extern "C" size_t la_dense_attention_workspace(const la_dense_attn_args *a) {
+  if (la::da_check(a) != LA_OK || a->Tq == 0) return 0;
+  return la::da_plan(a).bytes;
+}
+
+extern "C" int la_dense_attention(const la_dense_attn_args *a, void *stream) {
+  using namespace la;
+  if (int rc = da_check(a)) return rc;
+  if (a->Tq == 0) return LA_OK;
+  const int64_t esz = a->dtype == LA_F32 ? 4 : 2;
+  const int64_t osz = a->out_dtype == LA_F32 ? 4 : 2;
+  const bool packed = a->cu_q != nullptr;
+  auto sb = [&](int64_t s) { return packed || a->B == 1 ? 0 : s; };
+  if (int rc = da_rows_ok("q", a->q, esz, sb(a->q_sb), a->q_sh, a->q_st, a->Hq, a->Tq)) return rc;
+  if (a->Tk > 0) {
+    if (int rc = da_rows_ok("k", a->k, esz, sb(a->k_sb), a->k_sh, a->k_st, a->Hkv, a->Tk)) return rc;
+    if (int rc = da_rows_ok("v", a->v, esz, sb(a->v_sb), a->v_sh, a->v_st, a->Hkv, a->Tk)) return rc;
+  }
+  if (int rc = da_rows_ok("out", a->out, osz, sb(a->o_sb), a->o_sh, a->o_st, a->Hq, a->Tq)) return rc;
+  const DaPlan pl = da_plan(a);
+  if (pl.bytes > 0 && (!a->workspace || a->ws_bytes < (int64_t)pl.bytes))
+    return fail(LA_ERR_WORKSPACE, "la_dense_attention: workspace %lld < %lld bytes", (long long)a->ws_bytes,
+                (long long)pl.bytes);
+  LA_REQUIRE((uintptr_t)a->workspace % 256 == 0 || pl.bytes == 0, "la_dense_attention: workspace alignment");
+  const int64_t wgs = pl.ntile * a->Hkv * pl.splits;
+  LA_REQUIRE(pl.ntile < ((int64_t)1 << 31) && wgs < ((int64_t)1 << 31) / 64, "la_dense_attention: too many rows");
+  DaKP p{};
+  p.s = DaSeqs{a->cu_q, a->cu_k, a->q_len, a->k_len, a->Tq, a->Tk, (int32_t)a->B, (int32_t)(a->Hq / a->Hkv)};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.lse = a->lse;
+  p.ws_ml = (float *)a->workspace;
+  p.ws_acc = (float *)((char *)a->workspace + pl.ml);
+  p.q_sb = a->q_sb; p.q_sh = a->q_sh; p.q_st = a->q_st;
+  p.k_sb = a->k_sb; p.k_sh = a->k_sh; p.k_st = a->k_st;
+  p.v_sb = a->v_sb; p.v_sh = a->v_sh; p.v_st = a->v_st;
+  p.o_sb = a->o_sb; p.o_sh = a->o_sh; p.o_st = a->o_st;
+  p.l_sb = a->l_sb; p.l_sh = a->l_sh;
+  p.Hq = (int32_t)a->Hq; p.Hkv = (int32_t)a->Hkv;
+  p.ntile = (int32_t)pl.ntile; p.splits = (int32_t)pl.splits;
+  p.causal = a->causal != 0; p.out_dt = a->out_dtype; p.zero_rest = a->zero_rest != 0;
+  p.qscale = a->scale * 1.44269504088896340736f;
+  p.thr_gap = 8.f / p.qscale;
+  hipStream_t st = (hipStream_t)stream;
+  int rc;
+  if (a->dtype == LA_F32)
+    rc = a->D == 128 ? da_launch(dense_attn_f32_kernel<128>, wgs, 256, p, st)
+                     : da_launch(dense_attn_f32_kernel<64>, wgs, 256, p, st);
+  else if (a->dtype == LA_BF16)
+    rc = a->D == 128 ? da_launch16<DaBf16, 128>(pl, p, st) : da_launch16<DaBf16, 64>(pl, p, st);
+  else
+    rc = a->D == 128 ? da_launch16<DaF16, 128>(pl, p, st) : da_launch16<DaF16, 64>(pl, p, st);
+  if (rc != LA_OK || pl.splits == 1) return rc;
+  const int64_t rows = (packed ? 1 : a->B) * a->Tq * a->Hq;
+  const dim3 grid((uint32_t)ceil_div(rows, 4));
+  if (a->D == 128) dense_combine_kernel<128><<<grid, 256, 0, st>>>(p, rows);
+  else dense_combine_kernel<64><<<grid, 256, 0, st>>>(p, rows);
+  LA_LAUNCHED();
+  return LA_OK;
+}
