@@ -713,6 +713,44 @@ typedef struct {
 size_t la_dense_attention_workspace(const la_dense_attn_args *a);
 int la_dense_attention(const la_dense_attn_args *a, void *stream);
 
+/*
+ * The attention weight each key gathers, per KV head: what eviction ranks cached keys by.
+ *   w[s] = sum over the heads of the group and the last `last` queries t (0: all) that see s
+ *          of exp(scale q_t . k_s - lse[h][t])
+ * with the sequences, causality and layouts of la_dense_attention and its lse.  A query
+ * whose lse is -inf adds nothing.  out (fp32, strides w_sb, w_sh, 1) has a value for every
+ * key row: with accumulate != 0 the weights are added to what it holds; else they replace
+ * it, and keys past a sequence's length get 0 (packed: keys of no sequence with zero_rest).
+ * Sums are in a fixed order: the same call gives the same bits.
+ */
+typedef struct {
+  const void *q;
+  const void *k;
+  const float *lse;
+  float *out;
+  const int32_t *cu_q;
+  const int32_t *cu_k;
+  const int32_t *q_len;
+  const int32_t *k_len;
+  void *workspace;
+  int64_t ws_bytes;
+  int64_t B, Hq, Hkv, Tq, Tk, D;
+  int64_t q_sb, q_sh, q_st;
+  int64_t k_sb, k_sh, k_st;
+  int64_t l_sb, l_sh;
+  int64_t w_sb, w_sh;
+  int64_t last;
+  float scale;
+  int32_t causal;
+  int32_t dtype;
+  int32_t accumulate;
+  int32_t zero_rest;
+  int32_t reserved;
+} la_key_weights_args;
+
+size_t la_key_weights_workspace(const la_key_weights_args *a);
+int la_key_weights(const la_key_weights_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,6 +50,8 @@ EXPORTED = (
     "la_xattn_select",
     "la_dense_attention_workspace",
     "la_dense_attention",
+    "la_key_weights_workspace",
+    "la_key_weights",
     "la_device_status",
     "la_test_set_spin_limit",
 )
@@ -182,6 +184,16 @@ class LaDenseAttnArgs(ctypes.Structure):
                 ("out_dtype", _i32), ("zero_rest", _i32), ("reserved", _i32)]
 
 
+class LaKeyWeightsArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("lse", _vp), ("out", _vp), ("cu_q", _vp), ("cu_k", _vp),
+                ("q_len", _vp), ("k_len", _vp), ("workspace", _vp), ("ws_bytes", _i64),
+                ("B", _i64), ("Hq", _i64), ("Hkv", _i64), ("Tq", _i64), ("Tk", _i64), ("D", _i64),
+                ("q_sb", _i64), ("q_sh", _i64), ("q_st", _i64), ("k_sb", _i64), ("k_sh", _i64),
+                ("k_st", _i64), ("l_sb", _i64), ("l_sh", _i64), ("w_sb", _i64), ("w_sh", _i64),
+                ("last", _i64), ("scale", ctypes.c_float), ("causal", _i32), ("dtype", _i32),
+                ("accumulate", _i32), ("zero_rest", _i32), ("reserved", _i32)]
+
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -237,6 +249,9 @@ def load() -> ctypes.CDLL:
     L.la_dense_attention_workspace.argtypes = [P(LaDenseAttnArgs)]
     L.la_dense_attention_workspace.restype = ctypes.c_size_t
     L.la_dense_attention.argtypes = [P(LaDenseAttnArgs), _vp]
+    L.la_key_weights_workspace.argtypes = [P(LaKeyWeightsArgs)]
+    L.la_key_weights_workspace.restype = ctypes.c_size_t
+    L.la_key_weights.argtypes = [P(LaKeyWeightsArgs), _vp]
     L.la_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), _i32, _vp]
     L.la_test_set_spin_limit.argtypes = [ctypes.c_uint32]
     for name in EXPORTED:

@@ -1,0 +1,417 @@
+// The attention weight each key gathers (la_key_weights): column sums of the softmax
+// whose rows' log sums la_dense_attention returned.
+//
+// A workgroup takes a tile of keys of one KV head and keeps them in registers; it walks
+// the rows (query, head of the group) that see them, staged in LDS: S^T = K Q^T on the
+// matrix cores, P = exp2(c S - lse) in place, added lane by lane (a lane holds one row
+// and 16 keys of a product), and summed over the lanes once at the end.  Nothing is
+// normalised or joined on the way, so the rows of a tile can be split over workgroups;
+// their sums are added in order by a second kernel: no atomics.
+#include <algorithm>
+
+#include "dense_attn.h"
+
+namespace la {
+
+struct KwKP {
+  DaSeqs s;      // as given
+  DaSeqs tiles;  // keys as rows of one head: what da_tile cuts into tiles
+  const void *q, *k;
+  const float *lse;
+  float *out, *ws;  // ws: [split][what out has, densely]
+  int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, l_sb, l_sh, w_sb, w_sh, last, ws_split;
+  int32_t Hq, Hkv, ntile, splits, causal, accumulate, zero_rest;
+  float qscale;
+};
+
+// A tile's keys and the rows it walks.
+struct KwTile {
+  DaTile t;             // sequence (q0, k0, lq, lk as given), b < 0: none
+  int32_t s0;           // first key
+  int32_t row0, row1;   // this split's rows (query, head)
+};
+
+template <int KT>
+__device__ __forceinline__ KwTile kw_tile(const KwKP &p, int tix, int split) {
+  KwTile x;
+  x.t = da_tile(p.tiles, tix, p.ntile, KT);
+  x.s0 = x.row0 = x.row1 = 0;
+  if (x.t.b < 0) return x;
+  // da_tile's first tiles are the sequences' last; the first keys are seen by most rows
+  const int32_t n = p.s.cu_q ? x.t.lq : (int32_t)p.s.Tk;  // (rows of p.tiles: keys)
+  x.s0 = ((n + KT - 1) / KT) * KT - KT - x.t.r0;
+  da_seq(p.s, x.t);
+  if (x.s0 >= x.t.lk) return x;
+  const int G = p.s.G, diag = x.t.lk - x.t.lq;
+  int32_t t0 = p.last > 0 ? (int32_t)max((int64_t)x.t.lq - p.last, (int64_t)0) : 0;
+  if (p.causal) t0 = max(t0, x.s0 - diag);
+  const int64_t rows = (int64_t)max(x.t.lq - t0, 0) * G;
+  x.row0 = t0 * G + (int32_t)(rows * split / p.splits);
+  x.row1 = t0 * G + (int32_t)(rows * (split + 1) / p.splits);
+  return x;
+}
+
+// Where key s of the tile goes, and whether it is written here.
+template <class F>
+__device__ __forceinline__ void kw_put(const KwKP &p, const KwTile &x, int kvh, int split, int s, F value) {
+  const int64_t n = p.s.cu_q ? x.t.lk : p.s.Tk;
+  if (s >= n) return;
+  const float v = s < x.t.lk ? value() : 0.f;
+  const int64_t row = (p.s.cu_q ? x.t.k0 : 0) + s;
+  if (p.splits > 1) {
+    p.ws[split * p.ws_split + ((int64_t)(p.s.cu_q ? 0 : x.t.b) * p.Hkv + kvh) * p.s.Tk + row] = v;
+    return;
+  }
+  float *o = p.out + (p.s.cu_q ? 0 : x.t.b * p.w_sb) + kvh * p.w_sh + row;
+  *o = p.accumulate ? *o + v : v;
+}
+
+// Packed keys of no sequence, by the workgroups that got no tile.
+__device__ __forceinline__ void kw_rest(const KwKP &p, const KwTile &x, int kvh, int split, int tix) {
+  if (!p.zero_rest || split != 0 || x.t.b >= 0 || !p.s.cu_q) return;
+  const int32_t *ck = p.s.cu_k ? p.s.cu_k : p.s.cu_q;
+  const int64_t first = da_cu(ck, 0, p.s.Tk), last = max(first, (int64_t)da_cu(ck, p.s.B, p.s.Tk));
+  const int64_t n = first + p.s.Tk - last;
+  for (int64_t i = (int64_t)(tix - x.t.r0) * blockDim.x + threadIdx.x; i < n;
+       i += (int64_t)(p.ntile - x.t.r0) * blockDim.x)
+    p.out[kvh * p.w_sh + (i < first ? i : i + last - first)] = 0.f;
+}
+
+// Row r as (query, head of the group), moved on without dividing again.
+struct KwRow {
+  int32_t t, g;
+  __device__ __forceinline__ KwRow(int32_t r, int G) : t(r / G), g(r % G) {}
+  __device__ __forceinline__ void step(int32_t dt, int32_t dg, int G) {
+    t += dt;
+    g += dg;
+    if (g >= G) {
+      g -= G;
+      ++t;
+    }
+  }
+};
+
+// bf16 / fp16: four waves of 64 keys, rows staged 64 at a time by LDS-DMA, double buffered.
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
+  constexpr int NW = 4, KT = 64 * NW, BLK = DA_BS * D, CH = D / 8, RP = 64 / CH, NX = DA_BS / RP / NW;
+  constexpr int NS = D / 16;
+  typedef typename T::x8 x8;
+  typedef typename T::elem elem;
+  __shared__ __align__(16) uint16_t smem[2 * BLK];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hf = lane >> 5, r32 = lane & 31, G = p.s.G;
+  uint32_t stream, tix;
+  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, p.ntile, stream, tix);
+  const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
+  const KwTile x = kw_tile<KT>(p, (int)tix, split);
+  kw_rest(p, x, kvh, split, (int)tix);
+  if (x.t.b < 0) return;
+
+  const int s_w = x.s0 + 64 * w;  // this wave's keys
+  const int diag = x.t.lk - x.t.lq;
+  f32x16 acc[2];
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
+
+  const int nrow = x.row1 - x.row0;
+  if (nrow > 0) {
+    x8 kf[2][NS];  // A operand: key 32 kt + r32, dims 16 s + 8 hf ..
+    const elem *kbh = (const elem *)p.k + (p.s.cu_q ? x.t.k0 * p.k_st : x.t.b * p.k_sb) + kvh * p.k_sh;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int64_t key = min(s_w + 32 * kt + r32, x.t.lk - 1);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) kf[kt][s] = *(const x8 *)(kbh + key * p.k_st + 16 * s + 8 * hf);
+    }
+    const elem *qbh = (const elem *)p.q + (p.s.cu_q ? x.t.q0 * p.q_st : x.t.b * p.q_sb) + kvh * G * p.q_sh;
+    const float *lbh = p.lse + (p.s.cu_q ? x.t.q0 : x.t.b * p.l_sb) + kvh * G * p.l_sh;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
+    const int dt = DA_BS / G, dg = DA_BS % G;
+    const KwRow end(x.row1 - 1, G);
+    auto dma = [&](int j, int slot) {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int u = NW * i + w, rr = RP * u + lane / CH;
+        const KwRow r(min(x.row0 + j * DA_BS + rr, x.row1 - 1), G);
+        asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(qbh + r.t * p.q_st + r.g * p.q_sh +
+                                                             8 * ((lane % CH) ^ da_swz_k<D>(rr))),
+                     "{m0}"(lds0 + 2 * (slot * BLK + u * 512)) : "memory");
+      }
+    };
+    KwRow mine[2] = {KwRow(x.row0 + r32, G), KwRow(x.row0 + 32 + r32, G)};  // of each half of a tile
+    float ls[2];
+    int seen[2];
+    auto rows = [&](int j) {  // lse and last key seen of each half's row
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const KwRow &r = x.row0 + j * DA_BS + 32 * h + r32 < x.row1 ? mine[h] : end;
+        ls[h] = lbh[r.t + r.g * p.l_sh];
+        seen[h] = p.causal ? diag + r.t : x.t.lk - 1;
+        mine[h].step(dt, dg, G);
+      }
+    };
+    const int n = (nrow + DA_BS - 1) / DA_BS;
+    rows(0);
+    dma(0, 0);
+    for (int j = 0; j < n; ++j) {
+      wait_vmcnt<0>();
+      float nl[2];  // -lse in log2 units; -inf: the row adds nothing
+      int last[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        settle(ls[h]);
+        const bool none = x.row0 + j * DA_BS + 32 * h + r32 >= x.row1 || ls[h] == __int_as_float(0xff800000);
+        nl[h] = none ? __int_as_float(0xff800000) : -ls[h] * 1.44269504088896340736f;
+        last[h] = seen[h];
+      }
+      lds_barrier();
+      if (j + 1 < n) {
+        rows(j + 1);
+        dma(j + 1, (j + 1) & 1);
+      }
+      const uint16_t *sq = smem + (j & 1) * BLK;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int rl = 32 * h + r32, sw = da_swz_k<D>(rl);
+        x8 qf[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qf[s] = *(const x8 *)&sq[rl * D + 8 * ((2 * s + hf) ^ sw)];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          f32x16 st;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st[i] = 0.f;
+#pragma unroll
+          for (int s = 0; s < NS; ++s) st = T::mfma(kf[kt][s], qf[s], st);
+          // register i: key 8 (i / 4) + 4 hf + i % 4
+          const int d = last[h] - (s_w + 32 * kt + 4 * hf);
+          if (__ballot(d < 31 - 4 * hf) == 0) {  // all keys seen by all rows
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[kt][i] += fast_exp2(__builtin_fmaf(st[i], p.qscale, nl[h]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float e = fast_exp2(__builtin_fmaf(st[i], p.qscale, nl[h]));
+              acc[kt][i] += 8 * (i >> 2) + (i & 3) <= d ? e : 0.f;
+            }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float v = group_sum<32>(acc[kt][i]);
+      if (r32 == i) kw_put(p, x, kvh, split, s_w + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3), [&] { return v; });
+    }
+}
+
+// fp32: four waves of 32 keys on 16x16x4 products; lane (c, i) holds chunk 4 s + c of key
+// i, and of row i of the staged rows, as in dense_attn_f32_kernel.
+template <int D>
+__global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
+  constexpr int NW = 4, KT = 32 * NW, BS = 32, BLK = BS * D, CH = D / 4, RP = 64 / CH, NX = BS / RP / NW;
+  constexpr int NS = D / 16;
+  __shared__ __align__(16) float smem[2 * BLK];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane >> 4, ri = lane & 15, G = p.s.G;
+  uint32_t stream, tix;
+  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, p.ntile, stream, tix);
+  const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
+  const KwTile x = kw_tile<KT>(p, (int)tix, split);
+  kw_rest(p, x, kvh, split, (int)tix);
+  if (x.t.b < 0) return;
+  const int s_w = x.s0 + 32 * w, diag = x.t.lk - x.t.lq;
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  const int nrow = x.row1 - x.row0;
+  if (nrow > 0) {
+    f32x4 kf[2][NS];
+    const float *kbh = (const float *)p.k + (p.s.cu_q ? x.t.k0 * p.k_st : x.t.b * p.k_sb) + kvh * p.k_sh;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int64_t key = min(s_w + 16 * kt + ri, x.t.lk - 1);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) kf[kt][s] = *(const f32x4 *)(kbh + key * p.k_st + 16 * s + 4 * c);
+    }
+    const float *qbh = (const float *)p.q + (p.s.cu_q ? x.t.q0 * p.q_st : x.t.b * p.q_sb) + kvh * G * p.q_sh;
+    const float *lbh = p.lse + (p.s.cu_q ? x.t.q0 : x.t.b * p.l_sb) + kvh * G * p.l_sh;
+    auto swz = [](int r) { return 2 * (r & 7); };
+    auto dma = [&](int j, int slot) {
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int u = NW * i + w, rr = RP * u + lane / CH;
+        const KwRow r(min(x.row0 + j * BS + rr, x.row1 - 1), G);
+        dma16(qbh + r.t * p.q_st + r.g * p.q_sh + 4 * ((lane % CH) ^ swz(rr)), smem + slot * BLK + u * 256);
+      }
+    };
+    const int n = (nrow + BS - 1) / BS;
+    dma(0, 0);
+    for (int j = 0; j < n; ++j) {
+      float nl[2];
+      int seen[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int rr = x.row0 + j * BS + 16 * h + ri;
+        const KwRow r(min(rr, x.row1 - 1), G);
+        const float l = lbh[r.t + r.g * p.l_sh];
+        nl[h] = rr < x.row1 && l != __int_as_float(0xff800000) ? -l * 1.44269504088896340736f
+                                                              : __int_as_float(0xff800000);
+        seen[h] = p.causal ? diag + r.t : x.t.lk - 1;
+      }
+      wait_vmcnt<0>();
+      settle(nl[0]);
+      settle(nl[1]);
+      lds_barrier();
+      if (j + 1 < n) dma(j + 1, (j + 1) & 1);
+      const float *sq = smem + (j & 1) * BLK;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int rl = 16 * h + ri;
+        f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const f32x4 b = *(const f32x4 *)&sq[rl * D + 4 * ((4 * s + c) ^ swz(rl))];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              st[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[kt][s][e], b[e], st[kt], 0, 0, 0);
+        }
+        // register e: key 4 c + e
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          const int d = seen[h] - (s_w + 16 * kt + 4 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float pr = fast_exp2(__builtin_fmaf(st[kt][e], p.qscale, nl[h]));
+            acc[kt][e] += e <= d ? pr : 0.f;
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = group_sum<16>(acc[kt][e]);
+      if (ri == e) kw_put(p, x, kvh, split, s_w + 16 * kt + 4 * c + e, [&] { return v; });
+    }
+}
+
+// Adds the parts of a key in their order.  Packed keys of no sequence have no parts.
+__global__ __launch_bounds__(256) void key_weights_sum_kernel(KwKP p) {
+  const int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y;
+  if (s >= p.s.Tk) return;
+  if (p.s.cu_q) {
+    const int32_t *ck = p.s.cu_k ? p.s.cu_k : p.s.cu_q;
+    if (s < da_cu(ck, 0, p.s.Tk) || s >= da_cu(ck, p.s.B, p.s.Tk)) return;
+  }
+  const float *part = p.ws + bh * p.s.Tk + s;
+  float v = 0.f;
+  for (int i = 0; i < p.splits; ++i) v += part[i * p.ws_split];
+  float *o = p.out + (p.s.cu_q ? 0 : bh / p.Hkv * p.w_sb) + bh % p.Hkv * p.w_sh + s;
+  *o = p.accumulate ? *o + v : v;
+}
+
+// ------------------------------------------------------------------ host ----
+struct KwPlan {
+  int keys = 256;
+  int64_t ntile = 0, splits = 1;
+  size_t bytes = 0;
+};
+
+static KwPlan kw_plan(const la_key_weights_args *a) {
+  KwPlan pl;
+  const bool packed = a->cu_q != nullptr;
+  pl.keys = a->dtype == LA_F32 ? 128 : 256;
+  pl.ntile = da_tiles(packed, a->B, a->Tk, 1, pl.keys);
+  // Rows are split until there are eight workgroups a CU (causal tiles differ in length
+  // by far), down to four staged tiles each.
+  const int64_t wgs = pl.ntile * a->Hkv, G = a->Hq / a->Hkv;
+  int64_t rows = (packed ? ceil_div(a->Tq, a->B) : a->Tq) * G;
+  if (a->last > 0) rows = std::min(rows, a->last * G);
+  pl.splits = std::max<int64_t>(1, std::min<int64_t>({ceil_div((int64_t)8 * num_cus(), wgs), rows / 256, 64}));
+  if (pl.splits > 1) pl.bytes = (size_t)((packed ? 1 : a->B) * a->Hkv * a->Tk * pl.splits) * sizeof(float);
+  return pl;
+}
+
+static int kw_check(const la_key_weights_args *a) {
+  LA_REQUIRE(a != nullptr, "la_key_weights: null args");
+  LA_REQUIRE(a->B > 0 && a->Hq > 0 && a->Hkv > 0 && a->Tq >= 0 && a->Tk >= 0, "la_key_weights: sizes must be positive");
+  LA_REQUIRE(a->Hq % a->Hkv == 0, "la_key_weights: Hq must be a multiple of Hkv");
+  LA_REQUIRE(a->D == 64 || a->D == 128, "la_key_weights: head_dim %lld (64 or 128)", (long long)a->D);
+  LA_REQUIRE(a->dtype == LA_F32 || a->dtype == LA_BF16 || a->dtype == LA_F16, "la_key_weights: dtype");
+  LA_REQUIRE(a->scale > 0.f && a->scale < 1e30f, "la_key_weights: scale must be positive");
+  LA_REQUIRE(a->last >= 0, "la_key_weights: last must not be negative");
+  LA_REQUIRE(a->B < ((int64_t)1 << 24) && a->Tk < ((int64_t)1 << 30) && a->Tq * (a->Hq / a->Hkv) < ((int64_t)1 << 30),
+             "la_key_weights: sizes past 2^30 rows");
+  LA_REQUIRE(a->cu_q || !a->cu_k, "la_key_weights: cu_k without cu_q");
+  LA_REQUIRE(!(a->cu_q && (a->q_len || a->k_len)), "la_key_weights: lengths are for batched calls");
+  return LA_OK;
+}
+
+}  // namespace la
+
+extern "C" size_t la_key_weights_workspace(const la_key_weights_args *a) {
+  if (la::kw_check(a) != LA_OK || a->Tk == 0) return 0;
+  return la::kw_plan(a).bytes;
+}
+
+extern "C" int la_key_weights(const la_key_weights_args *a, void *stream) {
+  using namespace la;
+  if (int rc = kw_check(a)) return rc;
+  if (a->Tk == 0) return LA_OK;
+  const int64_t n16 = a->dtype == LA_F32 ? 4 : 8;
+  const bool packed = a->cu_q != nullptr;
+  LA_REQUIRE(a->k && a->out && ((a->q && a->lse) || a->Tq == 0), "la_key_weights: null pointer");
+  auto ok = [&](const void *x, int64_t sb, int64_t sh, int64_t st, int64_t heads, int64_t rows) {
+    return (uintptr_t)x % 16 == 0 && (packed || a->B == 1 || sb % n16 == 0) && (heads == 1 || sh % n16 == 0) &&
+           (rows == 1 || st % n16 == 0);
+  };
+  LA_REQUIRE(ok(a->k, a->k_sb, a->k_sh, a->k_st, a->Hkv, a->Tk) &&
+                 (a->Tq == 0 || ok(a->q, a->q_sb, a->q_sh, a->q_st, a->Hq, a->Tq)),
+             "la_key_weights: rows of q and k must be 16-byte aligned");
+  const KwPlan pl = kw_plan(a);
+  if (pl.bytes > 0 && (!a->workspace || a->ws_bytes < (int64_t)pl.bytes))
+    return fail(LA_ERR_WORKSPACE, "la_key_weights: workspace %lld < %lld bytes", (long long)a->ws_bytes,
+                (long long)pl.bytes);
+  const int64_t wgs = pl.ntile * a->Hkv * pl.splits;
+  const int64_t bh = (packed ? 1 : a->B) * a->Hkv;
+  LA_REQUIRE(wgs < ((int64_t)1 << 31) / 64 && bh < 65536, "la_key_weights: too many keys or heads");
+  KwKP p{};
+  p.s = DaSeqs{a->cu_q, a->cu_k, a->q_len, a->k_len, a->Tq, a->Tk, (int32_t)a->B, (int32_t)(a->Hq / a->Hkv)};
+  p.tiles = DaSeqs{packed ? (a->cu_k ? a->cu_k : a->cu_q) : nullptr, nullptr, nullptr, nullptr, a->Tk, a->Tk, (int32_t)a->B, 1};
+  p.q = a->q; p.k = a->k; p.lse = a->lse; p.out = a->out; p.ws = (float *)a->workspace;
+  p.q_sb = a->q_sb; p.q_sh = a->q_sh; p.q_st = a->q_st;
+  p.k_sb = a->k_sb; p.k_sh = a->k_sh; p.k_st = a->k_st;
+  p.l_sb = a->l_sb; p.l_sh = a->l_sh; p.w_sb = a->w_sb; p.w_sh = a->w_sh;
+  p.last = a->last; p.ws_split = bh * a->Tk;
+  p.Hq = (int32_t)a->Hq; p.Hkv = (int32_t)a->Hkv;
+  p.ntile = (int32_t)pl.ntile; p.splits = (int32_t)pl.splits;
+  p.causal = a->causal != 0; p.accumulate = a->accumulate != 0; p.zero_rest = a->zero_rest != 0 && !a->accumulate;
+  p.qscale = a->scale * 1.44269504088896340736f;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((uint32_t)wgs);
+  if (a->dtype == LA_F32) {
+    if (a->D == 128) key_weights_f32_kernel<128><<<grid, 256, 0, st>>>(p);
+    else key_weights_f32_kernel<64><<<grid, 256, 0, st>>>(p);
+  } else if (a->dtype == LA_BF16) {
+    if (a->D == 128) key_weights_kernel<DaBf16, 128><<<grid, 256, 0, st>>>(p);
+    else key_weights_kernel<DaBf16, 64><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (a->D == 128) key_weights_kernel<DaF16, 128><<<grid, 256, 0, st>>>(p);
+    else key_weights_kernel<DaF16, 64><<<grid, 256, 0, st>>>(p);
+  }
+  LA_LAUNCHED();
+  if (pl.splits > 1) {
+    key_weights_sum_kernel<<<dim3((uint32_t)ceil_div(a->Tk, 256), (uint32_t)bh), 256, 0, st>>>(p);
+    LA_LAUNCHED();
+  }
+  return LA_OK;
+}
