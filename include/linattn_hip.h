@@ -751,6 +751,92 @@ typedef struct {
 size_t la_key_weights_workspace(const la_key_weights_args *a);
 int la_key_weights(const la_key_weights_args *a, void *stream);
 
+/*
+ * Eviction: of each sequence's n cached entries keep `budget` per KV head, in order.
+ * Protected entries (positions below `sink`, or of the newest `recent`: >= pos - recent)
+ * come first, then the heaviest by weight; ties, and protected entries past the budget,
+ * go to the lowest index; a weight that is not a number ranks lowest.  n is lengths[b]
+ * (optional, int32 [B], clamped to [0, T]); an entry's position is positions[b][h][i]
+ * (optional int32, strides ps_sb, ps_sh and 1, with pos, int32 [B]: the position of the
+ * next token) or its index i (and pos n).
+ * The kept entries' rows of k and v, weights and positions go to slots 0 .. kept - 1 of
+ * k_out, v_out (B, Hkv, capacity, D), w_out and pos_out (B, Hkv, capacity), all
+ * contiguous; the slots behind them get zeros, weight 0 and position -1; len_out[b] is
+ * min(n, budget).  capacity >= budget >= sink + recent.
+ * Packed (cu non-null, int32 [B + 1]): sequence b's entries are rows cu[b] .. cu[b+1] - 1,
+ * T the tensors' rows and the *_sb strides unused.
+ * Rows of k and v: esize bytes per value, unit stride over D, 16-byte aligned.
+ * Workspace: la_evict_kv_workspace() bytes (the lists of kept entries).
+ */
+typedef struct {
+  const void *k;
+  const void *v;
+  const float *weights;
+  const int32_t *positions;
+  const int32_t *pos;
+  const int32_t *lengths;
+  const int32_t *cu;
+  void *k_out;
+  void *v_out;
+  float *w_out;
+  int32_t *pos_out;
+  int32_t *len_out;
+  void *workspace;
+  int64_t ws_bytes;
+  int64_t B, Hkv, T, D, esize;
+  int64_t k_sb, k_sh, k_st;
+  int64_t v_sb, v_sh, v_st;
+  int64_t w_sb, w_sh;
+  int64_t ps_sb, ps_sh;
+  int64_t budget, capacity, recent, sink;
+} la_evict_args;
+
+size_t la_evict_kv_workspace(const la_evict_args *a);
+int la_evict_kv(const la_evict_args *a, void *stream);
+
+/*
+ * One decode step over an evicted cache, in place: for each (b, KV head)
+ *   - the new token's slot is n = lengths[b] while the cache has room (n < C), else that
+ *     of the lightest entry that is not protected (position >= sink and < pos[b] - recent;
+ *     of equal weights the highest slot; a weight that is not a number is the lightest;
+ *     with every entry protected the highest slot);
+ *   - k_new, v_new, weight 0 and position pos[b] are written there;
+ *   - out = softmax(scale q k^T) v over the min(n + 1, C) entries, for each head of the
+ *     group, and every entry's weight grows by the group's weights on it.
+ * q, out (B, Hq, 1, D), k_new, v_new (B, Hkv, 1, D) (strides *_sb, *_sh, unit over D, rows
+ * 16-byte aligned); k, v (B, Hkv, C, D), weights and positions (B, Hkv, C), contiguous.
+ * lengths and pos (int32 [B]) are the caller's to advance.  dtype LA_F32, LA_BF16 or
+ * LA_F16, out_dtype that or LA_F32; D 64 or 128; Hq / Hkv at most 16; C < 2^24.
+ * Workspace: la_evict_decode_workspace() bytes, 256-byte aligned.
+ */
+typedef struct {
+  const void *q;
+  const void *k_new;
+  const void *v_new;
+  void *k;
+  void *v;
+  float *weights;
+  int32_t *positions;
+  const int32_t *lengths;
+  const int32_t *pos;
+  void *out;
+  void *workspace;
+  int64_t ws_bytes;
+  int64_t B, Hq, Hkv, C, D;
+  int64_t q_sb, q_sh;
+  int64_t kn_sb, kn_sh;
+  int64_t vn_sb, vn_sh;
+  int64_t o_sb, o_sh;
+  int64_t recent, sink;
+  float scale;
+  int32_t dtype;
+  int32_t out_dtype;
+  int32_t reserved;
+} la_evict_decode_args;
+
+size_t la_evict_decode_workspace(const la_evict_decode_args *a);
+int la_evict_decode(const la_evict_decode_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

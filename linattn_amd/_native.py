@@ -52,6 +52,10 @@ EXPORTED = (
     "la_dense_attention",
     "la_key_weights_workspace",
     "la_key_weights",
+    "la_evict_kv_workspace",
+    "la_evict_kv",
+    "la_evict_decode_workspace",
+    "la_evict_decode",
     "la_device_status",
     "la_test_set_spin_limit",
 )
@@ -194,6 +198,27 @@ class LaKeyWeightsArgs(ctypes.Structure):
                 ("accumulate", _i32), ("zero_rest", _i32), ("reserved", _i32)]
 
 
+class LaEvictArgs(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("weights", _vp), ("positions", _vp), ("pos", _vp),
+                ("lengths", _vp), ("cu", _vp), ("k_out", _vp), ("v_out", _vp), ("w_out", _vp),
+                ("pos_out", _vp), ("len_out", _vp), ("workspace", _vp), ("ws_bytes", _i64),
+                ("B", _i64), ("Hkv", _i64), ("T", _i64), ("D", _i64), ("esize", _i64),
+                ("k_sb", _i64), ("k_sh", _i64), ("k_st", _i64), ("v_sb", _i64), ("v_sh", _i64),
+                ("v_st", _i64), ("w_sb", _i64), ("w_sh", _i64), ("ps_sb", _i64), ("ps_sh", _i64),
+                ("budget", _i64), ("capacity", _i64), ("recent", _i64), ("sink", _i64)]
+
+
+class LaEvictDecodeArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k_new", _vp), ("v_new", _vp), ("k", _vp), ("v", _vp),
+                ("weights", _vp), ("positions", _vp), ("lengths", _vp), ("pos", _vp),
+                ("out", _vp), ("workspace", _vp), ("ws_bytes", _i64), ("B", _i64), ("Hq", _i64),
+                ("Hkv", _i64), ("C", _i64), ("D", _i64), ("q_sb", _i64), ("q_sh", _i64),
+                ("kn_sb", _i64), ("kn_sh", _i64), ("vn_sb", _i64), ("vn_sh", _i64),
+                ("o_sb", _i64), ("o_sh", _i64), ("recent", _i64), ("sink", _i64),
+                ("scale", ctypes.c_float), ("dtype", _i32), ("out_dtype", _i32),
+                ("reserved", _i32)]
+
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -252,6 +277,12 @@ def load() -> ctypes.CDLL:
     L.la_key_weights_workspace.argtypes = [P(LaKeyWeightsArgs)]
     L.la_key_weights_workspace.restype = ctypes.c_size_t
     L.la_key_weights.argtypes = [P(LaKeyWeightsArgs), _vp]
+    L.la_evict_kv_workspace.argtypes = [P(LaEvictArgs)]
+    L.la_evict_kv_workspace.restype = ctypes.c_size_t
+    L.la_evict_kv.argtypes = [P(LaEvictArgs), _vp]
+    L.la_evict_decode_workspace.argtypes = [P(LaEvictDecodeArgs)]
+    L.la_evict_decode_workspace.restype = ctypes.c_size_t
+    L.la_evict_decode.argtypes = [P(LaEvictDecodeArgs), _vp]
     L.la_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), _i32, _vp]
     L.la_test_set_spin_limit.argtypes = [ctypes.c_uint32]
     for name in EXPORTED:

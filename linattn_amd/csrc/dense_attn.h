@@ -15,12 +15,16 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int DA_BS = 64;  // keys of a staged tile
 
-// Element types on the matrix cores: 32 x 32 += (32 x 16) (16 x 32).
+// Element types on the matrix cores: 32 x 32 += (32 x 16) (16 x 32), or 16 x 16 += (16 x
+// 32) (32 x 16).
 struct DaBf16 {
   typedef bf16x8 x8;
   typedef __bf16 elem;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
 };
 struct DaF16 {
@@ -28,6 +32,9 @@ struct DaF16 {
   typedef _Float16 elem;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
 };
 

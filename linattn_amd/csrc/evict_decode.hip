@@ -1,0 +1,307 @@
+// One decode step over an evicted cache (la_evict_decode): the slot of the new token, the
+// attention over the cache with it, and the weights its entries gather.
+//
+// The K/V rows of a (sequence, KV head) are read once and bound the step; the heads of a
+// group are the rows of FewRows (few_rows.h), each wave of a workgroup on rounds of its
+// own, joined through LDS.  The slot's row is read from k_new / v_new, never from the
+// cache, so writing it there races with nothing.  Weights need the row's final sum: the
+// scores (a float per head and entry, 1/32 of the K/V bytes at four heads) are kept in
+// the workspace.  Where there are enough (sequence, head) pairs, one workgroup does all
+// of a pair; else its entries are split: evict_slot_kernel, evict_decode_kernel over the
+// parts, evict_join_kernel.
+#include <algorithm>
+
+#include "evict.h"
+#include "few_rows.h"
+
+namespace la {
+
+struct EdKP {
+  const void *q, *k_new, *v_new;
+  void *k, *v, *out;
+  float *weights;
+  int32_t *positions;
+  const int32_t *lengths, *pos;
+  int32_t *slots;   // [pair] (split form)
+  float *ml;        // [pair][split][G] (max in log2 units, sum)
+  float *vals;      // [pair][split][G][D]
+  float *scores;    // [pair][G][cs]
+  int64_t q_sb, q_sh, kn_sb, kn_sh, vn_sb, vn_sh, o_sb, o_sh, recent, sink, cs;
+  int32_t B, Hq, Hkv, G, C, splits, out_dt, chunks;
+  float qscale;
+};
+
+constexpr float ED_GAP = 8.f;  // headroom of the reference maximum, log2 units
+
+// The entry that makes room (of a full cache), by a workgroup of NT threads: the lowest
+// key, of equal ones the highest slot.
+template <int NT>
+__device__ __forceinline__ int32_t ed_victim(const EdKP &p, int64_t pair, int64_t pos) {
+  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+  typedef int32_t i4u __attribute__((ext_vector_type(4), aligned(4)));
+  __shared__ uint64_t best[NT / 64];
+  const float *w = p.weights + pair * p.C;
+  const int32_t *ps = p.positions + pair * p.C;
+  uint64_t mine = ~0ull;
+  auto look = [&](int32_t i, float x, int32_t at) {
+    const uint64_t k = ev_safe(at, pos, p.recent, p.sink) ? EV_SAFE : ev_key(x);
+    mine = min(mine, (k << 32) | (uint32_t)~i);
+  };
+  const int32_t whole = p.C & ~3;
+  for (int32_t i0 = 0; i0 < whole; i0 += 16 * NT) {
+    f4u x[4];
+    i4u y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int32_t i = min(i0 + 4 * (NT * j + (int32_t)threadIdx.x), whole - 4);
+      x[j] = *(const f4u *)(w + i);
+      y[j] = *(const i4u *)(ps + i);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int32_t i = min(i0 + 4 * (NT * j + (int32_t)threadIdx.x), whole - 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) look(i + e, x[j][e], y[j][e]);
+    }
+  }
+  if (whole + (int32_t)threadIdx.x < p.C) look(whole + threadIdx.x, w[whole + threadIdx.x], ps[whole + threadIdx.x]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) mine = min(mine, (uint64_t)__shfl_xor((unsigned long long)mine, o, 64));
+  if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  mine = best[0];
+#pragma unroll
+  for (int x = 1; x < NT / 64; ++x) mine = min(mine, best[x]);
+  return (int32_t)~(uint32_t)mine;
+}
+
+__device__ __forceinline__ int32_t ed_held(const EdKP &p, int b) { return min(max(p.lengths[b], 0), p.C); }
+
+__global__ __launch_bounds__(1024) void evict_slot_kernel(EdKP p) {
+  const int64_t pair = blockIdx.x;
+  const int b = (int)(pair / p.Hkv);
+  const int32_t n = ed_held(p, b);
+  const int32_t slot = n < p.C ? n : ed_victim<1024>(p, pair, p.pos[b]);
+  if (threadIdx.x == 0) p.slots[pair] = slot;
+}
+
+// Rows' weights over entries first .. end - 1 added to what they gathered; lse2 in LDS.
+template <int NT>
+__device__ __forceinline__ void ed_weights(const EdKP &p, int64_t pair, int32_t slot, int32_t first, int32_t end,
+                                           const float *lse2) {
+  const float *s = p.scores + pair * p.G * p.cs;
+  float *w = p.weights + pair * p.C;
+  for (int32_t i = first + (int32_t)threadIdx.x; i < end; i += NT) {
+    float sum = 0.f;
+    for (int g = 0; g < p.G; ++g) sum += fast_exp2(s[g * p.cs + i] - lse2[g]);
+    w[i] = (i == slot ? 0.f : w[i]) + sum;
+    if (i == slot) p.positions[pair * p.C + i] = p.pos[pair / p.Hkv];
+  }
+}
+
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
+  typedef FewRows<T, D> FR;
+  typedef typename FR::elem elem;
+  constexpr int NW = 4;
+  constexpr int LDS_MERGE = NW * (FR::VALS + 32) * 4;
+  constexpr int LDS = NW * FR::LDS_BYTES > LDS_MERGE ? NW * FR::LDS_BYTES : LDS_MERGE;
+  __shared__ __align__(16) char smem[LDS];
+  __shared__ float lse2[16];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t pair = blockIdx.x / (uint32_t)p.splits;
+  const int split = (int)(blockIdx.x % (uint32_t)p.splits);
+  const int b = (int)(pair / p.Hkv), kvh = (int)(pair % p.Hkv);
+  const int32_t held = ed_held(p, b), n = min(held + 1, p.C);
+  int32_t slot;
+  if (p.splits > 1) slot = p.slots[pair];
+  else slot = held < p.C ? held : ed_victim<256>(p, pair, p.pos[b]);
+  slot = __builtin_amdgcn_readfirstlane(slot);
+
+  const elem *kn = (const elem *)p.k_new + b * p.kn_sb + kvh * p.kn_sh;
+  const elem *vn = (const elem *)p.v_new + b * p.vn_sb + kvh * p.vn_sh;
+  elem *kc = (elem *)p.k + pair * p.C * D, *vc = (elem *)p.v + pair * p.C * D;
+  const int row = min(lane & 15, p.G - 1);
+  FR fr;
+  fr.begin((const elem *)p.q + b * p.q_sb + (kvh * p.G + row) * p.q_sh);
+  const int rounds = (n + FR::RK - 1) / FR::RK;
+  const int r0 = (int)((int64_t)rounds * split / p.splits), r1 = (int)((int64_t)rounds * (split + 1) / p.splits);
+  float *sc = p.scores + (pair * p.G + row) * p.cs;
+  const bool put = (lane & 15) < p.G;
+  fr.walk(r0 + w, NW, r1, n, n - 1, p.qscale, ED_GAP, (elem *)(smem + w * FR::LDS_BYTES),
+          [&](int key) { return key == slot ? kn : kc + (int64_t)key * D; },
+          [&](int key) { return key == slot ? vn : vc + (int64_t)key * D; },
+          [&](int key, f32x4 s) { if (put) *(f32x4 *)(sc + key) = s; });
+  // the new token's rows, by the part that holds its slot
+  if (slot / FR::RK >= r0 && slot / FR::RK < r1 && w == 0) {
+    constexpr int CHE = FR::CHE;
+    if (lane < D / CHE) {
+      *(uint4 *)(kc + (int64_t)slot * D + CHE * lane) = *(const uint4 *)(kn + CHE * lane);
+      *(uint4 *)(vc + (int64_t)slot * D + CHE * lane) = *(const uint4 *)(vn + CHE * lane);
+    }
+  }
+  __syncthreads();  // the waves' staged rows are read (and their scores written)
+  float *ml = (float *)smem, *vals = ml + NW * 32;
+  fr.put(ml + w * 32, vals + w * FR::VALS);
+  __syncthreads();
+  const float ninf = __int_as_float(0xff800000);
+  for (int e = threadIdx.x; e < p.G * D; e += 256) {
+    const int g = e / D, d = e % D;
+    float m = ninf;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) m = fmaxf(m, ml[x * 32 + 2 * g]);
+    float l = 0.f, a = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const float f = fast_exp2(ml[x * 32 + 2 * g] - (m == ninf ? 0.f : m));
+      l = __builtin_fmaf(ml[x * 32 + 2 * g + 1], f, l);
+      a = __builtin_fmaf(vals[x * FR::VALS + g * (D + 4) + d], f, a);
+    }
+    if (p.splits > 1) {
+      const int64_t at = (pair * p.splits + split) * p.G + g;
+      p.vals[at * D + d] = a;
+      if (d == 0) {
+        p.ml[2 * at] = m;
+        p.ml[2 * at + 1] = l;
+      }
+    } else {
+      store_from_f32(p.out, b * p.o_sb + (kvh * p.G + g) * p.o_sh + d, p.out_dt, a / l);
+      if (d == 0) lse2[g] = m + __log2f(l);
+    }
+  }
+  if (p.splits > 1) return;
+  __syncthreads();
+  ed_weights<256>(p, pair, slot, 0, n, lse2);
+}
+
+// Parts joined: a pair's output and the weights of 1024 entries a workgroup.
+constexpr int ED_CHUNK = 1024;
+template <int D>
+__global__ __launch_bounds__(256) void evict_join_kernel(EdKP p) {
+  __shared__ float lse2[16];
+  const int64_t pair = blockIdx.x / (uint32_t)p.chunks;
+  const int chunk = (int)(blockIdx.x % (uint32_t)p.chunks);
+  const int b = (int)(pair / p.Hkv), kvh = (int)(pair % p.Hkv);
+  const int32_t n = min(ed_held(p, b) + 1, p.C), slot = p.slots[pair];
+  const float ninf = __int_as_float(0xff800000);
+  const float *ml = p.ml + pair * p.splits * p.G * 2;
+  if (threadIdx.x < (uint32_t)p.G) {
+    const int g = threadIdx.x;
+    float m = ninf, l = 0.f;
+    for (int x = 0; x < p.splits; ++x) m = fmaxf(m, ml[2 * (x * p.G + g)]);
+    for (int x = 0; x < p.splits; ++x) l = __builtin_fmaf(ml[2 * (x * p.G + g) + 1],
+                                                          fast_exp2(ml[2 * (x * p.G + g)] - (m == ninf ? 0.f : m)), l);
+    lse2[g] = (m == ninf ? 0.f : m) + __log2f(l);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x + 256 * chunk; e < p.G * D; e += 256 * p.chunks) {
+    const int g = e / D, d = e % D;
+    float a = 0.f;
+    for (int x = 0; x < p.splits; ++x)
+      a = __builtin_fmaf(p.vals[((pair * p.splits + x) * p.G + g) * D + d], fast_exp2(ml[2 * (x * p.G + g)] - lse2[g]), a);
+    store_from_f32(p.out, b * p.o_sb + (kvh * p.G + g) * p.o_sh + d, p.out_dt, a);
+  }
+  ed_weights<256>(p, pair, slot, chunk * ED_CHUNK, min(n, (chunk + 1) * ED_CHUNK), lse2);
+}
+
+// ------------------------------------------------------------------ host ----
+struct EdPlan {
+  int64_t splits = 1, cs = 0;
+  size_t slots = 0, ml = 0, vals = 0, scores = 0, bytes = 0;
+};
+
+static EdPlan ed_plan(const la_evict_decode_args *a) {
+  EdPlan pl;
+  const int64_t pairs = a->B * a->Hkv, G = a->Hq / a->Hkv;
+  // two workgroups a CU, parts of at least 256 entries
+  pl.splits = std::max<int64_t>(1, std::min<int64_t>({(int64_t)2 * num_cus() / pairs, a->C / 256, 64}));
+  pl.cs = ceil_div(a->C, 32) * 32;
+  size_t at = 0;
+  auto take = [&](size_t n) { const size_t o = at; at += (n + 255) / 256 * 256; return o; };
+  pl.scores = take((size_t)(pairs * G * pl.cs) * sizeof(float));
+  if (pl.splits > 1) {
+    pl.slots = take((size_t)pairs * sizeof(int32_t));
+    pl.ml = take((size_t)(pairs * pl.splits * G * 2) * sizeof(float));
+    pl.vals = take((size_t)(pairs * pl.splits * G * a->D) * sizeof(float));
+  }
+  pl.bytes = at;
+  return pl;
+}
+
+static int ed_check(const la_evict_decode_args *a) {
+  LA_REQUIRE(a != nullptr, "la_evict_decode: null args");
+  LA_REQUIRE(a->B > 0 && a->Hq > 0 && a->Hkv > 0 && a->C > 0, "la_evict_decode: sizes must be positive");
+  LA_REQUIRE(a->Hq % a->Hkv == 0 && a->Hq / a->Hkv <= 16, "la_evict_decode: Hq must be 1 to 16 times Hkv");
+  LA_REQUIRE(a->D == 64 || a->D == 128, "la_evict_decode: head_dim %lld (64 or 128)", (long long)a->D);
+  LA_REQUIRE(a->dtype == LA_F32 || a->dtype == LA_BF16 || a->dtype == LA_F16, "la_evict_decode: dtype");
+  LA_REQUIRE(a->out_dtype == a->dtype || a->out_dtype == LA_F32, "la_evict_decode: out_dtype is dtype or fp32");
+  LA_REQUIRE(a->scale > 0.f && a->scale < 1e30f, "la_evict_decode: scale must be positive");
+  LA_REQUIRE(a->recent >= 0 && a->sink >= 0 && a->recent + a->sink < a->C,
+             "la_evict_decode: sink + recent must leave an entry of the cache to evict");
+  LA_REQUIRE(a->C < ((int64_t)1 << 24) && a->B * a->Hkv < ((int64_t)1 << 24), "la_evict_decode: too many entries");
+  return LA_OK;
+}
+
+template <class T, int D>
+static void ed_launch(const EdKP &p, int64_t pairs, hipStream_t st) {
+  evict_decode_kernel<T, D><<<(uint32_t)(pairs * p.splits), 256, 0, st>>>(p);
+}
+
+}  // namespace la
+
+extern "C" size_t la_evict_decode_workspace(const la_evict_decode_args *a) {
+  if (la::ed_check(a) != LA_OK) return 0;
+  return la::ed_plan(a).bytes;
+}
+
+extern "C" int la_evict_decode(const la_evict_decode_args *a, void *stream) {
+  using namespace la;
+  if (int rc = ed_check(a)) return rc;
+  LA_REQUIRE(a->q && a->k_new && a->v_new && a->k && a->v && a->weights && a->positions && a->lengths && a->pos && a->out,
+             "la_evict_decode: null pointer");
+  const int64_t n16 = a->dtype == LA_F32 ? 4 : 8;
+  auto ok = [&](const void *x, int64_t sb, int64_t sh, int64_t heads) {
+    return (uintptr_t)x % 16 == 0 && (a->B == 1 || sb % n16 == 0) && (heads == 1 || sh % n16 == 0);
+  };
+  LA_REQUIRE(ok(a->q, a->q_sb, a->q_sh, a->Hq) && ok(a->k_new, a->kn_sb, a->kn_sh, a->Hkv) &&
+                 ok(a->v_new, a->vn_sb, a->vn_sh, a->Hkv) && (uintptr_t)a->k % 16 == 0 && (uintptr_t)a->v % 16 == 0,
+             "la_evict_decode: rows must be 16-byte aligned");
+  const EdPlan pl = ed_plan(a);
+  if (!a->workspace || a->ws_bytes < (int64_t)pl.bytes)
+    return fail(LA_ERR_WORKSPACE, "la_evict_decode: workspace %lld < %lld bytes", (long long)a->ws_bytes,
+                (long long)pl.bytes);
+  LA_REQUIRE((uintptr_t)a->workspace % 256 == 0, "la_evict_decode: workspace alignment");
+  const int64_t pairs = a->B * a->Hkv;
+  EdKP p{};
+  p.q = a->q; p.k_new = a->k_new; p.v_new = a->v_new; p.k = a->k; p.v = a->v; p.out = a->out;
+  p.weights = a->weights; p.positions = a->positions; p.lengths = a->lengths; p.pos = a->pos;
+  char *ws = (char *)a->workspace;
+  p.scores = (float *)(ws + pl.scores);
+  p.slots = (int32_t *)(ws + pl.slots);
+  p.ml = (float *)(ws + pl.ml);
+  p.vals = (float *)(ws + pl.vals);
+  p.q_sb = a->q_sb; p.q_sh = a->q_sh; p.kn_sb = a->kn_sb; p.kn_sh = a->kn_sh;
+  p.vn_sb = a->vn_sb; p.vn_sh = a->vn_sh; p.o_sb = a->o_sb; p.o_sh = a->o_sh;
+  p.recent = a->recent; p.sink = a->sink; p.cs = pl.cs;
+  p.B = (int32_t)a->B; p.Hq = (int32_t)a->Hq; p.Hkv = (int32_t)a->Hkv; p.G = (int32_t)(a->Hq / a->Hkv);
+  p.C = (int32_t)a->C; p.splits = (int32_t)pl.splits; p.out_dt = a->out_dtype;
+  p.chunks = (int32_t)ceil_div(a->C, ED_CHUNK);
+  p.qscale = a->scale * 1.44269504088896340736f;
+  hipStream_t st = (hipStream_t)stream;
+  if (pl.splits > 1) {
+    evict_slot_kernel<<<(uint32_t)pairs, 1024, 0, st>>>(p);
+    LA_LAUNCHED();
+  }
+  const bool d128 = a->D == 128;
+  if (a->dtype == LA_F32) d128 ? ed_launch<DaF32, 128>(p, pairs, st) : ed_launch<DaF32, 64>(p, pairs, st);
+  else if (a->dtype == LA_BF16) d128 ? ed_launch<DaBf16, 128>(p, pairs, st) : ed_launch<DaBf16, 64>(p, pairs, st);
+  else d128 ? ed_launch<DaF16, 128>(p, pairs, st) : ed_launch<DaF16, 64>(p, pairs, st);
+  LA_LAUNCHED();
+  if (pl.splits > 1) {
+    const uint32_t grid = (uint32_t)(pairs * p.chunks);
+    if (d128) evict_join_kernel<128><<<grid, 256, 0, st>>>(p);
+    else evict_join_kernel<64><<<grid, 256, 0, st>>>(p);
+    LA_LAUNCHED();
+  }
+  return LA_OK;
+}

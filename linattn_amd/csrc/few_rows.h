@@ -1,0 +1,188 @@
+// Attention of up to 16 rows over many keys by one wave: what decode steps are made of.
+//
+// The keys are read once and bound everything, so a wave works on rounds of its own
+// (32 keys, 16 in fp32: 8 KiB of K and 8 of V at D = 128), with the next round's K on its
+// way into registers and V into the wave's own LDS while one is computed; no barrier.
+// S^T = K Q^T by 16x16x32 products straight from the loaded rows (16x16x4 in fp32);
+// O^T += V^T P^T with V^T by LDS transpose reads.  P enters that product as the sum of
+// two terms of the inputs' type (16 bits of each weight), which the matrix cores have
+// room for here.
+#pragma once
+
+#include "dense_attn.h"
+
+namespace la {
+
+struct DaF32 {
+  typedef f32x4 x8;
+  typedef float elem;
+};
+
+template <class T, int D>
+struct FewRows {
+  typedef typename T::elem elem;
+  typedef typename T::x8 x8;
+  static constexpr bool F32 = sizeof(elem) == 4;
+  static constexpr int RK = F32 ? 16 : 32;               // keys of a round
+  static constexpr int CHE = 16 / (int)sizeof(elem);     // values of a 16-byte chunk
+  static constexpr int CH = D / CHE, RP = 64 / CH;       // chunks of a row, rows of an LDS-DMA
+  static constexpr int NX = RK / RP;                     // LDS-DMAs of a round's V
+  static constexpr int STAGE = RK * D;                   // values of a staged round
+  static constexpr int NK = F32 ? D / 16 : D / 32;       // chunks of K a lane holds for 16 keys
+  static constexpr int LDS_BYTES = 2 * STAGE * (int)sizeof(elem);  // of one wave
+
+  x8 qf[NK];
+  f32x4 acc[D / 16];
+  float m, l, thr, nmu;
+
+  // chunk swizzle of a staged row: eight rows' pairs of chunks (fp32: four rows' four
+  // chunks, four apart) that are read together lie in different banks
+  static __device__ __forceinline__ int swz(int r) {
+    return F32 ? 4 * ((r >> 2) & 3) : D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3);
+  }
+
+  // qrow: row lane % 16 (any valid row where there are fewer)
+  __device__ __forceinline__ void begin(const elem *qrow) {
+    const int c = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int s = 0; s < NK; ++s) qf[s] = *(const x8 *)(qrow + (F32 ? 16 * s + 4 * c : 32 * s + 8 * c));
+    m = thr = __int_as_float(0xff800000);
+    l = nmu = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // Rounds first, first + step, ... below `rounds`, over keys round * RK ..  krow(key) and
+  // vrow(key) point at a key's rows and are asked for keys < end only (keys past it are
+  // the last one again, masked).  `lim` is the last key that row lane % 16 sees.  sink(key,
+  // s) gets the row's scores (log2 units, -inf where masked) of keys key .. key + 3.
+  template <class KRow, class VRow, class Sink>
+  __device__ __forceinline__ void walk(int first, int step, int rounds, int end, int lim, float qscale,
+                                       float thr_gap, elem *smem, KRow krow, VRow vrow, Sink sink) {
+    const int lane = threadIdx.x & 63, c = lane >> 4, ri = lane & 15;
+    const float ninf = __int_as_float(0xff800000);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
+    x8 kn[RK / 16][NK];
+    auto fetch = [&](int r, int slot) {
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        const int rr = RP * x + lane / CH;
+        const elem *src = vrow(min(r * RK + rr, end - 1)) + CHE * ((lane % CH) ^ swz(rr));
+        const uint32_t m0 = lds0 + (uint32_t)(slot * STAGE * (int)sizeof(elem) + x * 1024);
+        asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+      }
+#pragma unroll
+      for (int kt = 0; kt < RK / 16; ++kt) {
+        const elem *src = krow(min(r * RK + 16 * kt + ri, end - 1));
+#pragma unroll
+        for (int s = 0; s < NK; ++s) kn[kt][s] = *(const x8 *)(src + (F32 ? 16 * s + 4 * c : 32 * s + 8 * c));
+      }
+    };
+    if (first < rounds) fetch(first, 0);
+    int slot = 0;
+    for (int r = first; r < rounds; r += step) {
+      f32x4 st[RK / 16];
+      // this round's V is in LDS, and the round before is read out of the other half
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      x8 kc[RK / 16][NK];
+#pragma unroll
+      for (int kt = 0; kt < RK / 16; ++kt)
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+          kc[kt][s] = kn[kt][s];
+          settle(kc[kt][s]);
+        }
+      if (r + step < rounds) fetch(r + step, slot ^ 1);
+#pragma unroll
+      for (int kt = 0; kt < RK / 16; ++kt) {
+        st[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+          if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              st[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[kt][s][e], qf[s][e], st[kt], 0, 0, 0);
+          } else {
+            st[kt] = T::mfma16(kc[kt][s], qf[s], st[kt]);
+          }
+        }
+      }
+      // register e: key 4 c + e
+      const int d = lim - r * RK - 4 * c;
+      float mx = ninf;
+#pragma unroll
+      for (int kt = 0; kt < RK / 16; ++kt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          st[kt][e] = 16 * kt + e <= d ? st[kt][e] * qscale : ninf;
+          mx = fmaxf(mx, st[kt][e]);
+        }
+        sink(r * RK + 16 * kt + 4 * c, st[kt]);
+      }
+      if (__ballot(mx > thr) != 0) {
+        const float mn = fmaxf(m, pair32_max(pair16_max(mx)));
+        const float alpha = m == ninf ? 0.f : fast_exp2(m - mn);
+        m = mn;
+        thr = mn + thr_gap;
+        nmu = mn == ninf ? 0.f : -mn;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) acc[dt] *= alpha;
+      }
+#pragma unroll
+      for (int kt = 0; kt < RK / 16; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          st[kt][e] = fast_exp2(st[kt][e] + nmu);
+          l += st[kt][e];
+        }
+      const elem *sv = smem + slot * STAGE;
+      if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int kr = 4 * c + e;
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt)
+            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(sv[kr * D + 4 * ((4 * dt + (ri >> 2)) ^ swz(kr)) + (ri & 3)],
+                                                           st[0][e], acc[dt], 0, 0, 0);
+        }
+      } else {
+        x8 hi, lo;  // k index 8 c + j: key 4 c + j of the first 16, then of the second
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          hi[j] = (elem)st[j >> 2][j & 3];
+          lo[j] = (elem)(st[j >> 2][j & 3] - (float)hi[j]);
+        }
+        const int kr = 4 * c + (ri >> 2);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+          const int at = kr * D + 8 * ((2 * dt + ((ri & 3) >> 1)) ^ swz(kr)) + 4 * (ri & 1);
+          // (row kr + 16 has the same swizzle)
+          const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)((const uint16_t *)sv + at));
+          const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)((const uint16_t *)sv + at + 16 * D));
+          const x8 vt = __builtin_bit_cast(x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+          acc[dt] = T::mfma16(vt, hi, acc[dt]);
+          acc[dt] = T::mfma16(vt, lo, acc[dt]);
+        }
+      }
+      slot ^= 1;
+    }
+    l = pair32_sum(pair16_sum(l));
+  }
+
+  // The wave's state into LDS: (m, l) of row i at ml[2 i], its D values at vals[i D ..]
+  // (register e of dim tile dt: dim 16 dt + 4 c + e).
+  __device__ __forceinline__ void put(float *ml, float *vals) const {
+    const int lane = threadIdx.x & 63, c = lane >> 4, ri = lane & 15;
+    if (c == 0) {
+      ml[2 * ri] = m;
+      ml[2 * ri + 1] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+      *(f32x4 *)&vals[ri * (D + 4) + 16 * dt + 4 * c] = acc[dt];
+  }
+  static constexpr int VALS = 16 * (D + 4);  // floats of put's values
+};
+
+}  // namespace la

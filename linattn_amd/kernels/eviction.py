@@ -1,21 +1,24 @@
 """Eviction of cached keys by the attention weight they gather, on gfx950.
 
 ``key_weights`` sums, for each key and KV head, the weights that a prompt's (or a chunk's)
-queries give it, from the row sums ``dense_attention`` returned; ``packed_key_weights`` the
-same for packed sequences.
+queries give it, from the row sums ``dense_attention`` returned; ``evict_kv`` keeps the first,
+the newest and the heaviest entries of each cache up to a budget; ``packed_key_weights`` and
+``packed_evict_kv`` do the same for packed sequences.  ``evict_decode_step`` goes on from there
+token by token: evict, append, attend and gather weights in one call.  Each KV head keeps
+entries of its own.
 """
 
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from linattn_amd import _native as N
-from linattn_amd.kernels.dense import _check_qk, _cu, _int32, _rows, _scale
+from linattn_amd.kernels.dense import _TYPES, _check_qk, _cu, _int32, _out, _rows, _scale
 
-__all__ = ["key_weights", "packed_key_weights"]
+__all__ = ["key_weights", "packed_key_weights", "evict_kv", "packed_evict_kv", "evict_decode_step"]
 
 
 def _last(last: Optional[int]) -> int:
@@ -123,4 +126,184 @@ def packed_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor,
         a.l_sh, a.w_sh = lse.stride(0), out.stride(0)
         a.zero_rest = 0 if accumulate else 1
         _run_weights(what, a, q, k, lse, out, accumulate, causal, scale, last)
+    return out
+
+
+Evicted = Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
+
+
+def _budget(what: str, budget: int, recent: int, sink: int, capacity: Optional[int]) -> int:
+    if budget <= 0 or recent < 0 or sink < 0 or recent + sink > budget:
+        raise ValueError(f"{what}: sink + recent must fit a positive budget, got {sink} + {recent} of {budget}")
+    capacity = budget if capacity is None else capacity
+    if capacity < budget:
+        raise ValueError(f"{what}: capacity {capacity} is less than the budget {budget}")
+    return capacity
+
+
+def _run_evict(what: str, a: N.LaEvictArgs, B: int, k, v, weights, budget, recent, sink,
+               capacity) -> Evicted:
+    dev, Hkv, D = k.device, a.Hkv, k.shape[-1]
+    k_out = torch.empty(B, Hkv, capacity, D, dtype=k.dtype, device=dev)
+    v_out = torch.empty_like(k_out)
+    w_out = torch.empty(B, Hkv, capacity, dtype=torch.float32, device=dev)
+    pos_out = torch.empty(B, Hkv, capacity, dtype=torch.int32, device=dev)
+    len_out = torch.empty(B, dtype=torch.int32, device=dev)
+    if B > 0:
+        a.k, a.v, a.weights = k.data_ptr(), v.data_ptr(), weights.data_ptr()
+        a.k_out, a.v_out, a.w_out = k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr()
+        a.pos_out, a.len_out = pos_out.data_ptr(), len_out.data_ptr()
+        a.B, a.D, a.esize = B, D, k.element_size()
+        a.budget, a.capacity, a.recent, a.sink = budget, capacity, recent, sink
+        L = N.load()
+        with torch.cuda.device(dev):
+            nbytes = L.la_evict_kv_workspace(ctypes.byref(a))
+            ws = N.workspace(nbytes, dev)
+            a.workspace, a.ws_bytes = N.ptr(ws), nbytes
+            N.check(L.la_evict_kv(ctypes.byref(a), N.stream_handle(dev)), what)
+    return k_out, v_out, w_out, pos_out, len_out
+
+
+def _check_cache(what: str, k: torch.Tensor, v: torch.Tensor, dims: int) -> None:
+    if k.dim() != dims or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _TYPES:
+        raise ValueError(f"{what}: k and v must have {dims} dimensions, one shape and one of "
+                         "bfloat16, float16, float32")
+    if k.shape[-1] == 0 or k.shape[-1] * k.element_size() % 16:
+        raise ValueError(f"{what}: rows of k and v must be whole 16-byte chunks")
+    if k.shape[1] == 0:
+        raise ValueError(f"{what}: no KV heads")
+
+
+def evict_kv(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor, *, budget: int, recent: int,
+             sink: int = 0, lengths: Optional[torch.Tensor] = None,
+             positions: Optional[torch.Tensor] = None, pos: Optional[torch.Tensor] = None,
+             capacity: Optional[int] = None) -> Evicted:
+    """Keep ``budget`` entries of each cache: the first ``sink`` and the newest ``recent``
+    tokens, then the heaviest by ``weights`` (ties to the lowest index; NaN is lightest).
+
+    k/v (B, Hkv, T, D), ``weights`` (B, Hkv, T) float32 (``key_weights``), ``lengths`` (int32 (B,),
+    default T) the entries held.  An entry's token is its index, or ``positions`` (int32
+    (B, Hkv, T)) of a cache that was evicted before, with ``pos`` (int32 (B,)) the position
+    of the next token.  Returns new tensors (k, v, weights, positions, lengths) with room for
+    ``capacity`` (default ``budget``) entries: the kept ones in their order, then zeros with
+    weight 0 and position -1; a cache shorter than the budget is kept whole.  A capacity of
+    ``budget + 1`` is what ``evict_decode_step`` goes on with."""
+    what = "evict_kv"
+    dev = N.require_gpu(k, v, weights, lengths, positions, pos, what=what)
+    _check_cache(what, k, v, 4)
+    capacity = _budget(what, budget, recent, sink, capacity)
+    B, Hkv, T, _ = k.shape
+    if weights.dtype != torch.float32 or weights.shape != (B, Hkv, T):
+        raise ValueError(f"{what}: weights must be float32 (B, Hkv, T)")
+    if (positions is None) != (pos is None):
+        raise ValueError(f"{what}: pass both positions and pos, or neither")
+    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (B, Hkv, T)):
+        raise ValueError(f"{what}: positions must be int32 (B, Hkv, T)")
+    lengths, pos = _int32(lengths, (B,), "lengths"), _int32(pos, (B,), "pos")
+    k, v = _rows(k), _rows(v)
+    weights = weights if weights.stride(-1) == 1 else weights.contiguous()
+    a = N.LaEvictArgs()
+    if positions is not None:
+        positions = positions if positions.stride(-1) == 1 else positions.contiguous()
+        a.positions, a.pos = positions.data_ptr(), pos.data_ptr()
+        a.ps_sb, a.ps_sh = positions.stride()[:2]
+    a.lengths, a.Hkv, a.T = N.ptr(lengths), Hkv, T
+    a.k_sb, a.k_sh, a.k_st = k.stride()[:3]
+    a.v_sb, a.v_sh, a.v_st = v.stride()[:3]
+    a.w_sb, a.w_sh = weights.stride()[:2]
+    return _run_evict(what, a, B, k, v, weights, budget, recent, sink, capacity)
+
+
+def packed_evict_kv(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor,
+                    cu_seqlens: torch.Tensor, *, budget: int, recent: int, sink: int = 0,
+                    capacity: Optional[int] = None) -> Evicted:
+    """``evict_kv`` of packed sequences: k/v (Nk, Hkv, D), ``weights`` (Hkv, Nk) as
+    ``packed_key_weights`` returns them, sequence b's entries rows cu_seqlens[b] ..
+    cu_seqlens[b + 1] - 1.  Returns caches of their own, as ``evict_kv`` does; positions
+    count within each sequence."""
+    what = "packed_evict_kv"
+    N.require_gpu(k, v, weights, cu_seqlens, what=what)
+    _check_cache(what, k, v, 3)
+    capacity = _budget(what, budget, recent, sink, capacity)
+    Nk, Hkv, _ = k.shape
+    if weights.dtype != torch.float32 or weights.shape != (Hkv, Nk):
+        raise ValueError(f"{what}: weights must be float32 (Hkv, Nk)")
+    cu_seqlens = _cu(cu_seqlens, "cu_seqlens")
+    k, v = _rows(k), _rows(v)
+    weights = weights if weights.stride(-1) == 1 else weights.contiguous()
+    a = N.LaEvictArgs()
+    a.cu, a.Hkv, a.T = cu_seqlens.data_ptr(), Hkv, Nk
+    a.k_st, a.k_sh = k.stride()[:2]
+    a.v_st, a.v_sh = v.stride()[:2]
+    a.w_sh = weights.stride(0)
+    return _run_evict(what, a, cu_seqlens.shape[0] - 1, k, v, weights, budget, recent, sink, capacity)
+
+
+def evict_decode_step(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                      k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor,
+                      positions: torch.Tensor, lengths: torch.Tensor, pos: torch.Tensor, *,
+                      recent: int, sink: int = 0, scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None,
+                      out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """One token over caches that evict, updated in place.
+
+    q (B, Hq, 1, D), k_new/v_new (B, Hkv, 1, D), caches (B, Hkv, C, D) in the same dtype,
+    ``weights`` float32 and ``positions`` int32 (B, Hkv, C), ``lengths`` and ``pos`` int32 (B,):
+    the entries each cache holds and the new token's position.  For each (sequence, KV
+    head): a full cache loses its lightest entry that is neither among the first ``sink``
+    nor the newest ``recent`` tokens (position >= sink and < pos - recent; of equal weights
+    the highest slot; NaN is lightest; the highest slot if nothing else is left); the new
+    token takes its slot (or the next free one); the query heads attend the cache with it;
+    every entry's weight grows by the weights they gave it.  Returns (B, Hq, 1, D) in
+    ``out_dtype`` (default q's, or float32), or in ``out``.
+
+    The caller advances ``lengths`` (to at most C) and ``pos``.  Caches are contiguous, and
+    a call's are not another's: two streams may run two calls on caches of their own."""
+    what = "evict_decode_step"
+    dev = N.require_gpu(q, k_new, v_new, k_cache, v_cache, weights, positions, lengths, pos, out,
+                        what=what)
+    _check_qk(what, q, k_cache, 4, 1)
+    B, Hq, Tq, D = q.shape
+    Hkv, C = k_cache.shape[1], k_cache.shape[2]
+    if Tq != 1 or k_cache.shape[0] != B:
+        raise ValueError(f"{what}: one token of each sequence: q (B, Hq, 1, D)")
+    if Hq // Hkv > 16:
+        raise ValueError(f"{what}: at most 16 query heads per KV head")
+    if v_cache.shape != k_cache.shape or v_cache.dtype != q.dtype or \
+            not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"{what}: caches must be contiguous (B, Hkv, C, D) in q's dtype")
+    if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise ValueError(f"{what}: caches must be 16-byte aligned")
+    for t in (k_new, v_new):
+        if t.shape != (B, Hkv, 1, D) or t.dtype != q.dtype:
+            raise ValueError(f"{what}: k_new and v_new must be (B, Hkv, 1, D) in q's dtype")
+    if weights.dtype != torch.float32 or weights.shape != (B, Hkv, C) or not weights.is_contiguous():
+        raise ValueError(f"{what}: weights must be contiguous float32 (B, Hkv, C)")
+    if positions.dtype != torch.int32 or positions.shape != (B, Hkv, C) or \
+            not positions.is_contiguous():
+        raise ValueError(f"{what}: positions must be contiguous int32 (B, Hkv, C)")
+    lengths, pos = _int32(lengths, (B,), "lengths"), _int32(pos, (B,), "pos")
+    if recent < 0 or sink < 0 or recent + sink >= C:
+        raise ValueError(f"{what}: sink + recent must leave an entry of the cache to evict")
+    out = _out(what, out, q, out_dtype)
+    if B == 0:
+        return out
+    q, k_new, v_new = _rows(q), _rows(k_new), _rows(v_new)
+    a = N.LaEvictDecodeArgs()
+    a.q, a.k_new, a.v_new, a.out = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), out.data_ptr()
+    a.k, a.v, a.weights = k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr()
+    a.positions, a.lengths, a.pos = positions.data_ptr(), lengths.data_ptr(), pos.data_ptr()
+    a.B, a.Hq, a.Hkv, a.C, a.D = B, Hq, Hkv, C, D
+    a.q_sb, a.q_sh = q.stride()[:2]
+    a.kn_sb, a.kn_sh = k_new.stride()[:2]
+    a.vn_sb, a.vn_sh = v_new.stride()[:2]
+    a.o_sb, a.o_sh = out.stride()[:2]
+    a.recent, a.sink, a.scale = recent, sink, _scale(scale, D)
+    a.dtype, a.out_dtype = N.dtype_code(q.dtype), N.dtype_code(out.dtype)
+    L = N.load()
+    with torch.cuda.device(dev):
+        nbytes = L.la_evict_decode_workspace(ctypes.byref(a))
+        ws = N.workspace(nbytes, dev)
+        a.workspace, a.ws_bytes = N.ptr(ws), nbytes
+        N.check(L.la_evict_decode(ctypes.byref(a), N.stream_handle(dev)), what)
     return out

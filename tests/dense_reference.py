@@ -71,3 +71,25 @@ def close(got, want, tol, what=""):
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} off, worst "
                            f"{float(((got - want).abs() / tol)[bad].max()):.3g} times the bound, first at "
                            f"{bad.nonzero()[0].tolist()}")
+
+
+def keep(weights, n, budget, recent, sink, positions=None, pos=None):
+    """Indices a cache of n entries keeps, ascending."""
+    positions = list(range(n)) if positions is None else [int(x) for x in positions[:n]]
+    pos = n if pos is None else int(pos)
+
+    def rank(i):
+        if positions[i] < sink or positions[i] >= pos - recent:
+            return (0, 0.0, i)
+        w = float(weights[i])
+        return (2, 0.0, i) if math.isnan(w) else (1, -w, i)
+
+    return sorted(sorted(range(n), key=rank)[:budget])
+
+
+def victim(weights, recent, sink, positions, pos):
+    """The slot a full cache gives up."""
+    free = [i for i, p in enumerate(positions) if sink <= int(p) < int(pos) - recent]
+    if not free:
+        return len(positions) - 1
+    return max(free, key=lambda i: (1, 0.0, i) if math.isnan(float(weights[i])) else (0, -float(weights[i]), i))
