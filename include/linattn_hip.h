@@ -766,7 +766,7 @@ int la_key_weights(const la_key_weights_args *a, void *stream);
  * Packed (cu non-null, int32 [B + 1]): sequence b's entries are rows cu[b] .. cu[b+1] - 1,
  * T the tensors' rows and the *_sb strides unused.
  * Rows of k and v: esize bytes per value, unit stride over D, 16-byte aligned.
- * Workspace: la_evict_kv_workspace() bytes (the lists of kept entries).
+ * Workspace: la_evict_kv_workspace() bytes, 256-byte aligned (the lists of kept entries).
  */
 typedef struct {
   const void *k;

@@ -48,6 +48,8 @@ def _check(got, k, v, w, lists, capacity, positions=None):
 @pytest.mark.parametrize("T,budget,recent,sink,extra", [
     (1, 1, 0, 0, 0), (5, 8, 4, 2, 1), (64, 64, 0, 0, 0), (300, 64, 32, 4, 1), (300, 1, 0, 0, 0),
     (300, 64, 64, 0, 3), (1100, 1000, 0, 1000, 0), (2500, 777, 100, 3, 1),
+    (2048, 100, 10, 1, 1), (2049, 2000, 7, 0, 0), (16384, 500, 50, 4, 1), (16385, 500, 50, 4, 1),  # each form's ends
+    (40000, 39000, 100, 5, 1),
 ])
 def test_evict_keeps_the_heaviest(dev, dtype, D, T, budget, recent, sink, extra):
     B, Hkv = 2, 3
@@ -60,7 +62,17 @@ def test_evict_keeps_the_heaviest(dev, dtype, D, T, budget, recent, sink, extra)
 
 @pytest.mark.parametrize("kind", ["equal", "few", "odd", "tiny"])
 def test_ties_and_odd_weights(dev, kind):
-    B, Hkv, T, D = 2, 2, 3000, 64
+    _ties(dev, kind, 3000, (40, 1024, 2900, 2999))
+
+
+@pytest.mark.parametrize("kind", ["equal", "few", "odd", "tiny"])
+@pytest.mark.parametrize("T", [700, 20000])
+def test_ties_in_short_and_long_caches(dev, kind, T):
+    _ties(dev, kind, T, (T // 50 + 23, T // 3, T - 1))
+
+
+def _ties(dev, kind, T, budgets):
+    B, Hkv, D = 2, 2, 64
     k, v = _rand(0, B, Hkv, T, D), _rand(1, B, Hkv, T, D)
     w = torch.ones(B, Hkv, T) if kind == "equal" else _rand(2, B, Hkv, T)
     if kind == "few":
@@ -69,7 +81,7 @@ def test_ties_and_odd_weights(dev, kind):
         w[:, :, ::7], w[:, :, 1::11], w[:, :, 2::13] = math.nan, math.inf, -math.inf
     if kind == "tiny":
         w = w * 1e-44  # subnormal
-    for budget in (40, 1024, 2900, 2999):
+    for budget in budgets:
         got = evict_kv(k.to(dev), v.to(dev), w.to(dev), budget=budget, recent=20, sink=3)
         _check(got, k, v, w, [[keep(w[b, h], T, budget, 20, 3) for h in range(Hkv)] for b in range(B)], budget)
 
@@ -81,14 +93,27 @@ def test_evict_lengths_positions_and_layouts(dev):
     lens = [700, 0, 1, 130, 64]
     got = evict_kv(k.to(dev), v.to(dev), w.to(dev), budget=64, recent=16, sink=2, lengths=_i32(lens, dev))
     _check(got, k, v, w, [[keep(w[b, h], lens[b], 64, 16, 2) for h in range(Hkv)] for b in range(B)], 64)
+    _unordered(dev, k, v, w, lens, [2200, 2200, 10, 900, 2100], 100)
+
+
+@pytest.mark.parametrize("T", [5000, 18000])
+def test_long_caches_by_position(dev, T):
+    B, Hkv, D = 3, 2, 64
+    k, v, w = _rand(0, B, Hkv, T, D), _rand(1, B, Hkv, T, D), _rand(2, B, Hkv, T).exp()
+    w[1] = 1.0
+    _unordered(dev, k, v, w, [T, T - 7, 2100], [3 * T, 2 * T, 900], 1500)
+    _unordered(dev, k, v, w, [T, T - 7, 2100], [3 * T, 2 * T, 900], 40, recent=20)
+
+
+def _unordered(dev, k, v, w, lens, pos, budget, recent=30):
     # entries in no order, as a cache that decodes and evicts holds them
+    B, Hkv, T = w.shape
     g = torch.Generator().manual_seed(5)
     positions = torch.rand(B, Hkv, T, generator=g).argsort(-1).to(torch.int32) * 3
-    pos = [2200, 2200, 10, 900, 2100]
-    got = evict_kv(k.to(dev), v.to(dev), w.to(dev), budget=100, recent=30, sink=9, lengths=_i32(lens, dev),
-                   positions=positions.to(dev), pos=_i32(pos, dev), capacity=101)
-    lists = [[keep(w[b, h], lens[b], 100, 30, 9, positions[b, h], pos[b]) for h in range(Hkv)] for b in range(B)]
-    _check(got, k, v, w, lists, 101, positions)
+    got = evict_kv(k.to(dev), v.to(dev), w.to(dev), budget=budget, recent=recent, sink=9, lengths=_i32(lens, dev),
+                   positions=positions.to(dev), pos=_i32(pos, dev), capacity=budget + 1)
+    lists = [[keep(w[b, h], lens[b], budget, recent, 9, positions[b, h], pos[b]) for h in range(Hkv)] for b in range(B)]
+    _check(got, k, v, w, lists, budget + 1, positions)
 
 
 @pytest.mark.parametrize("lens", [[1], [300, 0, 1, 64, 65, 2000], [70000, 3]])
