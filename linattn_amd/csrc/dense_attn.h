@@ -69,15 +69,28 @@ __device__ __forceinline__ int32_t da_cu(const int32_t *cu, int i, int64_t rows)
   return (int32_t)min(max((int64_t)cu[i], (int64_t)0), rows);
 }
 
+// Sum and maximum over the wave, on the vector unit (as group_sum does it: a shuffle goes
+// through LDS, and the search below makes many).
+template <int CTRL>
+__device__ __forceinline__ int32_t da_dpp(int32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, false);
+}
+template <class F>
+__device__ __forceinline__ int32_t da_wave_fold(int32_t x, F f) {
+  x = f(x, da_dpp<0xB1>(x));
+  x = f(x, da_dpp<0x4E>(x));
+  x = f(x, da_dpp<0x141>(x));
+  x = f(x, da_dpp<0x140>(x));
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+  x = f((int32_t)a[0], (int32_t)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+  return __builtin_amdgcn_readfirstlane(f((int32_t)b[0], (int32_t)b[1]));
+}
 __device__ __forceinline__ int32_t da_wave_sum(int32_t x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-  return x;
+  return da_wave_fold(x, [](int32_t a, int32_t b) { return a + b; });
 }
 __device__ __forceinline__ int32_t da_wave_max(int32_t x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
-  return x;
+  return da_wave_fold(x, [](int32_t a, int32_t b) { return max(a, b); });
 }
 
 __device__ __forceinline__ void da_seq(const DaSeqs &s, DaTile &t) {
@@ -172,17 +185,12 @@ inline int64_t da_tiles(bool packed, int64_t B, int64_t Tq, int64_t G, int64_t R
   return packed ? Tq * G / R + B + 1 : B * ceil_div(Tq * G, R);
 }
 
-// Workgroup -> (KV head, tile).  Consecutive workgroups go to the 8 XCDs in turn: with a
-// multiple of 8 streams each XCD keeps the streams' keys in its own L2.
-__device__ __forceinline__ void da_stream(uint32_t wg, uint32_t ns, uint32_t nt, uint32_t &stream,
-                                          uint32_t &tix) {
-  if (ns % 8 == 0) {
-    stream = (wg & 7) + 8 * ((wg >> 3) / nt);
-    tix = (wg >> 3) % nt;
-  } else {
-    stream = wg % ns;
-    tix = wg / ns;
-  }
+// Workgroup -> (stream of tiles that share keys, tile): all streams' first tiles first, so
+// that the longest start first.  Consecutive workgroups go to the 8 XCDs in turn: with a
+// multiple of 8 streams each XCD has streams of its own, whose keys its L2 holds.
+__device__ __forceinline__ void da_stream(uint32_t wg, uint32_t ns, uint32_t &stream, uint32_t &tix) {
+  stream = wg % ns;
+  tix = wg / ns;
 }
 
 }  // namespace la

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hf = lane >> 5, r32 = lane & 31;
   uint32_t stream, tix;
-  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, p.ntile, stream, tix);
+  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
   const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R);
   const int G = p.s.G;
@@ -363,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane >> 4, ri = lane & 15;
   uint32_t stream, tix;
-  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, p.ntile, stream, tix);
+  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
   const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R);
   const int G = p.s.G;

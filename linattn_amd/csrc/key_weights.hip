@@ -8,6 +8,7 @@
 // normalised or joined on the way, so the rows of a tile can be split over workgroups;
 // their sums are added in order by a second kernel: no atomics.
 #include <algorithm>
+#include <type_traits>
 
 #include "dense_attn.h"
 
@@ -45,9 +46,11 @@ __device__ __forceinline__ KwTile kw_tile(const KwKP &p, int tix, int split) {
   const int G = p.s.G, diag = x.t.lk - x.t.lq;
   int32_t t0 = p.last > 0 ? (int32_t)max((int64_t)x.t.lq - p.last, (int64_t)0) : 0;
   if (p.causal) t0 = max(t0, x.s0 - diag);
-  const int64_t rows = (int64_t)max(x.t.lq - t0, 0) * G;
-  x.row0 = t0 * G + (int32_t)(rows * split / p.splits);
-  x.row1 = t0 * G + (int32_t)(rows * (split + 1) / p.splits);
+  const int32_t rows = max(x.t.lq - t0, 0) * G;
+  // parts of whole staged tiles
+  const int32_t per = (int32_t)(((uint32_t)rows + 64u * p.splits - 1u) / (64u * p.splits)) * 64;
+  x.row0 = t0 * G + min(per * split, rows);
+  x.row1 = t0 * G + min(per * (split + 1), rows);
   return x;
 }
 
@@ -80,6 +83,7 @@ __device__ __forceinline__ void kw_rest(const KwKP &p, const KwTile &x, int kvh,
 // Row r as (query, head of the group), moved on without dividing again.
 struct KwRow {
   int32_t t, g;
+  KwRow() = default;
   __device__ __forceinline__ KwRow(int32_t r, int G) : t(r / G), g(r % G) {}
   __device__ __forceinline__ void step(int32_t dt, int32_t dg, int G) {
     t += dt;
@@ -91,18 +95,22 @@ struct KwRow {
   }
 };
 
-// bf16 / fp16: four waves of 64 keys, rows staged 64 at a time by LDS-DMA, double buffered.
+// bf16 / fp16: four waves of 64 keys.  Rows are staged 64 at a time by LDS-DMA, with their
+// lse (each wave its own copy, so that every wave counts the same loads), NSLOT - 1 tiles
+// ahead; a tile's 128 products a workgroup and the 3 vector instructions of each of its
+// weights take about equally long.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
   constexpr int NW = 4, KT = 64 * NW, BLK = DA_BS * D, CH = D / 8, RP = 64 / CH, NX = DA_BS / RP / NW;
-  constexpr int NS = D / 16;
+  constexpr int NS = D / 16, NSLOT = 4;
   typedef typename T::x8 x8;
   typedef typename T::elem elem;
-  __shared__ __align__(16) uint16_t smem[2 * BLK];
+  __shared__ __align__(16) uint16_t smem[NSLOT * BLK];
+  __shared__ float s_lse[NSLOT][NW][DA_BS];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hf = lane >> 5, r32 = lane & 31, G = p.s.G;
   uint32_t stream, tix;
-  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, p.ntile, stream, tix);
+  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
   const KwTile x = kw_tile<KT>(p, (int)tix, split);
   kw_rest(p, x, kvh, split, (int)tix);
@@ -118,6 +126,53 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
 
   const int nrow = x.row1 - x.row0;
   if (nrow > 0) {
+    const elem *qbh = (const elem *)p.q + (p.s.cu_q ? x.t.q0 * p.q_st : x.t.b * p.q_sb) + kvh * G * p.q_sh;
+    const float *lbh = p.lse + (p.s.cu_q ? x.t.q0 : x.t.b * p.l_sb) + kvh * G * p.l_sh;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
+    const uint32_t ldl0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)s_lse);
+    // the rows this lane copies: of q, RP (NW i + w) + lane / CH, and one row's lse; moved
+    // on by 64 rows a tile (dt queries and dg heads, wrapping at the group), past the end
+    // the last one
+    const int dt = DA_BS / G, dg = DA_BS % G;
+    const KwRow end(x.row1 - 1, G);
+    const int64_t q_step = dt * p.q_st + dg * p.q_sh, q_wrap = p.q_st - G * p.q_sh;
+    const int64_t l_step = dt + dg * p.l_sh, l_wrap = 1 - G * p.l_sh;
+    const elem *q_end = qbh + end.t * p.q_st + end.g * p.q_sh;
+    const elem *q_ptr[NX];
+    int q_g[NX];
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const KwRow r(x.row0 + RP * (NW * i + w) + lane / CH, G);
+      q_ptr[i] = qbh + r.t * p.q_st + r.g * p.q_sh;
+      q_g[i] = r.g;
+    }
+    const KwRow r0(x.row0 + lane, G);
+    const float *l_ptr = lbh + r0.t + r0.g * p.l_sh, *l_end = lbh + end.t + end.g * p.l_sh;
+    int l_g = r0.g, left = x.row1 - x.row0;  // rows from this tile on
+    auto dma = [&](int slot) {  // the next tile
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int u = NW * i + w, rr = RP * u + lane / CH;
+        const elem *src = (rr < left ? q_ptr[i] : q_end) + 8 * ((lane % CH) ^ da_swz_k<D>(rr));
+        asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds0 + 2 * (slot * BLK + u * 512)) : "memory");
+        q_g[i] += dg;
+        q_ptr[i] += q_step;
+        if (q_g[i] >= G) {
+          q_g[i] -= G;
+          q_ptr[i] += q_wrap;
+        }
+      }
+      asm volatile("global_load_lds_dword %0, off" ::"v"(lane < left ? l_ptr : l_end),
+                   "{m0}"(ldl0 + 4 * ((slot * NW + w) * DA_BS)) : "memory");
+      l_g += dg;
+      l_ptr += l_step;
+      if (l_g >= G) {
+        l_g -= G;
+        l_ptr += l_wrap;
+      }
+      left -= DA_BS;
+    };
+    const int n = (nrow + DA_BS - 1) / DA_BS;
     x8 kf[2][NS];  // A operand: key 32 kt + r32, dims 16 s + 8 hf ..
     const elem *kbh = (const elem *)p.k + (p.s.cu_q ? x.t.k0 * p.k_st : x.t.b * p.k_sb) + kvh * p.k_sh;
 #pragma unroll
@@ -126,89 +181,91 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) kf[kt][s] = *(const x8 *)(kbh + key * p.k_st + 16 * s + 8 * hf);
     }
-    const elem *qbh = (const elem *)p.q + (p.s.cu_q ? x.t.q0 * p.q_st : x.t.b * p.q_sb) + kvh * G * p.q_sh;
-    const float *lbh = p.lse + (p.s.cu_q ? x.t.q0 : x.t.b * p.l_sb) + kvh * G * p.l_sh;
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
-    const int dt = DA_BS / G, dg = DA_BS % G;
-    const KwRow end(x.row1 - 1, G);
-    auto dma = [&](int j, int slot) {
-#pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const int u = NW * i + w, rr = RP * u + lane / CH;
-        const KwRow r(min(x.row0 + j * DA_BS + rr, x.row1 - 1), G);
-        asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(qbh + r.t * p.q_st + r.g * p.q_sh +
-                                                             8 * ((lane % CH) ^ da_swz_k<D>(rr))),
-                     "{m0}"(lds0 + 2 * (slot * BLK + u * 512)) : "memory");
-      }
-    };
-    KwRow mine[2] = {KwRow(x.row0 + r32, G), KwRow(x.row0 + 32 + r32, G)};  // of each half of a tile
-    float ls[2];
-    int seen[2];
-    auto rows = [&](int j) {  // lse and last key seen of each half's row
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const KwRow &r = x.row0 + j * DA_BS + 32 * h + r32 < x.row1 ? mine[h] : end;
-        ls[h] = lbh[r.t + r.g * p.l_sh];
-        seen[h] = p.causal ? diag + r.t : x.t.lk - 1;
-        mine[h].step(dt, dg, G);
-      }
-    };
-    const int n = (nrow + DA_BS - 1) / DA_BS;
-    rows(0);
-    dma(0, 0);
-    for (int j = 0; j < n; ++j) {
-      wait_vmcnt<0>();
-      float nl[2];  // -lse in log2 units; -inf: the row adds nothing
-      int last[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        settle(ls[h]);
-        const bool none = x.row0 + j * DA_BS + 32 * h + r32 >= x.row1 || ls[h] == __int_as_float(0xff800000);
-        nl[h] = none ? __int_as_float(0xff800000) : -ls[h] * 1.44269504088896340736f;
-        last[h] = seen[h];
-      }
-      lds_barrier();
-      if (j + 1 < n) {
-        rows(j + 1);
-        dma(j + 1, (j + 1) & 1);
-      }
-      const uint16_t *sq = smem + (j & 1) * BLK;
+    for (int j = 0; j < NSLOT - 1; ++j) {
+      if (j < n) dma(j);
+    }
+    // rows from these on see any, and all, of the wave's keys
+    const int row_any = p.causal ? max(s_w - diag, 0) * G : 0;
+    const int row_all = p.causal ? max(s_w + 63 - diag, 0) * G : s_w + 63 < x.t.lk ? 0 : INT32_MAX;
+    auto step = [&](auto mask, int j) __attribute__((always_inline)) {
+      const uint16_t *sq = smem + (j % NSLOT) * BLK;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int rl = 32 * h + r32, sw = da_swz_k<D>(rl);
-        x8 qf[NS];
+        f32x16 st[2];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) qf[s] = *(const x8 *)&sq[rl * D + 8 * ((2 * s + hf) ^ sw)];
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          f32x16 st;
+          for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) st[i] = 0.f;
+        for (int s = 0; s < NS; ++s) {
+          const x8 qf = *(const x8 *)&sq[rl * D + 8 * ((2 * s + hf) ^ sw)];
+          st[0] = T::mfma(kf[0][s], qf, st[0]);
+          st[1] = T::mfma(kf[1][s], qf, st[1]);
+        }
+        const float ls = s_lse[j % NSLOT][w][rl];
+        // -lse in log2 units; -inf: the row adds nothing
+        float nl = ls == __int_as_float(0xff800000) ? ls : -ls * 1.44269504088896340736f;
+        if constexpr (!decltype(mask)::value) {
 #pragma unroll
-          for (int s = 0; s < NS; ++s) st = T::mfma(kf[kt][s], qf[s], st);
-          // register i: key 8 (i / 4) + 4 hf + i % 4
-          const int d = last[h] - (s_w + 32 * kt + 4 * hf);
-          if (__ballot(d < 31 - 4 * hf) == 0) {  // all keys seen by all rows
+          for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[kt][i] += fast_exp2(__builtin_fmaf(st[i], p.qscale, nl[h]));
-          } else {
+            for (int i = 0; i < 16; ++i) acc[kt][i] += fast_exp2(__builtin_fmaf(st[kt][i], p.qscale, nl));
+        } else {
+          const int row = x.row0 + j * DA_BS + rl;
+          if (row >= x.row1) nl = __int_as_float(0xff800000);
+          const int seen = p.causal ? diag + min(row, x.row1 - 1) / G : x.t.lk - 1;
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            // register i: key 8 (i / 4) + 4 hf + i % 4
+            const int d = seen - (s_w + 32 * kt + 4 * hf);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float e = fast_exp2(__builtin_fmaf(st[i], p.qscale, nl[h]));
+              const float e = fast_exp2(__builtin_fmaf(st[kt][i], p.qscale, nl));
               acc[kt][i] += 8 * (i >> 2) + (i & 3) <= d ? e : 0.f;
             }
           }
         }
       }
+    };
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) settle(kf[kt][s]);  // (here, not in the loop, where it would wait for all tiles)
+    constexpr int PER = NX + 1;  // loads of a tile
+    for (int j = 0; j < n; ++j) {
+      // tile j has landed: the loads after it are those of the tiles ahead
+      if (j + 2 < n) wait_vmcnt<2 * PER>();
+      else if (j + 1 < n) wait_vmcnt<PER>();
+      else wait_vmcnt<0>();
+      lds_barrier();  // for every wave, and tile j - 1 is read
+      if (j + NSLOT - 1 < n) dma((j + NSLOT - 1) % NSLOT);
+      if (x.row0 + (j + 1) * DA_BS <= row_any) continue;
+      const bool whole = row_all <= x.row0 + j * DA_BS && (j + 1) * DA_BS <= nrow;
+      if (whole) step(std::false_type{}, j);
+      else step(std::true_type{}, j);
     }
   }
+  // sums over the 32 lanes of a half: each step adds two registers' halves of the lanes
+  // into one register, until lane l has register l / 2
 #pragma unroll
-  for (int kt = 0; kt < 2; ++kt)
+  for (int kt = 0; kt < 2; ++kt) {
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float v = group_sum<32>(acc[kt][i]);
-      if (r32 == i) kw_put(p, x, kvh, split, s_w + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3), [&] { return v; });
+    for (int i = 0; i < 8; ++i) {
+      const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[kt][i]), __float_as_uint(acc[kt][i + 8]), false, false);
+      v[i] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
     }
+    auto fold = [&](float lo, float hi, bool up, auto other) { return (up ? hi : lo) + other(up ? lo : hi); };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = fold(v[i], v[i + 4], lane & 8, [](float y) { return dpp_f32<0x128>(y); });
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v[i] = fold(v[i], v[i + 2], lane & 4, [](float y) { return dpp_f32<0x141>(y); });
+    v[0] = fold(v[0], v[1], lane & 2, [](float y) { return dpp_f32<0x1B>(y); });
+    v[0] += dpp_f32<0xB1>(v[0]);
+    const int i = r32 >> 1;
+    if ((lane & 1) == 0) kw_put(p, x, kvh, split, s_w + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3), [&] { return v[0]; });
+  }
 }
 
 // fp32: four waves of 32 keys on 16x16x4 products; lane (c, i) holds chunk 4 s + c of key
@@ -221,7 +278,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane >> 4, ri = lane & 15, G = p.s.G;
   uint32_t stream, tix;
-  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, p.ntile, stream, tix);
+  da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
   const KwTile x = kw_tile<KT>(p, (int)tix, split);
   kw_rest(p, x, kvh, split, (int)tix);
