@@ -109,12 +109,13 @@ __device__ __forceinline__ void da_seq(const DaSeqs &s, DaTile &t) {
   }
 }
 
-// Tile number i of R rows: the sequences' last tiles (the longest causal rows) first, so
-// that a launch does not end with its longest workgroups.  Packed sequences: of the tiles
-// ordered by their number within the sequence, descending, the i-th; every wave finds it
-// by counting, 64 sequences at a time.  Batched: every sequence has a tile of each number
-// (one past its length has no live rows).
-__device__ __forceinline__ DaTile da_tile(const DaSeqs &s, int32_t i, int32_t ntile, int R) {
+// Tile number i of R rows, of queries (times the group's heads) or, by_k, of keys: the
+// sequences' last tiles (the longest causal rows) first, so that a launch does not end
+// with its longest workgroups.  Packed sequences: of the tiles ordered by their number
+// within the sequence, descending, the i-th; every wave finds it by counting, the first 64
+// sequences from registers.  Batched: every sequence has a tile of each number (one past
+// its length has no live rows).
+__device__ __forceinline__ DaTile da_tile(const DaSeqs &s, int32_t i, int32_t ntile, int R, bool by_k) {
   DaTile t;
   t.b = -1;
   t.r0 = t.lq = t.lk = 0;
@@ -127,22 +128,16 @@ __device__ __forceinline__ DaTile da_tile(const DaSeqs &s, int32_t i, int32_t nt
     return t;
   }
   const int lane = threadIdx.x & 63;
-  auto tiles_of = [&](int b) -> int32_t {  // (b < B)
-    const int32_t n = max(da_cu(s.cu_q, b + 1, s.Tq) - da_cu(s.cu_q, b, s.Tq), 0);
-    return (int32_t)(((int64_t)n * s.G + R - 1) / R);
-  };
-  if (s.B == 1) {
-    const int32_t n = tiles_of(0);
-    if (i >= n) {
-      t.r0 = n;
-      return t;
-    }
-    t.b = 0;
-    t.r0 = (n - 1 - i) * R;
-    da_seq(s, t);
-    return t;
-  }
-  const int32_t mine = lane < s.B ? tiles_of(lane) : 0;  // (of the first 64)
+  const int32_t *cu_k = s.cu_k ? s.cu_k : s.cu_q, *cu = by_k ? cu_k : s.cu_q;
+  const int64_t rows = by_k ? s.Tk : s.Tq;
+  const int32_t mul = by_k ? 1 : s.G;
+  auto tiles = [&](int32_t n) -> int32_t { return (int32_t)(((int64_t)max(n, 0) * mul + R - 1) / R); };
+  auto tiles_of = [&](int b) -> int32_t { return tiles(da_cu(cu, b + 1, rows) - da_cu(cu, b, rows)); };  // (b < B)
+  // this lane's sequence, of the first 64: where its queries and keys begin and end
+  const int bl = min(lane, s.B - 1);
+  const int32_t qa = da_cu(s.cu_q, bl, s.Tq), qe = da_cu(s.cu_q, bl + 1, s.Tq);
+  const int32_t ka = da_cu(cu_k, bl, s.Tk), ke = da_cu(cu_k, bl + 1, s.Tk);
+  const int32_t mine = lane < s.B ? tiles(by_k ? ke - ka : qe - qa) : 0;
   auto above = [&](int32_t level) -> int32_t {  // tiles numbered `level` or more
     int32_t c = max(mine - level, 0);
     for (int b = 64 + lane; b < s.B; b += 64) c += max(tiles_of(b) - level, 0);
@@ -153,30 +148,44 @@ __device__ __forceinline__ DaTile da_tile(const DaSeqs &s, int32_t i, int32_t nt
     t.r0 = all;
     return t;
   }
-  int32_t most = mine;
-  for (int b = 64 + lane; b < s.B; b += 64) most = max(most, tiles_of(b));
-  int32_t lo = 0, hi = da_wave_max(most);  // above(lo) > i >= above(hi)
-  while (hi - lo > 1) {
-    const int32_t mid = (lo + hi) >> 1;
-    if (above(mid) > i) lo = mid;
-    else hi = mid;
-  }
-  int32_t rank = i - above(hi);
-  for (int b0 = 0; b0 < s.B; b0 += 64) {
-    const int b = b0 + lane;
-    const uint64_t has = __ballot((b0 == 0 ? mine : b < s.B ? tiles_of(b) : 0) > lo);
-    const int32_t c = __popcll(has);
-    if (rank < c) {
-      const int before = __popcll(has & ((1ull << lane) - 1ull));
-      const uint64_t at = __ballot(((has >> lane) & 1) && before == rank);
-      t.b = b0 + __ffsll((unsigned long long)at) - 1;
-      break;
+  int32_t lo;
+  if (s.B == 1) {
+    t.b = 0;
+    lo = all - 1 - i;
+  } else {
+    int32_t most = mine;
+    for (int b = 64 + lane; b < s.B; b += 64) most = max(most, tiles_of(b));
+    lo = 0;
+    int32_t hi = da_wave_max(most);  // above(lo) > i >= above(hi)
+    while (hi - lo > 1) {
+      const int32_t mid = (lo + hi) >> 1;
+      if (above(mid) > i) lo = mid;
+      else hi = mid;
     }
-    rank -= c;
+    int32_t rank = i - above(hi);
+    for (int b0 = 0; b0 < s.B; b0 += 64) {
+      const int b = b0 + lane;
+      const uint64_t has = __ballot((b0 == 0 ? mine : b < s.B ? tiles_of(b) : 0) > lo);
+      const int32_t c = __popcll(has);
+      if (rank < c) {
+        const int before = __popcll(has & ((1ull << lane) - 1ull));
+        const uint64_t at = __ballot(((has >> lane) & 1) && before == rank);
+        t.b = b0 + __ffsll((unsigned long long)at) - 1;
+        break;
+      }
+      rank -= c;
+    }
+    t.b = __builtin_amdgcn_readfirstlane(t.b);
   }
-  t.b = __builtin_amdgcn_readfirstlane(t.b);
   t.r0 = lo * R;
-  da_seq(s, t);
+  if (t.b >= 64) {
+    da_seq(s, t);
+    return t;
+  }
+  t.q0 = __builtin_amdgcn_readlane(qa, t.b);
+  t.lq = max(__builtin_amdgcn_readlane(qe, t.b) - (int32_t)t.q0, 0);
+  t.k0 = __builtin_amdgcn_readlane(ka, t.b);
+  t.lk = max(__builtin_amdgcn_readlane(ke, t.b) - (int32_t)t.k0, 0);
   return t;
 }
 

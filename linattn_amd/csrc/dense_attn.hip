@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
   uint32_t stream, tix;
   da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
-  const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R);
+  const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R, false);
   const int G = p.s.G;
   if (tl.b < 0 || tl.r0 + R > tl.lq * G) da_rest<D>(p, tl, R, kvh, split, (int)tix, w, NW);
   if (tl.b < 0 || tl.r0 >= tl.lq * G) return;
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   uint32_t stream, tix;
   da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
-  const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R);
+  const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R, false);
   const int G = p.s.G;
   if (tl.b < 0 || tl.r0 + R > tl.lq * G) da_rest<D>(p, tl, R, kvh, split, (int)tix, w, NW);
   if (tl.b < 0 || tl.r0 >= tl.lq * G) return;

@@ -8,15 +8,13 @@
 // normalised or joined on the way, so the rows of a tile can be split over workgroups;
 // their sums are added in order by a second kernel: no atomics.
 #include <algorithm>
-#include <type_traits>
 
 #include "dense_attn.h"
 
 namespace la {
 
 struct KwKP {
-  DaSeqs s;      // as given
-  DaSeqs tiles;  // keys as rows of one head: what da_tile cuts into tiles
+  DaSeqs s;
   const void *q, *k;
   const float *lse;
   float *out, *ws;  // ws: [split][what out has, densely]
@@ -35,13 +33,12 @@ struct KwTile {
 template <int KT>
 __device__ __forceinline__ KwTile kw_tile(const KwKP &p, int tix, int split) {
   KwTile x;
-  x.t = da_tile(p.tiles, tix, p.ntile, KT);
+  x.t = da_tile(p.s, tix, p.ntile, KT, true);
   x.s0 = x.row0 = x.row1 = 0;
   if (x.t.b < 0) return x;
   // da_tile's first tiles are the sequences' last; the first keys are seen by most rows
-  const int32_t n = p.s.cu_q ? x.t.lq : (int32_t)p.s.Tk;  // (rows of p.tiles: keys)
+  const int32_t n = p.s.cu_q ? x.t.lk : (int32_t)p.s.Tk;
   x.s0 = ((n + KT - 1) / KT) * KT - KT - x.t.r0;
-  da_seq(p.s, x.t);
   if (x.s0 >= x.t.lk) return x;
   const int G = p.s.G, diag = x.t.lk - x.t.lq;
   int32_t t0 = p.last > 0 ? (int32_t)max((int64_t)x.t.lq - p.last, (int64_t)0) : 0;
@@ -187,43 +184,63 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
     // rows from these on see any, and all, of the wave's keys
     const int row_any = p.causal ? max(s_w - diag, 0) * G : 0;
     const int row_all = p.causal ? max(s_w + 63 - diag, 0) * G : s_w + 63 < x.t.lk ? 0 : INT32_MAX;
-    auto step = [&](auto mask, int j) __attribute__((always_inline)) {
+    // products of a half of the staged rows; -lse of its rows in log2 units (-inf: adds nothing)
+    auto products = [&](int j, int h, f32x16 (&st)[2]) __attribute__((always_inline)) -> float {
       const uint16_t *sq = smem + (j % NSLOT) * BLK;
+      const int rl = 32 * h + r32, sw = da_swz_k<D>(rl);
+      const float ls = s_lse[j % NSLOT][w][rl];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const x8 qf = *(const x8 *)&sq[rl * D + 8 * ((2 * s + hf) ^ sw)];
+        st[0] = T::mfma(kf[0][s], qf, st[0]);
+        st[1] = T::mfma(kf[1][s], qf, st[1]);
+      }
+      return ls == __int_as_float(0xff800000) ? ls : -ls * 1.44269504088896340736f;
+    };
+    auto weigh = [&](const f32x16 (&st)[2], float nl) __attribute__((always_inline)) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[kt][i] += fast_exp2(__builtin_fmaf(st[kt][i], p.qscale, nl));
+    };
+    // a half's products while the half before is weighed: the matrix and the vector unit
+    // take about as long, and a wave's own instructions must fill both
+    auto interleave = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 64 / (2 * NS), 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 32 / (2 * NS), 0);
+        if (i % 2) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+    };
+    const float none = __int_as_float(0xff800000);
+    f32x16 sa[2], sb[2];
+    float nb = none;  // sb holds nothing yet
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sb[kt][i] = 0.f;
+    auto masked = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int rl = 32 * h + r32, sw = da_swz_k<D>(rl);
-        f32x16 st[2];
+        float nl = products(j, h, sa);
+        const int row = x.row0 + j * DA_BS + 32 * h + r32;
+        if (row >= x.row1) nl = none;
+        const int seen = p.causal ? diag + min(row, x.row1 - 1) / G : x.t.lk - 1;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt) {
+          // register i: key 8 (i / 4) + 4 hf + i % 4
+          const int d = seen - (s_w + 32 * kt + 4 * hf);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          const x8 qf = *(const x8 *)&sq[rl * D + 8 * ((2 * s + hf) ^ sw)];
-          st[0] = T::mfma(kf[0][s], qf, st[0]);
-          st[1] = T::mfma(kf[1][s], qf, st[1]);
-        }
-        const float ls = s_lse[j % NSLOT][w][rl];
-        // -lse in log2 units; -inf: the row adds nothing
-        float nl = ls == __int_as_float(0xff800000) ? ls : -ls * 1.44269504088896340736f;
-        if constexpr (!decltype(mask)::value) {
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[kt][i] += fast_exp2(__builtin_fmaf(st[kt][i], p.qscale, nl));
-        } else {
-          const int row = x.row0 + j * DA_BS + rl;
-          if (row >= x.row1) nl = __int_as_float(0xff800000);
-          const int seen = p.causal ? diag + min(row, x.row1 - 1) / G : x.t.lk - 1;
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt) {
-            // register i: key 8 (i / 4) + 4 hf + i % 4
-            const int d = seen - (s_w + 32 * kt + 4 * hf);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float e = fast_exp2(__builtin_fmaf(st[kt][i], p.qscale, nl));
-              acc[kt][i] += 8 * (i >> 2) + (i & 3) <= d ? e : 0.f;
-            }
+          for (int i = 0; i < 16; ++i) {
+            const float e = fast_exp2(__builtin_fmaf(sa[kt][i], p.qscale, nl));
+            acc[kt][i] += 8 * (i >> 2) + (i & 3) <= d ? e : 0.f;
           }
         }
       }
@@ -242,9 +259,18 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
       if (j + NSLOT - 1 < n) dma((j + NSLOT - 1) % NSLOT);
       if (x.row0 + (j + 1) * DA_BS <= row_any) continue;
       const bool whole = row_all <= x.row0 + j * DA_BS && (j + 1) * DA_BS <= nrow;
-      if (whole) step(std::false_type{}, j);
-      else step(std::true_type{}, j);
+      if (whole) {
+        const float na = products(j, 0, sa);
+        weigh(sb, nb);
+        interleave();
+        nb = products(j, 1, sb);
+        weigh(sa, na);
+        interleave();
+      } else {
+        masked(j);
+      }
     }
+    weigh(sb, nb);
   }
   // sums over the 32 lanes of a half: each step adds two registers' halves of the lanes
   // into one register, until lane l has register l / 2
@@ -388,12 +414,13 @@ static KwPlan kw_plan(const la_key_weights_args *a) {
   const bool packed = a->cu_q != nullptr;
   pl.keys = a->dtype == LA_F32 ? 128 : 256;
   pl.ntile = da_tiles(packed, a->B, a->Tk, 1, pl.keys);
-  // Rows are split until there are eight workgroups a CU (causal tiles differ in length
-  // by far), down to four staged tiles each.
+  // Rows are split until there are four workgroups a CU (causal tiles differ in length by
+  // far; 14567 packed tokens take 262 us unsplit, 167 with four, 180 with eight), down to
+  // four staged tiles each.
   const int64_t wgs = pl.ntile * a->Hkv, G = a->Hq / a->Hkv;
   int64_t rows = (packed ? ceil_div(a->Tq, a->B) : a->Tq) * G;
   if (a->last > 0) rows = std::min(rows, a->last * G);
-  pl.splits = std::max<int64_t>(1, std::min<int64_t>({ceil_div((int64_t)8 * num_cus(), wgs), rows / 256, 64}));
+  pl.splits = std::max<int64_t>(1, std::min<int64_t>({ceil_div((int64_t)4 * num_cus(), wgs), rows / 256, 64}));
   if (pl.splits > 1) pl.bytes = (size_t)((packed ? 1 : a->B) * a->Hkv * a->Tk * pl.splits) * sizeof(float);
   return pl;
 }
@@ -443,7 +470,6 @@ extern "C" int la_key_weights(const la_key_weights_args *a, void *stream) {
   LA_REQUIRE(wgs < ((int64_t)1 << 31) / 64 && bh < 65536, "la_key_weights: too many keys or heads");
   KwKP p{};
   p.s = DaSeqs{a->cu_q, a->cu_k, a->q_len, a->k_len, a->Tq, a->Tk, (int32_t)a->B, (int32_t)(a->Hq / a->Hkv)};
-  p.tiles = DaSeqs{packed ? (a->cu_k ? a->cu_k : a->cu_q) : nullptr, nullptr, nullptr, nullptr, a->Tk, a->Tk, (int32_t)a->B, 1};
   p.q = a->q; p.k = a->k; p.lse = a->lse; p.out = a->out; p.ws = (float *)a->workspace;
   p.q_sb = a->q_sb; p.q_sh = a->q_sh; p.q_st = a->q_st;
   p.k_sb = a->k_sb; p.k_sh = a->k_sh; p.k_st = a->k_st;
