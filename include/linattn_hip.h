@@ -679,7 +679,8 @@ int la_block_sparse_prefill(const la_prefill_args *a, void *stream);
  *    cu_q[b] .. cu_q[b+1] - 1 of q and out, cu_k (null: cu_q) its keys at those rows of
  *    k and v; Tq and Tk are the tensors' rows and the *_sb strides are unused.  Rows no
  *    sequence holds are left as they were, or zeroed (zero_rest).
- * Unit stride over D; every row 16-byte aligned.  D 64 or 128; dtype LA_F32, LA_BF16 or
+ * Unit stride over D; every row 16-byte aligned, key rows less than 2^24 values apart.
+ * D 64 or 128; dtype LA_F32, LA_BF16 or
  * LA_F16, out_dtype that or LA_F32.  lse (optional, fp32) has strides l_sb, l_sh and 1.
  * scale must be positive.  Workspace: la_dense_attention_workspace() bytes, 256-byte
  * aligned (the parts of few rows over many keys, which several workgroups share).

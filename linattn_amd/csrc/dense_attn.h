@@ -109,6 +109,23 @@ __device__ __forceinline__ void da_seq(const DaSeqs &s, DaTile &t) {
   }
 }
 
+// A pointer, and a tile, that every lane has the same of, in scalar registers.
+template <class P>
+__device__ __forceinline__ P *da_scalar(P *x) {
+  const uint64_t u = (uint64_t)(uintptr_t)x;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return (P *)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ DaTile da_uniform(DaTile t) {
+  t.b = __builtin_amdgcn_readfirstlane(t.b);
+  t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
+  t.lq = __builtin_amdgcn_readfirstlane(t.lq);
+  t.lk = __builtin_amdgcn_readfirstlane(t.lk);
+  t.q0 = __builtin_amdgcn_readfirstlane((int32_t)t.q0);
+  t.k0 = __builtin_amdgcn_readfirstlane((int32_t)t.k0);
+  return t;
+}
+
 // Tile number i of R rows, of queries (times the group's heads) or, by_k, of keys: the
 // sequences' last tiles (the longest causal rows) first, so that a launch does not end
 // with its longest workgroups.  Packed sequences: of the tiles ordered by their number

@@ -87,7 +87,7 @@ __device__ void da_rest(const DaKP &p, const DaTile &tl, int R, int kvh, int spl
 // i D / 64 ..).  For rows of a tile whose matrix products met an infinity or a NaN of V
 // that the row does not see (0 * inf): it reads nothing else.
 template <class E, int D>
-__device__ __noinline__ void da_row(const E *q, const E *k, const E *v, int64_t k_st, int64_t v_st, int a,
+__device__ __forceinline__ void da_row(const E *q, const E *k, const E *v, int64_t k_st, int64_t v_st, int a,
                                     int e, float qscale, float *m_out, float *l_out, float *acc) {
   constexpr int N = D / 64;
   const int lane = threadIdx.x & 63;
@@ -124,14 +124,16 @@ __device__ __noinline__ void da_row(const E *q, const E *k, const E *v, int64_t 
 // Rows of a wave (row number r_first + i, i < NR) whose results are not finite, of which
 // bit i of `bad` says so: those with an infinity or NaN of V among what their tiles (keys
 // a .. end - 1) held and they do not see are done again; the others stand.  (What a tile
-// holds past the last key is that key again.)  Returns the bits of the rows done.
+// holds past the last key is that key again.)  Called last, when the wave's rows are
+// stored and its registers free.
 template <class E, int D, int NR>
-__device__ __noinline__ uint32_t da_again(const DaKP &p, const DaTile &tl, int kvh, int split, int r_first,
+__device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kvh, int split, int r_first,
                                           uint32_t bad, int a, int end) {
   const int lane = threadIdx.x & 63, G = p.s.G;
   const E *kb = (const E *)p.k + (p.s.cu_q ? tl.k0 * p.k_st : tl.b * p.k_sb) + kvh * p.k_sh;
   const E *vb = (const E *)p.v + (p.s.cu_q ? tl.k0 * p.v_st : tl.b * p.v_sb) + kvh * p.v_sh;
-  uint32_t done = 0;
+  wait_vmcnt<0>();  // (stores over those)
+#pragma unroll 1
   for (int i = 0; i < NR; ++i) {
     if (!((bad >> i) & 1u)) continue;
     const int r = r_first + i, t = r / G, h = kvh * G + r % G;
@@ -141,7 +143,6 @@ __device__ __noinline__ uint32_t da_again(const DaKP &p, const DaTile &tl, int k
       for (int d = lane; d < D; d += 64)
         met = met || !(fabsf((float)vb[(int64_t)min(key, tl.lk - 1) * p.v_st + d]) < __int_as_float(0x7f800000));
     if (__ballot(met) == 0) continue;
-    done |= 1u << i;
     const E *q = (const E *)p.q + (p.s.cu_q ? (tl.q0 + t) * p.q_st : tl.b * p.q_sb + t * p.q_st) + h * p.q_sh;
     float m, l, acc[D / 64];
     da_row<E, D>(q, kb, vb, p.k_st, p.v_st, a, min(end, lim + 1), p.qscale, &m, &l, acc);
@@ -159,7 +160,6 @@ __device__ __noinline__ uint32_t da_again(const DaKP &p, const DaTile &tl, int k
       da_store1(p.out, o + lane * (D / 64) + x, p.out_dt, l == 0.f ? 0.f : acc[x] / l);
     if (p.lse && lane == 0) p.lse[da_lse_at(p, tl, t, h)] = l == 0.f ? da_ninf() : (m + __log2f(l)) * DA_LN2;
   }
-  return done;
 }
 
 // bf16 / fp16 rows: NW waves of 32 rows.  K and V tiles go global -> LDS by LDS-DMA,
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
   uint32_t stream, tix;
   da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
-  const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R, false);
+  const DaTile tl = da_uniform(da_tile(p.s, (int)tix, p.ntile, R, false));
   const int G = p.s.G;
   if (tl.b < 0 || tl.r0 + R > tl.lq * G) da_rest<D>(p, tl, R, kvh, split, (int)tix, w, NW);
   if (tl.b < 0 || tl.r0 >= tl.lq * G) return;
@@ -193,11 +193,17 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
   const bool live = r_first + r32 < nrow, wave_live = r_first < nrow;
   const int t = r_mine / G, h = kvh * G + r_mine % G;
   const int lim = limit(t);
-  const int lim_lo = limit(min(r_first, nrow - 1) / G);
-  const int lim_hi = limit(min(r_first + 31, nrow - 1) / G);
-  const int lim_tile = limit((min(tl.r0 + R, nrow) - 1) / G);
+  const int lim_lo = __builtin_amdgcn_readfirstlane(limit(min(r_first, nrow - 1) / G));
+  const int lim_hi = __builtin_amdgcn_readfirstlane(limit(min(r_first + 31, nrow - 1) / G));
+  const int lim_tile = __builtin_amdgcn_readfirstlane(limit((min(tl.r0 + R, nrow) - 1) / G));
   const int n_all = lim_tile < 0 ? 0 : lim_tile / DA_BS + 1;
-  const int j0 = (int)((int64_t)n_all * split / p.splits), j1 = (int)((int64_t)n_all * (split + 1) / p.splits);
+  int j0 = 0, j1 = n_all;
+  if (p.splits > 1) {
+    j0 = (int)((int64_t)n_all * split / p.splits);
+    j1 = (int)((int64_t)n_all * (split + 1) / p.splits);
+  }
+  j0 = __builtin_amdgcn_readfirstlane(j0);
+  j1 = __builtin_amdgcn_readfirstlane(j1);
 
   x8 qf[NS];  // B operand: dims 16 s + 8 hf ..
   {
@@ -209,25 +215,34 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
   const uint16_t *kbh = (const uint16_t *)p.k + (p.s.cu_q ? tl.k0 * p.k_st : tl.b * p.k_sb) + kvh * p.k_sh;
   const uint16_t *vbh = (const uint16_t *)p.v + (p.s.cu_q ? tl.k0 * p.v_st : tl.b * p.v_sb) + kvh * p.v_sh;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
-  // LDS-DMA: instruction x of wave w fills rows RP (NW x + w) + lane / CH
-  auto dma = [&](int kb, int slot) {
+  // LDS-DMA: instruction x of wave w fills rows RP (NW x + w) + lane / CH, from a scalar base
+  // and 32-bit offsets.  Rows past the last key are that key again (masked).
+  uint32_t ko[NX], vo[NX];
 #pragma unroll
-    for (int x = 0; x < NX; ++x) {
-      const int u = NW * x + w, rr = RP * u + lane / CH;
-      const int64_t key = min(kb * DA_BS + rr, tl.lk - 1);  // (past the end: masked)
-      const uint32_t m0 = lds0 + 2 * (slot * BLK + u * 512);
-      asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(kbh + key * p.k_st + 8 * ((lane % CH) ^ da_swz_k<D>(rr))),
-                   "{m0}"(m0) : "memory");
-    }
+  for (int x = 0; x < NX; ++x) {
+    const int rr = RP * (NW * x + w) + lane / CH;
+    ko[x] = (uint32_t)((rr * (uint32_t)p.k_st + 8 * ((lane % CH) ^ da_swz_k<D>(rr))) * 2);
+    vo[x] = (uint32_t)((rr * (uint32_t)p.v_st + 8 * ((lane % CH) ^ da_swz_v<D>(rr))) * 2);
+  }
+  auto dma = [&](const uint16_t *bh, int64_t st, const uint32_t (&off)[NX], int kb, int slot) __attribute__((always_inline)) {
+    const uint16_t *base = da_scalar(bh + (int64_t)kb * DA_BS * st);
+    const int last = tl.lk - 1 - kb * DA_BS;
+    if (last >= DA_BS - 1) {
 #pragma unroll
-    for (int x = 0; x < NX; ++x) {
-      const int u = NW * x + w, rr = RP * u + lane / CH;
-      const int64_t key = min(kb * DA_BS + rr, tl.lk - 1);
-      const uint32_t m0 = lds0 + 2 * ((2 + slot) * BLK + u * 512);
-      asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(vbh + key * p.v_st + 8 * ((lane % CH) ^ da_swz_v<D>(rr))),
-                   "{m0}"(m0) : "memory");
+      for (int x = 0; x < NX; ++x)
+        asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off[x]), "s"(base),
+                     "{m0}"(lds0 + 2 * (slot * BLK + (NW * x + w) * 512)) : "memory");
+    } else {
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        const int past = max(RP * (NW * x + w) + lane / CH - last, 0);  // rows back to the last key
+        asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off[x] - past * (uint32_t)st * 2u), "s"(base),
+                     "{m0}"(lds0 + 2 * (slot * BLK + (NW * x + w) * 512)) : "memory");
+      }
     }
   };
+  auto dma_k = [&](int kb) __attribute__((always_inline)) { dma(kbh, p.k_st, ko, kb, (kb - j0) & 1); };
+  auto dma_v = [&](int kb) __attribute__((always_inline)) { dma(vbh, p.v_st, vo, kb, 2 + ((kb - j0) & 1)); };
 
   float m = da_ninf(), thr = da_ninf(), l = 0.f, nmu = 0.f;
   f32x16 acc[ND];
@@ -236,15 +251,9 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
-  if (j0 < j1) dma(j0, 0);
-  for (int j = j0; j < j1; ++j) {
-    const int par = (j - j0) & 1;
-    wait_vmcnt<0>();
-    lds_barrier();  // tile j has landed for every wave, tile j - 1 is read
-    if (j + 1 < j1) dma(j + 1, par ^ 1);
-    if (!wave_live || j * DA_BS > lim_hi) continue;
-    const uint16_t *sk = smem + par * BLK, *sv = smem + (2 + par) * BLK;
-    f32x16 st[2];
+  // scores of tile j; register i of a half holds key 8 (i / 4) + 4 hf + i % 4
+  auto scores = [&](int j, f32x16 (&st)[2]) __attribute__((always_inline)) {
+    const uint16_t *sk = smem + ((j - j0) & 1) * BLK;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
@@ -254,7 +263,18 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
       for (int s = 0; s < NS; ++s)
         st[kt] = T::mfma(*(const x8 *)&sk[kr * D + 8 * ((2 * s + hf) ^ sw)], qf[s], st[kt]);
     }
-    // register i of a tile holds key 8 (i / 4) + 4 hf + i % 4
+  };
+  auto largest = [&](const f32x16 (&st)[2]) __attribute__((always_inline)) -> float {
+    float mx = fmaxf(st[0][0], st[0][1]);
+#pragma unroll
+    for (int i = 2; i < 16; i += 2) mx = fmaxf(fmaxf(mx, st[0][i]), st[0][i + 1]);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, st[1][i]), st[1][i + 1]);
+    return mx;
+  };
+  // masks tile j where it has to be, and raises the reference maximum only past 2^8 of
+  // headroom (the weights stay below 256); both halves of a row keep the same one
+  auto settle_max = [&](int j, f32x16 (&st)[2], float mx) __attribute__((always_inline)) {
     if (j * DA_BS + DA_BS - 1 > lim_lo) {
       const int d = lim - j * DA_BS - 4 * hf;
 #pragma unroll
@@ -262,14 +282,8 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           st[kt][i] = 32 * kt + 8 * (i >> 2) + (i & 3) <= d ? st[kt][i] : da_ninf();
+      mx = largest(st);
     }
-    float mx = st[0][0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, st[0][i]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[1][i]);
-    // the reference maximum is raised only past 2^8 of headroom (the weights stay below
-    // 256); both halves of a row keep the same one
     if (__ballot(mx > thr) != 0) {
       const float mn = fmaxf(m, pair32_max(mx));
       const float alpha = m == da_ninf() ? 0.f : fast_exp2((m - mn) * p.qscale);
@@ -282,32 +296,55 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
     }
+  };
+  // weights of half kt of a tile, and their product with V
+  auto weigh = [&](f32x16 &st, x8 (&pw)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int i = 0; i < 16; ++i) {
+      st[i] = fast_exp2(__builtin_fmaf(st[i], p.qscale, nmu));
+      l += st[i];
+      pw[i >> 3][i & 7] = (elem)st[i];
+    }
+  };
+  auto values = [&](int j, int kt, const x8 (&pw)[2]) __attribute__((always_inline)) {
+    const uint16_t *sv = smem + (2 + ((j - j0) & 1)) * BLK;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        st[kt][i] = fast_exp2(__builtin_fmaf(st[kt][i], p.qscale, nmu));
-        l += st[kt][i];
-      }
+    for (int ks = 0; ks < 2; ++ks) {
+      // V^T: 16-lane group c of the wave points at rows k0 + i / 4 and reads
+      // columns 32 dt + 16 (c % 2) + (its lane) of four keys
+      const int vr = 32 * kt + 16 * ks + 4 * hf + ((lane & 15) >> 2);
+      const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), ve = 4 * (lane & 1);
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        x8 pw;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pw[e] = (elem)st[kt][8 * ks + e];
-        // V^T: 16-lane group c of the wave points at rows k0 + i / 4 and reads
-        // columns 32 dt + 16 (c % 2) + (its lane) of four keys
-        const int vr = 32 * kt + 16 * ks + 4 * hf + ((lane & 15) >> 2);
-        const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), ve = 4 * (lane & 1);
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) {
-          const int at = vr * D + 8 * ((4 * dt + vc) ^ da_swz_v<D>(vr)) + ve;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sv + at));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sv + at + 8 * D));
-          const x8 a = __builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-          acc[dt] = T::mfma(a, pw, acc[dt]);
-        }
+      for (int dt = 0; dt < ND; ++dt) {
+        const int at = vr * D + 8 * ((4 * dt + vc) ^ da_swz_v<D>(vr)) + ve;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sv + at));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sv + at + 8 * D));
+        acc[dt] = T::mfma(__builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pw[ks], acc[dt]);
       }
     }
+  };
+
+  const int jw = wave_live && lim_hi >= 0 ? min(lim_hi / DA_BS, j1 - 1) : -1;  // this wave's last tile
+  if (j0 < j1) {
+    dma_k(j0);
+    dma_v(j0);
+  }
+  for (int j = j0; j < j1; ++j) {
+    wait_vmcnt<0>();
+    lds_barrier();  // tile j has landed for every wave, tile j - 1 is read
+    if (j + 1 < j1) {
+      dma_k(j + 1);
+      dma_v(j + 1);
+    }
+    if (j > jw) continue;
+    f32x16 st[2];
+    scores(j, st);
+    settle_max(j, st, largest(st));
+    x8 pw[2];
+    weigh(st[0], pw);
+    values(j, 0, pw);
+    weigh(st[1], pw);
+    values(j, 1, pw);
   }
   if (!wave_live) return;
   l = pair32_sum(l);
@@ -317,15 +354,9 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[dt][i], 0.f, sum);
-  uint64_t bad = __ballot(sum != 0.f);  // (NaN)
-  uint32_t done = 0;
-  if (bad != 0)
-    done = da_again<elem, D, 32>(p, tl, kvh, split, r_first,
-                                 (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
-                                 j0 * DA_BS, min(j1, lim_hi / DA_BS + 1) * DA_BS);
-  if (!live || ((done >> r32) & 1u)) return;
+  const uint64_t bad = __ballot(sum != 0.f);  // (NaN)
   // register i of dim tile dt holds dim 32 dt + 8 (i / 4) + 4 hf + i % 4
-  if (p.splits > 1) {
+  if (live && p.splits > 1) {
     const int64_t pi = da_part_at(p, tl, t, h, split);
     if (hf == 0) {
       p.ws_ml[2 * pi] = m == da_ninf() ? m : m * p.qscale;
@@ -337,18 +368,21 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
       for (int i = 0; i < 4; ++i)
         *(float4 *)(p.ws_acc + pi * D + 32 * dt + 8 * i + 4 * hf) =
             float4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
-    return;
+  } else if (live) {
+    const bool none = l == 0.f;  // no key seen
+    const float inv = none ? 0.f : 1.f / l;
+    const int64_t o = da_out_at(p, tl, t, h) + 4 * hf;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        da_store4(p.out, o + 32 * dt + 8 * i, p.out_dt, acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv,
+                  acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv);
+    if (p.lse && hf == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (m * p.qscale + __log2f(l)) * DA_LN2;
   }
-  const bool none = l == 0.f;  // no key seen
-  const float inv = none ? 0.f : 1.f / l;
-  const int64_t o = da_out_at(p, tl, t, h) + 4 * hf;
-#pragma unroll
-  for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      da_store4(p.out, o + 32 * dt + 8 * i, p.out_dt, acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv,
-                acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv);
-  if (p.lse && hf == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (m * p.qscale + __log2f(l)) * DA_LN2;
+  if (bad != 0)
+    da_again<elem, D, 32>(p, tl, kvh, split, r_first, (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
+                          j0 * DA_BS, min(j1, lim_hi / DA_BS + 1) * DA_BS);
 }
 
 // fp32 rows: four waves of 16 rows on 16x16x4 products, all of it fp32.  A staged tile is
@@ -365,7 +399,7 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   uint32_t stream, tix;
   da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
-  const DaTile tl = da_tile(p.s, (int)tix, p.ntile, R, false);
+  const DaTile tl = da_uniform(da_tile(p.s, (int)tix, p.ntile, R, false));
   const int G = p.s.G;
   if (tl.b < 0 || tl.r0 + R > tl.lq * G) da_rest<D>(p, tl, R, kvh, split, (int)tix, w, NW);
   if (tl.b < 0 || tl.r0 >= tl.lq * G) return;
@@ -377,11 +411,17 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   const bool live = r_first + ri < nrow, wave_live = r_first < nrow;
   const int t = r_mine / G, h = kvh * G + r_mine % G;
   const int lim = limit(t);
-  const int lim_lo = limit(min(r_first, nrow - 1) / G);
-  const int lim_hi = limit(min(r_first + 15, nrow - 1) / G);
-  const int lim_tile = limit((min(tl.r0 + R, nrow) - 1) / G);
+  const int lim_lo = __builtin_amdgcn_readfirstlane(limit(min(r_first, nrow - 1) / G));
+  const int lim_hi = __builtin_amdgcn_readfirstlane(limit(min(r_first + 15, nrow - 1) / G));
+  const int lim_tile = __builtin_amdgcn_readfirstlane(limit((min(tl.r0 + R, nrow) - 1) / G));
   const int n_all = lim_tile < 0 ? 0 : lim_tile / BS + 1;
-  const int j0 = (int)((int64_t)n_all * split / p.splits), j1 = (int)((int64_t)n_all * (split + 1) / p.splits);
+  int j0 = 0, j1 = n_all;
+  if (p.splits > 1) {
+    j0 = (int)((int64_t)n_all * split / p.splits);
+    j1 = (int)((int64_t)n_all * (split + 1) / p.splits);
+  }
+  j0 = __builtin_amdgcn_readfirstlane(j0);
+  j1 = __builtin_amdgcn_readfirstlane(j1);
 
   f32x4 qf[NS];
   {
@@ -473,16 +513,8 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(acc[dt][e], 0.f, sum);
   uint64_t bad = __ballot(sum != 0.f);
-  uint32_t done = 0;
-  if (bad != 0) {
-    bad |= bad >> 32;
-    done = da_again<float, D, 16>(p, tl, kvh, split, r_first,
-                                  (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
-                                  j0 * BS, min(j1, lim_hi / BS + 1) * BS);
-  }
-  if (!live || ((done >> ri) & 1u)) return;
   // register e of dim tile dt holds dim 16 dt + 4 c + e
-  if (p.splits > 1) {
+  if (live && p.splits > 1) {
     const int64_t pi = da_part_at(p, tl, t, h, split);
     if (c == 0) {
       p.ws_ml[2 * pi] = m == da_ninf() ? m : m * p.qscale;
@@ -491,15 +523,20 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
 #pragma unroll
     for (int dt = 0; dt < NS; ++dt)
       *(float4 *)(p.ws_acc + pi * D + 16 * dt + 4 * c) = float4{acc[dt][0], acc[dt][1], acc[dt][2], acc[dt][3]};
-    return;
-  }
-  const bool none = l == 0.f;
-  const float inv = none ? 0.f : 1.f / l;
-  const int64_t o = da_out_at(p, tl, t, h) + 4 * c;
+  } else if (live) {
+    const bool none = l == 0.f;
+    const float inv = none ? 0.f : 1.f / l;
+    const int64_t o = da_out_at(p, tl, t, h) + 4 * c;
 #pragma unroll
-  for (int dt = 0; dt < NS; ++dt)
-    da_store4(p.out, o + 16 * dt, p.out_dt, acc[dt][0] * inv, acc[dt][1] * inv, acc[dt][2] * inv, acc[dt][3] * inv);
-  if (p.lse && c == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (m * p.qscale + __log2f(l)) * DA_LN2;
+    for (int dt = 0; dt < NS; ++dt)
+      da_store4(p.out, o + 16 * dt, p.out_dt, acc[dt][0] * inv, acc[dt][1] * inv, acc[dt][2] * inv, acc[dt][3] * inv);
+    if (p.lse && c == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (m * p.qscale + __log2f(l)) * DA_LN2;
+  }
+  if (bad != 0) {
+    bad |= bad >> 32;
+    da_again<float, D, 16>(p, tl, kvh, split, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
+                           j0 * BS, min(j1, lim_hi / BS + 1) * BS);
+  }
 }
 
 // Joins the parts of a row: a wave a row.
@@ -633,6 +670,7 @@ extern "C" int la_dense_attention(const la_dense_attn_args *a, void *stream) {
   if (int rc = da_rows_ok("q", a->q, esz, sb(a->q_sb), a->q_sh, a->q_st, a->Hq, a->Tq)) return rc;
   if (a->Tk > 0) {
     if (int rc = da_rows_ok("k", a->k, esz, sb(a->k_sb), a->k_sh, a->k_st, a->Hkv, a->Tk)) return rc;
+    LA_REQUIRE(a->k_st < (1 << 24) && a->v_st < (1 << 24), "la_dense_attention: key rows 2^24 values apart or more");
     if (int rc = da_rows_ok("v", a->v, esz, sb(a->v_sb), a->v_sh, a->v_st, a->Hkv, a->Tk)) return rc;
   }
   if (int rc = da_rows_ok("out", a->out, osz, sb(a->o_sb), a->o_sh, a->o_st, a->Hq, a->Tq)) return rc;

@@ -33,7 +33,7 @@ struct KwTile {
 template <int KT>
 __device__ __forceinline__ KwTile kw_tile(const KwKP &p, int tix, int split) {
   KwTile x;
-  x.t = da_tile(p.s, tix, p.ntile, KT, true);
+  x.t = da_uniform(da_tile(p.s, tix, p.ntile, KT, true));
   x.s0 = x.row0 = x.row1 = 0;
   if (x.t.b < 0) return x;
   // da_tile's first tiles are the sequences' last; the first keys are seen by most rows

@@ -24,10 +24,11 @@ _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with rows the kernels can load 16 bytes at a time (a copy where they are not
-    contiguous and 16-byte aligned)."""
+    contiguous and 16-byte aligned, or very far apart)."""
     n = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
-            all(s % n == 0 for s, d in zip(t.stride()[:-1], t.shape) if d > 1):
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and \
+            all(s % n == 0 for s, d in zip(st[:-1], t.shape) if d > 1) and min(st[:-1]) < 1 << 24:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
