@@ -7,7 +7,7 @@
 // maximum and sum of a softmax: S^T = K Q^T, P = exp2(c S - m), O^T += V^T P^T.
 #include <algorithm>
 
-#include "dense_attn.h"
+#include "few_rows.h"
 
 namespace la {
 
@@ -162,20 +162,24 @@ __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kv
   }
 }
 
-// bf16 / fp16 rows: NW waves of 32 rows.  K and V tiles go global -> LDS by LDS-DMA,
-// double buffered, one barrier a tile.  S^T by 32x32x16 products (A = K rows, B = q held
+// bf16 / fp16 rows: NW waves of 32 rows.  K and V tiles go global -> LDS by LDS-DMA, K a
+// tile ahead into the other of two slots, V while its tile is scored: 48 KiB a workgroup
+// and at most 168 registers make three workgroups a CU, and with three waves a SIMD one
+// wave's softmax runs beside another's products (two waves and two slots each: 7.8 ms for
+// 32768 tokens of 32 heads on 8; three: 7.4, 1.19 PFLOP/s; tile j + 1 scored beside the
+// softmax of tile j in one wave's instructions: 10.5).  S^T by 32x32x16 products (A = K rows, B = q held
 // in registers) leaves a lane 16 scores of one row, so masks, maxima and sums are per
 // lane; O^T takes P from the same registers (the contraction index is mapped to the keys
 // a lane holds) and V^T by LDS transpose reads.  P is rounded to the inputs' type for
 // that product (to half a step, 2^-9 or 2^-12 of each weight, independently: as much as
 // the output's own rounding); its sum l, and with it lse, is of the fp32 values.
 template <class T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
+__global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
   constexpr int R = 32 * NW, BLK = DA_BS * D, CH = D / 8, RP = 64 / CH, NX = DA_BS / RP / NW;
   constexpr int NS = D / 16, ND = D / 32;
   typedef typename T::x8 x8;
   typedef typename T::elem elem;
-  __shared__ __align__(16) uint16_t smem[4 * BLK];  // K slots 0, 1, then V slots 0, 1
+  __shared__ __align__(16) uint16_t smem[3 * BLK];  // K slots 0, 1, then V
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hf = lane >> 5, r32 = lane & 31;
   uint32_t stream, tix;
@@ -242,7 +246,7 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
     }
   };
   auto dma_k = [&](int kb) __attribute__((always_inline)) { dma(kbh, p.k_st, ko, kb, (kb - j0) & 1); };
-  auto dma_v = [&](int kb) __attribute__((always_inline)) { dma(vbh, p.v_st, vo, kb, 2 + ((kb - j0) & 1)); };
+  auto dma_v = [&](int kb) __attribute__((always_inline)) { dma(vbh, p.v_st, vo, kb, 2); };
 
   float m = da_ninf(), thr = da_ninf(), l = 0.f, nmu = 0.f;
   f32x16 acc[ND];
@@ -251,17 +255,30 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
+  // Byte offsets of this lane's first reads of a slot.  Swizzles only flip the chunk bits,
+  // so the other reads are these with bits flipped (done anew for every tile: the
+  // registers are worth more).
+  //   K: row r32, chunk hf of each pair s
+  //   V^T: 16-lane group c of the wave points at rows k0 + i / 4 and reads columns 32 dt +
+  //   16 (c % 2) + (its lane) of four keys
+  const uint32_t k_at = 2 * (r32 * D + 8 * (hf ^ da_swz_k<D>(r32)));
+  const int v_row = 4 * hf + ((lane & 15) >> 2);
+  const uint32_t v_at = 2 * (2 * BLK + v_row * D + 8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ da_swz_v<D>(v_row)) +
+                             4 * (lane & 1));
+  const char *lds = (const char *)smem;
   // scores of tile j; register i of a half holds key 8 (i / 4) + 4 hf + i % 4
   auto scores = [&](int j, f32x16 (&st)[2]) __attribute__((always_inline)) {
-    const uint16_t *sk = smem + ((j - j0) & 1) * BLK;
+    const uint32_t at = k_at + 2 * ((j - j0) & 1) * BLK;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) st[kt][i] = 0.f;
-      const int kr = 32 * kt + r32, sw = da_swz_k<D>(kr);
+    }
 #pragma unroll
-      for (int s = 0; s < NS; ++s)
-        st[kt] = T::mfma(*(const x8 *)&sk[kr * D + 8 * ((2 * s + hf) ^ sw)], qf[s], st[kt]);
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)  // (row r32 + 32 has the same swizzle)
+        st[kt] = T::mfma(*(const x8 *)(lds + (at ^ (32 * s)) + 64 * kt * D), qf[s], st[kt]);
     }
   };
   auto largest = [&](const f32x16 (&st)[2]) __attribute__((always_inline)) -> float {
@@ -307,44 +324,41 @@ __global__ __launch_bounds__(64 * NW, 2) void dense_attn_kernel(DaKP p) {
     }
   };
   auto values = [&](int j, int kt, const x8 (&pw)[2]) __attribute__((always_inline)) {
-    const uint16_t *sv = smem + (2 + ((j - j0) & 1)) * BLK;
+    const uint32_t at = v_at;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      // V^T: 16-lane group c of the wave points at rows k0 + i / 4 and reads
-      // columns 32 dt + 16 (c % 2) + (its lane) of four keys
-      const int vr = 32 * kt + 16 * ks + 4 * hf + ((lane & 15) >> 2);
-      const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), ve = 4 * (lane & 1);
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) {
-        const int at = vr * D + 8 * ((4 * dt + vc) ^ da_swz_v<D>(vr)) + ve;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sv + at));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sv + at + 8 * D));
+        const char *v = lds + (at ^ (64 * dt)) + 2 * (32 * kt + 16 * ks) * D;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 16 * D));
         acc[dt] = T::mfma(__builtin_bit_cast(x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pw[ks], acc[dt]);
       }
     }
   };
 
   const int jw = wave_live && lim_hi >= 0 ? min(lim_hi / DA_BS, j1 - 1) : -1;  // this wave's last tile
-  if (j0 < j1) {
-    dma_k(j0);
-    dma_v(j0);
-  }
+  if (j0 < j1) dma_k(j0);
   for (int j = j0; j < j1; ++j) {
     wait_vmcnt<0>();
-    lds_barrier();  // tile j has landed for every wave, tile j - 1 is read
-    if (j + 1 < j1) {
-      dma_k(j + 1);
-      dma_v(j + 1);
-    }
-    if (j > jw) continue;
+    lds_barrier();  // K of tile j has landed for every wave, tile j - 1 is read
+    dma_v(j);
+    if (j + 1 < j1) dma_k(j + 1);
     f32x16 st[2];
-    scores(j, st);
-    settle_max(j, st, largest(st));
     x8 pw[2];
-    weigh(st[0], pw);
-    values(j, 0, pw);
-    weigh(st[1], pw);
-    values(j, 1, pw);
+    if (j <= jw) {
+      scores(j, st);
+      settle_max(j, st, largest(st));
+      weigh(st[0], pw);
+    }
+    if (j + 1 < j1) wait_vmcnt<NX>();
+    else wait_vmcnt<0>();
+    lds_barrier();  // V of tile j has landed
+    if (j <= jw) {
+      values(j, 0, pw);
+      weigh(st[1], pw);
+      values(j, 1, pw);
+    }
   }
   if (!wave_live) return;
   l = pair32_sum(l);
@@ -539,6 +553,73 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   }
 }
 
+// At most 16 rows a sequence and KV head (decode steps): the four waves of a workgroup
+// take rounds of keys in turn (few_rows.h) and join in LDS.
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void dense_few_kernel(DaKP p) {
+  typedef FewRows<T, D> FR;
+  typedef typename FR::elem elem;
+  constexpr int NW = 4;
+  constexpr int LDS_MERGE = NW * (FR::VALS + 32) * 4;
+  constexpr int LDS = NW * FR::LDS_BYTES > LDS_MERGE ? NW * FR::LDS_BYTES : LDS_MERGE;
+  __shared__ __align__(16) char smem[LDS];
+  __shared__ uint32_t s_bad;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t stream, split_u;
+  da_stream(blockIdx.x, (uint32_t)(p.Hkv * p.s.B), stream, split_u);
+  const int kvh = (int)(stream % (uint32_t)p.Hkv), split = (int)split_u, G = p.s.G;
+  DaTile tl{};
+  tl.b = (int32_t)(stream / (uint32_t)p.Hkv);
+  da_seq(p.s, tl);
+  tl = da_uniform(tl);
+  const int R = (int)p.s.Tq * G, nrow = tl.lq * G;
+  if (nrow < R) da_rest<D>(p, tl, R, kvh, split, 0, w, NW);
+  if (nrow == 0) return;
+  const int diag = tl.lk - tl.lq;
+  auto limit = [&](int t) { return p.causal ? diag + t : tl.lk - 1; };
+  const int row = min(lane & 15, nrow - 1), t = row / G;
+  const int last = __builtin_amdgcn_readfirstlane(limit(tl.lq - 1));  // the last key any row sees
+  const int rounds = last < 0 ? 0 : last / FR::RK + 1;
+  const int r0 = (int)((int64_t)rounds * split / p.splits), r1 = (int)((int64_t)rounds * (split + 1) / p.splits);
+  const elem *kb = (const elem *)p.k + tl.b * p.k_sb + kvh * p.k_sh, *vb = (const elem *)p.v + tl.b * p.v_sb + kvh * p.v_sh;
+  if (threadIdx.x == 0) s_bad = 0u;
+  FR fr;
+  fr.begin((const elem *)p.q + tl.b * p.q_sb + t * p.q_st + (kvh * G + row % G) * p.q_sh);
+  fr.walk(r0 + w, NW, r1, tl.lk, limit(t), p.qscale, 8.f, (elem *)(smem + w * FR::LDS_BYTES),
+          [&](int key) { return kb + key * p.k_st; }, [&](int key) { return vb + key * p.v_st; }, [](int, f32x4) {});
+  __syncthreads();
+  float *ml = (float *)smem, *vals = ml + NW * 32;
+  fr.put(ml + w * 32, vals + w * FR::VALS);
+  __syncthreads();
+  for (int e = threadIdx.x; e < nrow * D; e += 256) {
+    const int g = e / D, d = e % D, te = g / G, h = kvh * G + g % G;
+    float m = da_ninf();
+#pragma unroll
+    for (int x = 0; x < NW; ++x) m = fmaxf(m, ml[x * 32 + 2 * g]);
+    float l = 0.f, a = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const float f = fast_exp2(ml[x * 32 + 2 * g] - (m == da_ninf() ? 0.f : m));
+      l = __builtin_fmaf(ml[x * 32 + 2 * g + 1], f, l);
+      a = __builtin_fmaf(vals[x * FR::VALS + g * (D + 4) + d], f, a);
+    }
+    if (!(fabsf(a) < __int_as_float(0x7f800000))) atomicOr(&s_bad, 1u << g);
+    if (p.splits > 1) {
+      const int64_t pi = da_part_at(p, tl, te, h, split);
+      p.ws_acc[pi * D + d] = a;
+      if (d == 0) {
+        p.ws_ml[2 * pi] = m;
+        p.ws_ml[2 * pi + 1] = l;
+      }
+    } else {
+      da_store1(p.out, da_out_at(p, tl, te, h) + d, p.out_dt, l == 0.f ? 0.f : a / l);
+      if (p.lse && d == 0) p.lse[da_lse_at(p, tl, te, h)] = l == 0.f ? da_ninf() : (m + __log2f(l)) * DA_LN2;
+    }
+  }
+  __syncthreads();
+  if (s_bad != 0u && w == 0) da_again<elem, D, 16>(p, tl, kvh, split, 0, s_bad, r0 * FR::RK, r1 * FR::RK);
+}
+
 // Joins the parts of a row: a wave a row.
 template <int D>
 __global__ __launch_bounds__(256) void dense_combine_kernel(DaKP p, int64_t rows) {
@@ -583,7 +664,8 @@ __global__ __launch_bounds__(256) void dense_combine_kernel(DaKP p, int64_t rows
 
 // ------------------------------------------------------------------ host ----
 struct DaPlan {
-  int nw = 4, rows = 128;  // waves and rows of a workgroup
+  bool few = false;     // dense_few_kernel
+  int rows = 128;       // of a workgroup
   int64_t ntile = 0, splits = 1;
   size_t ml = 0, bytes = 0;
 };
@@ -592,18 +674,13 @@ static DaPlan da_plan(const la_dense_attn_args *a) {
   DaPlan pl;
   const bool packed = a->cu_q != nullptr, f32 = a->dtype == LA_F32;
   const int64_t G = a->Hq / a->Hkv;
-  auto tiles = [&](int64_t R) { return da_tiles(packed, a->B, a->Tq, G, R); };
-  if (f32) {
-    pl.nw = 4;
-    pl.rows = 64;
-  } else {
-    pl.nw = 4;
-    pl.rows = 128;
-  }
-  pl.ntile = tiles(pl.rows);
-  // parts of at least four staged tiles, two workgroups a CU
+  pl.few = !packed && a->Tq * G <= 16;
+  pl.rows = pl.few ? 16 : f32 ? 64 : 128;
+  pl.ntile = pl.few ? a->B : da_tiles(packed, a->B, a->Tq, G, pl.rows);
+  // parts of at least four staged tiles, two workgroups a CU (few rows: four, since the
+  // sequences' lengths differ)
   const int64_t wgs = pl.ntile * a->Hkv, keys = packed ? ceil_div(a->Tk, a->B) : a->Tk;
-  const int64_t want = (int64_t)2 * num_cus() / std::max<int64_t>(1, wgs);
+  const int64_t want = (int64_t)(pl.few ? 4 : 2) * num_cus() / std::max<int64_t>(1, wgs);
   pl.splits = std::max<int64_t>(1, std::min<int64_t>({want, keys / (4 * DA_BS), 64}));
   if (pl.splits > 1) {
     const int64_t parts = (packed ? 1 : a->B) * a->Tq * a->Hq * pl.splits;
@@ -644,12 +721,6 @@ static int da_launch(K kernel, int64_t wgs, int threads, const DaKP &p, hipStrea
   kernel<<<dim3((uint32_t)wgs), dim3(threads), 0, st>>>(p);
   LA_LAUNCHED();
   return LA_OK;
-}
-
-template <class T, int D>
-static int da_launch16(const DaPlan &pl, const DaKP &p, hipStream_t st) {
-  const int64_t wgs = pl.ntile * p.Hkv * pl.splits;
-  return da_launch(dense_attn_kernel<T, D, 4>, wgs, 256, p, st);
 }
 
 }  // namespace la
@@ -698,13 +769,21 @@ extern "C" int la_dense_attention(const la_dense_attn_args *a, void *stream) {
   p.thr_gap = 8.f / p.qscale;
   hipStream_t st = (hipStream_t)stream;
   int rc;
-  if (a->dtype == LA_F32)
-    rc = a->D == 128 ? da_launch(dense_attn_f32_kernel<128>, wgs, 256, p, st)
-                     : da_launch(dense_attn_f32_kernel<64>, wgs, 256, p, st);
-  else if (a->dtype == LA_BF16)
-    rc = a->D == 128 ? da_launch16<DaBf16, 128>(pl, p, st) : da_launch16<DaBf16, 64>(pl, p, st);
-  else
-    rc = a->D == 128 ? da_launch16<DaF16, 128>(pl, p, st) : da_launch16<DaF16, 64>(pl, p, st);
+  const bool d128 = a->D == 128;
+  if (pl.few) {
+    if (a->dtype == LA_F32)
+      rc = d128 ? da_launch(dense_few_kernel<DaF32, 128>, wgs, 256, p, st) : da_launch(dense_few_kernel<DaF32, 64>, wgs, 256, p, st);
+    else if (a->dtype == LA_BF16)
+      rc = d128 ? da_launch(dense_few_kernel<DaBf16, 128>, wgs, 256, p, st) : da_launch(dense_few_kernel<DaBf16, 64>, wgs, 256, p, st);
+    else
+      rc = d128 ? da_launch(dense_few_kernel<DaF16, 128>, wgs, 256, p, st) : da_launch(dense_few_kernel<DaF16, 64>, wgs, 256, p, st);
+  } else if (a->dtype == LA_F32) {
+    rc = d128 ? da_launch(dense_attn_f32_kernel<128>, wgs, 256, p, st) : da_launch(dense_attn_f32_kernel<64>, wgs, 256, p, st);
+  } else if (a->dtype == LA_BF16) {
+    rc = d128 ? da_launch(dense_attn_kernel<DaBf16, 128, 4>, wgs, 256, p, st) : da_launch(dense_attn_kernel<DaBf16, 64, 4>, wgs, 256, p, st);
+  } else {
+    rc = d128 ? da_launch(dense_attn_kernel<DaF16, 128, 4>, wgs, 256, p, st) : da_launch(dense_attn_kernel<DaF16, 64, 4>, wgs, 256, p, st);
+  }
   if (rc != LA_OK || pl.splits == 1) return rc;
   const int64_t rows = (packed ? 1 : a->B) * a->Tq * a->Hq;
   const dim3 grid((uint32_t)ceil_div(rows, 4));
