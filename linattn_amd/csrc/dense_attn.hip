@@ -640,20 +640,30 @@ __global__ __launch_bounds__(256) void dense_combine_kernel(DaKP p, int64_t rows
     o = b * p.o_sb + t * p.o_st + h * p.o_sh;
     lo = b * p.l_sb + t + h * p.l_sh;
   }
-  const float2 *ml = (const float2 *)p.ws_ml + row * p.splits;
-  float m = da_ninf();
-  for (int i = 0; i < p.splits; ++i) m = fmaxf(m, ml[i].x);
-  float l = 0.f, acc[N];
+  // a lane a part (at most 64)
+  const float2 ml = lane < p.splits ? ((const float2 *)p.ws_ml)[row * p.splits + lane] : float2{da_ninf(), 0.f};
+  float m = ml.x;
+#pragma unroll
+  for (int o2 = 32; o2 >= 1; o2 >>= 1) m = fmaxf(m, __shfl_xor(m, o2, 64));
+  const bool empty = ml.x == da_ninf() && ml.y == 0.f;
+  const float f = empty ? 0.f : fast_exp2(ml.x - (m == da_ninf() ? 0.f : m));
+  const float l = group_sum<64>(empty ? 0.f : ml.y * f);
+  float acc[N];
 #pragma unroll
   for (int x = 0; x < N; ++x) acc[x] = 0.f;
-  for (int i = 0; i < p.splits; ++i) {
-    const float2 part = ml[i];
-    if (part.x == da_ninf() && part.y == 0.f) continue;
-    const float f = fast_exp2(part.x - (m == da_ninf() ? 0.f : m));
-    l = __builtin_fmaf(part.y, f, l);
-    const float *a = p.ws_acc + (row * p.splits + i) * D + lane * N;
+  const float *a = p.ws_acc + row * p.splits * D + lane * N;
+  for (int i0 = 0; i0 < p.splits; i0 += 8) {
+    float v[8][N];
 #pragma unroll
-    for (int x = 0; x < N; ++x) acc[x] = __builtin_fmaf(a[x], f, acc[x]);
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int x = 0; x < N; ++x) v[i][x] = a[(int64_t)min(i0 + i, p.splits - 1) * D + x];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float fi = __shfl(i0 + i < p.splits ? f : 0.f, (i0 + i) & 63, 64);
+#pragma unroll
+      for (int x = 0; x < N; ++x) acc[x] = __builtin_fmaf(i0 + i < p.splits ? v[i][x] : 0.f, fi, acc[x]);
+    }
   }
   const bool none = l == 0.f;
   const float inv = none ? 0.f : 1.f / l;

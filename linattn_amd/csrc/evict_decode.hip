@@ -7,8 +7,9 @@
 // cache, so writing it there races with nothing.  Weights need the row's final sum: the
 // scores (a float per head and entry, 1/32 of the K/V bytes at four heads) are kept in
 // the workspace.  Where there are enough (sequence, head) pairs, one workgroup does all
-// of a pair; else its entries are split: evict_slot_kernel, evict_decode_kernel over the
-// parts, evict_join_kernel.
+// of a pair; else its entries are split over workgroups, each of which looks for the slot
+// on its own (all weights and positions of the pair: 8 bytes an entry, from L2 but for
+// the first), and evict_join_kernel joins the parts.
 #include <algorithm>
 
 #include "evict.h"
@@ -22,7 +23,7 @@ struct EdKP {
   float *weights;
   int32_t *positions;
   const int32_t *lengths, *pos;
-  int32_t *slots;   // [pair] (split form)
+  int32_t *slots;   // [pair] (split form, for evict_join_kernel)
   float *ml;        // [pair][split][G] (max in log2 units, sum)
   float *vals;      // [pair][split][G][D]
   float *scores;    // [pair][G][cs]
@@ -32,13 +33,13 @@ struct EdKP {
 };
 
 constexpr float ED_GAP = 8.f;  // headroom of the reference maximum, log2 units
+typedef float ed_f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef int32_t ed_i4 __attribute__((ext_vector_type(4), aligned(4)));
 
 // The entry that makes room (of a full cache), by a workgroup of NT threads: the lowest
 // key, of equal ones the highest slot.
 template <int NT>
 __device__ __forceinline__ int32_t ed_victim(const EdKP &p, int64_t pair, int64_t pos) {
-  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
-  typedef int32_t i4u __attribute__((ext_vector_type(4), aligned(4)));
   __shared__ uint64_t best[NT / 64];
   const float *w = p.weights + pair * p.C;
   const int32_t *ps = p.positions + pair * p.C;
@@ -48,18 +49,19 @@ __device__ __forceinline__ int32_t ed_victim(const EdKP &p, int64_t pair, int64_
     mine = min(mine, (k << 32) | (uint32_t)~i);
   };
   const int32_t whole = p.C & ~3;
-  for (int32_t i0 = 0; i0 < whole; i0 += 16 * NT) {
-    f4u x[4];
-    i4u y[4];
+  constexpr int NB = 8;  // loads of each in flight
+  for (int32_t i0 = 4 * (int32_t)threadIdx.x; i0 < whole; i0 += 4 * NB * NT) {
+    ed_f4 x[NB];
+    ed_i4 y[NB];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int32_t i = min(i0 + 4 * (NT * j + (int32_t)threadIdx.x), whole - 4);
-      x[j] = *(const f4u *)(w + i);
-      y[j] = *(const i4u *)(ps + i);
+    for (int j = 0; j < NB; ++j) {
+      const int32_t i = min(i0 + 4 * NT * j, whole - 4);
+      x[j] = *(const ed_f4 *)(w + i);
+      y[j] = *(const ed_i4 *)(ps + i);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int32_t i = min(i0 + 4 * (NT * j + (int32_t)threadIdx.x), whole - 4);
+    for (int j = 0; j < NB; ++j) {
+      const int32_t i = min(i0 + 4 * NT * j, whole - 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) look(i + e, x[j][e], y[j][e]);
     }
@@ -77,25 +79,45 @@ __device__ __forceinline__ int32_t ed_victim(const EdKP &p, int64_t pair, int64_
 
 __device__ __forceinline__ int32_t ed_held(const EdKP &p, int b) { return min(max(p.lengths[b], 0), p.C); }
 
-__global__ __launch_bounds__(1024) void evict_slot_kernel(EdKP p) {
-  const int64_t pair = blockIdx.x;
-  const int b = (int)(pair / p.Hkv);
-  const int32_t n = ed_held(p, b);
-  const int32_t slot = n < p.C ? n : ed_victim<1024>(p, pair, p.pos[b]);
-  if (threadIdx.x == 0) p.slots[pair] = slot;
-}
-
-// Rows' weights over entries first .. end - 1 added to what they gathered; lse2 in LDS.
+// Rows' weights over entries first .. end - 1 (first a multiple of 4) added to what they
+// gathered; lse2 in LDS.
 template <int NT>
 __device__ __forceinline__ void ed_weights(const EdKP &p, int64_t pair, int32_t slot, int32_t first, int32_t end,
                                            const float *lse2) {
   const float *s = p.scores + pair * p.G * p.cs;
   float *w = p.weights + pair * p.C;
-  for (int32_t i = first + (int32_t)threadIdx.x; i < end; i += NT) {
-    float sum = 0.f;
-    for (int g = 0; g < p.G; ++g) sum += fast_exp2(s[g * p.cs + i] - lse2[g]);
-    w[i] = (i == slot ? 0.f : w[i]) + sum;
-    if (i == slot) p.positions[pair * p.C + i] = p.pos[pair / p.Hkv];
+  for (int32_t i = first + 4 * (int32_t)threadIdx.x; i < end; i += 4 * NT) {
+    const bool whole = i + 4 <= end;
+    float sum[4], old[4];
+    if (whole) {
+      const ed_f4 o = *(const ed_f4 *)(w + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) old[e] = o[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) old[e] = i + e < end ? w[i + e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = 0.f;
+#pragma unroll 4
+    for (int g = 0; g < p.G; ++g) {
+      const float4 x = *(const float4 *)(s + g * p.cs + i);  // (scores are there for whole rounds)
+      const float l = lse2[g];
+      sum[0] += fast_exp2(x.x - l);
+      sum[1] += fast_exp2(x.y - l);
+      sum[2] += fast_exp2(x.z - l);
+      sum[3] += fast_exp2(x.w - l);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = (i + e == slot ? 0.f : old[e]) + sum[e];
+    if (whole) {
+      *(ed_f4 *)(w + i) = ed_f4{sum[0], sum[1], sum[2], sum[3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < end) w[i + e] = sum[e];
+    }
+    if (slot >= i && slot < min(i + 4, end)) p.positions[pair * p.C + slot] = p.pos[pair / p.Hkv];
   }
 }
 
@@ -113,10 +135,8 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
   const int split = (int)(blockIdx.x % (uint32_t)p.splits);
   const int b = (int)(pair / p.Hkv), kvh = (int)(pair % p.Hkv);
   const int32_t held = ed_held(p, b), n = min(held + 1, p.C);
-  int32_t slot;
-  if (p.splits > 1) slot = p.slots[pair];
-  else slot = held < p.C ? held : ed_victim<256>(p, pair, p.pos[b]);
-  slot = __builtin_amdgcn_readfirstlane(slot);
+  const int32_t slot = __builtin_amdgcn_readfirstlane(held < p.C ? held : ed_victim<256>(p, pair, p.pos[b]));
+  if (p.splits > 1 && split == 0 && threadIdx.x == 0) p.slots[pair] = slot;
 
   const elem *kn = (const elem *)p.k_new + b * p.kn_sb + kvh * p.kn_sh;
   const elem *vn = (const elem *)p.v_new + b * p.vn_sb + kvh * p.vn_sh;
@@ -178,27 +198,30 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
 constexpr int ED_CHUNK = 1024;
 template <int D>
 __global__ __launch_bounds__(256) void evict_join_kernel(EdKP p) {
-  __shared__ float lse2[16];
+  __shared__ float lse2[16], part[16][64];  // part: what each part's values count for
   const int64_t pair = blockIdx.x / (uint32_t)p.chunks;
-  const int chunk = (int)(blockIdx.x % (uint32_t)p.chunks);
+  const int chunk = (int)(blockIdx.x % (uint32_t)p.chunks), lane = threadIdx.x & 63;
   const int b = (int)(pair / p.Hkv), kvh = (int)(pair % p.Hkv);
   const int32_t n = min(ed_held(p, b) + 1, p.C), slot = p.slots[pair];
   const float ninf = __int_as_float(0xff800000);
-  const float *ml = p.ml + pair * p.splits * p.G * 2;
-  if (threadIdx.x < (uint32_t)p.G) {
-    const int g = threadIdx.x;
-    float m = ninf, l = 0.f;
-    for (int x = 0; x < p.splits; ++x) m = fmaxf(m, ml[2 * (x * p.G + g)]);
-    for (int x = 0; x < p.splits; ++x) l = __builtin_fmaf(ml[2 * (x * p.G + g) + 1],
-                                                          fast_exp2(ml[2 * (x * p.G + g)] - (m == ninf ? 0.f : m)), l);
-    lse2[g] = (m == ninf ? 0.f : m) + __log2f(l);
+  const float2 *ml = (const float2 *)p.ml + pair * p.splits * p.G;
+  for (int g = threadIdx.x >> 6; g < p.G; g += 4) {  // a lane a part
+    const float2 x = lane < p.splits ? ml[lane * p.G + g] : float2{ninf, 0.f};
+    float m = x.x;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    const float l = group_sum<64>(x.y * fast_exp2(x.x - (m == ninf ? 0.f : m)));
+    const float z = (m == ninf ? 0.f : m) + __log2f(l);
+    part[g][lane] = fast_exp2(x.x - z);
+    if (lane == 0) lse2[g] = z;
   }
   __syncthreads();
   for (int e = threadIdx.x + 256 * chunk; e < p.G * D; e += 256 * p.chunks) {
     const int g = e / D, d = e % D;
+    const float *v = p.vals + (pair * p.splits * p.G + g) * D + d;
     float a = 0.f;
-    for (int x = 0; x < p.splits; ++x)
-      a = __builtin_fmaf(p.vals[((pair * p.splits + x) * p.G + g) * D + d], fast_exp2(ml[2 * (x * p.G + g)] - lse2[g]), a);
+#pragma unroll 8
+    for (int x = 0; x < p.splits; ++x) a = __builtin_fmaf(v[(int64_t)x * p.G * D], part[g][x], a);
     store_from_f32(p.out, b * p.o_sb + (kvh * p.G + g) * p.o_sh + d, p.out_dt, a);
   }
   ed_weights<256>(p, pair, slot, chunk * ED_CHUNK, min(n, (chunk + 1) * ED_CHUNK), lse2);
@@ -288,10 +311,6 @@ extern "C" int la_evict_decode(const la_evict_decode_args *a, void *stream) {
   p.chunks = (int32_t)ceil_div(a->C, ED_CHUNK);
   p.qscale = a->scale * 1.44269504088896340736f;
   hipStream_t st = (hipStream_t)stream;
-  if (pl.splits > 1) {
-    evict_slot_kernel<<<(uint32_t)pairs, 1024, 0, st>>>(p);
-    LA_LAUNCHED();
-  }
   const bool d128 = a->D == 128;
   if (a->dtype == LA_F32) d128 ? ed_launch<DaF32, 128>(p, pairs, st) : ed_launch<DaF32, 64>(p, pairs, st);
   else if (a->dtype == LA_BF16) d128 ? ed_launch<DaBf16, 128>(p, pairs, st) : ed_launch<DaBf16, 64>(p, pairs, st);
