@@ -557,7 +557,7 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
 // take rounds of keys in turn (few_rows.h) and join in LDS.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void dense_few_kernel(DaKP p) {
-  typedef FewRows<T, D> FR;
+  typedef FewRows<T, D, false> FR;
   typedef typename FR::elem elem;
   constexpr int NW = 4;
   constexpr int LDS_MERGE = NW * (FR::VALS + 32) * 4;

@@ -123,7 +123,7 @@ __device__ __forceinline__ void ed_weights(const EdKP &p, int64_t pair, int32_t 
 
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
-  typedef FewRows<T, D> FR;
+  typedef FewRows<T, D, true> FR;
   typedef typename FR::elem elem;
   constexpr int NW = 4;
   constexpr int LDS_MERGE = NW * (FR::VALS + 32) * 4;

@@ -18,7 +18,11 @@ struct DaF32 {
   typedef float elem;
 };
 
-template <class T, int D>
+//
+// V is read past the caches (nt): 64 caches of 2049 entries 118 -> 110 us, decode over
+// 12345 keys 100 -> 93.  K is where NT_K is set, which the decode step gains from (110 ->
+// 109, four caches of 16385 entries 62 -> 59) and dense_few_kernel loses (93 -> 99).
+template <class T, int D, bool NT_K>
 struct FewRows {
   typedef typename T::elem elem;
   typedef typename T::x8 x8;
@@ -69,13 +73,17 @@ struct FewRows {
         const int rr = RP * x + lane / CH;
         const elem *src = vrow(min(r * RK + rr, end - 1)) + CHE * ((lane % CH) ^ swz(rr));
         const uint32_t m0 = lds0 + (uint32_t)(slot * STAGE * (int)sizeof(elem) + x * 1024);
-        asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+        asm volatile("global_load_lds_dwordx4 %0, off nt" ::"v"(src), "{m0}"(m0) : "memory");
       }
 #pragma unroll
       for (int kt = 0; kt < RK / 16; ++kt) {
         const elem *src = krow(min(r * RK + 16 * kt + ri, end - 1));
 #pragma unroll
-        for (int s = 0; s < NK; ++s) kn[kt][s] = *(const x8 *)(src + (F32 ? 16 * s + 4 * c : 32 * s + 8 * c));
+        for (int s = 0; s < NK; ++s) {
+          const x8 *x = (const x8 *)(src + (F32 ? 16 * s + 4 * c : 32 * s + 8 * c));
+          if constexpr (NT_K) kn[kt][s] = __builtin_nontemporal_load(x);
+          else kn[kt][s] = *x;
+        }
       }
     };
     if (first < rounds) fetch(first, 0);
