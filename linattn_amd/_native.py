@@ -330,7 +330,26 @@ def dtype_code(t: torch.dtype) -> int:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    if device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)  # (without a Stream object)
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` the current one, at no cost where it already is (its streams and
+    attributes are what a launch uses)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -22,14 +22,17 @@ __all__ = ["dense_attention", "packed_attention"]
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
+def _rows(t: torch.Tensor, token: int = -2) -> torch.Tensor:
     """``t`` with rows the kernels can load 16 bytes at a time (a copy where they are not
-    contiguous and 16-byte aligned, or very far apart)."""
-    n = 16 // t.element_size()
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and \
-            all(s % n == 0 for s, d in zip(st[:-1], t.shape) if d > 1) and min(st[:-1]) < 1 << 24:
-        return t
+    contiguous and 16-byte aligned, or the rows of dimension ``token`` very far apart)."""
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():  # (head sizes are whole 16-byte chunks)
+            return t
+        n = 16 // t.element_size()
+        st = t.stride()
+        if st[-1] == 1 and st[token] < 1 << 24 and \
+                all(s % n == 0 for s, d in zip(st[:-1], t.shape) if d > 1):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -84,18 +87,20 @@ def _out(what: str, out: Optional[torch.Tensor], q: torch.Tensor,
     return out
 
 
-def _run(what: str, a: N.LaDenseAttnArgs, q, k, v, out, causal, scale) -> None:
-    dev = q.device
-    D = q.shape[-1]
-    a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-    a.D, a.scale, a.causal = D, _scale(scale, D), 1 if causal else 0
-    a.dtype, a.out_dtype = N.dtype_code(q.dtype), N.dtype_code(out.dtype)
-    L = N.load()
-    with torch.cuda.device(dev):
-        nbytes = L.la_dense_attention_workspace(ctypes.byref(a))
-        ws = N.workspace(nbytes, dev)
-        a.workspace, a.ws_bytes = N.ptr(ws), nbytes
-        N.check(L.la_dense_attention(ctypes.byref(a), N.stream_handle(dev)), what)
+def _run(what: str, q, k, v, out, lse, cu_q, cu_k, q_len, k_len, shape, q_s, k_s, v_s, o_s, l_s,
+         causal, scale, zero_rest) -> None:
+    dev, D = q.device, q.shape[-1]
+    a = N.LaDenseAttnArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), N.ptr(lse), N.ptr(cu_q), N.ptr(cu_k),
+        N.ptr(q_len), N.ptr(k_len), None, 0, *shape, D, *q_s, *k_s, *v_s, *o_s, *l_s, _scale(scale, D),
+        1 if causal else 0, N.dtype_code(q.dtype), N.dtype_code(out.dtype), zero_rest, 0)
+    L, ref = N.load(), ctypes.byref(a)
+    with N.on_device(dev):
+        nbytes = L.la_dense_attention_workspace(ref)
+        if nbytes:
+            ws = N.workspace(nbytes, dev)
+            a.workspace, a.ws_bytes = ws.data_ptr(), nbytes
+        N.check(L.la_dense_attention(ref, N.stream_handle(dev)), what)
 
 
 def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = True,
@@ -128,15 +133,8 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=dev) if return_lse else None
     if B > 0 and Tq > 0:
         q, k, v = _rows(q), _rows(k), _rows(v)
-        a = N.LaDenseAttnArgs()
-        a.lse, a.q_len, a.k_len = N.ptr(lse), N.ptr(q_lengths), N.ptr(lengths)
-        a.B, a.Hq, a.Hkv, a.Tq, a.Tk = B, Hq, Hkv, Tq, Tk
-        a.q_sb, a.q_sh, a.q_st = q.stride()[:3]
-        a.k_sb, a.k_sh, a.k_st = k.stride()[:3]
-        a.v_sb, a.v_sh, a.v_st = v.stride()[:3]
-        a.o_sb, a.o_sh, a.o_st = out.stride()[:3]
-        a.l_sb, a.l_sh = Hq * Tq, Tq
-        _run(what, a, q, k, v, out, causal, scale)
+        _run(what, q, k, v, out, lse, None, None, q_lengths, lengths, (B, Hq, Hkv, Tq, Tk), q.stride()[:3],
+             k.stride()[:3], v.stride()[:3], out.stride()[:3], (Hq * Tq, Tq), causal, scale, 0)
     return (out, lse) if return_lse else out
 
 
@@ -174,15 +172,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         lse = torch.empty(Hq, Nq, dtype=torch.float32, device=dev) if zero_rest else \
             torch.full((Hq, Nq), float("-inf"), dtype=torch.float32, device=dev)
     if Nq > 0:
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        a = N.LaDenseAttnArgs()
-        a.lse, a.cu_q, a.cu_k = N.ptr(lse), cu_seqlens.data_ptr(), N.ptr(cu_seqlens_k)
-        a.B, a.Hq, a.Hkv, a.Tq, a.Tk = B, Hq, Hkv, Nq, Nk
-        a.q_st, a.q_sh = q.stride()[:2]
-        a.k_st, a.k_sh = k.stride()[:2]
-        a.v_st, a.v_sh = v.stride()[:2]
-        a.o_st, a.o_sh = out.stride()[:2]
-        a.l_sh = Nq
-        a.zero_rest = 1 if zero_rest else 0
-        _run(what, a, q, k, v, out, causal, scale)
+        q, k, v = _rows(q, 0), _rows(k, 0), _rows(v, 0)
+        (q_t, q_h, _), (k_t, k_h, _), (v_t, v_h, _), (o_t, o_h, _) = (x.stride() for x in (q, k, v, out))
+        _run(what, q, k, v, out, lse, cu_seqlens, cu_seqlens_k, None, None, (B, Hq, Hkv, Nq, Nk), (0, q_h, q_t),
+             (0, k_h, k_t), (0, v_h, v_t), (0, o_h, o_t), (0, Nq), causal, scale, 1 if zero_rest else 0)
     return (out, lse) if return_lse else out

@@ -42,18 +42,20 @@ def _lse(what: str, lse: torch.Tensor, shape) -> torch.Tensor:
     return lse if lse.stride(-1) == 1 else lse.contiguous()
 
 
-def _run_weights(what: str, a: N.LaKeyWeightsArgs, q, k, lse, out, accumulate, causal, scale,
-                 last) -> None:
+def _run_weights(what: str, q, k, lse, out, cu_q, cu_k, q_len, k_len, shape, q_s, k_s, l_s, w_s, last,
+                 causal, scale, accumulate, zero_rest) -> None:
     dev, D = k.device, q.shape[-1]
-    a.q, a.k, a.lse, a.out = q.data_ptr(), k.data_ptr(), lse.data_ptr(), out.data_ptr()
-    a.D, a.scale, a.causal, a.last = D, _scale(scale, D), 1 if causal else 0, last
-    a.dtype, a.accumulate = N.dtype_code(q.dtype), 1 if accumulate else 0
-    L = N.load()
-    with torch.cuda.device(dev):
-        nbytes = L.la_key_weights_workspace(ctypes.byref(a))
-        ws = N.workspace(nbytes, dev)
-        a.workspace, a.ws_bytes = N.ptr(ws), nbytes
-        N.check(L.la_key_weights(ctypes.byref(a), N.stream_handle(dev)), what)
+    a = N.LaKeyWeightsArgs(
+        q.data_ptr(), k.data_ptr(), lse.data_ptr(), out.data_ptr(), N.ptr(cu_q), N.ptr(cu_k), N.ptr(q_len),
+        N.ptr(k_len), None, 0, *shape, D, *q_s, *k_s, *l_s, *w_s, last, _scale(scale, D), 1 if causal else 0,
+        N.dtype_code(q.dtype), 1 if accumulate else 0, zero_rest, 0)
+    L, ref = N.load(), ctypes.byref(a)
+    with N.on_device(dev):
+        nbytes = L.la_key_weights_workspace(ref)
+        if nbytes:
+            ws = N.workspace(nbytes, dev)
+            a.workspace, a.ws_bytes = ws.data_ptr(), nbytes
+        N.check(L.la_key_weights(ref, N.stream_handle(dev)), what)
 
 
 def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, causal: bool = True,
@@ -82,14 +84,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, causal: 
     out = _weights_out(what, out, (B, Hkv, Tk), dev)
     if B > 0 and Tk > 0:
         q, k = _rows(q), _rows(k)
-        a = N.LaKeyWeightsArgs()
-        a.q_len, a.k_len = N.ptr(q_lengths), N.ptr(lengths)
-        a.B, a.Hq, a.Hkv, a.Tq, a.Tk = B, Hq, Hkv, Tq, Tk
-        a.q_sb, a.q_sh, a.q_st = q.stride()[:3]
-        a.k_sb, a.k_sh, a.k_st = k.stride()[:3]
-        a.l_sb, a.l_sh = lse.stride()[:2]
-        a.w_sb, a.w_sh = out.stride()[:2]
-        _run_weights(what, a, q, k, lse, out, accumulate, causal, scale, last)
+        _run_weights(what, q, k, lse, out, None, None, q_lengths, lengths, (B, Hq, Hkv, Tq, Tk), q.stride()[:3],
+                     k.stride()[:3], lse.stride()[:2], out.stride()[:2], last, causal, scale, accumulate, 0)
     return out
 
 
@@ -117,15 +113,11 @@ def packed_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor,
     accumulate = out is not None
     out = _weights_out(what, out, (Hkv, Nk), dev)
     if Nk > 0:
-        q, k = _rows(q), _rows(k)
-        a = N.LaKeyWeightsArgs()
-        a.cu_q, a.cu_k = cu_seqlens.data_ptr(), N.ptr(cu_seqlens_k)
-        a.B, a.Hq, a.Hkv, a.Tq, a.Tk = B, Hq, Hkv, Nq, Nk
-        a.q_st, a.q_sh = q.stride()[:2]
-        a.k_st, a.k_sh = k.stride()[:2]
-        a.l_sh, a.w_sh = lse.stride(0), out.stride(0)
-        a.zero_rest = 0 if accumulate else 1
-        _run_weights(what, a, q, k, lse, out, accumulate, causal, scale, last)
+        q, k = _rows(q, 0), _rows(k, 0)
+        (q_t, q_h, _), (k_t, k_h, _) = q.stride(), k.stride()
+        _run_weights(what, q, k, lse, out, cu_seqlens, cu_seqlens_k, None, None, (B, Hq, Hkv, Nq, Nk), (0, q_h, q_t),
+                     (0, k_h, k_t), (0, lse.stride(0)), (0, out.stride(0)), last, causal, scale, accumulate,
+                     0 if accumulate else 1)
     return out
 
 
@@ -155,12 +147,13 @@ def _run_evict(what: str, a: N.LaEvictArgs, B: int, k, v, weights, budget, recen
         a.pos_out, a.len_out = pos_out.data_ptr(), len_out.data_ptr()
         a.B, a.D, a.esize = B, D, k.element_size()
         a.budget, a.capacity, a.recent, a.sink = budget, capacity, recent, sink
-        L = N.load()
-        with torch.cuda.device(dev):
-            nbytes = L.la_evict_kv_workspace(ctypes.byref(a))
-            ws = N.workspace(nbytes, dev)
-            a.workspace, a.ws_bytes = N.ptr(ws), nbytes
-            N.check(L.la_evict_kv(ctypes.byref(a), N.stream_handle(dev)), what)
+        L, ref = N.load(), ctypes.byref(a)
+        with N.on_device(dev):
+            nbytes = L.la_evict_kv_workspace(ref)
+            if nbytes:
+                ws = N.workspace(nbytes, dev)
+                a.workspace, a.ws_bytes = ws.data_ptr(), nbytes
+            N.check(L.la_evict_kv(ref, N.stream_handle(dev)), what)
     return k_out, v_out, w_out, pos_out, len_out
 
 
@@ -289,21 +282,16 @@ def evict_decode_step(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     if B == 0:
         return out
     q, k_new, v_new = _rows(q), _rows(k_new), _rows(v_new)
-    a = N.LaEvictDecodeArgs()
-    a.q, a.k_new, a.v_new, a.out = q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), out.data_ptr()
-    a.k, a.v, a.weights = k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr()
-    a.positions, a.lengths, a.pos = positions.data_ptr(), lengths.data_ptr(), pos.data_ptr()
-    a.B, a.Hq, a.Hkv, a.C, a.D = B, Hq, Hkv, C, D
-    a.q_sb, a.q_sh = q.stride()[:2]
-    a.kn_sb, a.kn_sh = k_new.stride()[:2]
-    a.vn_sb, a.vn_sh = v_new.stride()[:2]
-    a.o_sb, a.o_sh = out.stride()[:2]
-    a.recent, a.sink, a.scale = recent, sink, _scale(scale, D)
-    a.dtype, a.out_dtype = N.dtype_code(q.dtype), N.dtype_code(out.dtype)
-    L = N.load()
-    with torch.cuda.device(dev):
-        nbytes = L.la_evict_decode_workspace(ctypes.byref(a))
-        ws = N.workspace(nbytes, dev)
-        a.workspace, a.ws_bytes = N.ptr(ws), nbytes
-        N.check(L.la_evict_decode(ctypes.byref(a), N.stream_handle(dev)), what)
+    a = N.LaEvictDecodeArgs(
+        q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        weights.data_ptr(), positions.data_ptr(), lengths.data_ptr(), pos.data_ptr(), out.data_ptr(), None, 0,
+        B, Hq, Hkv, C, D, *q.stride()[:2], *k_new.stride()[:2], *v_new.stride()[:2], *out.stride()[:2], recent,
+        sink, _scale(scale, D), N.dtype_code(q.dtype), N.dtype_code(out.dtype), 0)
+    L, ref = N.load(), ctypes.byref(a)
+    with N.on_device(dev):
+        nbytes = L.la_evict_decode_workspace(ref)
+        if nbytes:
+            ws = N.workspace(nbytes, dev)
+            a.workspace, a.ws_bytes = ws.data_ptr(), nbytes
+        N.check(L.la_evict_decode(ref, N.stream_handle(dev)), what)
     return out
