@@ -12,6 +12,9 @@
 // their keys cost on one CU (100 000 cycles for 65536, measured), so slices of a row have
 // workgroups of their own, and each digit a launch (evict_digit_kernel): the histograms
 // of a row's slices are added by whoever needs the sum, in place of atomics.
+// Slots that are not chosen by weight (the newest tokens, mostly half of the cache) wait
+// for no selection: the selecting launches, which leave the memory idle, copy them in
+// workgroups of their own.
 #include <algorithm>
 
 #include "evict.h"
@@ -32,6 +35,8 @@ struct EvKP {
   uint32_t *ahead;        // [pass][row][slice]: keys of earlier slices that the pass found above
   uint16_t *hist;         // [pass][row][slice][bin]
   int32_t B, Hkv, row16, slices;  // row16: 16-byte chunks of a row
+  int32_t sel;                    // workgroups of a launch that select
+  int32_t open, early;            // blocks of EV_SLOTS slots that wait for the lists, and after them that do not
 };
 
 typedef float ev_f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -73,8 +78,9 @@ __device__ __forceinline__ int32_t ev_slot(const EvRow &r, int32_t s) {
 
 constexpr int EV_SMALL = 2048, EV_MID = 16384, EV_SLOTS = 64;
 
-// Slots s0 .. s0 + ns - 1 of a row, at most EV_SLOTS, by a workgroup of 256: entries at[]
+// Slots s0 .. s0 + ns - 1 of a row, at most EV_SLOTS, by a workgroup of NT: entries at[]
 // (-1: none) of k and v, 16 bytes a lane, four of each in flight; weights and positions.
+template <int NT>
 __device__ __forceinline__ void ev_copy(const EvKP &p, const EvRow &r, int b, int h, const int32_t *at, int32_t s0,
                                         int32_t ns) {
   const int64_t bh = (int64_t)b * p.Hkv + h;
@@ -88,11 +94,11 @@ __device__ __forceinline__ void ev_copy(const EvKP &p, const EvRow &r, int b, in
   const char *vb = p.v + (p.cu ? r.first * p.v_st : b * p.v_sb) + h * p.v_sh;
   const int64_t o0 = 16 * (bh * p.capacity + s0) * p.row16;
   const uint32_t r16 = (uint32_t)p.row16, end = (uint32_t)ns * r16;
-  for (uint32_t x0 = threadIdx.x; x0 < end; x0 += 1024) {
+  for (uint32_t x0 = threadIdx.x; x0 < end; x0 += 4 * NT) {
     uint4 kk[4], vv[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t x = x0 + 256 * j;
+      const uint32_t x = x0 + NT * j;
       const int32_t i = x < end ? at[x / r16] : -1;
       const uint32_t ch = x % r16;
       kk[j] = vv[j] = uint4{0, 0, 0, 0};
@@ -103,13 +109,26 @@ __device__ __forceinline__ void ev_copy(const EvKP &p, const EvRow &r, int b, in
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t x = x0 + 256 * j;
+      const uint32_t x = x0 + NT * j;
       if (x < end) {
         *(uint4 *)(p.k_out + o0 + 16 * (int64_t)x) = kk[j];
         *(uint4 *)(p.v_out + o0 + 16 * (int64_t)x) = vv[j];
       }
     }
   }
+}
+
+// Block x (row by row) of those that wait for no list.
+template <int NT>
+__device__ __forceinline__ void ev_early(const EvKP &p, uint32_t x) {
+  __shared__ int32_t at[EV_SLOTS];
+  const int bh = x / (uint32_t)p.early, blk = p.open + x % (uint32_t)p.early, b = bh / p.Hkv, h = bh % p.Hkv;
+  if (bh >= p.B * p.Hkv) return;
+  const EvRow r = ev_row(p, b, h);
+  const int32_t s0 = blk * EV_SLOTS, ns = (int32_t)min((int64_t)EV_SLOTS, p.capacity - s0);
+  if (threadIdx.x < EV_SLOTS) at[threadIdx.x] = ev_slot(r, s0 + threadIdx.x);
+  __syncthreads();
+  ev_copy<NT>(p, r, b, h, at, s0, ns);
 }
 
 __device__ __forceinline__ uint32_t ev_below(uint64_t m) {  // set bits of lanes before this one
@@ -340,11 +359,15 @@ __global__ __launch_bounds__(256) void evict_small_kernel(EvKP p, int32_t parts)
       if (s >= s0 && s < s0 + ns) at[s - s0] = i;
     });
   __syncthreads();
-  ev_copy(p, r, b, h, at, s0, ns);
+  ev_copy<256>(p, r, b, h, at, s0, ns);
 }
 
 template <bool POS>
 __global__ __launch_bounds__(1024) void evict_select_kernel(EvKP p) {
+  if ((int)blockIdx.x >= p.sel) {
+    ev_early<1024>(p, blockIdx.x - p.sel);
+    return;
+  }
   const int b = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
   const EvRow r = ev_row(p, b, h);
   if (h == 0 && threadIdx.x == 0) p.len_out[b] = r.kept;
@@ -359,6 +382,10 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvKP p) {
 constexpr int EV_BINS = 2048;
 template <int PASS, bool POS>
 __global__ __launch_bounds__(256) void evict_digit_kernel(EvKP p) {
+  if ((int)blockIdx.x >= p.sel) {  // (this launch's share of them)
+    ev_early<256>(p, blockIdx.x - p.sel + PASS * (gridDim.x - p.sel));
+    return;
+  }
   constexpr int COPIES = 4;  // (see ev_choose)
   __shared__ __align__(16) uint32_t hist[PASS < 3 ? EV_BINS * COPIES : 4];
   __shared__ uint32_t part[4][2];
@@ -559,9 +586,9 @@ __global__ __launch_bounds__(256) void evict_digit_kernel(EvKP p) {
   }
 }
 
-__global__ __launch_bounds__(256) void evict_copy_kernel(EvKP p, int32_t blocks) {
+__global__ __launch_bounds__(256) void evict_copy_kernel(EvKP p) {
   __shared__ int32_t at[EV_SLOTS];
-  const int bh = blockIdx.x / blocks, blk = blockIdx.x % blocks, b = bh / p.Hkv, h = bh % p.Hkv;
+  const int bh = blockIdx.x / (uint32_t)p.open, blk = blockIdx.x % (uint32_t)p.open, b = bh / p.Hkv, h = bh % p.Hkv;
   const EvRow r = ev_row(p, b, h);
   const int32_t s0 = blk * EV_SLOTS, ns = (int32_t)min((int64_t)EV_SLOTS, p.capacity - s0);
   if (threadIdx.x < EV_SLOTS) {
@@ -569,7 +596,7 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(EvKP p, int32_t blocks)
     at[threadIdx.x] = s >= r.lead && s < r.kept - r.tail ? p.list[(int64_t)bh * p.budget + s] : ev_slot(r, s);
   }
   __syncthreads();
-  ev_copy(p, r, b, h, at, s0, ns);
+  ev_copy<256>(p, r, b, h, at, s0, ns);
 }
 
 static int ev_check(const la_evict_args *a) {
@@ -643,7 +670,8 @@ extern "C" int la_evict_kv(const la_evict_args *a, void *stream) {
     return fail(LA_ERR_WORKSPACE, "la_evict_kv: workspace %lld < %lld bytes", (long long)a->ws_bytes,
                 (long long)pl.bytes);
   LA_REQUIRE(pl.bytes == 0 || (uintptr_t)a->workspace % 256 == 0, "la_evict_kv: workspace alignment");
-  LA_REQUIRE((int64_t)a->B * a->Hkv * std::max<int64_t>(pl.slices, 1) < ((int64_t)1 << 31), "la_evict_kv: too many entries");
+  LA_REQUIRE(a->B * a->Hkv * (std::max<int64_t>(pl.slices, 1) + ceil_div(a->capacity, EV_SLOTS)) < ((int64_t)1 << 31),
+             "la_evict_kv: too many entries");
   EvKP p{};
   p.k = (const char *)a->k; p.v = (const char *)a->v; p.weights = a->weights;
   p.positions = a->positions; p.pos = a->pos; p.lengths = a->lengths; p.cu = a->cu;
@@ -667,11 +695,17 @@ extern "C" int la_evict_kv(const la_evict_args *a, void *stream) {
     LA_LAUNCHED();
     return LA_OK;
   }
+  // (of a row of more than budget entries; one of fewer has no chosen slots at all)
+  p.open = (int32_t)ceil_div(a->budget - (a->positions ? 0 : a->recent), EV_SLOTS);
+  p.early = parts - p.open;
+  const uint32_t early = rows * (uint32_t)p.early;
   if (a->T <= EV_MID) {
-    if (a->positions) evict_select_kernel<true><<<rows, 1024, 0, st>>>(p);
-    else evict_select_kernel<false><<<rows, 1024, 0, st>>>(p);
+    p.sel = (int32_t)rows;
+    if (a->positions) evict_select_kernel<true><<<rows + early, 1024, 0, st>>>(p);
+    else evict_select_kernel<false><<<rows + early, 1024, 0, st>>>(p);
   } else {
-    const uint32_t grid = rows * (uint32_t)pl.slices;
+    p.sel = (int32_t)(rows * (uint32_t)pl.slices);
+    const uint32_t grid = (uint32_t)p.sel + (early + 3) / 4;
     if (a->positions) {
       evict_digit_kernel<0, true><<<grid, 256, 0, st>>>(p);
       evict_digit_kernel<1, true><<<grid, 256, 0, st>>>(p);
@@ -685,7 +719,9 @@ extern "C" int la_evict_kv(const la_evict_args *a, void *stream) {
     }
   }
   LA_LAUNCHED();
-  evict_copy_kernel<<<rows * (uint32_t)parts, 256, 0, st>>>(p, parts);
-  LA_LAUNCHED();
+  if (p.open > 0) {
+    evict_copy_kernel<<<rows * (uint32_t)p.open, 256, 0, st>>>(p);
+    LA_LAUNCHED();
+  }
   return LA_OK;
 }
