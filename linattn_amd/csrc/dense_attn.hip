@@ -314,14 +314,18 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
         for (int i = 0; i < 16; ++i) acc[dt][i] *= alpha;
     }
   };
-  // weights of half kt of a tile, and their product with V
+  // weights of half kt of a tile, and their product with V.  The half's weights are added
+  // among themselves first: over 32768 keys one long chain of additions loses more than
+  // all other roundings of the log-sum.
   auto weigh = [&](f32x16 &st, x8 (&pw)[2]) __attribute__((always_inline)) {
+    float part[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       st[i] = fast_exp2(__builtin_fmaf(st[i], p.qscale, nmu));
-      l += st[i];
+      part[i & 1] = i < 2 ? st[i] : part[i & 1] + st[i];
       pw[i >> 3][i & 7] = (elem)st[i];
     }
+    l += part[0] + part[1];
   };
   auto values = [&](int j, int kt, const x8 (&pw)[2]) __attribute__((always_inline)) {
     const uint32_t at = v_at;
@@ -392,7 +396,7 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
       for (int i = 0; i < 4; ++i)
         da_store4(p.out, o + 32 * dt + 8 * i, p.out_dt, acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv,
                   acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv);
-    if (p.lse && hf == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (m * p.qscale + __log2f(l)) * DA_LN2;
+    if (p.lse && hf == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (__log2f(l) - nmu) * DA_LN2;  // (as rounded in the weights)
   }
   if (bad != 0)
     da_again<elem, D, 32>(p, tl, kvh, split, r_first, (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
@@ -506,18 +510,20 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
 #pragma unroll
       for (int dt = 0; dt < NS; ++dt) acc[dt] *= alpha;
     }
+    float part = 0.f;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float pr = fast_exp2(__builtin_fmaf(st[kt][e], p.qscale, nmu));
-        l += pr;
+        part += pr;
         const int kr = 16 * kt + 4 * c + e;
 #pragma unroll
         for (int dt = 0; dt < NS; ++dt)
           acc[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(
               sv[kr * D + 4 * ((4 * dt + (ri >> 2)) ^ swz_v(kr)) + (ri & 3)], pr, acc[dt], 0, 0, 0);
       }
+    l += part;
   }
   if (!wave_live) return;
   l = pair32_sum(pair16_sum(l));
@@ -544,7 +550,7 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
 #pragma unroll
     for (int dt = 0; dt < NS; ++dt)
       da_store4(p.out, o + 16 * dt, p.out_dt, acc[dt][0] * inv, acc[dt][1] * inv, acc[dt][2] * inv, acc[dt][3] * inv);
-    if (p.lse && c == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (m * p.qscale + __log2f(l)) * DA_LN2;
+    if (p.lse && c == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (__log2f(l) - nmu) * DA_LN2;
   }
   if (bad != 0) {
     bad |= bad >> 32;

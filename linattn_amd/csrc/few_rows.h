@@ -137,13 +137,15 @@ struct FewRows {
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) acc[dt] *= alpha;
       }
+      float part = 0.f;  // (a round's among themselves first: fewer roundings in l)
 #pragma unroll
       for (int kt = 0; kt < RK / 16; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           st[kt][e] = fast_exp2(st[kt][e] + nmu);
-          l += st[kt][e];
+          part += st[kt][e];
         }
+      l += part;
       const elem *sv = smem + slot * STAGE;
       if constexpr (F32) {
 #pragma unroll

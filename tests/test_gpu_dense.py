@@ -257,3 +257,25 @@ def test_streams_and_graph_replays(dev):
         eager, eager_lse = dense_attention(q, k, v, lengths=lengths, return_lse=True)
         assert torch.equal(out, eager) and torch.equal(lse, eager_lse)
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Tq", [1, 32])
+@pytest.mark.parametrize("gap", [0.25, 0.5, 1.1])
+def test_log_sum_of_equal_weights(dtype, Tq, gap):
+    """The first key's score is `gap` above all others', which are equal: a running sum that
+    took the equal weights one by one would drift by up to half a step of the sum for each."""
+    dev, n, D = "cuda", 20000, 64
+    q, k = torch.zeros(1, 1, Tq, D), torch.zeros(1, 1, n, D)
+    q[..., 0] = 1.0
+    k[..., 0, 0] = gap
+    q, k = q.to(dtype), k.to(dtype)
+    out, lse = dense_attention(q.to(dev), k.to(dev), torch.ones_like(k).to(dev), causal=False, scale=1.0,
+                               out_dtype=torch.float32, return_lse=True)
+    want = math.log(math.exp(float(k[0, 0, 0, 0])) + n - 1.0)
+    # a lane's share, n / 2 or fewer, in parts of 8 and more: n / 16 additions, 16 more within
+    # the parts and between lanes; a few steps of exp2, log2 and the scores
+    tol = (n / 16 + 24 + 2 * want) * 2.0 ** -24
+    assert (lse.double().cpu() - want).abs().max() <= tol
+    # O sums products of 4 (fp32) or more keys, each weight rounded to the inputs' type
+    assert (out.double().cpu() - 1.0).abs().max() <= torch.finfo(dtype).eps / 2 + tol + (n / 4 + 24) * 2.0 ** -24
