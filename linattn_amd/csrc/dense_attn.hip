@@ -757,7 +757,8 @@ extern "C" int la_dense_attention(const la_dense_attn_args *a, void *stream) {
   if (int rc = da_rows_ok("q", a->q, esz, sb(a->q_sb), a->q_sh, a->q_st, a->Hq, a->Tq)) return rc;
   if (a->Tk > 0) {
     if (int rc = da_rows_ok("k", a->k, esz, sb(a->k_sb), a->k_sh, a->k_st, a->Hkv, a->Tk)) return rc;
-    LA_REQUIRE(a->k_st < (1 << 24) && a->v_st < (1 << 24), "la_dense_attention: key rows 2^24 values apart or more");
+    LA_REQUIRE(a->Tk == 1 || (a->k_st >= 0 && a->v_st >= 0 && a->k_st < (1 << 24) && a->v_st < (1 << 24)),
+               "la_dense_attention: key rows 2^24 values apart or more");
     if (int rc = da_rows_ok("v", a->v, esz, sb(a->v_sb), a->v_sh, a->v_st, a->Hkv, a->Tk)) return rc;
   }
   if (int rc = da_rows_ok("out", a->out, osz, sb(a->o_sb), a->o_sh, a->o_st, a->Hq, a->Tq)) return rc;

@@ -20,34 +20,40 @@ struct KwKP {
   float *out, *ws;  // ws: [split][what out has, densely]
   int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, l_sb, l_sh, w_sb, w_sh, last, ws_split;
   int32_t Hq, Hkv, ntile, splits, causal, accumulate, zero_rest;
+  int32_t ms;  // log2 of the heads in a staged tile of rows
   float qscale;
 };
 
-// A tile's keys and the rows it walks.
+// A tile's keys, and the staged tiles of rows it walks: 2^ms heads by RT / 2^ms queries
+// each, from query t0 on, a group of heads after the other.
 struct KwTile {
-  DaTile t;             // sequence (q0, k0, lq, lk as given), b < 0: none
-  int32_t s0;           // first key
-  int32_t row0, row1;   // this split's rows (query, head)
+  DaTile t;       // sequence (q0, k0, lq, lk as given), b < 0: none
+  int32_t s0;     // first key
+  int32_t t0, n;  // first query; this split's staged tiles
+  int32_t tb, g;  // query and head of the group that the first of them begins with
 };
 
-template <int KT>
+template <int KT, int RT>
 __device__ __forceinline__ KwTile kw_tile(const KwKP &p, int tix, int split) {
   KwTile x;
   x.t = da_uniform(da_tile(p.s, tix, p.ntile, KT, true));
-  x.s0 = x.row0 = x.row1 = 0;
+  x.s0 = x.t0 = x.n = x.tb = x.g = 0;
   if (x.t.b < 0) return x;
   // da_tile's first tiles are the sequences' last; the first keys are seen by most rows
   const int32_t n = p.s.cu_q ? x.t.lk : (int32_t)p.s.Tk;
   x.s0 = ((n + KT - 1) / KT) * KT - KT - x.t.r0;
   if (x.s0 >= x.t.lk) return x;
-  const int G = p.s.G, diag = x.t.lk - x.t.lq;
-  int32_t t0 = p.last > 0 ? (int32_t)max((int64_t)x.t.lq - p.last, (int64_t)0) : 0;
-  if (p.causal) t0 = max(t0, x.s0 - diag);
-  const int32_t rows = max(x.t.lq - t0, 0) * G;
-  // parts of whole staged tiles
-  const int32_t per = (int32_t)(((uint32_t)rows + 64u * p.splits - 1u) / (64u * p.splits)) * 64;
-  x.row0 = t0 * G + min(per * split, rows);
-  x.row1 = t0 * G + min(per * (split + 1), rows);
+  x.t0 = p.last > 0 ? (int32_t)max((int64_t)x.t.lq - p.last, (int64_t)0) : 0;
+  if (p.causal) x.t0 = max(x.t0, x.s0 - (x.t.lk - x.t.lq));
+  const int qpt = RT >> p.ms;
+  const uint32_t ntq = (uint32_t)(max(x.t.lq - x.t0, 0) + qpt - 1) / (uint32_t)qpt;
+  const uint32_t all = ntq * (uint32_t)(p.s.G >> p.ms), per = (all + p.splits - 1) / p.splits;
+  const uint32_t i0 = min(per * split, all), i1 = min(i0 + per, all);
+  x.n = __builtin_amdgcn_readfirstlane(i1 - i0);
+  x.t0 = __builtin_amdgcn_readfirstlane(x.t0);
+  if (x.n == 0) return x;
+  x.g = __builtin_amdgcn_readfirstlane((i0 / ntq) << p.ms);
+  x.tb = __builtin_amdgcn_readfirstlane(x.t0 + (int)(i0 % ntq) * qpt);
   return x;
 }
 
@@ -77,20 +83,14 @@ __device__ __forceinline__ void kw_rest(const KwKP &p, const KwTile &x, int kvh,
     p.out[kvh * p.w_sh + (i < first ? i : i + last - first)] = 0.f;
 }
 
-// Row r as (query, head of the group), moved on without dividing again.
-struct KwRow {
-  int32_t t, g;
-  KwRow() = default;
-  __device__ __forceinline__ KwRow(int32_t r, int G) : t(r / G), g(r % G) {}
-  __device__ __forceinline__ void step(int32_t dt, int32_t dg, int G) {
-    t += dt;
-    g += dg;
-    if (g >= G) {
-      g -= G;
-      ++t;
-    }
+// The next staged tile of queries tb .. and heads g ..
+__device__ __forceinline__ void kw_next(const KwKP &p, const KwTile &x, int qpt, int &tb, int &g) {
+  tb += qpt;
+  if (tb >= x.t.lq) {
+    tb = x.t0;
+    g += 1 << p.ms;
   }
-};
+}
 
 // bf16 / fp16: four waves of 64 keys.  Rows are staged 64 at a time by LDS-DMA, with their
 // lse (each wave its own copy, so that every wave counts the same loads), NSLOT - 1 tiles
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
   uint32_t stream, tix;
   da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
-  const KwTile x = kw_tile<KT>(p, (int)tix, split);
+  const KwTile x = kw_tile<KT, DA_BS>(p, (int)tix, split);
   kw_rest(p, x, kvh, split, (int)tix);
   if (x.t.b < 0) return;
 
@@ -121,55 +121,45 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
 
-  const int nrow = x.row1 - x.row0;
-  if (nrow > 0) {
+  const int n = x.n, qs = 6 - p.ms, qpt = 1 << qs;
+  if (n > 0) {
     const elem *qbh = (const elem *)p.q + (p.s.cu_q ? x.t.q0 * p.q_st : x.t.b * p.q_sb) + kvh * G * p.q_sh;
     const float *lbh = p.lse + (p.s.cu_q ? x.t.q0 : x.t.b * p.l_sb) + kvh * G * p.l_sh;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
     const uint32_t ldl0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)s_lse);
-    // the rows this lane copies: of q, RP (NW i + w) + lane / CH, and one row's lse; moved
-    // on by 64 rows a tile (dt queries and dg heads, wrapping at the group), past the end
-    // the last one
-    const int dt = DA_BS / G, dg = DA_BS % G;
-    const KwRow end(x.row1 - 1, G);
-    const int64_t q_step = dt * p.q_st + dg * p.q_sh, q_wrap = p.q_st - G * p.q_sh;
-    const int64_t l_step = dt + dg * p.l_sh, l_wrap = 1 - G * p.l_sh;
-    const elem *q_end = qbh + end.t * p.q_st + end.g * p.q_sh;
-    const elem *q_ptr[NX];
-    int q_g[NX];
+    // what this lane copies of a staged tile, from a scalar base: of q, rows RP (NW i + w) +
+    // lane / CH, and one row's lse; queries past the last are copies of it
+    uint32_t qo[NX];
 #pragma unroll
     for (int i = 0; i < NX; ++i) {
-      const KwRow r(x.row0 + RP * (NW * i + w) + lane / CH, G);
-      q_ptr[i] = qbh + r.t * p.q_st + r.g * p.q_sh;
-      q_g[i] = r.g;
+      const int rr = RP * (NW * i + w) + lane / CH;
+      qo[i] = 2u * (uint32_t)((rr & (qpt - 1)) * p.q_st + (rr >> qs) * p.q_sh + 8 * ((lane % CH) ^ da_swz_k<D>(rr)));
     }
-    const KwRow r0(x.row0 + lane, G);
-    const float *l_ptr = lbh + r0.t + r0.g * p.l_sh, *l_end = lbh + end.t + end.g * p.l_sh;
-    int l_g = r0.g, left = x.row1 - x.row0;  // rows from this tile on
-    auto dma = [&](int slot) {  // the next tile
+    const uint32_t lo = 4u * (uint32_t)((lane & (qpt - 1)) + (lane >> qs) * p.l_sh);
+    int d_tb = x.tb, d_g = x.g;
+    auto dma = [&](int slot) __attribute__((always_inline)) {  // the next tile
+      const elem *qb = da_scalar(qbh + d_tb * p.q_st + d_g * p.q_sh);
+      const float *lb = da_scalar(lbh + d_tb + d_g * p.l_sh);
+      const int last = x.t.lq - 1 - d_tb;
+      if (last >= qpt - 1) {
 #pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        const int u = NW * i + w, rr = RP * u + lane / CH;
-        const elem *src = (rr < left ? q_ptr[i] : q_end) + 8 * ((lane % CH) ^ da_swz_k<D>(rr));
-        asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(lds0 + 2 * (slot * BLK + u * 512)) : "memory");
-        q_g[i] += dg;
-        q_ptr[i] += q_step;
-        if (q_g[i] >= G) {
-          q_g[i] -= G;
-          q_ptr[i] += q_wrap;
+        for (int i = 0; i < NX; ++i)
+          asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(qo[i]), "s"(qb),
+                       "{m0}"(lds0 + 2 * (slot * BLK + (NW * i + w) * 512)) : "memory");
+        asm volatile("global_load_lds_dword %0, %1" ::"v"(lo), "s"(lb),
+                     "{m0}"(ldl0 + 4 * ((slot * NW + w) * DA_BS)) : "memory");
+      } else {
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+          const int past = max(((RP * (NW * i + w) + lane / CH) & (qpt - 1)) - last, 0);
+          asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(qo[i] - past * (uint32_t)p.q_st * 2u), "s"(qb),
+                       "{m0}"(lds0 + 2 * (slot * BLK + (NW * i + w) * 512)) : "memory");
         }
+        asm volatile("global_load_lds_dword %0, %1" ::"v"(lo - 4u * (uint32_t)max((lane & (qpt - 1)) - last, 0)), "s"(lb),
+                     "{m0}"(ldl0 + 4 * ((slot * NW + w) * DA_BS)) : "memory");
       }
-      asm volatile("global_load_lds_dword %0, off" ::"v"(lane < left ? l_ptr : l_end),
-                   "{m0}"(ldl0 + 4 * ((slot * NW + w) * DA_BS)) : "memory");
-      l_g += dg;
-      l_ptr += l_step;
-      if (l_g >= G) {
-        l_g -= G;
-        l_ptr += l_wrap;
-      }
-      left -= DA_BS;
+      kw_next(p, x, qpt, d_tb, d_g);
     };
-    const int n = (nrow + DA_BS - 1) / DA_BS;
     x8 kf[2][NS];  // A operand: key 32 kt + r32, dims 16 s + 8 hf ..
     const elem *kbh = (const elem *)p.k + (p.s.cu_q ? x.t.k0 * p.k_st : x.t.b * p.k_sb) + kvh * p.k_sh;
 #pragma unroll
@@ -181,9 +171,10 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
     for (int j = 0; j < NSLOT - 1; ++j) {
       if (j < n) dma(j);
     }
-    // rows from these on see any, and all, of the wave's keys
-    const int row_any = p.causal ? max(s_w - diag, 0) * G : 0;
-    const int row_all = p.causal ? max(s_w + 63 - diag, 0) * G : s_w + 63 < x.t.lk ? 0 : INT32_MAX;
+    // queries from these on see any, and all, of the wave's keys
+    const int t_any = p.causal ? s_w - diag : 0;
+    const int t_all = p.causal ? s_w + 63 - diag : s_w + 63 < x.t.lk ? 0 : INT32_MAX;
+    int tb = x.tb, g = x.g;
     // products of a half of the staged rows; -lse of its rows in log2 units (-inf: adds nothing)
     auto products = [&](int j, int h, f32x16 (&st)[2]) __attribute__((always_inline)) -> float {
       const uint16_t *sq = smem + (j % NSLOT) * BLK;
@@ -230,9 +221,9 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float nl = products(j, h, sa);
-        const int row = x.row0 + j * DA_BS + 32 * h + r32;
-        if (row >= x.row1) nl = none;
-        const int seen = p.causal ? diag + min(row, x.row1 - 1) / G : x.t.lk - 1;
+        const int t = tb + ((32 * h + r32) & (qpt - 1));
+        if (t >= x.t.lq) nl = none;
+        const int seen = p.causal ? diag + t : x.t.lk - 1;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           // register i: key 8 (i / 4) + 4 hf + i % 4
@@ -250,15 +241,15 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
 #pragma unroll
       for (int s = 0; s < NS; ++s) settle(kf[kt][s]);  // (here, not in the loop, where it would wait for all tiles)
     constexpr int PER = NX + 1;  // loads of a tile
-    for (int j = 0; j < n; ++j) {
+    for (int j = 0; j < n; ++j, kw_next(p, x, qpt, tb, g)) {
       // tile j has landed: the loads after it are those of the tiles ahead
       if (j + 2 < n) wait_vmcnt<2 * PER>();
       else if (j + 1 < n) wait_vmcnt<PER>();
       else wait_vmcnt<0>();
       lds_barrier();  // for every wave, and tile j - 1 is read
       if (j + NSLOT - 1 < n) dma((j + NSLOT - 1) % NSLOT);
-      if (x.row0 + (j + 1) * DA_BS <= row_any) continue;
-      const bool whole = row_all <= x.row0 + j * DA_BS && (j + 1) * DA_BS <= nrow;
+      if (tb + qpt <= t_any) continue;
+      const bool whole = t_all <= tb && tb + qpt <= x.t.lq;
       if (whole) {
         const float na = products(j, 0, sa);
         weigh(sb, nb);
@@ -306,13 +297,13 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
   uint32_t stream, tix;
   da_stream(blockIdx.x, (uint32_t)p.Hkv * p.splits, stream, tix);
   const int kvh = (int)(stream / (uint32_t)p.splits), split = (int)(stream % (uint32_t)p.splits);
-  const KwTile x = kw_tile<KT>(p, (int)tix, split);
+  const KwTile x = kw_tile<KT, BS>(p, (int)tix, split);
   kw_rest(p, x, kvh, split, (int)tix);
   if (x.t.b < 0) return;
   const int s_w = x.s0 + 32 * w, diag = x.t.lk - x.t.lq;
   f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-  const int nrow = x.row1 - x.row0;
-  if (nrow > 0) {
+  const int n = x.n, qs = 5 - p.ms, qpt = 1 << qs;
+  if (n > 0) {
     f32x4 kf[2][NS];
     const float *kbh = (const float *)p.k + (p.s.cu_q ? x.t.k0 * p.k_st : x.t.b * p.k_sb) + kvh * p.k_sh;
 #pragma unroll
@@ -324,33 +315,33 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
     const float *qbh = (const float *)p.q + (p.s.cu_q ? x.t.q0 * p.q_st : x.t.b * p.q_sb) + kvh * G * p.q_sh;
     const float *lbh = p.lse + (p.s.cu_q ? x.t.q0 : x.t.b * p.l_sb) + kvh * G * p.l_sh;
     auto swz = [](int r) { return 2 * (r & 7); };
-    auto dma = [&](int j, int slot) {
+    int d_tb = x.tb, d_g = x.g, tb = x.tb, g = x.g;
+    auto dma = [&](int slot) {  // the next tile
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
         const int u = NW * i + w, rr = RP * u + lane / CH;
-        const KwRow r(min(x.row0 + j * BS + rr, x.row1 - 1), G);
-        dma16(qbh + r.t * p.q_st + r.g * p.q_sh + 4 * ((lane % CH) ^ swz(rr)), smem + slot * BLK + u * 256);
+        const int t = min(d_tb + (rr & (qpt - 1)), x.t.lq - 1);
+        dma16(qbh + t * p.q_st + (d_g + (rr >> qs)) * p.q_sh + 4 * ((lane % CH) ^ swz(rr)), smem + slot * BLK + u * 256);
       }
+      kw_next(p, x, qpt, d_tb, d_g);
     };
-    const int n = (nrow + BS - 1) / BS;
-    dma(0, 0);
-    for (int j = 0; j < n; ++j) {
+    dma(0);
+    for (int j = 0; j < n; ++j, kw_next(p, x, qpt, tb, g)) {
       float nl[2];
       int seen[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int rr = x.row0 + j * BS + 16 * h + ri;
-        const KwRow r(min(rr, x.row1 - 1), G);
-        const float l = lbh[r.t + r.g * p.l_sh];
-        nl[h] = rr < x.row1 && l != __int_as_float(0xff800000) ? -l * 1.44269504088896340736f
+        const int rr = 16 * h + ri, t = tb + (rr & (qpt - 1));
+        const float l = lbh[min(t, x.t.lq - 1) + (g + (rr >> qs)) * p.l_sh];
+        nl[h] = t < x.t.lq && l != __int_as_float(0xff800000) ? -l * 1.44269504088896340736f
                                                               : __int_as_float(0xff800000);
-        seen[h] = p.causal ? diag + r.t : x.t.lk - 1;
+        seen[h] = p.causal ? diag + t : x.t.lk - 1;
       }
       wait_vmcnt<0>();
       settle(nl[0]);
       settle(nl[1]);
       lds_barrier();
-      if (j + 1 < n) dma(j + 1, (j + 1) & 1);
+      if (j + 1 < n) dma((j + 1) & 1);
       const float *sq = smem + (j & 1) * BLK;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -461,6 +452,7 @@ extern "C" int la_key_weights(const la_key_weights_args *a, void *stream) {
   LA_REQUIRE(ok(a->k, a->k_sb, a->k_sh, a->k_st, a->Hkv, a->Tk) &&
                  (a->Tq == 0 || ok(a->q, a->q_sb, a->q_sh, a->q_st, a->Hq, a->Tq)),
              "la_key_weights: rows of q and k must be 16-byte aligned");
+  LA_REQUIRE(a->Tq <= 1 || (a->q_st >= 0 && a->q_st < (1 << 24)), "la_key_weights: query rows 2^24 values apart or more");
   const KwPlan pl = kw_plan(a);
   if (pl.bytes > 0 && (!a->workspace || a->ws_bytes < (int64_t)pl.bytes))
     return fail(LA_ERR_WORKSPACE, "la_key_weights: workspace %lld < %lld bytes", (long long)a->ws_bytes,
@@ -479,6 +471,13 @@ extern "C" int la_key_weights(const la_key_weights_args *a, void *stream) {
   p.ntile = (int32_t)pl.ntile; p.splits = (int32_t)pl.splits;
   p.causal = a->causal != 0; p.accumulate = a->accumulate != 0; p.zero_rest = a->zero_rest != 0 && !a->accumulate;
   p.qscale = a->scale * 1.44269504088896340736f;
+  // up to four heads a staged tile, so that short or causal ranges of queries fill it; where
+  // the heads are too far apart for 32-bit offsets, one
+  auto fits = [&](int64_t m) {
+    return p.s.G % m == 0 && a->q_sh >= 0 && (64 / m - 1) * a->q_st + (m - 1) * a->q_sh < ((int64_t)1 << 30) &&
+           a->l_sh >= 0 && (m - 1) * a->l_sh < ((int64_t)1 << 28);
+  };
+  p.ms = fits(4) ? 2 : fits(2) ? 1 : 0;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((uint32_t)wgs);
   if (a->dtype == LA_F32) {
