@@ -69,8 +69,22 @@ def _check_qk(what: str, q: torch.Tensor, k: torch.Tensor, dims: int, head: int)
         raise ValueError(f"{what}: the query heads must be a multiple of the KV heads")
 
 
+def _apart(what: str, out: torch.Tensor, *inputs: torch.Tensor) -> None:
+    """Refuses an ``out`` that holds a row twice, starts where an input does, or whose memory
+    is part of a contiguous input's (views that interleave with ``out`` pass)."""
+    if out.numel() == 0:
+        return
+    if any(s == 0 and d > 1 for s, d in zip(out.stride(), out.shape)):
+        raise ValueError(f"{what}: out holds some of its rows twice")
+    span = lambda t: t.data_ptr() + t.element_size() * (1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride())))
+    a, e, whole = out.data_ptr(), span(out), out.is_contiguous()
+    for t in inputs:
+        if t.numel() and (t.data_ptr() == a or (t.data_ptr() < e and a < span(t) and whole and t.is_contiguous())):
+            raise ValueError(f"{what}: out shares memory with an input")
+
+
 def _out(what: str, out: Optional[torch.Tensor], q: torch.Tensor,
-         out_dtype: Optional[torch.dtype]) -> torch.Tensor:
+         out_dtype: Optional[torch.dtype], *inputs: torch.Tensor) -> torch.Tensor:
     """(out, or a new one, checked)."""
     if out is None:
         dt = out_dtype or q.dtype
@@ -84,6 +98,7 @@ def _out(what: str, out: Optional[torch.Tensor], q: torch.Tensor,
     if out.stride(-1) != 1 or out.data_ptr() % 16 or \
             any(s % n for s, d in zip(out.stride()[:-1], out.shape) if d > 1):
         raise ValueError(f"{what}: rows of out must be contiguous and 16-byte aligned")
+    _apart(what, out, q, *inputs)
     return out
 
 
@@ -116,8 +131,8 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     the queries are the last of the keys' positions: query t of a sequence sees keys
     0 .. lengths - q_lengths + t (a prompt: both lengths; a chunk or one token behind a
     cache: the keys' alone).  Returns (B, Hq, Tq, D) in ``out_dtype`` (default q's, or
-    float32), or in ``out``, and with ``return_lse`` also the rows' log sums of exponentials
-    (B, Hq, Tq) in float32.  A query that sees no key, and one past ``q_lengths``, gets
+    float32), or in ``out`` (which shares no memory with the inputs), and with ``return_lse``
+    also the rows' log sums of exponentials (B, Hq, Tq) in float32.  A query that sees no key, and one past ``q_lengths``, gets
     zeros and -inf.  Infinities and NaN a query does not see do not reach it.  Forward
     only: no gradient is recorded."""
     what = "dense_attention"
@@ -129,7 +144,7 @@ def dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
         raise ValueError(f"{what}: k and v must be (B, Hkv, Tk, D) in q's batch and dtype")
     lengths = _int32(lengths, (B,), "lengths")
     q_lengths = _int32(q_lengths, (B,), "q_lengths")
-    out = _out(what, out, q, out_dtype)
+    out = _out(what, out, q, out_dtype, k, v)
     lse = torch.empty(B, Hq, Tq, dtype=torch.float32, device=dev) if return_lse else None
     if B > 0 and Tq > 0:
         q, k, v = _rows(q), _rows(k), _rows(v)
@@ -166,7 +181,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     elif Nk != Nq:
         raise ValueError(f"{what}: k has other rows than q: pass cu_seqlens_k")
     zero_rest = out is None
-    out = _out(what, out, q, out_dtype)
+    out = _out(what, out, q, out_dtype, k, v)
     lse = None
     if return_lse:  # (where out's rows are left, so would the lse's be)
         lse = torch.empty(Hq, Nq, dtype=torch.float32, device=dev) if zero_rest else \

@@ -16,7 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from linattn_amd import _native as N
-from linattn_amd.kernels.dense import _TYPES, _check_qk, _cu, _int32, _out, _rows, _scale
+from linattn_amd.kernels.dense import _TYPES, _apart, _check_qk, _cu, _int32, _out, _rows, _scale
 
 __all__ = ["key_weights", "packed_key_weights", "evict_kv", "packed_evict_kv", "evict_decode_step"]
 
@@ -27,12 +27,13 @@ def _last(last: Optional[int]) -> int:
     return last or 0
 
 
-def _weights_out(what: str, out: Optional[torch.Tensor], shape, dev) -> torch.Tensor:
+def _weights_out(what: str, out: Optional[torch.Tensor], shape, dev, *inputs) -> torch.Tensor:
     if out is None:
         return torch.empty(shape, dtype=torch.float32, device=dev)
     if out.dtype != torch.float32 or tuple(out.shape) != tuple(shape) or \
             (out.stride(-1) != 1 and out.shape[-1] > 1):
         raise ValueError(f"{what}: out must be float32 {tuple(shape)} with unit stride over the keys")
+    _apart(what, out, *inputs)
     return out
 
 
@@ -81,7 +82,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, causal: 
     lengths = _int32(lengths, (B,), "lengths")
     q_lengths = _int32(q_lengths, (B,), "q_lengths")
     accumulate = out is not None
-    out = _weights_out(what, out, (B, Hkv, Tk), dev)
+    out = _weights_out(what, out, (B, Hkv, Tk), dev, q, k, lse)
     if B > 0 and Tk > 0:
         q, k = _rows(q), _rows(k)
         _run_weights(what, q, k, lse, out, None, None, q_lengths, lengths, (B, Hq, Hkv, Tq, Tk), q.stride()[:3],
@@ -111,7 +112,7 @@ def packed_key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor,
         raise ValueError(f"{what}: k has other rows than q: pass cu_seqlens_k")
     lse = _lse(what, lse, (Hq, Nq))
     accumulate = out is not None
-    out = _weights_out(what, out, (Hkv, Nk), dev)
+    out = _weights_out(what, out, (Hkv, Nk), dev, q, k, lse)
     if Nk > 0:
         q, k = _rows(q, 0), _rows(k, 0)
         (q_t, q_h, _), (k_t, k_h, _) = q.stride(), k.stride()
@@ -278,7 +279,10 @@ def evict_decode_step(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     lengths, pos = _int32(lengths, (B,), "lengths"), _int32(pos, (B,), "pos")
     if recent < 0 or sink < 0 or recent + sink >= C:
         raise ValueError(f"{what}: sink + recent must leave an entry of the cache to evict")
-    out = _out(what, out, q, out_dtype)
+    if B > 0 and (k_cache.data_ptr() == v_cache.data_ptr() or weights.data_ptr() == positions.data_ptr() or
+                  {k_new.data_ptr(), v_new.data_ptr()} & {k_cache.data_ptr(), v_cache.data_ptr()}):
+        raise ValueError(f"{what}: caches, weights, positions and the new rows share memory")
+    out = _out(what, out, q, out_dtype, k_new, v_new, k_cache, v_cache, weights, positions)
     if B == 0:
         return out
     q, k_new, v_new = _rows(q), _rows(k_new), _rows(v_new)

@@ -78,6 +78,21 @@ def test_packed_attention_refuses(as_gpu, change):
         packed_attention(**a)
 
 
+def test_outputs_that_share_memory_are_refused(as_gpu):
+    q, kv = torch.zeros(2, 4, 8, 64), torch.zeros(2, 2, 8, 64)
+    for out in (q, q[:, :, :, :], torch.zeros(1, 4, 8, 64).expand(2, 4, 8, 64)):
+        with pytest.raises(ValueError, match="shares memory|twice"):
+            dense_attention(q, kv, kv.clone(), out=out)
+    whole = torch.zeros(3 * 8, 2, 64)  # q and out overlap by eight rows
+    cu = torch.tensor([0, 16], dtype=torch.int32)
+    k = torch.zeros(16, 2, 64)
+    with pytest.raises(ValueError, match="shares memory"):
+        packed_attention(whole[:16], k, k.clone(), cu, out=whole[8:])
+    both = torch.zeros(16, 4, 64)  # heads of one buffer, interleaved: no row is shared
+    with pytest.raises(AssertionError, match="not refused"):
+        packed_attention(both[:, :2], k, k.clone(), cu, out=both[:, 2:])
+
+
 @pytest.mark.parametrize("scale", [0.0, -1.0, math.inf, math.nan])
 def test_scale_is_positive(scale):
     with pytest.raises(ValueError):

@@ -103,12 +103,30 @@ def test_packed_evict_kv_refuses(as_gpu):
 ])
 def test_evict_decode_step_refuses(as_gpu, change):
     c = torch.zeros(2, 2, 9, 64)
-    a = dict(q=torch.zeros(2, 4, 1, 64), k_new=c[:, :, :1], v_new=c[:, :, :1], k_cache=c, v_cache=c.clone(),
+    a = dict(q=torch.zeros(2, 4, 1, 64), k_new=c[:, :, :1].clone(), v_new=c[:, :, :1].clone(), k_cache=c, v_cache=c.clone(),
              weights=torch.zeros(2, 2, 9), positions=torch.zeros(2, 2, 9, dtype=torch.int32), lengths=_i32(1, 2), pos=_i32(1, 2),
              recent=4, sink=2)
     a.update(change)
     with pytest.raises(ValueError):
         evict_decode_step(**a)
+
+
+def test_arguments_that_share_memory_are_refused(as_gpu):
+    c, w = torch.zeros(2, 2, 9, 64), torch.zeros(2, 2, 9)
+    new = torch.zeros(2, 2, 1, 64)
+    a = dict(q=torch.zeros(2, 2, 1, 64), k_new=new, v_new=new, k_cache=c, v_cache=c.clone(), weights=w,
+             positions=torch.zeros(2, 2, 9, dtype=torch.int32), lengths=_i32(1, 2), pos=_i32(1, 2), recent=4, sink=2)
+    for change in (dict(v_cache=c), dict(k_new=c[:, :, :1]), dict(v_new=c[:, :, :1]), dict(positions=w.view(torch.int32)),
+                   dict(out=a["q"]), dict(out=new), dict(out=torch.zeros(1, 2, 1, 64).expand(2, 2, 1, 64)),
+                   dict(out=c.view(-1)[128:384].view(2, 2, 1, 64))):
+        with pytest.raises(ValueError, match="share|twice"):
+            evict_decode_step(**{**a, **change})
+    with pytest.raises(AssertionError, match="not refused"):  # (the same new row twice is only read)
+        evict_decode_step(**a)
+    q, lse = torch.zeros(2, 2, 9, 64), torch.zeros(2, 2, 9)
+    for out in (lse, torch.zeros(2, 1, 9).expand(2, 2, 9)):
+        with pytest.raises(ValueError, match="share|twice"):
+            key_weights(q, c, lse, out=out)
 
 
 def test_c_entries_refuse_without_a_gpu():

@@ -318,3 +318,47 @@ def test_prompt_to_decode(dev, dtype):
             c = sorted((p if p >= 0 else int(pos[b]), x) for p, x in zip(p2[b, h, :int(n2[b])].tolist(), w2[b, h, :int(n2[b])].tolist()))
             assert [x for x, _ in a] == [x for x, _ in c]
             assert all(abs(x - y) < 1e-4 * (1 + abs(y)) for (_, x), (_, y) in zip(a, c))
+
+
+def test_prompts_captured_and_on_two_streams(dev):
+    """Attention, weights and eviction of packed prompts as one graph, replayed over other
+    sequences; two such chains at once on two streams."""
+    N, Hq, Hkv, D, budget = 20000, 4, 2, 64, 600
+    q, k, v = (_rand(i, N, h, D, dtype=torch.bfloat16).to(dev) for i, h in ((0, Hq), (1, Hkv), (2, Hkv)))
+    cu = torch.tensor([0, 18000, 20000], dtype=torch.int32, device=dev)
+
+    def chain():
+        out, lse = packed_attention(q, k, v, cu, return_lse=True)
+        w = packed_key_weights(q, k, lse, cu, last=64)
+        return (out, lse, w, *packed_evict_kv(k, v, w, cu, budget=budget, recent=200, sink=4, capacity=budget + 1))
+
+    cuts = [[0, 18000, 20000], [0, 700, 20000], [5, 5, 19000], [0, 18000, 20000]]
+    want = []
+    for c in cuts:
+        cu.copy_(torch.tensor(c, dtype=torch.int32))
+        want.append([x.clone() for x in chain()])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for c, ref in zip(cuts, want):
+        cu.copy_(torch.tensor(c, dtype=torch.int32))
+        for x in got:
+            x.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, ref):
+            assert torch.equal(x, y)
+        assert torch.equal(chain()[3], ref[3])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    results = [[], []]
+    for _ in range(3):
+        for s, r in zip(streams, results):
+            with torch.cuda.stream(s):
+                r.append(chain())
+    torch.cuda.synchronize()
+    for r in results:
+        for once in r:
+            for x, y in zip(once, want[-1]):
+                assert torch.equal(x, y)

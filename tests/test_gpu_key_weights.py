@@ -171,3 +171,22 @@ def test_weights_of_chunks_add_up(dev):
     assert torch.equal(w2, whole)
     # every query's weights sum to one
     assert abs(float(whole.sum()) - Hkv * G * T) < 1e-3 * Hkv * G
+
+
+@pytest.mark.parametrize("G,Tq,last,far", [(4, 40, None, 6_000_000), (4, 129, None, 18_000_000), (2, 300, 17, 18_000_000),
+                                           (5, 20, 3, 18_000_000)])
+def test_heads_far_apart(dev, G, Tq, last, far):
+    """Head strides that with three and with one of them pass 32 bits: a staged tile holds
+    fewer heads."""
+    D, far = 64, 64 * far
+    q, k = _rand(0, 1, G, Tq, D, dtype=torch.bfloat16), _rand(1, 1, 1, Tq, D, dtype=torch.bfloat16)
+    lse = _lse(q, k, [Tq], [Tq])
+    big = torch.empty(far * (G - 1) + Tq * D, dtype=torch.bfloat16, device=dev)
+    wide = big.as_strided((1, G, Tq, D), (0, far, D, 1))
+    wide.copy_(q.to(dev))
+    w = key_weights(wide, k.to(dev), lse.to(dev), last=last)
+    _check(w, q, k, lse, [Tq], [Tq], last=last)
+    near = key_weights(q.to(dev), k.to(dev), lse.to(dev), last=last)
+    _check(near, q, k, lse, [Tq], [Tq], last=last)
+    del big, wide
+    torch.cuda.empty_cache()
