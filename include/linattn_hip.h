@@ -722,6 +722,7 @@ int la_dense_attention(const la_dense_attn_args *a, void *stream);
  * whose lse is -inf adds nothing.  out (fp32, strides w_sb, w_sh, 1) has a value for every
  * key row: with accumulate != 0 the weights are added to what it holds; else they replace
  * it, and keys past a sequence's length get 0 (packed: keys of no sequence with zero_rest).
+ * Rows of q less than 2^24 values apart (q_st).  Inputs and out share no memory.
  * Sums are in a fixed order: the same call gives the same bits.
  */
 typedef struct {

@@ -171,7 +171,7 @@ __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kv
 // in registers) leaves a lane 16 scores of one row, so masks, maxima and sums are per
 // lane; O^T takes P from the same registers (the contraction index is mapped to the keys
 // a lane holds) and V^T by LDS transpose reads.  P is rounded to the inputs' type for
-// that product (to half a step, 2^-9 or 2^-12 of each weight, independently: as much as
+// that product (to half a step, 2^-8 or 2^-11 of each weight, independently: as much as
 // the output's own rounding); its sum l, and with it lse, is of the fp32 values.
 template <class T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
@@ -209,13 +209,6 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
   j0 = __builtin_amdgcn_readfirstlane(j0);
   j1 = __builtin_amdgcn_readfirstlane(j1);
 
-  x8 qf[NS];  // B operand: dims 16 s + 8 hf ..
-  {
-    const elem *qp = (const elem *)p.q + (p.s.cu_q ? (tl.q0 + t) * p.q_st : tl.b * p.q_sb + t * p.q_st) +
-                     h * p.q_sh + 8 * hf;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) qf[s] = *(const x8 *)(qp + 16 * s);
-  }
   const uint16_t *kbh = (const uint16_t *)p.k + (p.s.cu_q ? tl.k0 * p.k_st : tl.b * p.k_sb) + kvh * p.k_sh;
   const uint16_t *vbh = (const uint16_t *)p.v + (p.s.cu_q ? tl.k0 * p.v_st : tl.b * p.v_sb) + kvh * p.v_sh;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
@@ -247,6 +240,20 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
   };
   auto dma_k = [&](int kb) __attribute__((always_inline)) { dma(kbh, p.k_st, ko, kb, (kb - j0) & 1); };
   auto dma_v = [&](int kb) __attribute__((always_inline)) { dma(vbh, p.v_st, vo, kb, 2); };
+  if (j0 < j1) {  // (the first tile is on its way while q is loaded)
+    dma_k(j0);
+    dma_v(j0);
+  }
+
+  x8 qf[NS];  // B operand: dims 16 s + 8 hf ..
+  {
+    const elem *qp = (const elem *)p.q + (p.s.cu_q ? (tl.q0 + t) * p.q_st : tl.b * p.q_sb + t * p.q_st) +
+                     h * p.q_sh + 8 * hf;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = *(const x8 *)(qp + 16 * s);
+  }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) settle(qf[s]);
 
   float m = da_ninf(), thr = da_ninf(), l = 0.f, nmu = 0.f;
   f32x16 acc[ND];
@@ -342,11 +349,10 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
   };
 
   const int jw = wave_live && lim_hi >= 0 ? min(lim_hi / DA_BS, j1 - 1) : -1;  // this wave's last tile
-  if (j0 < j1) dma_k(j0);
   for (int j = j0; j < j1; ++j) {
     wait_vmcnt<0>();
     lds_barrier();  // K of tile j has landed for every wave, tile j - 1 is read
-    dma_v(j);
+    if (j > j0) dma_v(j);
     if (j + 1 < j1) dma_k(j + 1);
     f32x16 st[2];
     x8 pw[2];
@@ -389,13 +395,30 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
   } else if (live) {
     const bool none = l == 0.f;  // no key seen
     const float inv = none ? 0.f : 1.f / l;
-    const int64_t o = da_out_at(p, tl, t, h) + 4 * hf;
+    const int64_t o = da_out_at(p, tl, t, h);
+    if (p.out_dt == LA_F32) {
 #pragma unroll
-    for (int dt = 0; dt < ND; ++dt)
+      for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        da_store4(p.out, o + 32 * dt + 8 * i, p.out_dt, acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv,
-                  acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv);
+        for (int i = 0; i < 4; ++i)
+          *(float4 *)((float *)p.out + o + 32 * dt + 8 * i + 4 * hf) =
+              float4{acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv, acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv};
+    } else {  // the halves of a row trade fours, so that a lane stores eight values
+      typedef elem x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          uint2 y[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            y[x] = __builtin_bit_cast(uint2, x4{(elem)(acc[dt][4 * (i + x)] * inv), (elem)(acc[dt][4 * (i + x) + 1] * inv),
+                                                (elem)(acc[dt][4 * (i + x) + 2] * inv), (elem)(acc[dt][4 * (i + x) + 3] * inv)});
+          const auto a = __builtin_amdgcn_permlane32_swap(y[0].x, y[1].x, false, false);
+          const auto c = __builtin_amdgcn_permlane32_swap(y[0].y, y[1].y, false, false);
+          *(uint4 *)((elem *)p.out + o + 32 * dt + 8 * (i + hf)) = uint4{a[0], c[0], a[1], c[1]};
+        }
+    }
     if (p.lse && hf == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (__log2f(l) - nmu) * DA_LN2;  // (as rounded in the weights)
   }
   if (bad != 0)
