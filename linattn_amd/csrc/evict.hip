@@ -14,7 +14,9 @@
 // of a row's slices are added by whoever needs the sum, in place of atomics.
 // Slots that are not chosen by weight (the newest tokens, mostly half of the cache) wait
 // for no selection: the selecting launches, which leave the memory idle, copy them in
-// workgroups of their own.
+// workgroups of their own (four caches of 6572 to 66473 entries of 8 heads cut to 4096: 61
+// us without, 55.7 with; passes 7, 11, 11 and 11 us, the rest of the rows 12, of which 28
+// would move all bytes at the rate of a large copy).
 #include <algorithm>
 
 #include "evict.h"
@@ -345,6 +347,7 @@ __device__ __forceinline__ void ev_choose(const EvRow &r, List list) {
   });
 }
 
+// (Two caches of 660 and 740 entries of 8 heads cut to 256: 9.4 us, the search's barriers.)
 template <bool POS>
 __global__ __launch_bounds__(256) void evict_small_kernel(EvKP p, int32_t parts) {
   __shared__ int32_t at[EV_SLOTS];
@@ -362,6 +365,7 @@ __global__ __launch_bounds__(256) void evict_small_kernel(EvKP p, int32_t parts)
   ev_copy<256>(p, r, b, h, at, s0, ns);
 }
 
+// (One cache of 16000 entries of 8 heads cut to 4096, with the copies: 20 us.)
 template <bool POS>
 __global__ __launch_bounds__(1024) void evict_select_kernel(EvKP p) {
   if ((int)blockIdx.x >= p.sel) {

@@ -95,7 +95,12 @@ __device__ __forceinline__ void kw_next(const KwKP &p, const KwTile &x, int qpt,
 // bf16 / fp16: four waves of 64 keys.  Rows are staged 64 at a time by LDS-DMA, with their
 // lse (each wave its own copy, so that every wave counts the same loads), NSLOT - 1 tiles
 // ahead; a tile's 128 products a workgroup and the 3 vector instructions of each of its
-// weights take about equally long.
+// weights take about equally long, which is what bounds it: 14567 tokens of 32 heads on 8
+// run at 0.95 PFLOP/s as one sequence, and as twelve of 115 to 3039 at 0.8 (162 us).  For
+// few queries the keys bound it, and that they must arrive before a workgroup's first
+// product: the last 64 queries of 50001 tokens, 105 MB, 52 us.  (Two waves of 64 keys a
+// workgroup: 254 and 86 us, the copies' instructions double; eight: 191 and 68, nothing runs
+// beside a workgroup's loads; three workgroups a CU without the interleaving: 249 and 60.)
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
   constexpr int NW = 4, KT = 64 * NW, BLK = DA_BS * D, CH = D / 8, RP = 64 / CH, NX = DA_BS / RP / NW;
@@ -286,7 +291,8 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
 }
 
 // fp32: four waves of 32 keys on 16x16x4 products; lane (c, i) holds chunk 4 s + c of key
-// i, and of row i of the staged rows, as in dense_attn_f32_kernel.
+// i, and of row i of the staged rows, as in dense_attn_f32_kernel.  Bound by the fp32 matrix
+// rate: 8192 tokens of 32 heads on 8, D = 128, 2.5 ms, 110 TFLOP/s.
 template <int D>
 __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
   constexpr int NW = 4, KT = 32 * NW, BS = 32, BLK = BS * D, CH = D / 4, RP = 64 / CH, NX = BS / RP / NW;
@@ -378,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
     }
 }
 
-// Adds the parts of a key in their order.  Packed keys of no sequence have no parts.
+// Adds the parts of a key in their order (5 us, its launch).  Packed keys of no sequence have no parts.
 __global__ __launch_bounds__(256) void key_weights_sum_kernel(KwKP p) {
   const int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y;
   if (s >= p.s.Tk) return;
@@ -406,7 +412,7 @@ static KwPlan kw_plan(const la_key_weights_args *a) {
   pl.keys = a->dtype == LA_F32 ? 128 : 256;
   pl.ntile = da_tiles(packed, a->B, a->Tk, 1, pl.keys);
   // Rows are split until there are four workgroups a CU (causal tiles differ in length by
-  // far; 14567 packed tokens take 262 us unsplit, 167 with four, 180 with eight), down to
+  // far; 14567 packed tokens took 262 us unsplit, 167 with four, 180 with eight), down to
   // four staged tiles each.
   const int64_t wgs = pl.ntile * a->Hkv, G = a->Hq / a->Hkv;
   int64_t rows = (packed ? ceil_div(a->Tq, a->B) : a->Tq) * G;
