@@ -362,13 +362,14 @@ def require_gpu(*tensors: Optional[torch.Tensor], what: str) -> torch.device:
     for t in tensors:
         if t is None:
             continue
+        if dev is not None and t.device == dev:
+            continue
         if not t.is_cuda:
             raise RuntimeError(f"{what}: the HIP backend needs GPU tensors (got {t.device}); "
                                "the CPU oracle lives in oracle/ and is not a fallback")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if dev is not None:
             raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        dev = t.device
     if dev is None:
         raise ValueError(f"{what}: no tensors")
     return dev

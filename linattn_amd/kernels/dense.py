@@ -59,13 +59,14 @@ def _scale(scale: Optional[float], D: int) -> float:
 
 
 def _check_qk(what: str, q: torch.Tensor, k: torch.Tensor, dims: int, head: int) -> None:
-    if q.dim() != dims or k.dim() != dims:
+    qs, ks, dt = q.shape, k.shape, q.dtype
+    if len(qs) != dims or len(ks) != dims:
         raise ValueError(f"{what}: q and k must have {dims} dimensions")
-    if q.dtype != k.dtype or q.dtype not in _TYPES:
+    if dt != k.dtype or dt not in _TYPES:
         raise ValueError(f"{what}: q, k and v must share one of bfloat16, float16, float32")
-    if q.shape[-1] not in (64, 128) or k.shape[-1] != q.shape[-1]:
+    if qs[-1] not in (64, 128) or ks[-1] != qs[-1]:
         raise ValueError(f"{what}: head_dim must be 64 or 128, and the same in q and k")
-    if k.shape[head] == 0 or q.shape[head] == 0 or q.shape[head] % k.shape[head]:
+    if ks[head] == 0 or qs[head] == 0 or qs[head] % ks[head]:
         raise ValueError(f"{what}: the query heads must be a multiple of the KV heads")
 
 
@@ -87,10 +88,9 @@ def _out(what: str, out: Optional[torch.Tensor], q: torch.Tensor,
          out_dtype: Optional[torch.dtype], *inputs: torch.Tensor) -> torch.Tensor:
     """(out, or a new one, checked)."""
     if out is None:
-        dt = out_dtype or q.dtype
-        if dt not in (q.dtype, torch.float32):
+        if out_dtype is not None and out_dtype not in (q.dtype, torch.float32):
             raise ValueError(f"{what}: out_dtype is q's or float32")
-        return torch.empty(q.shape, dtype=dt, device=q.device)
+        return torch.empty_like(q, dtype=out_dtype, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype not in (q.dtype, torch.float32) or \
             (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"{what}: out must be q's shape in q's dtype (or float32)")

@@ -140,7 +140,7 @@ def _run_evict(what: str, a: N.LaEvictArgs, B: int, k, v, weights, budget, recen
     k_out = torch.empty(B, Hkv, capacity, D, dtype=k.dtype, device=dev)
     v_out = torch.empty_like(k_out)
     w_out = torch.empty(B, Hkv, capacity, dtype=torch.float32, device=dev)
-    pos_out = torch.empty(B, Hkv, capacity, dtype=torch.int32, device=dev)
+    pos_out = torch.empty_like(w_out, dtype=torch.int32)
     len_out = torch.empty(B, dtype=torch.int32, device=dev)
     if B > 0:
         a.k, a.v, a.weights = k.data_ptr(), v.data_ptr(), weights.data_ptr()
