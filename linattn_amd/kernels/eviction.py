@@ -134,20 +134,19 @@ def _budget(what: str, budget: int, recent: int, sink: int, capacity: Optional[i
     return capacity
 
 
-def _run_evict(what: str, a: N.LaEvictArgs, B: int, k, v, weights, budget, recent, sink,
-               capacity) -> Evicted:
-    dev, Hkv, D = k.device, a.Hkv, k.shape[-1]
+def _run_evict(what: str, k, v, weights, positions, pos, lengths, cu, B: int, Hkv: int, T: int, k_s, v_s, w_s,
+               ps_s, budget, recent, sink, capacity) -> Evicted:
+    dev, D = k.device, k.shape[-1]
     k_out = torch.empty(B, Hkv, capacity, D, dtype=k.dtype, device=dev)
     v_out = torch.empty_like(k_out)
     w_out = torch.empty(B, Hkv, capacity, dtype=torch.float32, device=dev)
     pos_out = torch.empty_like(w_out, dtype=torch.int32)
     len_out = torch.empty(B, dtype=torch.int32, device=dev)
     if B > 0:
-        a.k, a.v, a.weights = k.data_ptr(), v.data_ptr(), weights.data_ptr()
-        a.k_out, a.v_out, a.w_out = k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr()
-        a.pos_out, a.len_out = pos_out.data_ptr(), len_out.data_ptr()
-        a.B, a.D, a.esize = B, D, k.element_size()
-        a.budget, a.capacity, a.recent, a.sink = budget, capacity, recent, sink
+        a = N.LaEvictArgs(
+            k.data_ptr(), v.data_ptr(), weights.data_ptr(), N.ptr(positions), N.ptr(pos), N.ptr(lengths), N.ptr(cu),
+            k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr(), pos_out.data_ptr(), len_out.data_ptr(), None, 0,
+            B, Hkv, T, D, k.element_size(), *k_s, *v_s, *w_s, *ps_s, budget, capacity, recent, sink)
         L, ref = N.load(), ctypes.byref(a)
         with N.on_device(dev):
             nbytes = L.la_evict_kv_workspace(ref)
@@ -196,16 +195,12 @@ def evict_kv(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor, *, budget:
     lengths, pos = _int32(lengths, (B,), "lengths"), _int32(pos, (B,), "pos")
     k, v = _rows(k), _rows(v)
     weights = weights if weights.stride(-1) == 1 else weights.contiguous()
-    a = N.LaEvictArgs()
+    ps_s = (0, 0)
     if positions is not None:
         positions = positions if positions.stride(-1) == 1 else positions.contiguous()
-        a.positions, a.pos = positions.data_ptr(), pos.data_ptr()
-        a.ps_sb, a.ps_sh = positions.stride()[:2]
-    a.lengths, a.Hkv, a.T = N.ptr(lengths), Hkv, T
-    a.k_sb, a.k_sh, a.k_st = k.stride()[:3]
-    a.v_sb, a.v_sh, a.v_st = v.stride()[:3]
-    a.w_sb, a.w_sh = weights.stride()[:2]
-    return _run_evict(what, a, B, k, v, weights, budget, recent, sink, capacity)
+        ps_s = positions.stride()[:2]
+    return _run_evict(what, k, v, weights, positions, pos, lengths, None, B, Hkv, T, k.stride()[:3], v.stride()[:3],
+                      weights.stride()[:2], ps_s, budget, recent, sink, capacity)
 
 
 def packed_evict_kv(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor,
@@ -225,12 +220,9 @@ def packed_evict_kv(k: torch.Tensor, v: torch.Tensor, weights: torch.Tensor,
     cu_seqlens = _cu(cu_seqlens, "cu_seqlens")
     k, v = _rows(k), _rows(v)
     weights = weights if weights.stride(-1) == 1 else weights.contiguous()
-    a = N.LaEvictArgs()
-    a.cu, a.Hkv, a.T = cu_seqlens.data_ptr(), Hkv, Nk
-    a.k_st, a.k_sh = k.stride()[:2]
-    a.v_st, a.v_sh = v.stride()[:2]
-    a.w_sh = weights.stride(0)
-    return _run_evict(what, a, cu_seqlens.shape[0] - 1, k, v, weights, budget, recent, sink, capacity)
+    (k_t, k_h, _), (v_t, v_h, _) = k.stride(), v.stride()
+    return _run_evict(what, k, v, weights, None, None, None, cu_seqlens, cu_seqlens.shape[0] - 1, Hkv, Nk,
+                      (0, k_h, k_t), (0, v_h, v_t), (0, weights.stride(0)), (0, 0), budget, recent, sink, capacity)
 
 
 def evict_decode_step(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
