@@ -4,7 +4,7 @@
 // A workgroup takes a tile of keys of one KV head and keeps them in registers; it walks
 // the rows (query, head of the group) that see them, staged in LDS: S^T = K Q^T on the
 // matrix cores, P = exp2(c S - lse) in place, added lane by lane (a lane holds one row
-// and 16 keys of a product), and summed over the lanes once at the end.  Nothing is
+// and 16 keys of a product), and summed over the lanes every 32 staged tiles.  Nothing is
 // normalised or joined on the way, so the rows of a tile can be split over workgroups;
 // their sums are added in order by a second kernel: no atomics.
 #include <algorithm>
@@ -92,6 +92,10 @@ __device__ __forceinline__ void kw_next(const KwKP &p, const KwTile &x, int qpt,
   }
 }
 
+// Staged tiles after which a tile's running sums are added to its totals: over 128 000 rows
+// a chain of additions a lane loses five times what the weights' own roundings do.
+constexpr int KW_RUN = 32;
+
 // bf16 / fp16: four waves of 64 keys.  Rows are staged 64 at a time by LDS-DMA, with their
 // lse (each wave its own copy, so that every wave counts the same loads), NSLOT - 1 tiles
 // ahead; a tile's 128 products a workgroup and the 3 vector instructions of each of its
@@ -125,6 +129,31 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
+
+  // What acc gathered added to total, and acc begun again: sums over the 32 lanes of a
+  // half, each step adding two registers' halves of the lanes into one register, until
+  // lane l has register l / 2.
+  float total[2] = {0.f, 0.f};
+  auto fold_in = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[kt][i]), __float_as_uint(acc[kt][i + 8]), false, false);
+        v[i] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+      }
+      auto fold = [&](float lo, float hi, bool up, auto other) { return (up ? hi : lo) + other(up ? lo : hi); };
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = fold(v[i], v[i + 4], lane & 8, [](float y) { return dpp_f32<0x128>(y); });
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] = fold(v[i], v[i + 2], lane & 4, [](float y) { return dpp_f32<0x141>(y); });
+      v[0] = fold(v[0], v[1], lane & 2, [](float y) { return dpp_f32<0x1B>(y); });
+      total[kt] += v[0] + dpp_f32<0xB1>(v[0]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[kt][i] = 0.f;
+    }
+  };
 
   const int n = x.n, qs = 6 - p.ms, qpt = 1 << qs;
   if (n > 0) {
@@ -253,6 +282,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
       else wait_vmcnt<0>();
       lds_barrier();  // for every wave, and tile j - 1 is read
       if (j + NSLOT - 1 < n) dma((j + NSLOT - 1) % NSLOT);
+      if (j % KW_RUN == KW_RUN - 1) fold_in();
       if (tb + qpt <= t_any) continue;
       const bool whole = t_all <= tb && tb + qpt <= x.t.lq;
       if (whole) {
@@ -267,26 +297,12 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
       }
     }
     weigh(sb, nb);
+    fold_in();
   }
-  // sums over the 32 lanes of a half: each step adds two registers' halves of the lanes
-  // into one register, until lane l has register l / 2
 #pragma unroll
   for (int kt = 0; kt < 2; ++kt) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[kt][i]), __float_as_uint(acc[kt][i + 8]), false, false);
-      v[i] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
-    }
-    auto fold = [&](float lo, float hi, bool up, auto other) { return (up ? hi : lo) + other(up ? lo : hi); };
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = fold(v[i], v[i + 4], lane & 8, [](float y) { return dpp_f32<0x128>(y); });
-#pragma unroll
-    for (int i = 0; i < 2; ++i) v[i] = fold(v[i], v[i + 2], lane & 4, [](float y) { return dpp_f32<0x141>(y); });
-    v[0] = fold(v[0], v[1], lane & 2, [](float y) { return dpp_f32<0x1B>(y); });
-    v[0] += dpp_f32<0xB1>(v[0]);
     const int i = r32 >> 1;
-    if ((lane & 1) == 0) kw_put(p, x, kvh, split, s_w + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3), [&] { return v[0]; });
+    if ((lane & 1) == 0) kw_put(p, x, kvh, split, s_w + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3), [&] { return total[kt]; });
   }
 }
 
@@ -308,6 +324,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
   if (x.t.b < 0) return;
   const int s_w = x.s0 + 32 * w, diag = x.t.lk - x.t.lq;
   f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  f32x4 total[2] = {acc[0], acc[1]};
   const int n = x.n, qs = 5 - p.ms, qpt = 1 << qs;
   if (n > 0) {
     f32x4 kf[2][NS];
@@ -348,6 +365,13 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
       settle(nl[1]);
       lds_barrier();
       if (j + 1 < n) dma((j + 1) & 1);
+      if (j % KW_RUN == KW_RUN - 1) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          total[kt] += acc[kt];
+          acc[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+      }
       const float *sq = smem + (j & 1) * BLK;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -379,7 +403,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
   for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float v = group_sum<16>(acc[kt][e]);
+      const float v = group_sum<16>(total[kt][e] + acc[kt][e]);
       if (ri == e) kw_put(p, x, kvh, split, s_w + 16 * kt + 4 * c + e, [&] { return v; });
     }
 }

@@ -190,3 +190,20 @@ def test_heads_far_apart(dev, G, Tq, last, far):
     _check(near, q, k, lse, [Tq], [Tq], last=last)
     del big, wide
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lse", [0.3, 0.7, 1.3])
+def test_many_equal_weights(dev, dtype, lse):
+    """Keys that gather equal weights from up to 131072 rows: a running sum that took all of a
+    lane's rows one by one would drift by up to half a step of the sum for each."""
+    Hkv, G, T, D = 8, 4, 32768, 64
+    q = torch.zeros(T, Hkv * G, D, dtype=dtype, device=dev)
+    k = torch.zeros(T, Hkv, D, dtype=dtype, device=dev)
+    row = torch.full((Hkv * G, T), lse, dtype=torch.float32, device=dev)
+    w = packed_key_weights(q, k, row, torch.tensor([0, T], dtype=torch.int32, device=dev)).double().cpu()
+    want = G * torch.arange(T, 0, -1).double() * math.exp(-float(torch.tensor(lse, dtype=torch.float32)))
+    # runs of 32 staged tiles, 64 additions a lane (2 of each tile), 5 between lanes, and the
+    # runs' sums: 64 of 64 rows' tiles, 128 of 32 rows'; a few steps of exp2 and its argument
+    tol = (64 + 5 + (64 if dtype != torch.float32 else 128) + 8 + 2 * lse) * 2.0 ** -24
+    assert ((w - want).abs() <= tol * want).all()
