@@ -492,9 +492,11 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   };
 
   float m = da_ninf(), thr = da_ninf(), l = 0.f, nmu = 0.f;
-  f32x4 acc[NS];
+  // acc of 16 tiles at a time is added to total: one long chain of products' sums, four
+  // keys a step, would round as often as there are steps
+  f32x4 acc[NS], total[NS];
 #pragma unroll
-  for (int dt = 0; dt < NS; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < NS; ++dt) acc[dt] = total[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   if (j0 < j1) dma(j0, 0);
   for (int j = j0; j < j1; ++j) {
@@ -537,7 +539,10 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
       nmu = mn == da_ninf() ? 0.f : -mn * p.qscale;
       l *= alpha;
 #pragma unroll
-      for (int dt = 0; dt < NS; ++dt) acc[dt] *= alpha;
+      for (int dt = 0; dt < NS; ++dt) {
+        acc[dt] *= alpha;
+        total[dt] *= alpha;
+      }
     }
     float part = 0.f;
 #pragma unroll
@@ -553,8 +558,17 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
               sv[kr * D + 4 * ((4 * dt + (ri >> 2)) ^ swz_v(kr)) + (ri & 3)], pr, acc[dt], 0, 0, 0);
       }
     l += part;
+    if ((j - j0) % 16 == 15) {
+#pragma unroll
+      for (int dt = 0; dt < NS; ++dt) {
+        total[dt] += acc[dt];
+        acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
   }
   if (!wave_live) return;
+#pragma unroll
+  for (int dt = 0; dt < NS; ++dt) acc[dt] += total[dt];
   l = pair32_sum(pair16_sum(l));
   float sum = 0.f;
 #pragma unroll
