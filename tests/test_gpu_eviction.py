@@ -362,3 +362,29 @@ def test_prompts_captured_and_on_two_streams(dev):
         for once in r:
             for x, y in zip(once, want[-1]):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_to_read(dev, dtype):
+    """No keys, no queries, no entries: zeros, -inf and empty caches, from tensors without rows."""
+    z = lambda *s: torch.zeros(*s, dtype=dtype, device=dev)
+    cu, none = _i32([0, 3, 5], dev), _i32([0, 0, 0], dev)
+    for Tq in (1, 40):
+        out, lse = dense_attention(z(2, 4, Tq, 64) + 1, z(2, 2, 0, 64), z(2, 2, 0, 64), return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    out, lse = packed_attention(z(5, 4, 64) + 1, z(0, 2, 64), z(0, 2, 64), cu, none, return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    out, lse = packed_attention(z(0, 4, 64), z(5, 2, 64), z(5, 2, 64), none, cu, return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
+    w = key_weights(z(2, 4, 0, 64), z(2, 2, 70, 64), torch.zeros(2, 4, 0, device=dev))
+    assert w.shape == (2, 2, 70) and (w == 0).all()
+    w = packed_key_weights(z(0, 4, 64), z(5, 2, 64), torch.zeros(4, 0, device=dev), none, cu)
+    assert w.shape == (2, 5) and (w == 0).all()
+    assert key_weights(z(2, 4, 3, 64), z(2, 2, 0, 64), torch.zeros(2, 4, 3, device=dev)).shape == (2, 2, 0)
+    for got in (evict_kv(z(2, 2, 0, 64), z(2, 2, 0, 64), torch.zeros(2, 2, 0, device=dev), budget=4, recent=2, capacity=5),
+                packed_evict_kv(z(0, 2, 64), z(0, 2, 64), torch.zeros(2, 0, device=dev), none, budget=4, recent=2, capacity=5)):
+        k, v, w, pos, n = got
+        assert (k == 0).all() and (v == 0).all() and (w == 0).all() and (pos == -1).all() and (n == 0).all()
+        assert k.shape == (2, 2, 5, 64)
+    k, v, w, pos, n = evict_kv(z(0, 2, 9, 64), z(0, 2, 9, 64), torch.zeros(0, 2, 9, device=dev), budget=4, recent=2)
+    assert k.shape == (0, 2, 4, 64) and n.shape == (0,)
