@@ -83,69 +83,32 @@ __device__ void da_rest(const DaKP &p, const DaTile &tl, int R, int kvh, int spl
   }
 }
 
-// One row over keys a .. e - 1, by a wave, key by key (m in log2 units; lane i holds dims
-// i D / 64 ..).  For rows of a tile whose matrix products met an infinity or a NaN of V
-// that the row does not see (0 * inf): it reads nothing else.
-template <class E, int D>
-__device__ __forceinline__ void da_row(const E *q, const E *k, const E *v, int64_t k_st, int64_t v_st, int a,
-                                    int e, float qscale, float *m_out, float *l_out, float *acc) {
-  constexpr int N = D / 64;
-  const int lane = threadIdx.x & 63;
-  float m = da_ninf(), l = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  for (int key0 = a; key0 < e; key0 += 64) {
-    const int key = min(key0 + lane, e - 1);
-    float s = 0.f;
-    for (int d = 0; d < D; ++d) s = __builtin_fmaf((float)q[d], (float)k[key * k_st + d], s);
-    s = key0 + lane < e ? s * qscale : da_ninf();
-    float mx = s;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    const float mn = fmaxf(m, mx);
-    const float alpha = m == da_ninf() ? 0.f : fast_exp2(m - mn);
-    const float pr = fast_exp2(s - (mn == da_ninf() ? 0.f : mn));
-    m = mn;
-    l = l * alpha + group_sum<64>(pr);
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] *= alpha;
-    const int n = min(64, e - key0);
-    for (int j = 0; j < n; ++j) {
-      const float w = __shfl(pr, j, 64);
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        acc[i] = __builtin_fmaf(w, (float)v[(int64_t)(key0 + j) * v_st + lane * N + i], acc[i]);
-    }
-  }
-  *m_out = m;
-  *l_out = l;
-}
-
-// Rows of a wave (row number r_first + i, i < NR) whose results are not finite, of which
+// Rows r_first + i, i = i0, i0 + step, .. below NR, whose results are not finite, of which
 // bit i of `bad` says so: those with an infinity or NaN of V among what their tiles (keys
-// a .. end - 1) held and they do not see are done again; the others stand.  (What a tile
-// holds past the last key is that key again.)  Called last, when the wave's rows are
-// stored and its registers free.
-template <class E, int D, int NR>
+// a .. end - 1) held and they do not see are done again; the others stand, but for ALL
+// (few_row).  (What a tile holds past the last key is that key again.)  Called last, when
+// the rows are stored and the registers free.
+template <class E, int D, int NR, bool ALL>
 __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kvh, int split, int r_first,
-                                          uint32_t bad, int a, int end) {
+                                          uint32_t bad, int a, int end, int i0, int step) {
   const int lane = threadIdx.x & 63, G = p.s.G;
   const E *kb = (const E *)p.k + (p.s.cu_q ? tl.k0 * p.k_st : tl.b * p.k_sb) + kvh * p.k_sh;
   const E *vb = (const E *)p.v + (p.s.cu_q ? tl.k0 * p.v_st : tl.b * p.v_sb) + kvh * p.v_sh;
   wait_vmcnt<0>();  // (stores over those)
 #pragma unroll 1
-  for (int i = 0; i < NR; ++i) {
+  for (int i = i0; i < NR; i += step) {
     if (!((bad >> i) & 1u)) continue;
     const int r = r_first + i, t = r / G, h = kvh * G + r % G;
     const int lim = p.causal ? min(tl.lk - 1, tl.lk - tl.lq + t) : tl.lk - 1;
-    bool met = false;
-    for (int key = max(max(lim + 1, a), 0); key < end; ++key)
+    bool met = ALL;
+    for (int key = max(max(lim + 1, a), 0); key < end && !ALL; ++key)
       for (int d = lane; d < D; d += 64)
         met = met || !(fabsf((float)vb[(int64_t)min(key, tl.lk - 1) * p.v_st + d]) < __int_as_float(0x7f800000));
     if (__ballot(met) == 0) continue;
     const E *q = (const E *)p.q + (p.s.cu_q ? (tl.q0 + t) * p.q_st : tl.b * p.q_sb + t * p.q_st) + h * p.q_sh;
     float m, l, acc[D / 64];
-    da_row<E, D>(q, kb, vb, p.k_st, p.v_st, a, min(end, lim + 1), p.qscale, &m, &l, acc);
+    few_row<E, D>(q, [&](int key) { return kb + key * p.k_st; }, [&](int key) { return vb + key * p.v_st; }, a,
+                  min(end, lim + 1), p.qscale, &m, &l, acc);
     if (p.splits > 1) {
       const int64_t pi = da_part_at(p, tl, t, h, split);
       if (lane == 0) {
@@ -426,8 +389,8 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
     if (p.lse && hf == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (__log2f(l) - nmu) * DA_LN2;  // (as rounded in the weights)
   }
   if (bad != 0)
-    da_again<elem, D, 32>(p, tl, kvh, split, r_first, (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
-                          j0 * DA_BS, min(j1, lim_hi / DA_BS + 1) * DA_BS);
+    da_again<elem, D, 32, false>(p, tl, kvh, split, r_first, (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
+                                 j0 * DA_BS, min(j1, lim_hi / DA_BS + 1) * DA_BS, 0, 1);
 }
 
 // fp32 rows: four waves of 16 rows on 16x16x4 products, all of it fp32.  A staged tile is
@@ -597,8 +560,8 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   }
   if (bad != 0) {
     bad |= bad >> 32;
-    da_again<float, D, 16>(p, tl, kvh, split, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
-                           j0 * BS, min(j1, lim_hi / BS + 1) * BS);
+    da_again<float, D, 16, false>(p, tl, kvh, split, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
+                                  j0 * BS, min(j1, lim_hi / BS + 1) * BS, 0, 1);
   }
 }
 
@@ -654,7 +617,8 @@ __global__ __launch_bounds__(256, 2) void dense_few_kernel(DaKP p) {
       l = __builtin_fmaf(ml[x * 32 + 2 * g + 1], f, l);
       a = __builtin_fmaf(vals[x * FR::VALS + g * (D + 4) + d], f, a);
     }
-    if (!(fabsf(a) < __int_as_float(0x7f800000))) atomicOr(&s_bad, 1u << g);
+    // (with scores that are not numbers, l is not, and the row stands)
+    if (!(fabsf(a) < __int_as_float(0x7f800000)) && l < __int_as_float(0x7f800000)) atomicOr(&s_bad, 1u << g);
     if (p.splits > 1) {
       const int64_t pi = da_part_at(p, tl, te, h, split);
       p.ws_acc[pi * D + d] = a;
@@ -668,7 +632,10 @@ __global__ __launch_bounds__(256, 2) void dense_few_kernel(DaKP p) {
     }
   }
   __syncthreads();
-  if (s_bad != 0u && w == 0) da_again<elem, D, 16>(p, tl, kvh, split, 0, s_bad, r0 * FR::RK, r1 * FR::RK);
+  if (s_bad == 0u) return;
+  wait_vmcnt<0>();
+  __syncthreads();  // (every wave's stores are done, which those of the rows done again replace)
+  da_again<elem, D, 16, true>(p, tl, kvh, split, 0, s_bad, r0 * FR::RK, r1 * FR::RK, w, NW);
 }
 
 // Joins the parts of a row: a wave a row (4-6 us, its launch).

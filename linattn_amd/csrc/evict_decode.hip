@@ -132,6 +132,7 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
   constexpr int LDS = NW * FR::LDS_BYTES > LDS_MERGE ? NW * FR::LDS_BYTES : LDS_MERGE;
   __shared__ __align__(16) char smem[LDS];
   __shared__ float lse2[16];
+  __shared__ uint32_t s_bad;  // rows to be done again (few_row)
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t pair = blockIdx.x / (uint32_t)p.splits;
   const int split = (int)(blockIdx.x % (uint32_t)p.splits);
@@ -150,9 +151,10 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
   const int r0 = (int)((int64_t)rounds * split / p.splits), r1 = (int)((int64_t)rounds * (split + 1) / p.splits);
   float *sc = p.scores + (pair * p.G + row) * p.cs;
   const bool put = (lane & 15) < p.G;
-  fr.walk(r0 + w, NW, r1, n, n - 1, p.qscale, ED_GAP, (elem *)(smem + w * FR::LDS_BYTES),
-          [&](int key) { return key == slot ? kn : kc + (int64_t)key * D; },
-          [&](int key) { return key == slot ? vn : vc + (int64_t)key * D; },
+  if (threadIdx.x == 0) s_bad = 0u;
+  auto krow = [&](int key) -> const elem * { return key == slot ? kn : kc + (int64_t)key * D; };
+  auto vrow = [&](int key) -> const elem * { return key == slot ? vn : vc + (int64_t)key * D; };
+  fr.walk(r0 + w, NW, r1, n, n - 1, p.qscale, ED_GAP, (elem *)(smem + w * FR::LDS_BYTES), krow, vrow,
           [&](int key, f32x4 s) { if (put) *(f32x4 *)(sc + key) = s; });
   // the new token's rows, by the part that holds its slot
   if (slot / FR::RK >= r0 && slot / FR::RK < r1 && w == 0) {
@@ -179,6 +181,8 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
       l = __builtin_fmaf(ml[x * 32 + 2 * g + 1], f, l);
       a = __builtin_fmaf(vals[x * FR::VALS + g * (D + 4) + d], f, a);
     }
+    // (with scores that are not numbers, l is not, and the row stands)
+    if (!(fabsf(a) < __int_as_float(0x7f800000)) && l < __int_as_float(0x7f800000)) atomicOr(&s_bad, 1u << g);
     if (p.splits > 1) {
       const int64_t at = (pair * p.splits + split) * p.G + g;
       p.vals[at * D + d] = a;
@@ -191,8 +195,28 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
       if (d == 0) lse2[g] = m + __log2f(l);
     }
   }
-  if (p.splits > 1) return;
   __syncthreads();
+  if (s_bad != 0u) {
+    wait_vmcnt<0>();
+    __syncthreads();  // (every wave's stores are done, which those of the rows done again replace)
+    for (int g = w; g < p.G; g += NW) {
+      if (!((s_bad >> g) & 1u)) continue;
+      constexpr int N = D / 64;
+      float m, l, a[N];
+      few_row<elem, D>((const elem *)p.q + b * p.q_sb + (kvh * p.G + g) * p.q_sh, krow, vrow, r0 * FR::RK,
+                       min(n, r1 * FR::RK), p.qscale, &m, &l, a);
+      const int64_t at = (pair * p.splits + split) * p.G + g;
+      if (p.splits > 1 && lane == 0) {
+        p.ml[2 * at] = m;
+        p.ml[2 * at + 1] = l;
+      }
+      for (int x = 0; x < N; ++x) {
+        if (p.splits > 1) p.vals[at * D + lane * N + x] = a[x];
+        else store_from_f32(p.out, b * p.o_sb + (kvh * p.G + g) * p.o_sh + lane * N + x, p.out_dt, a[x] / l);
+      }
+    }
+  }
+  if (p.splits > 1) return;
   ed_weights<256>(p, pair, slot, 0, n, lse2);
 }
 

@@ -11,6 +11,12 @@
 
 #include "dense_attn.h"
 
+//
+// An infinity of V that a row sees meets weights of both signs in that sum (the second
+// term's), and what is past the last key is that key again with weight 0: 0 and inf - inf
+// where the result is infinite.  The caller looks for sums that are not finite and does
+// those rows again (few_row).
+
 namespace la {
 
 struct DaF32 {
@@ -194,5 +200,44 @@ struct FewRows {
   }
   static constexpr int VALS = 16 * (D + 4);  // floats of put's values
 };
+
+// One row over keys a .. e - 1 (krow(key), vrow(key)), by a wave, key by key in fp32 (m in
+// log2 units; lane i holds dims i D / 64 ..).  For rows whose matrix products met an
+// infinity or a NaN of V in a way that the definition does not: it reads nothing else.
+template <class E, int D, class KRow, class VRow>
+__device__ __forceinline__ void few_row(const E *q, KRow krow, VRow vrow, int a, int e, float qscale, float *m_out,
+                                        float *l_out, float *acc) {
+  constexpr int N = D / 64;
+  const int lane = threadIdx.x & 63;
+  const float ninf = __int_as_float(0xff800000);
+  float m = ninf, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int key0 = a; key0 < e; key0 += 64) {
+    const E *k = krow(min(key0 + lane, e - 1));
+    float s = 0.f;
+    for (int d = 0; d < D; ++d) s = __builtin_fmaf((float)q[d], (float)k[d], s);
+    s = key0 + lane < e ? s * qscale : ninf;
+    float mx = s;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+    const float mn = fmaxf(m, mx);
+    const float alpha = m == ninf ? 0.f : fast_exp2(m - mn);
+    const float pr = fast_exp2(s - (mn == ninf ? 0.f : mn));
+    m = mn;
+    l = l * alpha + group_sum<64>(pr);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] *= alpha;
+    const int n = min(64, e - key0);
+    for (int j = 0; j < n; ++j) {
+      const float w = __shfl(pr, j, 64);
+      const E *v = vrow(key0 + j) + lane * N;
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = __builtin_fmaf(w, (float)v[i], acc[i]);
+    }
+  }
+  *m_out = m;
+  *l_out = l;
+}
 
 }  // namespace la
