@@ -19,7 +19,7 @@ struct DaKP {
   float *ws_ml, *ws_acc;  // parts: [row of q][head][split] (max, sum) and D values
   int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, o_sb, o_sh, o_st, l_sb, l_sh;
   int32_t Hq, Hkv, ntile, splits, causal, out_dt, zero_rest;
-  float qscale, thr_gap;  // log2(e) scale; 8 / qscale
+  float qscale, thr_gap;  // log2(e) scale; the type's GAP / qscale
 };
 
 constexpr float DA_LN2 = 0.69314718055994530942f;
@@ -135,7 +135,8 @@ __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kv
 // lane; O^T takes P from the same registers (the contraction index is mapped to the keys
 // a lane holds) and V^T by LDS transpose reads.  P is rounded to the inputs' type for
 // that product (to half a step, 2^-8 or 2^-11 of each weight, independently: as much as
-// the output's own rounding); its sum l, and with it lse, is of the fp32 values.
+// the output's own rounding; for fp16 of weights down to 2^-29 of the largest, DaF16); its
+// sum l, and with it lse, is of the fp32 values.
 // What bounds it is the softmax's vector work beside the products (a large bf16 product
 // reaches 1.4 PFLOP/s), and for short sequences a workgroup's beginning and end: 14567
 // tokens of 32 heads on 8 run at 1.12 PFLOP/s as one sequence, 1.05 as four, 0.84 as
@@ -263,8 +264,8 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
     for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, st[1][i]), st[1][i + 1]);
     return mx;
   };
-  // masks tile j where it has to be, and raises the reference maximum only past 2^8 of
-  // headroom (the weights stay below 256); both halves of a row keep the same one
+  // masks tile j where it has to be, and raises the reference maximum only past its
+  // headroom (T::GAP); both halves of a row keep the same one
   auto settle_max = [&](int j, f32x16 (&st)[2], float mx) __attribute__((always_inline)) {
     if (j * DA_BS + DA_BS - 1 > lim_lo) {
       const int d = lim - j * DA_BS - 4 * hf;
@@ -280,7 +281,7 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
       const float alpha = m == da_ninf() ? 0.f : fast_exp2((m - mn) * p.qscale);
       m = mn;
       thr = mn + p.thr_gap;
-      nmu = mn == da_ninf() ? 0.f : -mn * p.qscale;
+      nmu = da_ref<T>(mn, p.qscale);
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt)
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
   if (live && p.splits > 1) {
     const int64_t pi = da_part_at(p, tl, t, h, split);
     if (hf == 0) {
-      p.ws_ml[2 * pi] = m == da_ninf() ? m : m * p.qscale;
+      p.ws_ml[2 * pi] = m == da_ninf() ? m : -nmu;
       p.ws_ml[2 * pi + 1] = l;
     }
 #pragma unroll
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   if (live && p.splits > 1) {
     const int64_t pi = da_part_at(p, tl, t, h, split);
     if (c == 0) {
-      p.ws_ml[2 * pi] = m == da_ninf() ? m : m * p.qscale;
+      p.ws_ml[2 * pi] = m == da_ninf() ? m : -nmu;
       p.ws_ml[2 * pi + 1] = l;
     }
 #pragma unroll
@@ -599,7 +600,7 @@ __global__ __launch_bounds__(256, 2) void dense_few_kernel(DaKP p) {
   if (threadIdx.x == 0) s_bad = 0u;
   FR fr;
   fr.begin((const elem *)p.q + tl.b * p.q_sb + t * p.q_st + (kvh * G + row % G) * p.q_sh);
-  fr.walk(r0 + w, NW, r1, tl.lk, limit(t), p.qscale, 8.f, (elem *)(smem + w * FR::LDS_BYTES),
+  fr.walk(r0 + w, NW, r1, tl.lk, limit(t), p.qscale, (elem *)(smem + w * FR::LDS_BYTES),
           [&](int key) { return kb + key * p.k_st; }, [&](int key) { return vb + key * p.v_st; }, [](int, f32x4) {});
   __syncthreads();
   float *ml = (float *)smem, *vals = ml + NW * 32;
@@ -796,7 +797,7 @@ extern "C" int la_dense_attention(const la_dense_attn_args *a, void *stream) {
   p.ntile = (int32_t)pl.ntile; p.splits = (int32_t)pl.splits;
   p.causal = a->causal != 0; p.out_dt = a->out_dtype; p.zero_rest = a->zero_rest != 0;
   p.qscale = a->scale * 1.44269504088896340736f;
-  p.thr_gap = 8.f / p.qscale;
+  p.thr_gap = std::min((a->dtype == LA_F16 ? DaF16::GAP : DaBf16::GAP) / p.qscale, 3e38f);  // (finite: -inf + it stays)
   hipStream_t st = (hipStream_t)stream;
   int rc;
   const bool d128 = a->D == 128;

@@ -34,7 +34,6 @@ struct EdKP {
   float qscale;
 };
 
-constexpr float ED_GAP = 8.f;  // headroom of the reference maximum, log2 units
 typedef float ed_f4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef int32_t ed_i4 __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -154,7 +153,7 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
   if (threadIdx.x == 0) s_bad = 0u;
   auto krow = [&](int key) -> const elem * { return key == slot ? kn : kc + (int64_t)key * D; };
   auto vrow = [&](int key) -> const elem * { return key == slot ? vn : vc + (int64_t)key * D; };
-  fr.walk(r0 + w, NW, r1, n, n - 1, p.qscale, ED_GAP, (elem *)(smem + w * FR::LDS_BYTES), krow, vrow,
+  fr.walk(r0 + w, NW, r1, n, n - 1, p.qscale, (elem *)(smem + w * FR::LDS_BYTES), krow, vrow,
           [&](int key, f32x4 s) { if (put) *(f32x4 *)(sc + key) = s; });
   // the new token's rows, by the part that holds its slot
   if (slot / FR::RK >= r0 && slot / FR::RK < r1 && w == 0) {

@@ -5,8 +5,8 @@
 // way into registers and V into the wave's own LDS while one is computed; no barrier.
 // S^T = K Q^T by 16x16x32 products straight from the loaded rows (16x16x4 in fp32);
 // O^T += V^T P^T with V^T by LDS transpose reads.  P enters that product as the sum of
-// two terms of the inputs' type (16 bits of each weight), which the matrix cores have
-// room for here.
+// two terms of the inputs' type (16 bits of each weight, in fp16 down to 2^-23 of the row's
+// largest), which the matrix cores have room for here.
 #pragma once
 
 #include "dense_attn.h"
@@ -20,6 +20,7 @@
 namespace la {
 
 struct DaF32 {
+  static constexpr float GAP = 8.f, BIAS = 0.f;
   typedef f32x4 x8;
   typedef float elem;
 };
@@ -68,7 +69,7 @@ struct FewRows {
   // s) gets the row's scores (log2 units, -inf where masked) of keys key .. key + 3.
   template <class KRow, class VRow, class Sink>
   __device__ __forceinline__ void walk(int first, int step, int rounds, int end, int lim, float qscale,
-                                       float thr_gap, elem *smem, KRow krow, VRow vrow, Sink sink) {
+                                       elem *smem, KRow krow, VRow vrow, Sink sink) {
     const int lane = threadIdx.x & 63, c = lane >> 4, ri = lane & 15;
     const float ninf = __int_as_float(0xff800000);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
@@ -137,8 +138,8 @@ struct FewRows {
         const float mn = fmaxf(m, pair32_max(pair16_max(mx)));
         const float alpha = m == ninf ? 0.f : fast_exp2(m - mn);
         m = mn;
-        thr = mn + thr_gap;
-        nmu = mn == ninf ? 0.f : -mn;
+        thr = mn + T::GAP;
+        nmu = da_ref<T>(mn, 1.f);
         l *= alpha;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) acc[dt] *= alpha;
@@ -186,12 +187,12 @@ struct FewRows {
     l = pair32_sum(pair16_sum(l));
   }
 
-  // The wave's state into LDS: (m, l) of row i at ml[2 i], its D values at vals[i D ..]
+  // The wave's state into LDS: (m - BIAS, l) of row i at ml[2 i], its D values at vals[i D ..]
   // (register e of dim tile dt: dim 16 dt + 4 c + e).
   __device__ __forceinline__ void put(float *ml, float *vals) const {
     const int lane = threadIdx.x & 63, c = lane >> 4, ri = lane & 15;
     if (c == 0) {
-      ml[2 * ri] = m;
+      ml[2 * ri] = m == __int_as_float(0xff800000) ? m : -nmu;
       ml[2 * ri + 1] = l;
     }
 #pragma unroll
