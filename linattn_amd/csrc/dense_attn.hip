@@ -86,14 +86,35 @@ __device__ void da_rest(const DaKP &p, const DaTile &tl, int R, int kvh, int spl
 // Rows r_first + i, i = i0, i0 + step, .. below NR, whose results are not finite, of which
 // bit i of `bad` says so: those with an infinity or NaN of V among what their tiles (keys
 // a .. end - 1) held and they do not see are done again; the others stand, but for ALL
-// (few_row).  (What a tile holds past the last key is that key again.)  Called last, when
-// the rows are stored and the registers free.
-template <class E, int D, int NR, bool ALL>
+// (few_row), and in fp16, where a weight below 2^-40 of the row's largest is 0 and its
+// product with an infinity NaN: a dim's first keys with NaN and either infinity say what it
+// is for each row.  (What a tile holds past the last key is that key again.)  Called last,
+// when the rows are stored and the registers free.
+template <class T, int D, int NR, bool ALL>
 __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kvh, int split, int r_first,
                                           uint32_t bad, int a, int end, int i0, int step) {
+  typedef typename T::elem E;
   const int lane = threadIdx.x & 63, G = p.s.G;
   const E *kb = (const E *)p.k + (p.s.cu_q ? tl.k0 * p.k_st : tl.b * p.k_sb) + kvh * p.k_sh;
   const E *vb = (const E *)p.v + (p.s.cu_q ? tl.k0 * p.v_st : tl.b * p.v_sb) + kvh * p.v_sh;
+  constexpr bool LOST = !ALL && T::BIAS > 0.f;
+  constexpr int N = D / 64;
+  const float inf = __int_as_float(0x7f800000);
+  int32_t at[3][N];  // of dim lane + 64 x
+#pragma unroll
+  for (int x = 0; x < N; ++x) at[0][x] = at[1][x] = at[2][x] = INT32_MAX;
+  if constexpr (LOST) {
+    const int32_t e = min(end, tl.lk);
+#pragma unroll 8
+    for (int32_t key = a; key < e; ++key)
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const float v = (float)vb[key * p.v_st + lane + 64 * x];
+        at[0][x] = min(at[0][x], v != v ? key : INT32_MAX);
+        at[1][x] = min(at[1][x], v == inf ? key : INT32_MAX);
+        at[2][x] = min(at[2][x], v == -inf ? key : INT32_MAX);
+      }
+  }
   wait_vmcnt<0>();  // (stores over those)
 #pragma unroll 1
   for (int i = i0; i < NR; i += step) {
@@ -103,10 +124,20 @@ __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kv
     bool met = ALL;
     for (int key = max(max(lim + 1, a), 0); key < end && !ALL; ++key)
       for (int d = lane; d < D; d += 64)
-        met = met || !(fabsf((float)vb[(int64_t)min(key, tl.lk - 1) * p.v_st + d]) < __int_as_float(0x7f800000));
-    if (__ballot(met) == 0) continue;
+        met = met || !(fabsf((float)vb[(int64_t)min(key, tl.lk - 1) * p.v_st + d]) < inf);
+    if (__ballot(met) == 0) {
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        const bool up = at[1][x] <= lim, down = at[2][x] <= lim, nan = at[0][x] <= lim || (up && down);
+        if (!nan && !up && !down) continue;
+        const float y = nan ? __int_as_float(0x7fc00000) : up ? inf : -inf;
+        if (p.splits > 1) p.ws_acc[da_part_at(p, tl, t, h, split) * D + lane + 64 * x] = y;
+        else da_store1(p.out, da_out_at(p, tl, t, h) + lane + 64 * x, p.out_dt, y);
+      }
+      continue;
+    }
     const E *q = (const E *)p.q + (p.s.cu_q ? (tl.q0 + t) * p.q_st : tl.b * p.q_sb + t * p.q_st) + h * p.q_sh;
-    float m, l, acc[D / 64];
+    float m, l, acc[N];
     few_row<E, D>(q, [&](int key) { return kb + key * p.k_st; }, [&](int key) { return vb + key * p.v_st; }, a,
                   min(end, lim + 1), p.qscale, &m, &l, acc);
     if (p.splits > 1) {
@@ -115,12 +146,12 @@ __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kv
         p.ws_ml[2 * pi] = m;
         p.ws_ml[2 * pi + 1] = l;
       }
-      for (int x = 0; x < D / 64; ++x) p.ws_acc[pi * D + lane * (D / 64) + x] = acc[x];
+      for (int x = 0; x < N; ++x) p.ws_acc[pi * D + lane * N + x] = acc[x];
       continue;
     }
     const int64_t o = da_out_at(p, tl, t, h);
-    for (int x = 0; x < D / 64; ++x)
-      da_store1(p.out, o + lane * (D / 64) + x, p.out_dt, l == 0.f ? 0.f : acc[x] / l);
+    for (int x = 0; x < N; ++x)
+      da_store1(p.out, o + lane * N + x, p.out_dt, l == 0.f ? 0.f : acc[x] / l);
     if (p.lse && lane == 0) p.lse[da_lse_at(p, tl, t, h)] = l == 0.f ? da_ninf() : (m + __log2f(l)) * DA_LN2;
   }
 }
@@ -340,13 +371,13 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
   }
   if (!wave_live) return;
   l = pair32_sum(l);
-  // results that are not finite, and what their rows do not see
+  // results that are not finite (with scores that are not numbers, l is not, and the row stands)
   float sum = 0.f;
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[dt][i], 0.f, sum);
-  const uint64_t bad = __ballot(sum != 0.f);  // (NaN)
+  const uint64_t bad = __ballot(sum != 0.f && l < __int_as_float(0x7f800000));  // (sum: NaN)
   // register i of dim tile dt holds dim 32 dt + 8 (i / 4) + 4 hf + i % 4
   if (live && p.splits > 1) {
     const int64_t pi = da_part_at(p, tl, t, h, split);
@@ -390,7 +421,7 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
     if (p.lse && hf == 0) p.lse[da_lse_at(p, tl, t, h)] = none ? da_ninf() : (__log2f(l) - nmu) * DA_LN2;  // (as rounded in the weights)
   }
   if (bad != 0)
-    da_again<elem, D, 32, false>(p, tl, kvh, split, r_first, (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
+    da_again<T, D, 32, false>(p, tl, kvh, split, r_first, (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
                                  j0 * DA_BS, min(j1, lim_hi / DA_BS + 1) * DA_BS, 0, 1);
 }
 
@@ -539,7 +570,7 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   for (int dt = 0; dt < NS; ++dt)
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(acc[dt][e], 0.f, sum);
-  uint64_t bad = __ballot(sum != 0.f);
+  uint64_t bad = __ballot(sum != 0.f && l < __int_as_float(0x7f800000));
   // register e of dim tile dt holds dim 16 dt + 4 c + e
   if (live && p.splits > 1) {
     const int64_t pi = da_part_at(p, tl, t, h, split);
@@ -561,7 +592,7 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
   }
   if (bad != 0) {
     bad |= bad >> 32;
-    da_again<float, D, 16, false>(p, tl, kvh, split, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
+    da_again<DaF32, D, 16, false>(p, tl, kvh, split, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
                                   j0 * BS, min(j1, lim_hi / BS + 1) * BS, 0, 1);
   }
 }
@@ -636,7 +667,7 @@ __global__ __launch_bounds__(256, 2) void dense_few_kernel(DaKP p) {
   if (s_bad == 0u) return;
   wait_vmcnt<0>();
   __syncthreads();  // (every wave's stores are done, which those of the rows done again replace)
-  da_again<elem, D, 16, true>(p, tl, kvh, split, 0, s_bad, r0 * FR::RK, r1 * FR::RK, w, NW);
+  da_again<T, D, 16, true>(p, tl, kvh, split, 0, s_bad, r0 * FR::RK, r1 * FR::RK, w, NW);
 }
 
 // Joins the parts of a row: a wave a row (4-6 us, its launch).

@@ -78,3 +78,21 @@ def test_decode_step(dev, dtype, D, B, Hkv, G, C, lens):
             m = plain.n[b]
             assert torch.equal(vd[b, :, :m].cpu(), plain.v[b, :, :m])
             close(wd[b, :, :m], plain.w[b, :, :m], plain.tol[b, :, :m], where)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,T", [(1, 300), (4, 150)])
+def test_prompt_with_weights_of_every_size(dev, dtype, G, T):
+    """Whole prompts, the infinities at keys whose weights lie up to 70 powers of two below the
+    row's largest."""
+    D = 64
+    q, k, v = (_rand(i, 1, h, T, D, dtype=dtype) for i, h in ((0, G), (1, 1), (2, 1)))
+    q[..., 0], k[..., 0] = 1.0, torch.linspace(0.0, -48.0, T).to(dtype)
+    v[0, 0, 3, 1], v[0, 0, T // 2, 2], v[0, 0, T - 9, 3], v[0, 0, T - 9, 4] = math.inf, -math.inf, math.inf, math.nan
+    v[0, 0, 20, 3], v[0, 0, 21, 5], v[0, 0, T - 30, 5] = math.inf, math.inf, -math.inf
+    out, lse = (y.cpu() for y in dense_attention(q.to(dev), k.to(dev), v.to(dev), scale=1.0, return_lse=True))
+    for h in range(G):
+        o, ls, tol, tol_l = attention(q[0, h], k[0, 0], v[0, 0], True, 1.0, HALF_STEP[dtype])
+        assert torch.equal(out[0, h].isnan(), o.isnan())
+        close(out[0, h].nan_to_num(0, math.inf, -math.inf), o.nan_to_num(0, math.inf, -math.inf), tol.nan_to_num(0, math.inf))
+        close(lse[0, h], ls, tol_l)
