@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
         float nl = products(j, h, sa);
         const int t = tb + ((32 * h + r32) & (qpt - 1));
         if (t >= x.t.lq) nl = none;
-        const int seen = p.causal ? diag + t : x.t.lk - 1;
+        const int seen = nl == none ? -1 : p.causal ? diag + t : x.t.lk - 1;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           // register i: key 8 (i / 4) + 4 hf + i % 4
@@ -280,11 +280,13 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
       if (j + 2 < n) wait_vmcnt<2 * PER>();
       else if (j + 1 < n) wait_vmcnt<PER>();
       else wait_vmcnt<0>();
+      // (a row with lse -inf adds nothing even where its scores are not numbers; the wave's own copy)
+      const uint64_t absent = __ballot(s_lse[j % NSLOT][w][lane] == none);
       lds_barrier();  // for every wave, and tile j - 1 is read
       if (j + NSLOT - 1 < n) dma((j + NSLOT - 1) % NSLOT);
       if (j % KW_RUN == KW_RUN - 1) fold_in();
       if (tb + qpt <= t_any) continue;
-      const bool whole = t_all <= tb && tb + qpt <= x.t.lq;
+      const bool whole = t_all <= tb && tb + qpt <= x.t.lq && absent == 0;
       if (whole) {
         const float na = products(j, 0, sa);
         weigh(sb, nb);
@@ -361,8 +363,11 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
         seen[h] = p.causal ? diag + t : x.t.lk - 1;
       }
       wait_vmcnt<0>();
-      settle(nl[0]);
-      settle(nl[1]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        settle(nl[h]);
+        if (nl[h] == __int_as_float(0xff800000)) seen[h] = -1;
+      }
       lds_barrier();
       if (j + 1 < n) dma((j + 1) & 1);
       if (j % KW_RUN == KW_RUN - 1) {

@@ -67,8 +67,9 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, *, causal: 
     of its group and the last ``last`` queries (default all) of exp(scale q . k_s - lse).
 
     q (B, Hq, Tq, D), k (B, Hkv, Tk, D), ``lse`` (B, Hq, Tq) as ``dense_attention`` returned it
-    for the same ``causal``, ``scale``, ``lengths`` and ``q_lengths``.  Returns (B, Hkv, Tk)
-    in float32, 0 past a sequence's keys; with ``out`` the weights are added to it (the
+    for the same ``causal``, ``scale``, ``lengths`` and ``q_lengths``; a query whose lse is -inf
+    adds nothing, whatever its row of q holds.  Returns (B, Hkv, Tk) in float32, 0 past a
+    sequence's keys; with ``out`` the weights are added to it (the
     weights of chunk after chunk of a prompt).  Sums are in a fixed order."""
     what = "key_weights"
     dev = N.require_gpu(q, k, lse, lengths, q_lengths, out, what=what)
