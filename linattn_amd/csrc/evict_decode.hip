@@ -81,10 +81,10 @@ __device__ __forceinline__ int32_t ed_victim(const EdKP &p, int64_t pair, int64_
 __device__ __forceinline__ int32_t ed_held(const EdKP &p, int b) { return min(max(p.lengths[b], 0), p.C); }
 
 // Rows' weights over entries first .. end - 1 (first a multiple of 4) added to what they
-// gathered; lse2 in LDS.
+// gathered; in LDS their references (log2 units) and the reciprocals of their sums.
 template <int NT>
 __device__ __forceinline__ void ed_weights(const EdKP &p, int64_t pair, int32_t slot, int32_t first, int32_t end,
-                                           const float *lse2) {
+                                           const float *ref, const float *inv) {
   const float *s = p.scores + pair * p.G * p.cs;
   float *w = p.weights + pair * p.C;
   for (int32_t i = first + 4 * (int32_t)threadIdx.x; i < end; i += 4 * NT) {
@@ -103,11 +103,11 @@ __device__ __forceinline__ void ed_weights(const EdKP &p, int64_t pair, int32_t 
 #pragma unroll 4
     for (int g = 0; g < p.G; ++g) {
       const float4 x = *(const float4 *)(s + g * p.cs + i);  // (scores are there for whole rounds)
-      const float l = lse2[g];
-      sum[0] += fast_exp2(x.x - l);
-      sum[1] += fast_exp2(x.y - l);
-      sum[2] += fast_exp2(x.z - l);
-      sum[3] += fast_exp2(x.w - l);
+      const float m = ref[g], f = inv[g];
+      sum[0] += fast_exp2(__builtin_fmaf(x.x, p.qscale, -m)) * f;
+      sum[1] += fast_exp2(__builtin_fmaf(x.y, p.qscale, -m)) * f;
+      sum[2] += fast_exp2(__builtin_fmaf(x.z, p.qscale, -m)) * f;
+      sum[3] += fast_exp2(__builtin_fmaf(x.w, p.qscale, -m)) * f;
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] = (i + e == slot ? 0.f : old[e]) + sum[e];
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
   constexpr int LDS_MERGE = NW * (FR::VALS + 32) * 4;
   constexpr int LDS = NW * FR::LDS_BYTES > LDS_MERGE ? NW * FR::LDS_BYTES : LDS_MERGE;
   __shared__ __align__(16) char smem[LDS];
-  __shared__ float lse2[16];
+  __shared__ float ref[16], inv[16];
   __shared__ uint32_t s_bad;  // rows to be done again (few_row)
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t pair = blockIdx.x / (uint32_t)p.splits;
@@ -191,7 +191,10 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
       }
     } else {
       store_from_f32(p.out, b * p.o_sb + (kvh * p.G + g) * p.o_sh + d, p.out_dt, a / l);
-      if (d == 0) lse2[g] = m + __log2f(l);
+      if (d == 0) {
+        ref[g] = m;
+        inv[g] = 1.f / l;
+      }
     }
   }
   __syncthreads();
@@ -216,14 +219,14 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
     }
   }
   if (p.splits > 1) return;
-  ed_weights<256>(p, pair, slot, 0, n, lse2);
+  ed_weights<256>(p, pair, slot, 0, n, ref, inv);
 }
 
 // Parts joined: a pair's output and the weights of 1024 entries a workgroup.
 constexpr int ED_CHUNK = 1024;
 template <int D>
 __global__ __launch_bounds__(256) void evict_join_kernel(EdKP p) {
-  __shared__ float lse2[16], part[16][64];  // part: what each part's values count for
+  __shared__ float ref[16], inv[16], part[16][64];  // part: what each part's values count for
   const int64_t pair = blockIdx.x / (uint32_t)p.chunks;
   const int chunk = (int)(blockIdx.x % (uint32_t)p.chunks), lane = threadIdx.x & 63;
   const int b = (int)(pair / p.Hkv), kvh = (int)(pair % p.Hkv);
@@ -235,10 +238,12 @@ __global__ __launch_bounds__(256) void evict_join_kernel(EdKP p) {
     float m = x.x;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    const float l = group_sum<64>(x.y * fast_exp2(x.x - (m == ninf ? 0.f : m)));
-    const float z = (m == ninf ? 0.f : m) + __log2f(l);
-    part[g][lane] = fast_exp2(x.x - z);
-    if (lane == 0) lse2[g] = z;
+    const float f = fast_exp2(x.x - (m == ninf ? 0.f : m)), f_l = 1.f / group_sum<64>(x.y * f);
+    part[g][lane] = f * f_l;
+    if (lane == 0) {
+      ref[g] = m;
+      inv[g] = f_l;
+    }
   }
   __syncthreads();
   for (int e = threadIdx.x + 256 * chunk; e < p.G * D; e += 256 * p.chunks) {
@@ -249,7 +254,7 @@ __global__ __launch_bounds__(256) void evict_join_kernel(EdKP p) {
     for (int x = 0; x < p.splits; ++x) a = __builtin_fmaf(v[(int64_t)x * p.G * D], part[g][x], a);
     store_from_f32(p.out, b * p.o_sb + (kvh * p.G + g) * p.o_sh + d, p.out_dt, a);
   }
-  ed_weights<256>(p, pair, slot, chunk * ED_CHUNK, min(n, (chunk + 1) * ED_CHUNK), lse2);
+  ed_weights<256>(p, pair, slot, chunk * ED_CHUNK, min(n, (chunk + 1) * ED_CHUNK), ref, inv);
 }
 
 // ------------------------------------------------------------------ host ----

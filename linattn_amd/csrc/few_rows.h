@@ -66,12 +66,15 @@ struct FewRows {
   // Rounds first, first + step, ... below `rounds`, over keys round * RK ..  krow(key) and
   // vrow(key) point at a key's rows and are asked for keys < end only (keys past it are
   // the last one again, masked).  `lim` is the last key that row lane % 16 sees.  sink(key,
-  // s) gets the row's scores (log2 units, -inf where masked) of keys key .. key + 3.
+  // s) gets the row's scores (not scaled, -inf where masked) of keys key .. key + 3.  A weight
+  // takes its score, the scale and the reference in one fma: what is rounded is their
+  // difference, not a score that may be far larger.
   template <class KRow, class VRow, class Sink>
   __device__ __forceinline__ void walk(int first, int step, int rounds, int end, int lim, float qscale,
                                        elem *smem, KRow krow, VRow vrow, Sink sink) {
     const int lane = threadIdx.x & 63, c = lane >> 4, ri = lane & 15;
     const float ninf = __int_as_float(0xff800000);
+    const float thr_gap = fminf(T::GAP / qscale, 3e38f);  // (finite: -inf + it stays)
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
     x8 kn[RK / 16][NK];
     auto fetch = [&](int r, int slot) {
@@ -111,15 +114,21 @@ struct FewRows {
 #pragma unroll
       for (int kt = 0; kt < RK / 16; ++kt) {
         st[kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        // four sums: one chain of all dims would round four times as often (one token over 9000
+        // fp32 keys: outputs off by 3.4e-7 of their norm in place of 1.1e-6)
+        if constexpr (F32) {
+          f32x4 part[4];
 #pragma unroll
-        for (int s = 0; s < NK; ++s) {
-          if constexpr (F32) {
+          for (int e = 0; e < 4; ++e) {
+            part[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              st[kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[kt][s][e], qf[s][e], st[kt], 0, 0, 0);
-          } else {
-            st[kt] = T::mfma16(kc[kt][s], qf[s], st[kt]);
+            for (int s = 0; s < NK; ++s)
+              part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kc[kt][s][e], qf[s][e], part[e], 0, 0, 0);
           }
+          st[kt] = (part[0] + part[1]) + (part[2] + part[3]);
+        } else {
+#pragma unroll
+          for (int s = 0; s < NK; ++s) st[kt] = T::mfma16(kc[kt][s], qf[s], st[kt]);
         }
       }
       // register e: key 4 c + e
@@ -129,17 +138,17 @@ struct FewRows {
       for (int kt = 0; kt < RK / 16; ++kt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          st[kt][e] = 16 * kt + e <= d ? st[kt][e] * qscale : ninf;
+          st[kt][e] = 16 * kt + e <= d ? st[kt][e] : ninf;
           mx = fmaxf(mx, st[kt][e]);
         }
         sink(r * RK + 16 * kt + 4 * c, st[kt]);
       }
       if (__ballot(mx > thr) != 0) {
         const float mn = fmaxf(m, pair32_max(pair16_max(mx)));
-        const float alpha = m == ninf ? 0.f : fast_exp2(m - mn);
+        const float alpha = m == ninf ? 0.f : fast_exp2((m - mn) * qscale);
         m = mn;
-        thr = mn + T::GAP;
-        nmu = da_ref<T>(mn, 1.f);
+        thr = mn + thr_gap;
+        nmu = da_ref<T>(mn, qscale);
         l *= alpha;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) acc[dt] *= alpha;
@@ -149,7 +158,7 @@ struct FewRows {
       for (int kt = 0; kt < RK / 16; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          st[kt][e] = fast_exp2(st[kt][e] + nmu);
+          st[kt][e] = fast_exp2(__builtin_fmaf(st[kt][e], qscale, nmu));
           part += st[kt][e];
         }
       l += part;
@@ -187,7 +196,7 @@ struct FewRows {
     l = pair32_sum(pair16_sum(l));
   }
 
-  // The wave's state into LDS: (m - BIAS, l) of row i at ml[2 i], its D values at vals[i D ..]
+  // The wave's state into LDS: (reference in log2 units, l) of row i at ml[2 i], its D values at vals[i D ..]
   // (register e of dim tile dt: dim 16 dt + 4 c + e).
   __device__ __forceinline__ void put(float *ml, float *vals) const {
     const int lane = threadIdx.x & 63, c = lane >> 4, ri = lane & 15;
