@@ -682,8 +682,9 @@ int la_block_sparse_prefill(const la_prefill_args *a, void *stream);
  * Unit stride over D; every row 16-byte aligned, key rows less than 2^24 values apart.
  * D 64 or 128; dtype LA_F32, LA_BF16 or
  * LA_F16, out_dtype that or LA_F32.  lse (optional, fp32) has strides l_sb, l_sh and 1.
- * scale must be positive.  Workspace: la_dense_attention_workspace() bytes, 256-byte
- * aligned (the parts of few rows over many keys, which several workgroups share).
+ * scale must be positive; out shares no memory with q, k and v.  Workspace:
+ * la_dense_attention_workspace() bytes, 256-byte aligned (the parts of few rows over many
+ * keys, which several workgroups share).
  */
 typedef struct {
   const void *q;
@@ -808,7 +809,8 @@ int la_evict_kv(const la_evict_args *a, void *stream);
  * q, out (B, Hq, 1, D), k_new, v_new (B, Hkv, 1, D) (strides *_sb, *_sh, unit over D, rows
  * 16-byte aligned); k, v (B, Hkv, C, D), weights and positions (B, Hkv, C), contiguous.
  * lengths and pos (int32 [B]) are the caller's to advance.  dtype LA_F32, LA_BF16 or
- * LA_F16, out_dtype that or LA_F32; D 64 or 128; Hq / Hkv at most 16; C < 2^24.
+ * LA_F16, out_dtype that or LA_F32; D 64 or 128; Hq / Hkv at most 16; C < 2^24.  What is
+ * written (k, v, weights, positions, out) shares no memory with anything else.
  * Workspace: la_evict_decode_workspace() bytes, 256-byte aligned.
  */
 typedef struct {

@@ -43,6 +43,35 @@ int indexer_status(uint32_t *bits, bool clear, hipStream_t st);
       return ::la::fail(LA_ERR_HIP, "kernel launch failed: %s", hipGetErrorString(_e)); \
   } while (0)
 
+// What a tensor covers: runs of `run` bytes from `p` on, by dims of (stride in bytes, count).
+struct Cover {
+  struct Dim {
+    int64_t stride, count;
+  };
+  int64_t p, run, end;  // (run 0: nothing; p is its lowest byte, end is behind its last)
+  Dim dim[3];
+  Cover(const void *at, int64_t bytes, Dim x = {0, 1}, Dim y = {0, 1}, Dim z = {0, 1})
+      : p((int64_t)(uintptr_t)at), run(at ? bytes : 0), dim{x, y, z} {
+    int64_t up = run;
+    for (Dim &d : dim) {
+      if (d.count <= 0) run = 0;
+      if (d.count <= 1) d = Dim{0, 1};
+      (d.stride < 0 ? p : up) += d.stride * (d.count - 1);
+      if (d.stride < 0) {
+        up -= d.stride * (d.count - 1);
+        d.stride = -d.stride;
+      }
+    }
+    end = p + up;
+  }
+};
+// Whether two of them have a byte in common.  Exact for strides that nest, as those of views
+// do; true where the search grows past a few thousand steps.
+bool overlap_runs(const Cover &a, const Cover &b);
+inline bool overlap(const Cover &a, const Cover &b) {
+  return a.run > 0 && b.run > 0 && a.p < b.end && b.p < a.end && overlap_runs(a, b);
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 inline int ilog2(int64_t x) {

@@ -807,6 +807,15 @@ extern "C" int la_dense_attention(const la_dense_attn_args *a, void *stream) {
     if (int rc = da_rows_ok("v", a->v, esz, sb(a->v_sb), a->v_sh, a->v_st, a->Hkv, a->Tk)) return rc;
   }
   if (int rc = da_rows_ok("out", a->out, osz, sb(a->o_sb), a->o_sh, a->o_st, a->Hq, a->Tq)) return rc;
+  const int64_t nb = packed ? 1 : a->B;
+  auto cover = [&](const void *x, int64_t es, int64_t b, int64_t h, int64_t t, int64_t heads, int64_t rows) {
+    return Cover(x, a->D * es, {b * es, nb}, {h * es, heads}, {t * es, rows});
+  };
+  const Cover out = cover(a->out, osz, a->o_sb, a->o_sh, a->o_st, a->Hq, a->Tq);
+  LA_REQUIRE(!overlap(out, cover(a->q, esz, a->q_sb, a->q_sh, a->q_st, a->Hq, a->Tq)) &&
+                 !overlap(out, cover(a->k, esz, a->k_sb, a->k_sh, a->k_st, a->Hkv, a->Tk)) &&
+                 !overlap(out, cover(a->v, esz, a->v_sb, a->v_sh, a->v_st, a->Hkv, a->Tk)),
+             "la_dense_attention: out shares memory with an input");
   const DaPlan pl = da_plan(a);
   if (pl.bytes > 0 && (!a->workspace || a->ws_bytes < (int64_t)pl.bytes))
     return fail(LA_ERR_WORKSPACE, "la_dense_attention: workspace %lld < %lld bytes", (long long)a->ws_bytes,

@@ -319,6 +319,17 @@ extern "C" int la_evict_decode(const la_evict_decode_args *a, void *stream) {
   LA_REQUIRE(ok(a->q, a->q_sb, a->q_sh, a->Hq) && ok(a->k_new, a->kn_sb, a->kn_sh, a->Hkv) &&
                  ok(a->v_new, a->vn_sb, a->vn_sh, a->Hkv) && (uintptr_t)a->k % 16 == 0 && (uintptr_t)a->v % 16 == 0,
              "la_evict_decode: rows must be 16-byte aligned");
+  const int64_t es = a->dtype == LA_F32 ? 4 : 2, os = a->out_dtype == LA_F32 ? 4 : 2, slots = a->B * a->Hkv * a->C;
+  auto rows = [&](const void *x, int64_t e, int64_t sb, int64_t sh, int64_t heads) {
+    return Cover(x, a->D * e, {sb * e, a->B}, {sh * e, heads});
+  };
+  const Cover cov[] = {Cover(a->k, slots * a->D * es), Cover(a->v, slots * a->D * es), Cover(a->weights, slots * 4),
+                       Cover(a->positions, slots * 4), rows(a->out, os, a->o_sb, a->o_sh, a->Hq),  // written
+                       rows(a->q, es, a->q_sb, a->q_sh, a->Hq), rows(a->k_new, es, a->kn_sb, a->kn_sh, a->Hkv),
+                       rows(a->v_new, es, a->vn_sb, a->vn_sh, a->Hkv), Cover(a->lengths, a->B * 4), Cover(a->pos, a->B * 4)};
+  for (int i = 0; i < 5; ++i)
+    for (int j = i + 1; j < 10; ++j)
+      LA_REQUIRE(!overlap(cov[i], cov[j]), "la_evict_decode: caches, weights, positions, out or inputs share memory");
   const EdPlan pl = ed_plan(a);
   if (!a->workspace || a->ws_bytes < (int64_t)pl.bytes)
     return fail(LA_ERR_WORKSPACE, "la_evict_decode: workspace %lld < %lld bytes", (long long)a->ws_bytes,

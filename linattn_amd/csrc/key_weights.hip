@@ -488,6 +488,12 @@ extern "C" int la_key_weights(const la_key_weights_args *a, void *stream) {
                  (a->Tq == 0 || ok(a->q, a->q_sb, a->q_sh, a->q_st, a->Hq, a->Tq)),
              "la_key_weights: rows of q and k must be 16-byte aligned");
   LA_REQUIRE(a->Tq <= 1 || (a->q_st >= 0 && a->q_st < (1 << 24)), "la_key_weights: query rows 2^24 values apart or more");
+  const int64_t nb = packed ? 1 : a->B, es = a->dtype == LA_F32 ? 4 : 2;
+  const Cover out(a->out, 4 * a->Tk, {4 * a->w_sb, nb}, {4 * a->w_sh, a->Hkv});
+  LA_REQUIRE(!overlap(out, Cover(a->q, a->D * es, {es * a->q_sb, nb}, {es * a->q_sh, a->Hq}, {es * a->q_st, a->Tq})) &&
+                 !overlap(out, Cover(a->k, a->D * es, {es * a->k_sb, nb}, {es * a->k_sh, a->Hkv}, {es * a->k_st, a->Tk})) &&
+                 !overlap(out, Cover(a->lse, 4 * a->Tq, {4 * a->l_sb, nb}, {4 * a->l_sh, a->Hq})),
+             "la_key_weights: out shares memory with an input");
   const KwPlan pl = kw_plan(a);
   if (pl.bytes > 0 && (!a->workspace || a->ws_bytes < (int64_t)pl.bytes))
     return fail(LA_ERR_WORKSPACE, "la_key_weights: workspace %lld < %lld bytes", (long long)a->ws_bytes,

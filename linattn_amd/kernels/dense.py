@@ -72,7 +72,8 @@ def _check_qk(what: str, q: torch.Tensor, k: torch.Tensor, dims: int, head: int)
 
 def _apart(what: str, out: torch.Tensor, *inputs: torch.Tensor) -> None:
     """Refuses an ``out`` that holds a row twice, starts where an input does, or whose memory
-    is part of a contiguous input's (views that interleave with ``out`` pass)."""
+    is part of a contiguous input's (the library looks at what is left, byte by byte: views
+    that interleave with ``out`` pass)."""
     if out.numel() == 0:
         return
     if any(s == 0 and d > 1 for s, d in zip(out.stride(), out.shape)):

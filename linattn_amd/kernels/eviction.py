@@ -244,8 +244,9 @@ def evict_decode_step(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     every entry's weight grows by the weights they gave it.  Returns (B, Hq, 1, D) in
     ``out_dtype`` (default q's, or float32), or in ``out``.
 
-    The caller advances ``lengths`` (to at most C) and ``pos``.  Caches are contiguous, and
-    a call's are not another's: two streams may run two calls on caches of their own."""
+    The caller advances ``lengths`` (to at most C) and ``pos``.  Caches are contiguous, share
+    no memory with one another or with other arguments, and a call's are not another's: two
+    streams may run two calls on caches of their own."""
     what = "evict_decode_step"
     dev = N.require_gpu(q, k_new, v_new, k_cache, v_cache, weights, positions, lengths, pos, out,
                         what=what)
@@ -259,7 +260,8 @@ def evict_decode_step(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     if v_cache.shape != k_cache.shape or v_cache.dtype != q.dtype or \
             not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError(f"{what}: caches must be contiguous (B, Hkv, C, D) in q's dtype")
-    if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+    kp, vp, wp, pp = k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr(), positions.data_ptr()
+    if kp % 16 or vp % 16:
         raise ValueError(f"{what}: caches must be 16-byte aligned")
     for t in (k_new, v_new):
         if t.shape != (B, Hkv, 1, D) or t.dtype != q.dtype:
@@ -272,16 +274,15 @@ def evict_decode_step(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
     lengths, pos = _int32(lengths, (B,), "lengths"), _int32(pos, (B,), "pos")
     if recent < 0 or sink < 0 or recent + sink >= C:
         raise ValueError(f"{what}: sink + recent must leave an entry of the cache to evict")
-    if B > 0 and (k_cache.data_ptr() == v_cache.data_ptr() or weights.data_ptr() == positions.data_ptr() or
-                  {k_new.data_ptr(), v_new.data_ptr()} & {k_cache.data_ptr(), v_cache.data_ptr()}):
+    if B > 0 and (kp == vp or wp == pp or k_new.data_ptr() in (kp, vp) or v_new.data_ptr() in (kp, vp)):
         raise ValueError(f"{what}: caches, weights, positions and the new rows share memory")
     out = _out(what, out, q, out_dtype, k_new, v_new, k_cache, v_cache, weights, positions)
     if B == 0:
         return out
     q, k_new, v_new = _rows(q), _rows(k_new), _rows(v_new)
     a = N.LaEvictDecodeArgs(
-        q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-        weights.data_ptr(), positions.data_ptr(), lengths.data_ptr(), pos.data_ptr(), out.data_ptr(), None, 0,
+        q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), kp, vp, wp, pp, lengths.data_ptr(), pos.data_ptr(),
+        out.data_ptr(), None, 0,
         B, Hq, Hkv, C, D, *q.stride()[:2], *k_new.stride()[:2], *v_new.stride()[:2], *out.stride()[:2], recent,
         sink, _scale(scale, D), N.dtype_code(q.dtype), N.dtype_code(out.dtype), 0)
     L, ref = N.load(), ctypes.byref(a)
