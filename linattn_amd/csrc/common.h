@@ -72,6 +72,9 @@ inline bool overlap(const Cover &a, const Cover &b) {
   return a.run > 0 && b.run > 0 && a.p < b.end && b.p < a.end && overlap_runs(a, b);
 }
 
+// Whether a launch may have that many workgroups (2^32 threads are too many).
+inline bool grid_fits(int64_t workgroups, int64_t threads) { return workgroups < ((int64_t)1 << 32) / threads; }
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 inline int ilog2(int64_t x) {

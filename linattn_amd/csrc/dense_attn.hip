@@ -822,7 +822,7 @@ extern "C" int la_dense_attention(const la_dense_attn_args *a, void *stream) {
                 (long long)pl.bytes);
   LA_REQUIRE((uintptr_t)a->workspace % 256 == 0 || pl.bytes == 0, "la_dense_attention: workspace alignment");
   const int64_t wgs = pl.ntile * a->Hkv * pl.splits;
-  LA_REQUIRE(pl.ntile < ((int64_t)1 << 31) && wgs < ((int64_t)1 << 31) / 64, "la_dense_attention: too many rows");
+  LA_REQUIRE(grid_fits(wgs, 256), "la_dense_attention: too many rows");
   DaKP p{};
   p.s = DaSeqs{a->cu_q, a->cu_k, a->q_len, a->k_len, a->Tq, a->Tk, (int32_t)a->B, (int32_t)(a->Hq / a->Hkv)};
   p.q = a->q; p.k = a->k; p.v = a->v; p.out = a->out; p.lse = a->lse;

@@ -674,8 +674,6 @@ extern "C" int la_evict_kv(const la_evict_args *a, void *stream) {
     return fail(LA_ERR_WORKSPACE, "la_evict_kv: workspace %lld < %lld bytes", (long long)a->ws_bytes,
                 (long long)pl.bytes);
   LA_REQUIRE(pl.bytes == 0 || (uintptr_t)a->workspace % 256 == 0, "la_evict_kv: workspace alignment");
-  LA_REQUIRE(a->B * a->Hkv * (std::max<int64_t>(pl.slices, 1) + ceil_div(a->capacity, EV_SLOTS)) < ((int64_t)1 << 31),
-             "la_evict_kv: too many entries");
   EvKP p{};
   p.k = (const char *)a->k; p.v = (const char *)a->v; p.weights = a->weights;
   p.positions = a->positions; p.pos = a->pos; p.lengths = a->lengths; p.cu = a->cu;
@@ -694,6 +692,7 @@ extern "C" int la_evict_kv(const la_evict_args *a, void *stream) {
   const uint32_t rows = (uint32_t)(a->B * a->Hkv);
   const int32_t parts = (int32_t)ceil_div(a->capacity, EV_SLOTS);
   if (a->T <= EV_SMALL) {
+    LA_REQUIRE(grid_fits((int64_t)rows * parts, 256), "la_evict_kv: too many slots");
     if (a->positions) evict_small_kernel<true><<<rows * (uint32_t)parts, 256, 0, st>>>(p, parts);
     else evict_small_kernel<false><<<rows * (uint32_t)parts, 256, 0, st>>>(p, parts);
     LA_LAUNCHED();
@@ -703,13 +702,16 @@ extern "C" int la_evict_kv(const la_evict_args *a, void *stream) {
   p.open = (int32_t)ceil_div(a->budget - (a->positions ? 0 : a->recent), EV_SLOTS);
   p.early = parts - p.open;
   const uint32_t early = rows * (uint32_t)p.early;
+  LA_REQUIRE(grid_fits((int64_t)rows * p.open, 256), "la_evict_kv: too many slots");
   if (a->T <= EV_MID) {
+    LA_REQUIRE(grid_fits((int64_t)rows + early, 1024), "la_evict_kv: too many slots");
     p.sel = (int32_t)rows;
     if (a->positions) evict_select_kernel<true><<<rows + early, 1024, 0, st>>>(p);
     else evict_select_kernel<false><<<rows + early, 1024, 0, st>>>(p);
   } else {
     p.sel = (int32_t)(rows * (uint32_t)pl.slices);
     const uint32_t grid = (uint32_t)p.sel + (early + 3) / 4;
+    LA_REQUIRE(grid_fits(grid, 256), "la_evict_kv: too many entries");
     if (a->positions) {
       evict_digit_kernel<0, true><<<grid, 256, 0, st>>>(p);
       evict_digit_kernel<1, true><<<grid, 256, 0, st>>>(p);

@@ -501,7 +501,7 @@ extern "C" int la_key_weights(const la_key_weights_args *a, void *stream) {
   const int64_t wgs = pl.ntile * a->Hkv * pl.splits;
   const int64_t bh = (packed ? 1 : a->B) * a->Hkv;
   // (rows are only split, and key_weights_sum_kernel's gridDim.y only bh, of fewer workgroups)
-  LA_REQUIRE(wgs < ((int64_t)1 << 31) / 64 && (pl.splits == 1 || bh < 65536), "la_key_weights: too many keys or heads");
+  LA_REQUIRE(grid_fits(wgs, 256) && (pl.splits == 1 || bh < 65536), "la_key_weights: too many keys or heads");
   KwKP p{};
   p.s = DaSeqs{a->cu_q, a->cu_k, a->q_len, a->k_len, a->Tq, a->Tk, (int32_t)a->B, (int32_t)(a->Hq / a->Hkv)};
   p.q = a->q; p.k = a->k; p.lse = a->lse; p.out = a->out; p.ws = (float *)a->workspace;
