@@ -137,13 +137,13 @@ __device__ __forceinline__ uint32_t ev_below(uint64_t m) {  // set bits of lanes
   return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
 }
 
-// The entries of a row kept for their weight, in order: list(slot, entry) for the slots
-// from `lead` on.  By a workgroup of NT threads, whose wave w holds NJ * 256 entries of
-// round x from (x * NW + w) * seg on: 4 lane .. 4 lane + 3 of each 256.
-template <int NT, int NJ, int BITS, bool POS, class List>
+// The entries of a row (at most MOST) kept for their weight, in order: list(slot, entry) for
+// the slots from `lead` on.  By a workgroup of NT threads, whose wave w holds the keys of up
+// to 256 NJ entries from w * seg on: 4 lane .. 4 lane + 3 of each 256.
+template <int NT, int MOST, int BITS, bool POS, class List>
 __device__ __forceinline__ void ev_choose(const EvRow &r, List list) {
-  constexpr int NW = NT / 64, BINS = 1 << BITS, PER = BINS / NT;
-  static_assert(PER >= 1, "a thread has a bin");
+  constexpr int NW = NT / 64, NJ = MOST / (4 * NT), BINS = 1 << BITS, PER = BINS / NT;
+  static_assert(PER >= 1 && 4 * NT * NJ == MOST, "a thread has a bin, and the workgroup all keys");
   // a bin's count in COPIES parts, by lane: weights crowd into a few exponents, and lanes
   // that meet in one LDS word wait for each other
   constexpr int COPIES = 4;
@@ -160,48 +160,38 @@ __device__ __forceinline__ void ev_choose(const EvRow &r, List list) {
   uint32_t want = (uint32_t)(r.kept - r.lead - r.tail);
   if (want == 0) return;
   const float *wr = r.w + r.lead;
-  const int32_t rounds = (n + NT * 4 * NJ - 1) / (NT * 4 * NJ);
-  const int32_t seg = rounds == 1 ? ((n + NT * 4 - 1) / (NT * 4)) * 256 : 256 * NJ;
+  const int32_t seg = ((n + NT * 4 - 1) / (NT * 4)) * 256;
+  const int32_t s0 = w * seg, s1 = min(s0 + seg, n);
   uint32_t key[NJ][4];  // 0: no entry
-  auto load = [&](int32_t x) __attribute__((always_inline)) {
-    const int32_t s0 = (x * NW + w) * seg, s1 = min(s0 + seg, n);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {  // (every load in flight before the first is used)
-      const int32_t c0 = s0 + 256 * j, i = c0 + 4 * lane;
-      if (c0 + 256 <= s1) {
-        const ev_i4 v = *(const ev_i4 *)(wr + i);
+  for (int j = 0; j < NJ; ++j) {  // (every load in flight before the first is used)
+    const int32_t c0 = s0 + 256 * j, i = c0 + 4 * lane;
+    if (c0 + 256 <= s1) {
+      const ev_i4 v = *(const ev_i4 *)(wr + i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) key[j][e] = (uint32_t)v[e];
-      } else {
+      for (int e = 0; e < 4; ++e) key[j][e] = (uint32_t)v[e];
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) key[j][e] = __float_as_uint(wr[min(i + e, n - 1)]);
-      }
+      for (int e = 0; e < 4; ++e) key[j][e] = __float_as_uint(wr[min(i + e, n - 1)]);
     }
+  }
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int32_t c0 = s0 + 256 * j, i = c0 + 4 * lane;
+  for (int j = 0; j < NJ; ++j) {
+    const int32_t c0 = s0 + 256 * j, i = c0 + 4 * lane;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t k = ev_key(__uint_as_float(key[j][e]));
-        if constexpr (POS) {
-          const int32_t at = r.ps[min(i + e, n - 1)];
-          k = at >= r.lo && at < r.hi ? k : EV_SAFE;
-        }
-        key[j][e] = k;
+    for (int e = 0; e < 4; ++e) {
+      uint32_t k = ev_key(__uint_as_float(key[j][e]));
+      if constexpr (POS) {
+        const int32_t at = r.ps[min(i + e, n - 1)];
+        k = at >= r.lo && at < r.hi ? k : EV_SAFE;
       }
-      if (c0 + 256 > s1) {
+      key[j][e] = k;
+    }
+    if (c0 + 256 > s1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) key[j][e] = i + e < s1 ? key[j][e] : 0u;
-      }
+      for (int e = 0; e < 4; ++e) key[j][e] = i + e < s1 ? key[j][e] : 0u;
     }
-  };
-  auto each = [&](auto f) __attribute__((always_inline)) {
-    for (int32_t x = 0; x < rounds; ++x) {
-      if (rounds > 1) load(x);
-      f(x);
-    }
-  };
-  if (rounds == 1) load(0);
+  }
   // kept: keys above thr, and the first `want` of those equal to it
   uint32_t thr = 0;
   int shift = 32;
@@ -220,15 +210,13 @@ __device__ __forceinline__ void ev_choose(const EvRow &r, List list) {
       for (uint32_t i = tid; i < few; i += NT)
         if (((cand[i] ^ thr) >> up) == 0u) count(cand[i]);
     } else {
-      each([&](int32_t) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t k = key[j][e];
-            if (k != 0u && (up == 32 || ((k ^ thr) >> (up & 31)) == 0u)) count(k);
-          }
-      });
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t k = key[j][e];
+          if (k != 0u && (up == 32 || ((k ^ thr) >> (up & 31)) == 0u)) count(k);
+        }
     }
     __syncthreads();
     // from the highest bin down, PER bins a thread: where the count reaches `want`
@@ -271,80 +259,72 @@ __device__ __forceinline__ void ev_choose(const EvRow &r, List list) {
     want -= found[1];
     if (up == 32 && found[2] <= (uint32_t)CAND) {
       few = found[2];
-      each([&](int32_t) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (((key[j][e] ^ thr) >> shift) == 0u && key[j][e] != 0u)
-              cand[atomicAdd(&ncand, 1u)] = key[j][e];
-      });
+        for (int e = 0; e < 4; ++e)
+          if (((key[j][e] ^ thr) >> shift) == 0u && key[j][e] != 0u)
+            cand[atomicAdd(&ncand, 1u)] = key[j][e];
       // (in any order: only their number in each bin counts)
       __syncthreads();
     }
     // (part and found are written again after further barriers)
   }
   // what each wave keeps, and from where on
-  uint32_t gt0 = 0, eq0 = 0;  // in the rounds before
-  each([&](int32_t x) {
-    uint32_t gt = 0, eq = 0;
+  uint32_t gt = 0, eq = 0;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+  for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        gt += (uint32_t)__popcll(__ballot(key[j][e] > thr));  // (thr is 1 or more)
-        eq += (uint32_t)__popcll(__ballot(key[j][e] == thr));
-      }
-    __syncthreads();
-    if (lane == 0) {
-      part[w][0] = gt;
-      part[w][1] = eq;
+    for (int e = 0; e < 4; ++e) {
+      gt += (uint32_t)__popcll(__ballot(key[j][e] > thr));  // (thr is 1 or more)
+      eq += (uint32_t)__popcll(__ballot(key[j][e] == thr));
     }
-    __syncthreads();
-    uint32_t g = gt0, q = eq0;
+  __syncthreads();
+  if (lane == 0) {
+    part[w][0] = gt;
+    part[w][1] = eq;
+  }
+  __syncthreads();
+  uint32_t g = 0, q = 0;  // above thr, and equal to it, in the waves before
 #pragma unroll
-    for (int y = 0; y < NW; ++y) {
-      g += y < w ? part[y][0] : 0u;
-      q += y < w ? part[y][1] : 0u;
-      gt0 += part[y][0];
-      eq0 += part[y][1];
+  for (int y = 0; y < NW; ++y) {
+    g += y < w ? part[y][0] : 0u;
+    q += y < w ? part[y][1] : 0u;
+  }
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    uint64_t any = 0;
+    uint32_t gl = g;  // above thr, of earlier lanes (and, below, of this lane's earlier entries)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint64_t m = __ballot(key[j][e] > thr);
+      gl += ev_below(m);
+      g += (uint32_t)__popcll(m);
+      any |= __ballot(key[j][e] == thr);
     }
-    const int32_t s0 = (x * NW + w) * seg + 4 * lane + r.lead;
+    const int32_t i = s0 + 4 * lane + r.lead + 256 * j;
+    if (any == 0) {
+      int32_t slot = r.lead + (int32_t)(gl + min(q, want));
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      uint64_t any = 0;
-      uint32_t gl = g;  // above thr, of earlier lanes (and, below, of this lane's earlier entries)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint64_t m = __ballot(key[j][e] > thr);
-        gl += ev_below(m);
-        g += (uint32_t)__popcll(m);
-        any |= __ballot(key[j][e] == thr);
-      }
-      const int32_t i = s0 + 256 * j;
-      if (any == 0) {
-        int32_t slot = r.lead + (int32_t)(gl + min(q, want));
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key[j][e] > thr) list(slot++, i + e);
-        continue;
-      }
-      uint32_t ql = q;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint64_t m = __ballot(key[j][e] == thr);
-        ql += ev_below(m);
-        q += (uint32_t)__popcll(m);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool above = key[j][e] > thr, same = key[j][e] == thr;
-        if (above || (same && ql < want)) list(r.lead + (int32_t)(gl + min(ql, want)), i + e);
-        gl += above ? 1u : 0u;
-        ql += same ? 1u : 0u;
-      }
+      for (int e = 0; e < 4; ++e)
+        if (key[j][e] > thr) list(slot++, i + e);
+      continue;
     }
-  });
+    uint32_t ql = q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint64_t m = __ballot(key[j][e] == thr);
+      ql += ev_below(m);
+      q += (uint32_t)__popcll(m);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool above = key[j][e] > thr, same = key[j][e] == thr;
+      if (above || (same && ql < want)) list(r.lead + (int32_t)(gl + min(ql, want)), i + e);
+      gl += above ? 1u : 0u;
+      ql += same ? 1u : 0u;
+    }
+  }
 }
 
 // (Two caches of 660 and 740 entries of 8 heads cut to 256: 9.4 us, the search's barriers.)
@@ -358,7 +338,7 @@ __global__ __launch_bounds__(256) void evict_small_kernel(EvKP p, int32_t parts)
   if (threadIdx.x < EV_SLOTS) at[threadIdx.x] = ev_slot(r, s0 + threadIdx.x);
   __syncthreads();
   if (s0 + ns > r.lead && s0 < r.kept - r.tail)  // (some slot is chosen by weight)
-    ev_choose<256, EV_SMALL / 1024, 8, POS>(r, [&](int32_t s, int32_t i) {
+    ev_choose<256, EV_SMALL, 8, POS>(r, [&](int32_t s, int32_t i) {
       if (s >= s0 && s < s0 + ns) at[s - s0] = i;
     });
   __syncthreads();
@@ -377,7 +357,7 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvKP p) {
   if (h == 0 && threadIdx.x == 0) p.len_out[b] = r.kept;
   if (r.n <= r.kept) return;
   int32_t *list = p.list + (int64_t)blockIdx.x * p.budget;
-  ev_choose<1024, EV_MID / 4096, 11, POS>(r, [&](int32_t s, int32_t i) { list[s] = i; });
+  ev_choose<1024, EV_MID, 11, POS>(r, [&](int32_t s, int32_t i) { list[s] = i; });
 }
 
 // A slice of a row of a long cache: pass 0 counts the first digits; passes 1 and 2 find the
