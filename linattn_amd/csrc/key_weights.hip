@@ -254,10 +254,10 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KwKP p) {
     auto masked = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float nl = products(j, h, sa);
+        const float nl = products(j, h, sa);
         const int t = tb + ((32 * h + r32) & (qpt - 1));
-        if (t >= x.t.lq) nl = none;
-        const int seen = nl == none ? -1 : p.causal ? diag + t : x.t.lk - 1;
+        const bool out = t >= x.t.lq || s_lse[j % NSLOT][w][32 * h + r32] == none;
+        const int seen = out ? -1 : p.causal ? diag + t : x.t.lk - 1;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
           // register i: key 8 (i / 4) + 4 hf + i % 4
@@ -357,16 +357,15 @@ __global__ __launch_bounds__(256, 2) void key_weights_f32_kernel(KwKP p) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int rr = 16 * h + ri, t = tb + (rr & (qpt - 1));
-        const float l = lbh[min(t, x.t.lq - 1) + (g + (rr >> qs)) * p.l_sh];
-        nl[h] = t < x.t.lq && l != __int_as_float(0xff800000) ? -l * 1.44269504088896340736f
-                                                              : __int_as_float(0xff800000);
-        seen[h] = p.causal ? diag + t : x.t.lk - 1;
+        nl[h] = lbh[min(t, x.t.lq - 1) + (g + (rr >> qs)) * p.l_sh];
+        seen[h] = t >= x.t.lq ? -1 : p.causal ? diag + t : x.t.lk - 1;
       }
       wait_vmcnt<0>();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         settle(nl[h]);
         if (nl[h] == __int_as_float(0xff800000)) seen[h] = -1;
+        else nl[h] *= -1.44269504088896340736f;
       }
       lds_barrier();
       if (j + 1 < n) dma((j + 1) & 1);
