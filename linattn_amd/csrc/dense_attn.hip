@@ -160,17 +160,20 @@ __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kv
 // tile ahead into the other of two slots, V while its tile is scored: 48 KiB a workgroup
 // and at most 168 registers make three workgroups a CU, and with three waves a SIMD one
 // wave's softmax runs beside another's products (two waves and two slots each: 7.8 ms for
-// 32768 tokens of 32 heads on 8; three: 7.4, 1.19 PFLOP/s; tile j + 1 scored beside the
-// softmax of tile j in one wave's instructions: 10.5).  S^T by 32x32x16 products (A = K rows, B = q held
+// 32768 tokens of 32 heads on 8; three, on the same machine: 7.4, on others to 7.95, 1.11
+// to 1.20 PFLOP/s; tile j + 1 scored beside the softmax of tile j in one wave's
+// instructions: 10.5).  S^T by 32x32x16 products (A = K rows, B = q held
 // in registers) leaves a lane 16 scores of one row, so masks, maxima and sums are per
 // lane; O^T takes P from the same registers (the contraction index is mapped to the keys
 // a lane holds) and V^T by LDS transpose reads.  P is rounded to the inputs' type for
 // that product (to half a step, 2^-8 or 2^-11 of each weight, independently: as much as
 // the output's own rounding; for fp16 of weights down to 2^-29 of the largest, DaF16); its
 // sum l, and with it lse, is of the fp32 values.
-// What bounds it is the softmax's vector work beside the products (a large bf16 product
-// reaches 1.4 PFLOP/s), and for short sequences a workgroup's beginning and end: 14567
-// tokens of 32 heads on 8 run at 1.12 PFLOP/s as one sequence, 1.05 as four, 0.84 as
+// Bound by matrix and vector work together: over 32768 tokens the matrix unit is busy for
+// 67 % of the cycles and the vector unit for 55 (the clock, 1.6 GHz then, gives way to
+// both; a large bf16 product reaches 1.4 PFLOP/s).  Short sequences are bound by a
+// workgroup's beginning and end: both units are busy for 49 % over twelve sequences of
+// 14567 tokens; 14567 tokens of 32 heads on 8 run at 1.12 PFLOP/s as one sequence, 1.05 as four, 0.84 as
 // twelve and 0.61 as twenty-four.
 template <class T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {

@@ -11,7 +11,8 @@
 // on its own (all weights and positions of the pair: 8 bytes an entry, from L2 but for
 // the first), and evict_join_kernel joins the parts.
 // 64 caches of 2049 entries of 8 heads, bf16, D = 128: 109 us, 5.0 TB/s; four of 16385, 58
-// (46 and a join of 6); one of 257 entries in fp32, 11 us, dependent loads and barriers.
+// (53 and a join of 6; their bytes alone 46); one of 257 entries in fp32, 12 us, dependent
+// loads and barriers.
 #include <algorithm>
 
 #include "evict.h"

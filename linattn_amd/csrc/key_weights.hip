@@ -98,11 +98,12 @@ constexpr int KW_RUN = 32;
 
 // bf16 / fp16: four waves of 64 keys.  Rows are staged 64 at a time by LDS-DMA, with their
 // lse (each wave its own copy, so that every wave counts the same loads), NSLOT - 1 tiles
-// ahead; a tile's 128 products a workgroup and the 3 vector instructions of each of its
-// weights take about equally long, which is what bounds it: 14567 tokens of 32 heads on 8
-// run at 0.95 PFLOP/s as one sequence, and as twelve of 115 to 3039 at 0.8 (162 us).  For
-// few queries the keys bound it, and that they must arrive before a workgroup's first
-// product: the last 64 queries of 50001 tokens, 105 MB, 52 us.  (Two waves of 64 keys a
+// ahead.  14567 tokens of 32 heads on 8 run at 0.95 PFLOP/s as one sequence, and as twelve
+// of 115 to 3039 at 0.8 (162 to 166 us): there the vector unit (fma, exp and add of each
+// weight) is busy for 52 % of the cycles, the matrix unit for 35, and waves wait for the
+// staged tiles that their own keys skip (the diagonal) and for one another.  For few
+// queries it is latency, the keys having to arrive before a workgroup's first product: the
+// last 64 queries of 50001 tokens, 105 MB, take 51 to 54 us, vector unit 35 %, matrix 18.  (Two waves of 64 keys a
 // workgroup: 254 and 86 us, the copies' instructions double; eight: 191 and 68, nothing runs
 // beside a workgroup's loads; three workgroups a CU without the interleaving: 249 and 60.)
 template <class T, int D>
