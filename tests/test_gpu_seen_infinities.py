@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from dense_reference import HALF_STEP, attention, close
-from linattn_amd.kernels.dense import dense_attention
+from linattn_amd.kernels.dense import dense_attention, packed_attention
 from linattn_amd.kernels.eviction import evict_decode_step
 from test_gpu_eviction import _Plain
 
@@ -96,3 +96,27 @@ def test_prompt_with_weights_of_every_size(dev, dtype, G, T):
         assert torch.equal(out[0, h].isnan(), o.isnan())
         close(out[0, h].nan_to_num(0, math.inf, -math.inf), o.nan_to_num(0, math.inf, -math.inf), tol.nan_to_num(0, math.inf))
         close(lse[0, h], ls, tol_l)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,Tq,Tk,packed", [(64, 40, 3000, False), (128, 17, 2100, False), (64, 200, 260, True), (64, 3, 2500, False)])
+def test_chunks_with_weights_of_every_size(dev, dtype, D, Tq, Tk, packed):
+    """Keys split over workgroups, sequences packed at an offset, few rows: infinities and NaN
+    before and behind the rows' last keys, at weights up to 70 powers of two below the largest."""
+    q, k, v = (_rand(i, 1, 1, t, D, dtype=dtype) for i, t in ((0, Tq), (1, Tk), (2, Tk)))
+    q[..., 0], k[..., 0] = 1.0, torch.linspace(-48.0, 0.0, Tk).to(dtype)
+    v[0, 0, 3, 1], v[0, 0, Tk // 2, 2], v[0, 0, 5, 3], v[0, 0, Tk // 3, 3] = math.inf, -math.inf, math.inf, -math.inf
+    v[0, 0, Tk - 2, 4], v[0, 0, Tk - 1, 5], v[0, 0, Tk // 2, 6] = math.nan, math.inf, math.nan
+    if packed:
+        lead = 5
+        qd, kd, vd = (torch.cat([torch.full_like(x[0, 0, :lead], math.nan), x[0, 0]])[:, None].to(dev) for x in (q, k, v))
+        cu = [_i32([lead, lead + n], dev) for n in (Tq, Tk)]
+        out, lse = packed_attention(qd, kd, vd, *cu, scale=1.0, return_lse=True)
+        out, lse = out[lead:, 0].cpu(), lse[0, lead:].cpu()
+    else:
+        out, lse = dense_attention(q.to(dev), k.to(dev), v.to(dev), scale=1.0, return_lse=True)
+        out, lse = out[0, 0].cpu(), lse[0, 0].cpu()
+    o, ls, tol, tol_l = attention(q[0, 0], k[0, 0], v[0, 0], True, 1.0, HALF_STEP[dtype])
+    assert torch.equal(out.isnan(), o.isnan())
+    close(out.nan_to_num(0, math.inf, -math.inf), o.nan_to_num(0, math.inf, -math.inf), tol.nan_to_num(0, math.inf))
+    close(lse, ls, tol_l)
