@@ -170,7 +170,7 @@ __device__ __forceinline__ void da_again(const DaKP &p, const DaTile &tl, int kv
 // the output's own rounding; for fp16 of weights down to 2^-29 of the largest, DaF16); its
 // sum l, and with it lse, is of the fp32 values.
 // Bound by matrix and vector work together: over 32768 tokens the matrix unit is busy for
-// 67 % of the cycles and the vector unit for 55 (the clock, 1.6 GHz then, gives way to
+// 67 % of the cycles and the vector unit for 54 (the clock, 1.6 GHz then, gives way to
 // both; a large bf16 product reaches 1.4 PFLOP/s).  Short sequences are bound by a
 // workgroup's beginning and end: both units are busy for 49 % over twelve sequences of
 // 14567 tokens; 14567 tokens of 32 heads on 8 run at 1.12 PFLOP/s as one sequence, 1.05 as four, 0.84 as
@@ -311,11 +311,11 @@ __global__ __launch_bounds__(64 * NW, 3) void dense_attn_kernel(DaKP p) {
       mx = largest(st);
     }
     if (__ballot(mx > thr) != 0) {
-      const float mn = fmaxf(m, pair32_max(mx));
-      const float alpha = m == da_ninf() ? 0.f : fast_exp2((m - mn) * p.qscale);
+      const float mn = fmaxf(m, pair32_max(mx)), to = da_ref<T>(mn, p.qscale);
+      const float alpha = m == da_ninf() ? 0.f : fast_exp2(to - nmu);  // (both as rounded in the weights)
       m = mn;
       thr = mn + p.thr_gap;
-      nmu = da_ref<T>(mn, p.qscale);
+      nmu = to;
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt)
@@ -530,11 +530,11 @@ __global__ __launch_bounds__(256, 2) void dense_attn_f32_kernel(DaKP p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) mx = fmaxf(mx, st[kt][e]);
     if (__ballot(mx > thr) != 0) {
-      const float mn = fmaxf(m, pair32_max(pair16_max(mx)));
-      const float alpha = m == da_ninf() ? 0.f : fast_exp2((m - mn) * p.qscale);
+      const float mn = fmaxf(m, pair32_max(pair16_max(mx))), to = da_ref<DaF32>(mn, p.qscale);
+      const float alpha = m == da_ninf() ? 0.f : fast_exp2(to - nmu);
       m = mn;
       thr = mn + p.thr_gap;
-      nmu = mn == da_ninf() ? 0.f : -mn * p.qscale;
+      nmu = to;
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < NS; ++dt) {

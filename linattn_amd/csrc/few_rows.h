@@ -144,11 +144,11 @@ struct FewRows {
         sink(r * RK + 16 * kt + 4 * c, st[kt]);
       }
       if (__ballot(mx > thr) != 0) {
-        const float mn = fmaxf(m, pair32_max(pair16_max(mx)));
-        const float alpha = m == ninf ? 0.f : fast_exp2((m - mn) * qscale);
+        const float mn = fmaxf(m, pair32_max(pair16_max(mx))), to = da_ref<T>(mn, qscale);
+        const float alpha = m == ninf ? 0.f : fast_exp2(to - nmu);  // (both as rounded in the weights)
         m = mn;
         thr = mn + thr_gap;
-        nmu = da_ref<T>(mn, qscale);
+        nmu = to;
         l *= alpha;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) acc[dt] *= alpha;

@@ -60,3 +60,34 @@ def test_decode_step_far_from_zero(dev, C):
                             torch.zeros(1, 1, C, dtype=torch.int32, device=dev), i32(n - 1), i32(n - 1), recent=8, scale=1.0)
     assert ((out[0, 0, 0].double().cpu() - want).abs() <= tol).all()
     assert ((w[0, 0, :n].double().cpu() - want).abs() <= tol).all() and (w[0, 0, n:] == 0).all()
+
+
+def _rising(n, D=64):
+    """Scores from 1000 to 1032, exact in fp32: the reference maximum is raised again and again.
+    Output dim i is the weight of the i-th of D stretches of keys."""
+    q, k, v = torch.zeros(1, 1, 1, D), torch.zeros(1, 1, n, D), torch.zeros(1, 1, n, D)
+    q[..., 0] = 1.0
+    x = 1000.0 + 32.0 * torch.arange(n) / n
+    k[0, 0, :, 0] = x
+    v[0, 0, torch.arange(n), torch.arange(n) // (n // D)] = 1.0
+    want = torch.softmax(x.double(), 0).view(D, -1).sum(1)
+    # a weight rounds 4 times (its argument, exp2 and the product); the reference is raised at
+    # most 8 times, each for 4 roundings of what was before; a lane adds at most 32 parts of 8
+    # weights, which 8 more additions join; the quotient
+    return q, k, v, want, want * (4 + 8 * 4 + 32 + 8 + 8 + 2) * F32
+
+
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_rising_scores(dev, Tq):
+    q, k, v, want, tol = _rising(1024)
+    out = dense_attention(q.expand(1, 1, Tq, 64).to(dev), k.to(dev), v.to(dev), causal=False, scale=1.0)
+    assert ((out[0, 0].double().cpu() - want).abs() <= tol).all()
+
+
+def test_decode_step_with_rising_scores(dev):
+    q, k, v, want, tol = _rising(1024)
+    i32 = lambda x: torch.tensor([x], dtype=torch.int32, device=dev)
+    out = evict_decode_step(q.to(dev), k[:, :, 1023:].to(dev), v[:, :, 1023:].to(dev), k.to(dev), v.to(dev),
+                            torch.zeros(1, 1, 1024, device=dev), torch.zeros(1, 1, 1024, dtype=torch.int32, device=dev),
+                            i32(1023), i32(1023), recent=8, scale=1.0)
+    assert ((out[0, 0, 0].double().cpu() - want).abs() <= tol).all()
