@@ -653,7 +653,8 @@ __global__ __launch_bounds__(256, 2) void dense_few_kernel(DaKP p) {
       a = __builtin_fmaf(vals[x * FR::VALS + g * (D + 4) + d], f, a);
     }
     // (with scores that are not numbers, l is not, and the row stands)
-    if (!(fabsf(a) < __int_as_float(0x7f800000)) && l < __int_as_float(0x7f800000)) atomicOr(&s_bad, 1u << g);
+    if (!(fabsf(a) < __int_as_float(0x7f800000)) && l > 0.f && l < __int_as_float(0x7f800000)) atomicOr(&s_bad, 1u << g);
+    if (l == 0.f) a = 0.f;  // (no key seen)
     if (p.splits > 1) {
       const int64_t pi = da_part_at(p, tl, te, h, split);
       p.ws_acc[pi * D + d] = a;
@@ -668,8 +669,21 @@ __global__ __launch_bounds__(256, 2) void dense_few_kernel(DaKP p) {
   }
   __syncthreads();
   if (s_bad == 0u) return;
+  uint32_t *marks = (uint32_t *)smem;  // (of which all is read)
+  if (threadIdx.x < D) marks[threadIdx.x] = 0u;
   wait_vmcnt<0>();
-  __syncthreads();  // (every wave's stores are done, which those of the rows done again replace)
+  __syncthreads();  // (every wave's stores are done, which those below replace)
+  if (!p.causal || tl.lq == 1) {  // (every row sees every key)
+    few_marks<elem, D, NW>(marks, [&](int key) { return vb + key * p.v_st; }, r0 * FR::RK, min(tl.lk, r1 * FR::RK));
+    __syncthreads();
+    for (int e = threadIdx.x; e < nrow * D; e += 256) {
+      const int g = e / D, d = e % D, te = g / G, h = kvh * G + g % G;
+      if (!((s_bad >> g) & 1u) || marks[d] == 0u) continue;
+      if (p.splits > 1) p.ws_acc[da_part_at(p, tl, te, h, split) * D + d] = few_mark(marks[d]);
+      else da_store1(p.out, da_out_at(p, tl, te, h) + d, p.out_dt, few_mark(marks[d]));
+    }
+    return;
+  }
   da_again<T, D, 16, true>(p, tl, kvh, split, 0, s_bad, r0 * FR::RK, r1 * FR::RK, w, NW);
 }
 

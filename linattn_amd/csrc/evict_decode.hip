@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
   constexpr int LDS = NW * FR::LDS_BYTES > LDS_MERGE ? NW * FR::LDS_BYTES : LDS_MERGE;
   __shared__ __align__(16) char smem[LDS];
   __shared__ float ref[16], inv[16];
-  __shared__ uint32_t s_bad;  // rows to be done again (few_row)
+  __shared__ uint32_t s_bad;  // rows whose sums are not finite
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t pair = blockIdx.x / (uint32_t)p.splits;
   const int split = (int)(blockIdx.x % (uint32_t)p.splits);
@@ -182,7 +182,8 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
       a = __builtin_fmaf(vals[x * FR::VALS + g * (D + 4) + d], f, a);
     }
     // (with scores that are not numbers, l is not, and the row stands)
-    if (!(fabsf(a) < __int_as_float(0x7f800000)) && l < __int_as_float(0x7f800000)) atomicOr(&s_bad, 1u << g);
+    if (!(fabsf(a) < __int_as_float(0x7f800000)) && l > 0.f && l < __int_as_float(0x7f800000)) atomicOr(&s_bad, 1u << g);
+    if (l == 0.f) a = 0.f;  // (every score -inf)
     if (p.splits > 1) {
       const int64_t at = (pair * p.splits + split) * p.G + g;
       p.vals[at * D + d] = a;
@@ -200,23 +201,18 @@ __global__ __launch_bounds__(256, 2) void evict_decode_kernel(EdKP p) {
   }
   __syncthreads();
   if (s_bad != 0u) {
+    uint32_t *marks = (uint32_t *)smem;  // (of which all is read)
+    if (threadIdx.x < D) marks[threadIdx.x] = 0u;
     wait_vmcnt<0>();
-    __syncthreads();  // (every wave's stores are done, which those of the rows done again replace)
-    for (int g = w; g < p.G; g += NW) {
-      if (!((s_bad >> g) & 1u)) continue;
-      constexpr int N = D / 64;
-      float m, l, a[N];
-      few_row<elem, D>((const elem *)p.q + b * p.q_sb + (kvh * p.G + g) * p.q_sh, krow, vrow, r0 * FR::RK,
-                       min(n, r1 * FR::RK), p.qscale, &m, &l, a);
-      const int64_t at = (pair * p.splits + split) * p.G + g;
-      if (p.splits > 1 && lane == 0) {
-        p.ml[2 * at] = m;
-        p.ml[2 * at + 1] = l;
-      }
-      for (int x = 0; x < N; ++x) {
-        if (p.splits > 1) p.vals[at * D + lane * N + x] = a[x];
-        else store_from_f32(p.out, b * p.o_sb + (kvh * p.G + g) * p.o_sh + lane * N + x, p.out_dt, a[x] / l);
-      }
+    __syncthreads();  // (every wave's stores are done, which those below replace)
+    few_marks<elem, D, NW>(marks, vrow, r0 * FR::RK, min(n, r1 * FR::RK));
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.G * D; e += 256) {
+      const int g = e / D, d = e % D;
+      if (!((s_bad >> g) & 1u) || marks[d] == 0u) continue;
+      const float a = few_mark(marks[d]);
+      if (p.splits > 1) p.vals[((pair * p.splits + split) * p.G + g) * D + d] = a;
+      else store_from_f32(p.out, b * p.o_sb + (kvh * p.G + g) * p.o_sh + d, p.out_dt, a);
     }
   }
   if (p.splits > 1) return;

@@ -14,8 +14,9 @@
 //
 // An infinity of V that a row sees meets weights of both signs in that sum (the second
 // term's), and what is past the last key is that key again with weight 0: 0 and inf - inf
-// where the result is infinite.  The caller looks for sums that are not finite and does
-// those rows again (few_row).
+// where the result is infinite.  The caller looks for sums that are not finite: where its
+// rows see every key, which dims of V hold a NaN or an infinity says what they are
+// (few_marks, few_mark); else those rows are done again (few_row).
 
 namespace la {
 
@@ -211,10 +212,36 @@ struct FewRows {
   static constexpr int VALS = 16 * (D + 4);  // floats of put's values
 };
 
+// Into marks[d] (LDS, D of them, cleared), by all NW waves of a workgroup: whether dim d of V
+// holds a NaN (1), an infinity (2) or the negative one (4) for any of the keys a .. e - 1.
+template <class E, int D, int NW, class VRow>
+__device__ __forceinline__ void few_marks(uint32_t *marks, VRow vrow, int a, int e) {
+  constexpr int CHE = 16 / (int)sizeof(E), CH = D / CHE, RP = 64 / CH;
+  typedef E x8 __attribute__((ext_vector_type(CHE)));
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const float inf = __int_as_float(0x7f800000);
+  uint32_t m = 0;  // three bits of each of the lane's dims
+#pragma unroll 4
+  for (int key = a + RP * w; key < e; key += RP * NW) {
+    const x8 x = *(const x8 *)(vrow(min(key + lane / CH, e - 1)) + CHE * (lane % CH));
+#pragma unroll
+    for (int i = 0; i < CHE; ++i) {
+      const float v = (float)x[i];
+      m |= (v != v ? 1u : v == inf ? 2u : v == -inf ? 4u : 0u) << (3 * i);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < CHE; ++i)
+    if ((m >> (3 * i)) & 7u) atomicOr(&marks[CHE * (lane % CH) + i], (m >> (3 * i)) & 7u);
+}
+// The sum of a row that sees all those keys, where the mark is not 0.
+__device__ __forceinline__ float few_mark(uint32_t mark) {
+  return __int_as_float(mark == 2u ? 0x7f800000 : mark == 4u ? 0xff800000 : 0x7fc00000);
+}
+
 // One row over keys a .. e - 1 (krow(key), vrow(key)), by a wave, key by key in fp32 (m in
 // log2 units; lane i holds dims i D / 64 ..).  For rows whose matrix products met an
-// infinity or a NaN of V in a way that the definition does not: it reads nothing else.  (A
-// step over 64 caches of 2049 entries, every one with such a value, 0.8 ms in place of 0.09.)
+// infinity or a NaN of V in a way that the definition does not: it reads nothing else.
 template <class E, int D, class KRow, class VRow>
 __device__ __forceinline__ void few_row(const E *q, KRow krow, VRow vrow, int a, int e, float qscale, float *m_out,
                                         float *l_out, float *acc) {
