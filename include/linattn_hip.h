@@ -768,7 +768,8 @@ int la_key_weights(const la_key_weights_args *a, void *stream);
  * min(n, budget).  capacity >= budget >= sink + recent.
  * Packed (cu non-null, int32 [B + 1]): sequence b's entries are rows cu[b] .. cu[b+1] - 1,
  * T the tensors' rows and the *_sb strides unused.
- * Rows of k and v: esize bytes per value, unit stride over D, 16-byte aligned.
+ * Rows of k and v: esize bytes per value, unit stride over D, 16-byte aligned.  Outputs
+ * share no memory with inputs.
  * Workspace: la_evict_kv_workspace() bytes, 256-byte aligned (the lists of kept entries).
  */
 typedef struct {
