@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define LA_ABI_VERSION 15
+#define LA_ABI_VERSION 16
 
 /* element types */
 enum {
@@ -841,6 +841,92 @@ typedef struct {
 
 size_t la_evict_decode_workspace(const la_evict_decode_args *a);
 int la_evict_decode(const la_evict_decode_args *a, void *stream);
+
+/*
+ * Rotary positions on several axes: the first 2 n of each row's D values are turned by
+ * frequency i's angle p[axis_i] inv_freq[i]:
+ *   a' = a cos - b sin,  b' = b cos + a sin
+ * for the pairs (i, n + i), or (2 i, 2 i + 1) with interleaved != 0; the rest of a row is
+ * copied.  inverse != 0 turns back (the gradient of what was turned).  Angles are products
+ * in 64 bits, turns and rows in 32; a row is rounded once.
+ * q, q_out (B, Hq, T, D), k, k_out (B, Hkv, T, D) (Hkv 0: none) at strides *_sb, *_sh, *_st,
+ * unit stride over D; positions (int32) of axis a, token (b, t) at a p_sa + b p_sb + t p_st;
+ * inv_freq fp32 [n]; axes (int32 [n], clamped to 0 .. A - 1; null with A = 1).  D at most
+ * 512.  q_out may be q and k_out may be k, else outputs share no memory with anything.
+ */
+typedef struct {
+  const void *q;
+  const void *k;
+  void *q_out;
+  void *k_out;
+  const int32_t *positions;
+  const float *inv_freq;
+  const int32_t *axes;
+  int64_t B, T, Hq, Hkv, D, n, A;
+  int64_t q_sb, q_sh, q_st;
+  int64_t k_sb, k_sh, k_st;
+  int64_t qo_sb, qo_sh, qo_st;
+  int64_t ko_sb, ko_sh, ko_st;
+  int64_t p_sa, p_sb, p_st;
+  int32_t dtype;
+  int32_t interleaved;
+  int32_t inverse;
+  int32_t reserved;
+} la_rotary_args;
+
+int la_rotary(const la_rotary_args *a, void *stream);
+
+/*
+ * New tokens into a paged cache, turned by their positions on the way: q (optional, Hq 0:
+ * none) and k_new as la_rotary turns them, q into q_out (which may be q), k_new and v_new
+ * into k_pool, v_pool (n_phys, Hkv, pool_page, D), contiguous.  New token i of sequence b
+ * sits at place positions[b] + i: slot place % pool_page of page page_table[b][place /
+ * pool_page]; a token whose place or page is outside of the table or the pool is not stored.
+ *  - batched (cu null): q, k_new, v_new (B, H, T, D), T new tokens of each sequence;
+ *  - packed: cu (int32 [B + 1], ascending): sequence b's tokens are rows cu[b] .. cu[b+1] - 1
+ *    of T, the *_sb strides are unused; rows of q_out that no sequence holds are left, or
+ *    zeroed (zero_rest).
+ * Angles go by rot_positions (as in la_rotary, packed: axis a, row t), or, null, by the
+ * tokens' places.  The pool holds the inputs' dtype (LA_F32, LA_BF16, LA_F16), or e4m3 codes
+ * with fp32 scales (n_phys, Hkv, pool_page) at stride s_stride: scale = max(largest, 1e-8) /
+ * 448 of the row as turned in fp32, codes = e4m3(x / scale).
+ * page_min, page_max (optional, not with fp8; the dtype of k_new): the least and largest keys
+ * of pages of meta_page tokens, (B, Hkv, n_pages, D) at m_sb, m_sh, m_sp, m_sd; those that the
+ * new tokens touch are brought up to date (a page that starts among them holds only them).
+ * Unit stride over D, D at most 512; what is written shares no memory with anything else.
+ */
+typedef struct {
+  const void *q;
+  const void *k_new;
+  const void *v_new;
+  void *q_out;
+  void *k_pool;
+  void *v_pool;
+  float *k_scale;
+  float *v_scale;
+  const int32_t *page_table;
+  const int32_t *positions;
+  const int32_t *cu;
+  const int32_t *rot_positions;
+  const float *inv_freq;
+  const int32_t *axes;
+  void *page_min;
+  void *page_max;
+  int64_t B, T, Hq, Hkv, D, n, A;
+  int64_t q_sb, q_sh, q_st;
+  int64_t kn_sb, kn_sh, kn_st;
+  int64_t vn_sb, vn_sh, vn_st;
+  int64_t o_sb, o_sh, o_st;
+  int64_t p_sa, p_sb, p_st;
+  int64_t n_phys, pool_page, pt_sb, pt_pages, s_stride;
+  int64_t meta_page, n_pages, m_sb, m_sh, m_sp, m_sd;
+  int32_t dtype;
+  int32_t pool_dtype;
+  int32_t interleaved;
+  int32_t zero_rest;
+} la_rotary_append_args;
+
+int la_rotary_append(const la_rotary_append_args *a, void *stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblinattn_hip.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 LIST_READS_PARTS = 256  # LA_LIST_READS_PARTS
 
 LA_F32, LA_BF16, LA_F16, LA_FP8_E4M3, LA_F64 = 0, 1, 2, 3, 4
@@ -56,6 +56,8 @@ EXPORTED = (
     "la_evict_kv",
     "la_evict_decode_workspace",
     "la_evict_decode",
+    "la_rotary",
+    "la_rotary_append",
     "la_device_status",
     "la_test_set_spin_limit",
 )
@@ -219,6 +221,31 @@ class LaEvictDecodeArgs(ctypes.Structure):
                 ("reserved", _i32)]
 
 
+class LaRotaryArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp), ("positions", _vp),
+                ("inv_freq", _vp), ("axes", _vp), ("B", _i64), ("T", _i64), ("Hq", _i64),
+                ("Hkv", _i64), ("D", _i64), ("n", _i64), ("A", _i64), ("q_sb", _i64),
+                ("q_sh", _i64), ("q_st", _i64), ("k_sb", _i64), ("k_sh", _i64), ("k_st", _i64),
+                ("qo_sb", _i64), ("qo_sh", _i64), ("qo_st", _i64), ("ko_sb", _i64),
+                ("ko_sh", _i64), ("ko_st", _i64), ("p_sa", _i64), ("p_sb", _i64), ("p_st", _i64),
+                ("dtype", _i32), ("interleaved", _i32), ("inverse", _i32), ("reserved", _i32)]
+
+
+class LaRotaryAppendArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k_new", _vp), ("v_new", _vp), ("q_out", _vp), ("k_pool", _vp),
+                ("v_pool", _vp), ("k_scale", _vp), ("v_scale", _vp), ("page_table", _vp),
+                ("positions", _vp), ("cu", _vp), ("rot_positions", _vp), ("inv_freq", _vp),
+                ("axes", _vp), ("page_min", _vp), ("page_max", _vp), ("B", _i64), ("T", _i64),
+                ("Hq", _i64), ("Hkv", _i64), ("D", _i64), ("n", _i64), ("A", _i64),
+                ("q_sb", _i64), ("q_sh", _i64), ("q_st", _i64), ("kn_sb", _i64), ("kn_sh", _i64),
+                ("kn_st", _i64), ("vn_sb", _i64), ("vn_sh", _i64), ("vn_st", _i64),
+                ("o_sb", _i64), ("o_sh", _i64), ("o_st", _i64), ("p_sa", _i64), ("p_sb", _i64),
+                ("p_st", _i64), ("n_phys", _i64), ("pool_page", _i64), ("pt_sb", _i64),
+                ("pt_pages", _i64), ("s_stride", _i64), ("meta_page", _i64), ("n_pages", _i64),
+                ("m_sb", _i64), ("m_sh", _i64), ("m_sp", _i64), ("m_sd", _i64), ("dtype", _i32),
+                ("pool_dtype", _i32), ("interleaved", _i32), ("zero_rest", _i32)]
+
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -283,6 +310,8 @@ def load() -> ctypes.CDLL:
     L.la_evict_decode_workspace.argtypes = [P(LaEvictDecodeArgs)]
     L.la_evict_decode_workspace.restype = ctypes.c_size_t
     L.la_evict_decode.argtypes = [P(LaEvictDecodeArgs), _vp]
+    L.la_rotary.argtypes = [P(LaRotaryArgs), _vp]
+    L.la_rotary_append.argtypes = [P(LaRotaryAppendArgs), _vp]
     L.la_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), _i32, _vp]
     L.la_test_set_spin_limit.argtypes = [ctypes.c_uint32]
     for name in EXPORTED:

@@ -8,19 +8,23 @@ Quest page bounds -- the KV concatenation of AttentionVariant.push_kv
 pages.  For an fp8 pool the codec of kv/quant.py:76-93 (per-token scales,
 group = head_dim) runs in the same kernel.  Sequences may sit at different
 positions (ragged batches).
+
+``rotary_kv_append`` does this for whole prompts, chunks and single tokens together, and
+turns the new queries and keys by their rotary positions on the way.
 """
 
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from linattn_amd import _native as N
 from linattn_amd.kernels.block_sparse import _paged_scale_stride
+from linattn_amd.kernels.rotary import (_TYPES, _frequencies, _out_rows, _positions, _strides, _unit_rows)
 
-__all__ = ["paged_kv_append"]
+__all__ = ["paged_kv_append", "rotary_kv_append"]
 
 
 def paged_kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
@@ -103,3 +107,134 @@ def paged_kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
     a.in_dtype = N.dtype_code(k_new.dtype)
     a.pool_dtype = N.dtype_code(k_pool.dtype)
     N.check(N.load().la_paged_kv_append(ctypes.byref(a), N.stream_handle(dev)), "paged_kv_append")
+
+
+def _pools(what: str, k_pool: torch.Tensor, v_pool: torch.Tensor, dtype: torch.dtype, Hkv: int, D: int,
+           k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor]) -> Tuple[bool, int]:
+    """(whether the pools hold fp8 codes, the stride of their scales), checked."""
+    if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or k_pool.shape[1] != Hkv or k_pool.shape[3] != D \
+            or k_pool.numel() == 0:
+        raise ValueError(f"{what}: pools must be (n_phys, {Hkv}, page_size, {D}), and not empty")
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError(f"{what}: pools must be contiguous")
+    fp8 = k_pool.dtype == torch.float8_e4m3fn
+    if k_pool.dtype != v_pool.dtype or not (fp8 or k_pool.dtype == dtype):
+        raise ValueError(f"{what}: the pools hold the queries' dtype, or float8_e4m3fn codes")
+    if not fp8:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"{what}: scales are for fp8 pools")
+        return False, 1
+    for s in (k_scale, v_scale):
+        if s is None or s.dtype != torch.float32 or s.shape != k_pool.shape[:3]:
+            raise ValueError(f"{what}: fp8 pools need fp32 k_scale / v_scale (n_phys, Hkv, page_size)")
+    if k_scale.stride() != v_scale.stride():
+        raise ValueError(f"{what}: k_scale / v_scale must share strides")
+    return True, _paged_scale_stride(k_scale, k_pool)
+
+
+def _table(what: str, page_table: torch.Tensor, B: int) -> None:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B \
+            or page_table.shape[1] == 0 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"{what}: page_table must be int32 ({B}, pages) with unit column stride")
+
+
+def rotary_kv_append(q: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
+                     v_pool: torch.Tensor, page_table: torch.Tensor, positions: torch.Tensor,
+                     inv_freq: torch.Tensor, *, cu_seqlens: Optional[torch.Tensor] = None,
+                     rotary_positions: Optional[torch.Tensor] = None, axes: Optional[torch.Tensor] = None,
+                     interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
+                     page_min: Optional[torch.Tensor] = None, page_max: Optional[torch.Tensor] = None,
+                     page_size: Optional[int] = None, k_scale: Optional[torch.Tensor] = None,
+                     v_scale: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Turns the queries and keys of new tokens by their rotary positions and stores the keys
+    and their values in the pages of their sequences; returns the turned queries.
+
+    q (B, Hq, Tn, D), k_new / v_new (B, Hkv, Tn, D), or packed (N, H, D) with ``cu_seqlens``
+    (int32 (B + 1,), ascending, on the device): sequence b's tokens are rows cu_seqlens[b] ..
+    cu_seqlens[b + 1] - 1, none to many; q may be None.  bfloat16, float16 or float32.
+    New token i of sequence b goes to place ``positions[b]`` + i (int32 (B,)), that is to slot
+    place % pool_page of page ``page_table[b, place // pool_page]`` of the pools (n_phys, Hkv,
+    pool_page, D); a token whose place lies outside of the table, or whose page outside of the
+    pool, is not stored.  The pools hold k_new's dtype, or float8_e4m3fn codes with ``k_scale`` /
+    ``v_scale`` (as ``paged_kv_append``; codes are of the row as it was turned in fp32).
+    Angles: ``inv_freq``, ``axes`` and ``interleaved`` as in ``rotary``, by the tokens' places, or by
+    ``rotary_positions`` (int32, (B, Tn) or (N,); with ``axes`` (A, B, Tn) or (A, N)).
+    ``page_min`` / ``page_max`` (B, Hkv, n_pages, D) in k_new's dtype, with ``page_size``: Quest's
+    bounds of the pages that the new tokens touch are kept as in ``paged_kv_append`` (the keys
+    as they are stored).  Queries go to a new tensor (rows of no sequence are zeros), or to
+    ``q_out`` (those rows are left), which may be q itself.  Forward only."""
+    what = "rotary_kv_append"
+    dev = N.require_gpu(k_new, v_new, q, k_pool, v_pool, page_table, positions, inv_freq, cu_seqlens,
+                        rotary_positions, axes, q_out, page_min, page_max, k_scale, v_scale, what=what)
+    packed = cu_seqlens is not None
+    if k_new.dim() != (3 if packed else 4) or v_new.shape != k_new.shape:
+        raise ValueError(f"{what}: k_new / v_new must be (B, Hkv, Tn, D), or with cu_seqlens (N, Hkv, D)")
+    if k_new.dtype not in _TYPES or v_new.dtype != k_new.dtype:
+        raise ValueError(f"{what}: k_new / v_new must both be bfloat16, float16 or float32")
+    Hkv, D = k_new.shape[1], k_new.shape[-1]
+    if Hkv == 0:
+        raise ValueError(f"{what}: no KV heads")
+    if q is not None and (q.dim() != k_new.dim() or q.dtype != k_new.dtype or q.shape[0] != k_new.shape[0]
+                          or q.shape[2:] != k_new.shape[2:] or q.shape[1] % Hkv):
+        raise ValueError(f"{what}: q must have k_new's dtype, tokens and head_dim, and a multiple of its heads")
+    if packed:
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+            raise ValueError(f"{what}: cu_seqlens must be int32 (B + 1,)")
+        cu_seqlens = cu_seqlens.contiguous()
+        B, T = cu_seqlens.shape[0] - 1, k_new.shape[0]
+    else:
+        B, T = k_new.shape[0], k_new.shape[2]
+    fp8, s_stride = _pools(what, k_pool, v_pool, k_new.dtype, Hkv, D, k_scale, v_scale)
+    _table(what, page_table, B)
+    if positions.dtype != torch.int32 or positions.shape != (B,):
+        raise ValueError(f"{what}: positions must be int32 ({B},)")
+    positions = positions.contiguous()
+    _frequencies(what, inv_freq, axes, D)
+    A, p_s = 1, (0, 0, 0)
+    if rotary_positions is not None:
+        A, p_s = _positions(what, rotary_positions, axes, (T,) if packed else (B, T))
+    elif axes is not None:
+        raise ValueError(f"{what}: axes need rotary_positions")
+    if (page_min is None) != (page_max is None):
+        raise ValueError(f"{what}: pass both page_min and page_max, or neither")
+    meta = (0, 0, 0, 0, 0, 0)
+    if page_min is not None:
+        if fp8:
+            raise ValueError(f"{what}: fp8 pools take no page bounds")
+        if page_size is None or not 0 < int(page_size) < 1 << 30:
+            raise ValueError(f"{what}: page bounds need page_size")
+        if page_min.dim() != 4 or page_min.shape[:2] != (B, Hkv) or page_min.shape[3] != D \
+                or page_max.shape != page_min.shape or page_min.stride() != page_max.stride():
+            raise ValueError(f"{what}: page_min / page_max must be (B, Hkv, n_pages, D) with equal strides")
+        if page_min.dtype != k_new.dtype or page_max.dtype != k_new.dtype:
+            raise ValueError(f"{what}: page bounds are stored in the key dtype")
+        meta = (int(page_size), page_min.shape[2], *page_min.stride())
+        if page_min.numel() == 0:
+            page_min = page_max = None
+    elif page_size is not None:
+        raise ValueError(f"{what}: page_size is for page bounds")
+    zero_rest = q_out is None
+    if q is None:
+        if q_out is not None:
+            raise ValueError(f"{what}: q_out without q")
+    else:
+        q_out = _out_rows(what, "q_out", q_out, q)
+    if B == 0 or T == 0:
+        return q_out
+    q = None if q is None else _unit_rows(what, "q", q)
+    k_new, v_new = _unit_rows(what, "k_new", k_new), _unit_rows(what, "v_new", v_new)
+    inv_freq = inv_freq.contiguous()
+    axes = None if axes is None else axes.contiguous()
+    Hq = 0 if q is None else q.shape[1]
+    none = (0, 0, 0)
+    a = N.LaRotaryAppendArgs(
+        N.ptr(q), k_new.data_ptr(), v_new.data_ptr(), N.ptr(q_out), k_pool.data_ptr(), v_pool.data_ptr(),
+        N.ptr(k_scale), N.ptr(v_scale), page_table.data_ptr(), positions.data_ptr(), N.ptr(cu_seqlens),
+        N.ptr(rotary_positions), inv_freq.data_ptr(), N.ptr(axes), N.ptr(page_min), N.ptr(page_max),
+        B, T, Hq, Hkv, D, inv_freq.shape[0], A, *(_strides(q) if Hq else none), *_strides(k_new), *_strides(v_new),
+        *(_strides(q_out) if Hq else none), *p_s, k_pool.shape[0], k_pool.shape[2], page_table.stride(0),
+        page_table.shape[1], s_stride, *meta, N.dtype_code(k_new.dtype), N.dtype_code(k_pool.dtype),
+        1 if interleaved else 0, 1 if zero_rest else 0)
+    with N.on_device(dev):
+        N.check(N.load().la_rotary_append(ctypes.byref(a), N.stream_handle(dev)), what)
+    return q_out

@@ -1,0 +1,136 @@
+"""Rotary positions on gfx950, on one axis or on several (time, height and width of a video).
+
+``rotary`` turns the rows of q and k by their tokens' positions before
+``linattn_amd.kernels.dense`` or ``linattn_amd.kernels.prefill`` attends over them;
+``linattn_amd.kernels.kv_cache.rotary_kv_append`` does it on the way into a paged cache.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from linattn_amd import _native as N
+from linattn_amd.kernels.dense import _apart
+
+__all__ = ["rotary", "rotary_axes"]
+
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def rotary_axes(sections: Sequence[int], interleaved: bool = False,
+                device: Optional[torch.device] = None) -> torch.Tensor:
+    """Which axis each frequency goes by, int32: ``sections[a]`` frequencies on axis a, one
+    section behind the other, or the axes in turn, as long as each has some left."""
+    if not sections or any(int(s) != s or s < 0 for s in sections) or sum(sections) == 0:
+        raise ValueError(f"sections must be whole numbers that are not negative, got {sections}")
+    if not interleaved:
+        axes = [a for a, s in enumerate(sections) for _ in range(int(s))]
+    else:
+        axes = [a for i in range(int(max(sections))) for a, s in enumerate(sections) if i < s]
+    return torch.tensor(axes, dtype=torch.int32, device=device)
+
+
+def _unit_rows(what: str, name: str, t: torch.Tensor) -> torch.Tensor:
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        return t.contiguous()
+    return t
+
+
+def _frequencies(what: str, inv_freq: torch.Tensor, axes: Optional[torch.Tensor], D: int) -> None:
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= D <= 512:
+        raise ValueError(f"{what}: inv_freq must be float32 (n,) with 2 n <= head_dim <= 512")
+    if axes is not None and (axes.dtype != torch.int32 or axes.shape != inv_freq.shape):
+        raise ValueError(f"{what}: axes must be int32 with an entry for each frequency")
+
+
+def _positions(what: str, positions: torch.Tensor, axes: Optional[torch.Tensor],
+               tokens: Tuple[int, ...]) -> Tuple[int, Tuple[int, int, int]]:
+    """(axes, strides by axis, sequence and token) of positions (*tokens) or (A, *tokens)."""
+    if positions.dtype != torch.int32:
+        raise ValueError(f"{what}: positions must be int32")
+    shape, st = tuple(positions.shape), positions.stride()
+    if axes is None:
+        if shape != tokens:
+            raise ValueError(f"{what}: positions must be {tokens} (with several axes, pass `axes`), got {shape}")
+        A, st = 1, (0, *st)
+    else:
+        if len(shape) != len(tokens) + 1 or shape[1:] != tokens or shape[0] == 0:
+            raise ValueError(f"{what}: positions must be (axes, {', '.join(map(str, tokens))}), got {shape}")
+        A = shape[0]
+    return A, (st if len(tokens) == 2 else (st[0], 0, st[1]))
+
+
+def _out_rows(what: str, name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    if out.shape != x.shape or out.dtype != x.dtype or (out.shape[-1] > 1 and out.stride(-1) != 1):
+        raise ValueError(f"{what}: {name} must have its input's shape and dtype, and contiguous rows")
+    if out is not x and out.data_ptr() != x.data_ptr():
+        _apart(what, out, x)
+    elif out is not x and out.numel() and any(a != b for a, b, d in zip(out.stride(), x.stride(), x.shape) if d > 1):
+        raise ValueError(f"{what}: {name} shares memory with its input, but does not hold the same rows")
+    return out
+
+
+def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
+    """(sequence, head, token) of (B, H, T, D), or packed (T, H, D)."""
+    s = t.stride()
+    return (s[0], s[1], s[2]) if len(s) == 4 else (0, s[1], s[0])
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
+           axes: Optional[torch.Tensor] = None, interleaved: bool = False, inverse: bool = False,
+           q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None
+           ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """The rows of q and k turned by their tokens' positions.
+
+    q (B, Hq, T, D) and k (B, Hkv, T, D), or packed (N, Hq, D) and (N, Hkv, D), bfloat16,
+    float16 or float32, D up to 512; k may be None.  ``inv_freq`` (float32 (n,), 2 n <= D):
+    frequency i turns the pair (i, n + i) of a row, or with ``interleaved`` (2 i, 2 i + 1), by
+    the angle position * inv_freq[i]; what is behind the first 2 n values is copied.
+    ``positions`` (int32) is (B, T) or (N,); with ``axes`` (int32 (n,), see ``rotary_axes``) it
+    is (A, B, T) or (A, N), and frequency i goes by positions[axes[i]].  ``inverse`` turns back:
+    the gradient of a turn is the turn back of its output's gradient (no gradient is recorded).
+    Angles are counted in 64 bits, so far positions keep their phase; rows are turned in 32 and
+    rounded once.  Returns new tensors (q alone where k is None), or ``q_out`` / ``k_out``, which
+    may be q and k themselves (in place)."""
+    what = "rotary"
+    dev = N.require_gpu(q, k, positions, inv_freq, axes, q_out, k_out, what=what)
+    if q.dim() not in (3, 4) or q.dtype not in _TYPES:
+        raise ValueError(f"{what}: q must be (B, Hq, T, D) or (N, Hq, D) in bfloat16, float16 or float32")
+    batched = q.dim() == 4
+    if k is not None and (k.dim() != q.dim() or k.dtype != q.dtype or k.shape[0] != q.shape[0]
+                          or k.shape[2:] != q.shape[2:]):
+        raise ValueError(f"{what}: k must have q's dtype, tokens and head_dim")
+    D, Hq = q.shape[-1], q.shape[1]
+    Hkv = 0 if k is None else k.shape[1]
+    B, T = (q.shape[0], q.shape[2]) if batched else (1, q.shape[0])
+    _frequencies(what, inv_freq, axes, D)
+    A, p_s = _positions(what, positions, axes, (B, T) if batched else (T,))
+    if k is None and k_out is not None:
+        raise ValueError(f"{what}: k_out without k")
+    q_out = _out_rows(what, "q_out", q_out, q)
+    if k is not None:
+        k_out = _out_rows(what, "k_out", k_out, k)
+    if q_out.numel() or (k is not None and k_out.numel()):
+        inv_freq = inv_freq.contiguous()
+        axes = None if axes is None else axes.contiguous()
+        q = _unit_rows(what, "q", q)
+        k = None if k is None else _unit_rows(what, "k", k)
+        none = (0, 0, 0)
+        kv = k is not None and Hkv > 0
+        if Hq == 0:  # (the rows of k alone)
+            if kv:
+                rotary(k, None, positions, inv_freq, axes=axes, interleaved=interleaved, inverse=inverse, q_out=k_out)
+            return q_out, k_out
+        a = N.LaRotaryArgs(
+            q.data_ptr(), k.data_ptr() if kv else None, q_out.data_ptr(), k_out.data_ptr() if kv else None,
+            positions.data_ptr(), inv_freq.data_ptr(), N.ptr(axes), B, T, Hq, Hkv, D, inv_freq.shape[0], A,
+            *_strides(q), *(_strides(k) if kv else none), *_strides(q_out), *(_strides(k_out) if kv else none),
+            *p_s, N.dtype_code(q.dtype), 1 if interleaved else 0, 1 if inverse else 0, 0)
+        with N.on_device(dev):
+            N.check(N.load().la_rotary(ctypes.byref(a), N.stream_handle(dev)), what)
+    return q_out if k is None else (q_out, k_out)
