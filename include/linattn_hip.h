@@ -928,6 +928,54 @@ typedef struct {
 
 int la_rotary_append(const la_rotary_append_args *a, void *stream);
 
+/*
+ * la_dense_attention of new tokens over a paged cache: query t of sequence b, one of its last
+ * Lq positions, sees keys 0 .. Lk - Lq + t (causal; else all Lk), Lk = lengths[b] (int32 [B],
+ * clamped to 0 .. pt_pages * page), key s in slot s % page of page page_table[b][s / page]
+ * of k_pool, v_pool (n_phys, Hkv, page, D), contiguous.  Slots past Lk are not read; a page
+ * outside of the pool is read as the nearest that is in it.
+ *  - batched (cu_q null): q, out (B, Hq, Tq, D); q_len (optional, int32 [B]) gives each
+ *    sequence's Lq (clamped to 0 .. Tq); rows at or past it are zeros (lse -inf);
+ *  - packed: cu_q (int32 [B + 1], ascending): rows cu_q[b] .. cu_q[b+1] - 1 of Tq; rows no
+ *    sequence holds are left as they were, or zeroed (zero_rest).
+ * A query that sees no key gets zeros and lse -inf.  The cache holds dtype (LA_F32, LA_BF16,
+ * LA_F16), or, with 16-bit dtype, e4m3 codes with fp32 scales of K and V per token (n_phys,
+ * Hkv, page) at stride s_stride.  out_dtype is dtype or LA_F32; D 64 or 128; rows of q and out
+ * 16-byte aligned; lse (optional, fp32) has strides l_sb, l_sh and 1.  The cache has less than
+ * 2^32 rows.  scale must be positive; out shares no memory with q and the cache.  Workspace:
+ * la_paged_attention_workspace() bytes, 256-byte aligned (the parts of tiles that several
+ * workgroups share).  The same call gives the same bits.
+ */
+typedef struct {
+  const void *q;
+  const void *k_pool;
+  const void *v_pool;
+  void *out;
+  float *lse;
+  const float *k_scale;
+  const float *v_scale;
+  const int32_t *page_table;
+  const int32_t *lengths;
+  const int32_t *cu_q;
+  const int32_t *q_len;
+  void *workspace;
+  int64_t ws_bytes;
+  int64_t B, Hq, Hkv, Tq, D;
+  int64_t q_sb, q_sh, q_st;
+  int64_t o_sb, o_sh, o_st;
+  int64_t l_sb, l_sh;
+  int64_t n_phys, page, pt_sb, pt_pages, s_stride;
+  float scale;
+  int32_t causal;
+  int32_t dtype;
+  int32_t kv_dtype;
+  int32_t out_dtype;
+  int32_t zero_rest;
+} la_paged_attn_args;
+
+size_t la_paged_attention_workspace(const la_paged_attn_args *a);
+int la_paged_attention(const la_paged_attn_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -58,6 +58,8 @@ EXPORTED = (
     "la_evict_decode",
     "la_rotary",
     "la_rotary_append",
+    "la_paged_attention_workspace",
+    "la_paged_attention",
     "la_device_status",
     "la_test_set_spin_limit",
 )
@@ -246,6 +248,18 @@ class LaRotaryAppendArgs(ctypes.Structure):
                 ("pool_dtype", _i32), ("interleaved", _i32), ("zero_rest", _i32)]
 
 
+class LaPagedAttnArgs(ctypes.Structure):
+    _fields_ = [("q", _vp), ("k_pool", _vp), ("v_pool", _vp), ("out", _vp), ("lse", _vp),
+                ("k_scale", _vp), ("v_scale", _vp), ("page_table", _vp), ("lengths", _vp),
+                ("cu_q", _vp), ("q_len", _vp), ("workspace", _vp), ("ws_bytes", _i64), ("B", _i64),
+                ("Hq", _i64), ("Hkv", _i64), ("Tq", _i64), ("D", _i64), ("q_sb", _i64),
+                ("q_sh", _i64), ("q_st", _i64), ("o_sb", _i64), ("o_sh", _i64), ("o_st", _i64),
+                ("l_sb", _i64), ("l_sh", _i64), ("n_phys", _i64), ("page", _i64), ("pt_sb", _i64),
+                ("pt_pages", _i64), ("s_stride", _i64), ("scale", ctypes.c_float),
+                ("causal", _i32), ("dtype", _i32), ("kv_dtype", _i32), ("out_dtype", _i32),
+                ("zero_rest", _i32)]
+
+
 _LIB: Optional[ctypes.CDLL] = None
 
 
@@ -312,6 +326,9 @@ def load() -> ctypes.CDLL:
     L.la_evict_decode.argtypes = [P(LaEvictDecodeArgs), _vp]
     L.la_rotary.argtypes = [P(LaRotaryArgs), _vp]
     L.la_rotary_append.argtypes = [P(LaRotaryAppendArgs), _vp]
+    L.la_paged_attention_workspace.argtypes = [P(LaPagedAttnArgs)]
+    L.la_paged_attention_workspace.restype = ctypes.c_size_t
+    L.la_paged_attention.argtypes = [P(LaPagedAttnArgs), _vp]
     L.la_device_status.argtypes = [ctypes.POINTER(ctypes.c_uint32), _i32, _vp]
     L.la_test_set_spin_limit.argtypes = [ctypes.c_uint32]
     for name in EXPORTED:

@@ -1,0 +1,193 @@
+// Dense attention over a paged cache: which keys of which rows a workgroup takes, where they
+// lie, and how parts of rows are joined.  Used by paged_attn.hip.
+//
+// Rows: row r of a sequence and KV head is query r / G of head r % G of its group (so the heads of
+// a group share every staged key); R of them are a tile, which walks the keys its last row sees.
+//
+// The lengths are known on the device only, and a batch holds single tokens beside long chunks, so
+// the work is shared out there: all tiles of a KV head in a line, sequence after sequence, each
+// as long as its keys (and a little, for its beginning and end); of that line every workgroup
+// takes an equal stretch, from its place on, across the ends of tiles.  A tile that
+// lies in one stretch is finished by its workgroup; of one that does not, each workgroup
+// leaves its part (unnormalised sums, reference and weight sum of each row) and the join, a
+// second launch, adds them up.
+#pragma once
+
+#include "few_rows.h"
+
+namespace la {
+
+struct PaKP {
+  const void *q, *k, *v;
+  void *out;
+  float *lse;
+  const float *k_scale, *v_scale;
+  const int32_t *page_table, *lengths, *cu_q, *q_len;
+  float *ws_ml, *ws_acc;  // parts: [workgroup][first, last][row] (reference, sum) and D values
+  int4 *ws_join;          // [workgroup]: sequence, tile, parts (0: none), of the tile that begins last there
+  int64_t Tq, q_sb, q_sh, q_st, o_sb, o_sh, o_st, l_sb, l_sh, pt_sb, s_stride, n_phys;
+  int64_t least;  // of a stretch
+  int32_t B, G, Hq, Hkv, D, W, part_rows;  // W: workgroups of a KV head
+  int32_t page, pt_pages, causal, out_dt, zero_rest;
+  float qscale, thr_gap;
+};
+
+constexpr int PA_AHEAD = 160;  // what a tile's beginning and end cost, in keys
+
+struct PaSeq {
+  int32_t lq, lk;
+  int64_t q0;  // packed: its first row
+};
+
+__device__ __forceinline__ PaSeq pa_seq(const PaKP &p, int b) {
+  PaSeq s;
+  if (p.cu_q) {
+    const int32_t a = da_cu(p.cu_q, b, p.Tq), e = da_cu(p.cu_q, b + 1, p.Tq);
+    s.q0 = a;
+    s.lq = max(e - a, 0);
+  } else {
+    s.q0 = 0;
+    s.lq = (int32_t)(p.q_len ? min(max((int64_t)p.q_len[b], (int64_t)0), p.Tq) : p.Tq);
+  }
+  s.lk = min(max(p.lengths[b], 0), p.pt_pages * p.page);  // (below 2^31)
+  return s;
+}
+
+// A sequence's tiles: tile i costs a + step (i + 1), in keys times G.
+struct PaTiles {
+  int64_t a, step;
+  int32_t n;
+  __device__ __forceinline__ int64_t upto(int64_t i) const { return i * a + step * (i * (i + 1) / 2); }
+  __device__ __forceinline__ int64_t cost(int64_t i) const { return a + step * (i + 1); }
+};
+template <int R>
+__device__ __forceinline__ PaTiles pa_tiles(const PaKP &p, const PaSeq &s) {
+  PaTiles t;
+  t.n = (int32_t)(((int64_t)s.lq * p.G + R - 1) / R);
+  t.a = (int64_t)p.G * ((p.causal ? max(s.lk - s.lq, 0) : s.lk) + PA_AHEAD);
+  t.step = p.causal ? R : 0;
+  return t;
+}
+
+__device__ __forceinline__ int64_t pa_shfl(int64_t x, int lane) { return __shfl((long long)x, lane, 64); }
+__device__ __forceinline__ int64_t pa_uniform(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// Where stretch w of a KV head's line begins: sequence b, tile i, `off` into the tile; `left` is
+// the stretch's length (0: none) and `quota` that of every full one.
+struct PaStretch {
+  int32_t b, i;
+  int64_t off, left, quota;
+};
+template <int R>
+__device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w) {
+  const int lane = threadIdx.x & 63;
+  auto cost = [&](int b) -> int64_t {
+    if (b >= p.B) return 0;
+    const PaTiles t = pa_tiles<R>(p, pa_seq(p, b));
+    return t.upto(t.n);
+  };
+  const int64_t mine = cost(lane);
+  int64_t all = mine;
+  for (int b = 64 + lane; b < p.B; b += 64) all += cost(b);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor((long long)all, o, 64);
+  PaStretch s;
+  all = pa_uniform(all);
+  s.quota = max((all + p.W - 1) / p.W, p.least);
+  s.off = s.quota * w;
+  s.left = min(s.quota, all - s.off);
+  s.b = s.i = 0;
+  if (s.left <= 0) {
+    s.left = 0;
+    return s;
+  }
+  for (int b0 = 0;; b0 += 64) {
+    const int64_t c = b0 == 0 ? mine : cost(b0 + lane);
+    int64_t sum = c;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t y = __shfl_up((long long)sum, o, 64);
+      if (lane >= o) sum += y;
+    }
+    const int64_t here = pa_uniform(pa_shfl(sum, 63));
+    if (s.off >= here && b0 + 64 < p.B) {
+      s.off -= here;
+      continue;
+    }
+    const int at = __ffsll((unsigned long long)__ballot(sum > s.off)) - 1;  // (off is below the line's end)
+    s.b = __builtin_amdgcn_readfirstlane(b0 + at);
+    s.off -= pa_uniform(pa_shfl(sum - c, at));
+    break;
+  }
+  const PaTiles t = pa_tiles<R>(p, pa_seq(p, s.b));
+  // upto(i) <= off < upto(i + 1): the quadratic's root, and what its rounding may have missed
+  int64_t i;
+  if (t.step == 0) {
+    i = s.off / t.a;
+  } else {
+    const double h = (double)t.a + 0.5 * (double)t.step;
+    i = (int64_t)((sqrt(h * h + 2.0 * (double)t.step * (double)s.off) - h) / (double)t.step);
+  }
+  i = min(max(i, (int64_t)0), (int64_t)t.n - 1);
+  while (i > 0 && t.upto(i) > s.off) --i;
+  while (i + 1 < t.n && t.upto(i + 1) <= s.off) ++i;
+  s.i = __builtin_amdgcn_readfirstlane((int32_t)i);
+  s.off = pa_uniform(s.off - t.upto(i));
+  s.left = pa_uniform(s.left);
+  return s;
+}
+
+// Of a tile of `n` staged blocks of keys and cost C, those before place c.
+__device__ __forceinline__ int pa_blocks(int n, int64_t c, int64_t C) {
+  if (c <= 0) return 0;
+  if (c >= C) return n;
+  return min((int)((double)n * ((double)c / (double)C)), n);
+}
+
+// The cache's row of (page entry of key, KV head): its place among the pool's rows.
+__device__ __forceinline__ uint32_t pa_row(const PaKP &p, const int32_t *pages, int key, int kvh) {
+  const uint32_t at = (uint32_t)key / (uint32_t)p.page;
+  const int64_t phys = min(max((int64_t)pages[at], (int64_t)0), p.n_phys - 1);
+  return (uint32_t)((phys * p.Hkv + kvh) * p.page + ((uint32_t)key - at * (uint32_t)p.page));
+}
+
+__device__ __forceinline__ int64_t pa_q_at(const PaKP &p, int b, const PaSeq &s, int t, int h) {
+  return (p.cu_q ? (s.q0 + t) * p.q_st : b * p.q_sb + t * p.q_st) + h * p.q_sh;
+}
+__device__ __forceinline__ int64_t pa_out_at(const PaKP &p, int b, const PaSeq &s, int t, int h) {
+  return (p.cu_q ? (s.q0 + t) * p.o_st : b * p.o_sb + t * p.o_st) + h * p.o_sh;
+}
+__device__ __forceinline__ int64_t pa_lse_at(const PaKP &p, int b, const PaSeq &s, int t, int h) {
+  return (p.cu_q ? s.q0 + t : b * p.l_sb + t) + h * p.l_sh;
+}
+
+// Rows of the call that no sequence holds: zeros, lse -inf; shared out over the workgroups.
+template <int D>
+__device__ __forceinline__ void pa_rest(const PaKP &p, int kvh) {
+  const float ninf = __int_as_float(0xff800000);
+  auto zero = [&](int64_t o, int64_t l) {
+    for (int e = threadIdx.x; e < p.G * D; e += blockDim.x)
+      store_from_f32(p.out, o + (kvh * p.G + e / D) * p.o_sh + e % D, p.out_dt, 0.f);
+    if (p.lse)
+      for (int g = threadIdx.x; g < p.G; g += blockDim.x) p.lse[l + (kvh * p.G + g) * p.l_sh] = ninf;
+  };
+  const int64_t first = blockIdx.x / (uint32_t)p.Hkv, step = p.W;
+  if (p.cu_q) {
+    if (!p.zero_rest) return;
+    const int64_t lo = da_cu(p.cu_q, 0, p.Tq), hi = max(lo, (int64_t)da_cu(p.cu_q, p.B, p.Tq));
+    for (int64_t i = first; i < lo + p.Tq - hi; i += step) {
+      const int64_t t = i < lo ? i : hi + i - lo;
+      zero(t * p.o_st, t);
+    }
+  } else if (p.q_len) {
+    for (int64_t i = first; i < (int64_t)p.B * p.Tq; i += step) {
+      const int64_t b = i / p.Tq, t = i % p.Tq;
+      if (t >= p.q_len[b]) zero(b * p.o_sb + t * p.o_st, b * p.l_sb + t);
+    }
+  }
+}
+
+}  // namespace la

@@ -4,7 +4,8 @@
 causal, grouped heads) over the framework's (B, H, T, D) tensors, ``packed_attention`` the
 same over sequences of different lengths packed one behind the other.  Nothing of the
 (Tq, Tk) score matrix is stored.  Both can return each row's log sum of exponentials,
-which ``linattn_amd.kernels.eviction`` weighs cached keys by.
+which ``linattn_amd.kernels.eviction`` weighs cached keys by.  ``paged_attention`` reads keys
+and values from the pages of a cache, as ``linattn_amd.kernels.kv_cache`` fills it.
 """
 
 from __future__ import annotations
@@ -16,8 +17,9 @@ from typing import Optional, Tuple, Union
 import torch
 
 from linattn_amd import _native as N
+from linattn_amd.kernels.block_sparse import _paged_scale_stride
 
-__all__ = ["dense_attention", "packed_attention"]
+__all__ = ["dense_attention", "packed_attention", "paged_attention"]
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -192,4 +194,111 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         (q_t, q_h, _), (k_t, k_h, _), (v_t, v_h, _), (o_t, o_h, _) = (x.stride() for x in (q, k, v, out))
         _run(what, q, k, v, out, lse, cu_seqlens, cu_seqlens_k, None, None, (B, Hq, Hkv, Nq, Nk), (0, q_h, q_t),
              (0, k_h, k_t), (0, v_h, v_t), (0, o_h, o_t), (0, Nq), causal, scale, 1 if zero_rest else 0)
+    return (out, lse) if return_lse else out
+
+
+def _pools(what: str, k_pool: torch.Tensor, v_pool: torch.Tensor, dtype: torch.dtype, Hkv: int, D: int,
+           k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor]) -> Tuple[bool, int]:
+    """(whether the pools hold fp8 codes, the stride of their scales), checked."""
+    if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or k_pool.shape[1] != Hkv or k_pool.shape[3] != D \
+            or k_pool.numel() == 0:
+        raise ValueError(f"{what}: pools must be (n_phys, {Hkv}, page_size, {D}), and not empty")
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError(f"{what}: pools must be contiguous")
+    fp8 = k_pool.dtype == torch.float8_e4m3fn
+    if k_pool.dtype != v_pool.dtype or not (fp8 or k_pool.dtype == dtype):
+        raise ValueError(f"{what}: the pools hold the queries' dtype, or float8_e4m3fn codes")
+    if not fp8:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"{what}: scales are for fp8 pools")
+        return False, 1
+    for s in (k_scale, v_scale):
+        if s is None or s.dtype != torch.float32 or s.shape != k_pool.shape[:3]:
+            raise ValueError(f"{what}: fp8 pools need fp32 k_scale / v_scale (n_phys, Hkv, page_size)")
+    if k_scale.stride() != v_scale.stride():
+        raise ValueError(f"{what}: k_scale / v_scale must share strides")
+    return True, _paged_scale_stride(k_scale, k_pool)
+
+
+def _table(what: str, page_table: torch.Tensor, B: int) -> None:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B \
+            or page_table.shape[1] == 0 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError(f"{what}: page_table must be int32 ({B}, pages) with unit column stride")
+
+
+def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
+                    lengths: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, *, causal: bool = True,
+                    scale: Optional[float] = None, q_lengths: Optional[torch.Tensor] = None,
+                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                    return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """``dense_attention`` of new tokens over the pages of a cache that holds their keys already:
+    chunks of prompts and single tokens, in one call.
+
+    q (N, Hq, D) with ``cu_seqlens`` (int32 (B + 1,), ascending, on the device): sequence b's
+    queries are rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1, none to many; or (B, Hq, Tq, D),
+    with ``q_lengths`` (int32 (B,), default Tq) queries of each.  ``lengths`` (int32 (B,)) gives
+    the keys of each sequence, the new ones among them; key s lies in slot s % page_size of
+    page ``page_table[b, s // page_size]`` (int32 (B, pages)) of the pools (n_phys, Hkv,
+    page_size, D), any page size.  Slots past a sequence's length are never read; lengths past
+    the table are the table's; a page outside of the pool is read as the nearest that is in it.
+    With ``causal`` the queries are the last of the keys' positions.
+    bfloat16, float16 or float32, D 64 or 128; pools in q's dtype, or float8_e4m3fn codes with
+    ``k_scale`` / ``v_scale`` (float32 (n_phys, Hkv, page_size), contiguous or the halves of
+    ``fp8_scale_pairs``) and 16-bit q.
+    Returns as ``packed_attention``: (N, Hq, D), with ``return_lse`` (Hq, N), rows that no
+    sequence holds left as they were in an ``out`` that is passed; or as ``dense_attention``:
+    (B, Hq, Tq, D) and (B, Hq, Tq).  Lengths and pages are read on the device, and the work is
+    shared out there, so a captured call may be replayed with others.  Forward only."""
+    what = "paged_attention"
+    dev = N.require_gpu(q, k_pool, v_pool, page_table, lengths, cu_seqlens, q_lengths, k_scale, v_scale, out, what=what)
+    packed = cu_seqlens is not None
+    if q.dim() != (3 if packed else 4):
+        raise ValueError(f"{what}: q must be (N, Hq, D) with cu_seqlens, or (B, Hq, Tq, D)")
+    if q.dtype not in _TYPES:
+        raise ValueError(f"{what}: q must be bfloat16, float16 or float32")
+    Hq, D = q.shape[1], q.shape[-1]
+    if D not in (64, 128):
+        raise ValueError(f"{what}: head_dim must be 64 or 128")
+    Hkv = k_pool.shape[1] if k_pool.dim() == 4 else 0
+    fp8, s_stride = _pools(what, k_pool, v_pool, q.dtype, Hkv, D, k_scale, v_scale)
+    if fp8 and q.dtype == torch.float32:
+        raise ValueError(f"{what}: fp8 pools take bfloat16 or float16 queries")
+    if Hq == 0 or Hq % Hkv:
+        raise ValueError(f"{what}: the query heads must be a multiple of the KV heads")
+    if packed:
+        cu_seqlens = _cu(cu_seqlens, "cu_seqlens")
+        if q_lengths is not None:
+            raise ValueError(f"{what}: q_lengths are for batched queries")
+        B, Tq = cu_seqlens.shape[0] - 1, q.shape[0]
+    else:
+        B, Tq = q.shape[0], q.shape[2]
+        q_lengths = _int32(q_lengths, (B,), "q_lengths")
+    _table(what, page_table, B)
+    lengths = _int32(lengths, (B,), "lengths")
+    if lengths is None:
+        raise ValueError(f"{what}: lengths must be int32 ({B},)")
+    zero_rest = out is None
+    out = _out(what, out, q, out_dtype, k_pool, v_pool)
+    lse, l_s = None, (0, 0)
+    if return_lse:
+        lse = torch.empty((Hq, Tq) if packed else (B, Hq, Tq), dtype=torch.float32, device=dev) if zero_rest or not packed \
+            else torch.full((Hq, Tq), float("-inf"), dtype=torch.float32, device=dev)
+        l_s = (0, Tq) if packed else (Hq * Tq, Tq)
+    if B > 0 and Tq > 0:
+        q = _rows(q, 0 if packed else -2)
+        q_s, o_s = (((0, t.stride(1), t.stride(0)) if packed else t.stride()[:3]) for t in (q, out))
+        a = N.LaPagedAttnArgs(
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), N.ptr(lse), N.ptr(k_scale),
+            N.ptr(v_scale), page_table.data_ptr(), lengths.data_ptr(), N.ptr(cu_seqlens), N.ptr(q_lengths), None, 0,
+            B, Hq, Hkv, Tq, D, *q_s, *o_s, *l_s, k_pool.shape[0], k_pool.shape[2], page_table.stride(0),
+            page_table.shape[1], s_stride, _scale(scale, D), 1 if causal else 0, N.dtype_code(q.dtype),
+            N.dtype_code(k_pool.dtype), N.dtype_code(out.dtype), 1 if zero_rest else 0)
+        L, ref = N.load(), ctypes.byref(a)
+        with N.on_device(dev):
+            nbytes = L.la_paged_attention_workspace(ref)
+            if nbytes:
+                ws = N.workspace(nbytes, dev)
+                a.workspace, a.ws_bytes = ws.data_ptr(), nbytes
+            N.check(L.la_paged_attention(ref, N.stream_handle(dev)), what)
     return (out, lse) if return_lse else out

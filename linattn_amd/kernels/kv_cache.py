@@ -22,7 +22,8 @@ import torch
 
 from linattn_amd import _native as N
 from linattn_amd.kernels.block_sparse import _paged_scale_stride
-from linattn_amd.kernels.rotary import (_TYPES, _frequencies, _out_rows, _positions, _strides, _unit_rows)
+from linattn_amd.kernels.dense import _pools, _table
+from linattn_amd.kernels.rotary import _TYPES, _frequencies, _out_rows, _positions, _strides, _unit_rows
 
 __all__ = ["paged_kv_append", "rotary_kv_append"]
 
@@ -107,35 +108,6 @@ def paged_kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tens
     a.in_dtype = N.dtype_code(k_new.dtype)
     a.pool_dtype = N.dtype_code(k_pool.dtype)
     N.check(N.load().la_paged_kv_append(ctypes.byref(a), N.stream_handle(dev)), "paged_kv_append")
-
-
-def _pools(what: str, k_pool: torch.Tensor, v_pool: torch.Tensor, dtype: torch.dtype, Hkv: int, D: int,
-           k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor]) -> Tuple[bool, int]:
-    """(whether the pools hold fp8 codes, the stride of their scales), checked."""
-    if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or k_pool.shape[1] != Hkv or k_pool.shape[3] != D \
-            or k_pool.numel() == 0:
-        raise ValueError(f"{what}: pools must be (n_phys, {Hkv}, page_size, {D}), and not empty")
-    if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
-        raise ValueError(f"{what}: pools must be contiguous")
-    fp8 = k_pool.dtype == torch.float8_e4m3fn
-    if k_pool.dtype != v_pool.dtype or not (fp8 or k_pool.dtype == dtype):
-        raise ValueError(f"{what}: the pools hold the queries' dtype, or float8_e4m3fn codes")
-    if not fp8:
-        if k_scale is not None or v_scale is not None:
-            raise ValueError(f"{what}: scales are for fp8 pools")
-        return False, 1
-    for s in (k_scale, v_scale):
-        if s is None or s.dtype != torch.float32 or s.shape != k_pool.shape[:3]:
-            raise ValueError(f"{what}: fp8 pools need fp32 k_scale / v_scale (n_phys, Hkv, page_size)")
-    if k_scale.stride() != v_scale.stride():
-        raise ValueError(f"{what}: k_scale / v_scale must share strides")
-    return True, _paged_scale_stride(k_scale, k_pool)
-
-
-def _table(what: str, page_table: torch.Tensor, B: int) -> None:
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B \
-            or page_table.shape[1] == 0 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError(f"{what}: page_table must be int32 ({B}, pages) with unit column stride")
 
 
 def rotary_kv_append(q: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
