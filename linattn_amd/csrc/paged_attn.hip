@@ -33,10 +33,10 @@ __device__ __forceinline__ int64_t pa_part(const PaKP &p, int wg, bool last) { r
 
 // Rows r_first + i of which bit i of `bad` is set, whose results are not finite: those with an
 // infinity or NaN of V among what their blocks (keys a .. end - 1) held and they do not see are done
-// again, key by key, in fp32; the others stand, but in fp16, where a weight below 2^-40 of the
+// again, key by key, in fp32 (ALL: and the others); the others stand, but in fp16 (LOST), where a weight below 2^-40 of the
 // row's largest is 0 and its product with an infinity NaN: a dim's first keys with NaN and either
 // infinity say what it is for each row.  (What a block holds past the last key is that key again.)
-template <class E, int D, int NR, bool KV8, bool LOST>
+template <class E, int D, int NR, bool KV8, bool ALL, bool LOST>
 __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t part, int r_tile, int r_first, uint32_t bad, int a, int end) {
   const int lane = threadIdx.x & 63, G = p.G;
   const int32_t *pages = p.page_table + b * p.pt_sb;
@@ -66,8 +66,8 @@ __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t
     if (!((bad >> i) & 1u)) continue;
     const int r = r_first + i, t = r / G, h = kvh * G + r % G;
     const int lim = p.causal ? min(sq.lk - 1, sq.lk - sq.lq + t) : sq.lk - 1;
-    bool met = false;
-    for (int key = max(max(lim + 1, a), 0); key < end; ++key)
+    bool met = ALL;
+    for (int key = max(max(lim + 1, a), 0); key < end && !ALL; ++key)
       for (int d = lane; d < D; d += 64) met = met || !(fabsf(V.at(row(key), d)) < inf);
     if (__ballot(met) == 0) {
 #pragma unroll
@@ -125,231 +125,505 @@ __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t
   }
 }
 
-// What follows a piece: the next tile of the stretch, or the join's note of the tile that is left open.
+// A workgroup's way along its stretch.  It lies in LDS, and the call's arguments are read anew
+// (pa_args) at either end of a piece, so that nothing of it takes registers in between.
 struct PaWalk {
   PaStretch s;
   PaSeq seq;
-  PaTiles tiles;
-  int wg, w, kvh;
-  template <int R>
-  __device__ __forceinline__ bool begin(const PaKP &p) {
-    wg = blockIdx.x;
-    kvh = wg % p.Hkv;
-    w = wg / p.Hkv;
-    s = pa_stretch<R>(p, w);
-    if (s.left == 0) {
-      if (threadIdx.x == 0) p.ws_join[wg] = int4{0, 0, 0, 0};
-      return false;
-    }
-    load<R>(p);
-    return true;
+  int64_t a, step;  // (of the sequence's tiles)
+  int32_t n;
+};
+
+// The lane's number, of which nothing is worked out ahead (it would take registers, or memory, from
+// there on).
+__device__ __forceinline__ int pa_lane() {
+  int x = threadIdx.x & 63;
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+typedef const __attribute__((address_space(4))) PaKP PaArgs;
+__device__ __forceinline__ const PaKP &pa_args() {
+  PaArgs *x = (PaArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(x));
+  return *(const PaKP *)x;
+}
+
+template <int R>
+__device__ __forceinline__ void pa_load(const PaKP &p, PaWalk &w) {
+  w.seq = pa_seq(p, w.s.b);
+  const PaTiles t = pa_tiles<R>(p, w.seq);
+  w.a = t.a;
+  w.step = t.step;
+  w.n = t.n;
+}
+
+// The stretch's beginning, by every wave; false: there is none.
+template <int R>
+__device__ __forceinline__ bool pa_begin(PaWalk *walk) {
+  const PaKP &p = pa_args();
+  PaWalk w;
+  w.s = pa_stretch<R>(p, blockIdx.x / (uint32_t)p.Hkv);
+  if (w.s.left == 0) {
+    if (threadIdx.x == 0) p.ws_join[blockIdx.x] = int4{0, 0, 0, 0};
+    return false;
   }
-  template <int R>
-  __device__ __forceinline__ void load(const PaKP &p) {
-    seq = pa_seq(p, s.b);
-    seq.lq = __builtin_amdgcn_readfirstlane(seq.lq);
-    seq.lk = __builtin_amdgcn_readfirstlane(seq.lk);
-    seq.q0 = pa_uniform(seq.q0);
-    tiles = pa_tiles<R>(p, seq);
-  }
-  // (false: the stretch is done)
-  template <int R>
-  __device__ __forceinline__ bool next(const PaKP &p, int64_t cost, int64_t upto) {
-    s.left -= upto - s.off;
-    if (s.left <= 0) {
-      const bool open = s.off == 0 && upto < cost;
-      const int parts = open ? 1 + (int)((cost - upto + s.quota - 1) / s.quota) : 0;
-      if (threadIdx.x == 0) p.ws_join[wg] = int4{s.b, s.i, parts, 0};
-      return false;
+  pa_load<R>(p, w);
+  if (threadIdx.x == 0) *walk = w;
+  __syncthreads();
+  return true;
+}
+
+// The next tile of the stretch, or the join's note of the tile that is left open (false: the stretch
+// is done).  By every wave.
+template <int R>
+__device__ __forceinline__ bool pa_next(PaWalk *walk) {
+  const PaKP &p = pa_args();
+  PaWalk w = *walk;
+  lds_barrier();  // (every wave has read it)
+  const int64_t cost = w.a + w.step * (w.s.i + 1), upto = min(cost, w.s.off + w.s.left);
+  w.s.left -= upto - w.s.off;
+  const bool more = __builtin_amdgcn_readfirstlane(w.s.left > 0);
+  if (threadIdx.x == 0) {
+    if (!more) {
+      const int parts = w.s.off == 0 && upto < cost ? 1 + (int)((cost - upto + w.s.quota - 1) / w.s.quota) : 0;
+      p.ws_join[blockIdx.x] = int4{w.s.b, w.s.i, parts, 0};
+    } else {
+      w.s.off = 0;
+      if (++w.s.i >= w.n) {
+        w.s.i = 0;
+        do {
+          ++w.s.b;
+          pa_load<R>(p, w);
+        } while (w.n == 0 && w.s.b + 1 < p.B);
+      }
+      *walk = w;
     }
-    s.off = 0;
-    if (++s.i < tiles.n) return true;
-    s.i = 0;
-    do {
-      ++s.b;
-      load<R>(p);
-    } while (tiles.n == 0 && s.b + 1 < p.B);
-    return true;
+  }
+  __syncthreads();
+  return more;
+}
+
+// The piece that the walk is at, in scalar registers: rows r0 .. of a sequence, and which of its
+// blocks of BS keys.
+struct PaPiece {
+  PaSeq sq;
+  int32_t b, r0, kvh, j0, j1;
+  int64_t part;  // (-1: the whole tile)
+};
+template <int R, int BS>
+__device__ __forceinline__ PaPiece pa_piece(const PaKP &p, const PaWalk *walk) {
+  asm volatile("" ::: "memory");
+  PaWalk w = *walk;
+  PaPiece x;
+  x.sq.lq = __builtin_amdgcn_readfirstlane(w.seq.lq);
+  x.sq.lk = __builtin_amdgcn_readfirstlane(w.seq.lk);
+  x.sq.q0 = pa_uniform(w.seq.q0);
+  x.b = __builtin_amdgcn_readfirstlane(w.s.b);
+  x.r0 = __builtin_amdgcn_readfirstlane(w.s.i) * R;
+  x.kvh = (int)(blockIdx.x % (uint32_t)p.Hkv);
+  const int last = (min(x.r0 + R, x.sq.lq * p.G) - 1) / p.G;  // its last query
+  const int lim = p.causal ? x.sq.lk - x.sq.lq + last : x.sq.lk - 1;
+  const int n_all = lim < 0 ? 0 : lim / BS + 1;
+  const int64_t cost = w.a + w.step * (w.s.i + 1), upto = min(cost, w.s.off + w.s.left);
+  x.j0 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, w.s.off, cost));
+  x.j1 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, upto, cost));
+  x.part = pa_uniform(w.s.off == 0 && upto == cost ? -1 : pa_part(p, blockIdx.x, w.s.off == 0));
+  return x;
+}
+
+// The cache's rows of a wave's sixteen keys of each block of 64: pages of whole sixteens (EVEN):
+// of block jb + lane, the first of the sixteen; else of block jb + lane / 16, key lane % 16 of them.
+template <bool EVEN>
+struct PaRows {
+  static constexpr int SPAN = EVEN ? 64 : 4;
+  const int32_t *pages;
+  uint32_t rows;
+  int jb, key0, last;  // first key of the wave's sixteen in a block; the sequence's last
+  __device__ __forceinline__ void look(const PaKP &p, int kvh, int j) {
+    jb = j;
+    const int lane = pa_lane();
+    const int key = EVEN ? (j + lane) * DA_BS + key0 : (j + lane / 16) * DA_BS + key0 + lane % 16;
+    rows = pa_row(p, pages, min(key, last), kvh);
+    settle(rows);
+  }
+  // EVEN: the first row of block j's sixteen, and how many keys there are behind it
+  __device__ __forceinline__ uint32_t first(int j) const { return (uint32_t)__builtin_amdgcn_readlane((int)rows, j - jb); }
+  __device__ __forceinline__ int behind(int j) const { return last - min(j * DA_BS + key0, last); }
+  // this lane's row for key rr (keys past the last: that again)
+  __device__ __forceinline__ uint32_t of(int j, int rr) const {
+    if constexpr (EVEN) return first(j) + min(rr, behind(j));
+    else return (uint32_t)__shfl((int)rows, (j - jb) * 16 + rr, 64);
+  }
+  // Sixteen rows of RB bytes each of block j into LDS at `to`, 16-byte chunk c of row r at c ^ swz(r)
+  // (swz takes the same values for rows PER apart): 64 lanes x 16 bytes a load.
+  template <int RB, int PER, class Swz>
+  __device__ __forceinline__ void load(const void *pool, int j, uint32_t to, int lane, Swz swz) const {
+    constexpr int CH = RB / 16, RP = 64 / CH, NX = 16 / RP;
+    if constexpr (EVEN) {
+      const int n = behind(j);
+      const char *base = (const char *)pool + (uint64_t)first(j) * RB;
+      if (n >= 15) {
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+          constexpr int STEP = PER / RP > 0 ? PER / RP : 1;  // loads after which the offsets come again
+          const int rr = RP * (x % STEP) + lane / CH;
+          asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"((uint32_t)(rr * RB + 16 * ((lane % CH) ^ swz(rr)))),
+                       "s"(base + RP * (x - x % STEP) * RB), "{m0}"(to + x * 1024) : "memory");
+        }
+      } else {
+        lane = pa_lane();
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+          const int rr = RP * x + lane / CH;
+          asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"((uint32_t)(min(rr, n) * RB + 16 * ((lane % CH) ^ swz(rr)))),
+                       "s"(base), "{m0}"(to + x * 1024) : "memory");
+        }
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        const int rr = RP * x + lane / CH;
+        const char *src = (const char *)pool + (uint64_t)of(j, rr) * RB + 16 * ((lane % CH) ^ swz(rr));
+        asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src), "{m0}"(to + x * 1024) : "memory");
+      }
+    }
   }
 };
+
+// Four codes as two pairs of bf16 or fp16 (exactly).
+template <class T>
+__device__ __forceinline__ uint2 pa_widen(uint32_t codes) {
+  if constexpr (std::is_same<T, DaBf16>::value)
+    return uint2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.f, true))};
+  else
+    return uint2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.f, true))};
+}
+
+// 16 x 16 += (16 x 16) (16 x 16)
+template <class T>
+__device__ __forceinline__ f32x4 pa_mfma16(s16x4 a, s16x4 b, f32x4 c) {
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  if constexpr (std::is_same<T, DaBf16>::value) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
+
+constexpr int PA_WAVE_LDS = 12288;  // of a wave, where the waves of a workgroup go their own ways
+
+// At most 16 rows of a sequence and KV head (single tokens): the waves take a quarter of each block's
+// keys each, without barriers, and join in LDS.  Bound by the reads: a wave has three pieces of
+// sixteen rows of K or V on their way into LDS of its own (fp8: four), of which one is used.
+// S^T = K Q^T by 16x16x32 products, O^T += V^T P^T by 16x16x16, P as the sum of two
+// terms of the type (16 bits of each weight), which the matrix cores have room for here.
+template <class T, int D, bool KV8, bool EVEN>
+__device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale, uint32_t *s_bad) {
+  typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V
+  typedef typename T::x8 x8;
+  typedef typename T::elem elem;
+  typedef typename TP::elem pelem;
+  typedef pelem px4 __attribute__((ext_vector_type(4)));
+  constexpr int NW = 4, NK = D / 32, RB = KV8 ? D : 2 * D, UNIT = 16 * RB, NU = KV8 ? 4 : 3, NX = UNIT / 1024;
+  constexpr int CH = D / 8;
+  const int lane = pa_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane >> 4, ri = lane & 15;
+  char *mine = smem + w * PA_WAVE_LDS;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)mine);
+  const uint32_t sc0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)((char *)s_scale + w * 768));
+  // 16-byte chunk swizzles.  K: the sixteen rows of one chunk lie in all banks; V (two bytes a
+  // value): eight rows' pairs of chunks (FewRows).
+  auto swz_k = [](int r) { return D == 128 && !KV8 ? r & 15 : D == 128 || !KV8 ? (r >> 1) & 7 : (r >> 2) & 3; };
+  auto swz_v = [](int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); };
+  x8 qf[NK];
+  f32x4 acc[D / 16];
+  float m = pa_ninf(), thr = pa_ninf(), l = 0.f, nmu = 0.f;
+  {
+    const PaKP &p = pa_args();
+    const PaPiece x = pa_piece<128, DA_BS>(p, walk);
+    const int nrow = x.sq.lq * p.G, row = min(ri, nrow - 1), t = row / p.G;
+    const int lim = p.causal ? x.sq.lk - x.sq.lq + t : x.sq.lk - 1;  // last key seen
+    const float qscale = p.qscale, thr_gap = p.thr_gap;
+    const int64_t s_stride = p.s_stride;
+    const void *kp = p.k, *vp = p.v;
+    const float *k_scale = p.k_scale, *v_scale = p.v_scale;
+    PaRows<EVEN> rows;
+    rows.pages = p.page_table + x.b * p.pt_sb;
+    rows.key0 = 16 * w;
+    rows.last = x.sq.lk - 1;
+    const int n = x.j1 - x.j0;
+    // piece u of K or V rows: K of block j0 + u / 2, then V
+    auto load = [&](int u) {
+      const int j = x.j0 + (u >> 1);
+      if ((u & 1) == 0 && j - rows.jb == PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j);
+      const uint32_t to = lds0 + (uint32_t)(u % NU) * UNIT;
+      if (u & 1) {
+        if constexpr (KV8) rows.template load<RB, 16>(vp, j, to, lane, [](int) { return 0; });
+        else rows.template load<RB, 8>(vp, j, to, lane, swz_v);
+      } else {
+        rows.template load<RB, 16>(kp, j, to, lane, swz_k);
+        if constexpr (KV8) {  // the keys' scales and their values', 16 each (and again)
+          const float *src = (lane & 16 ? v_scale : k_scale) + rows.of(j, ri) * (uint64_t)s_stride;
+          const uint32_t m0 = sc0 + (uint32_t)((u >> 1) % 3) * 256;
+          asm volatile("global_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+        }
+      }
+    };
+    const elem *qp = (const elem *)p.q + pa_q_at(p, x.b, x.sq, t, x.kvh * p.G + row % p.G);
+#pragma unroll
+    for (int s = 0; s < NK; ++s) qf[s] = *(const x8 *)(qp + 32 * s + 8 * c);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (n > 0) {
+      rows.look(p, x.kvh, x.j0);
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        if (u < 2 * n) load(u);
+    }
+#pragma unroll
+    for (int s = 0; s < NK; ++s) settle(qf[s]);
+    for (int i = 0; i < n; ++i) {
+      const int j = x.j0 + i;
+      // newer pieces on their way: V of this block, and K (fp8: and V) of the next
+      if (i + 1 < n) wait_vmcnt<(NU - 1) * NX + (KV8 ? 1 : 0)>();
+      else wait_vmcnt<NX>();
+      const float *sc = (const float *)((const char *)s_scale + w * 768 + (i % 3) * 256);
+      f32x4 st = f32x4{0.f, 0.f, 0.f, 0.f};
+      const char *sk = mine + ((2 * i) % NU) * UNIT;
+#pragma unroll
+      for (int s = 0; s < NK; ++s) {
+        if constexpr (KV8) {
+          const uint2 codes = *(const uint2 *)(sk + ri * RB + 16 * ((2 * s + (c >> 1)) ^ swz_k(ri)) + 8 * (c & 1));
+          const uint2 a = pa_widen<T>(codes.x), b = pa_widen<T>(codes.y);
+          st = T::mfma16(__builtin_bit_cast(x8, uint4{a.x, a.y, b.x, b.y}), qf[s], st);
+        } else {
+          st = T::mfma16(*(const x8 *)(sk + ri * RB + 16 * ((4 * s + c) ^ swz_k(ri))), qf[s], st);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its place is free
+      if (2 * i + NU < 2 * n) load(2 * i + NU);
+      if constexpr (KV8) {
+        // register e: key 4 c + e
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[e] *= sc[4 * c + e];
+      }
+      const int d = lim - j * DA_BS - 16 * w - 4 * c;
+      float mx = pa_ninf();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        st[e] = e <= d ? st[e] : pa_ninf();
+        mx = fmaxf(mx, st[e]);
+      }
+      if (__ballot(mx > thr) != 0) {
+        const float mn = fmaxf(m, pair32_max(pair16_max(mx))), to = da_ref<TP>(mn, qscale);
+        const float alpha = m == pa_ninf() ? 0.f : fast_exp2(to - nmu);
+        m = mn;
+        thr = mn + thr_gap;
+        nmu = to;
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) acc[dt] *= alpha;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        st[e] = fast_exp2(__builtin_fmaf(st[e], qscale, nmu));
+        sum += st[e];
+      }
+      l += sum;
+      if constexpr (KV8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st[e] *= sc[16 + 4 * c + e];
+      }
+      px4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        hi[e] = (pelem)st[e];
+        lo[e] = (pelem)(st[e] - (float)hi[e]);
+      }
+      // newer: K and V of the next block, and (fp8) K of the one behind it
+      if (KV8 && i + 2 < n) wait_vmcnt<3 * NX + 2>();
+      else if (i + 1 < n) wait_vmcnt<2 * NX + (KV8 ? 1 : 0)>();
+      else wait_vmcnt<0>();
+      const uint16_t *sv = (const uint16_t *)(mine + ((2 * i + 1) % NU) * UNIT);
+      if constexpr (KV8) {  // widened into a place of its own
+        sv = (const uint16_t *)(mine + NU * UNIT);
+#pragma unroll
+        for (int y = 0; y < NX; ++y) {
+          const int at = 64 * y + lane, r = at / (RB / 16), ch = at % (RB / 16);
+          const uint4 codes = *(const uint4 *)(mine + ((2 * i + 1) % NU) * UNIT + 16 * at);
+          const uint2 a = pa_widen<TP>(codes.x), b = pa_widen<TP>(codes.y), e = pa_widen<TP>(codes.z), f = pa_widen<TP>(codes.w);
+          *(uint4 *)((char *)sv + 2 * r * D + 16 * ((2 * ch) ^ swz_v(r))) = uint4{a.x, a.y, b.x, b.y};
+          *(uint4 *)((char *)sv + 2 * r * D + 16 * ((2 * ch + 1) ^ swz_v(r))) = uint4{e.x, e.y, f.x, f.y};
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      const int kr = 4 * c + (ri >> 2);
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) {
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4 *)(sv + kr * D + 8 * ((2 * dt + ((ri & 3) >> 1)) ^ swz_v(kr)) + 4 * (ri & 1)));
+        acc[dt] = pa_mfma16<TP>(a, __builtin_bit_cast(s16x4, hi), acc[dt]);
+        acc[dt] = pa_mfma16<TP>(a, __builtin_bit_cast(s16x4, lo), acc[dt]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V is read
+      if (2 * i + 1 + NU < 2 * n) load(2 * i + 1 + NU);
+    }
+    l = pair32_sum(pair16_sum(l));
+  }
+  // the waves' states into LDS, and together
+  float *ml = (float *)mine, *vals = ml + 32;
+  if (c == 0) {
+    ml[2 * ri] = m == pa_ninf() ? m : -nmu;
+    ml[2 * ri + 1] = l;
+  }
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) *(f32x4 *)&vals[ri * (D + 4) + 16 * dt + 4 * c] = acc[dt];
+  if (threadIdx.x == 0) *s_bad = 0u;
+  lds_barrier();
+  const PaKP &p = pa_args();
+  const PaPiece x = pa_piece<128, DA_BS>(p, walk);
+  const int nrow = x.sq.lq * p.G;
+  for (int e = threadIdx.x; e < nrow * D; e += 64 * NW) {
+    const int g = e / D, dim = e % D;
+    float mm = pa_ninf();
+#pragma unroll
+    for (int y = 0; y < NW; ++y) mm = fmaxf(mm, ((const float *)(smem + y * PA_WAVE_LDS))[2 * g]);
+    float ll = 0.f, a = 0.f;
+#pragma unroll
+    for (int y = 0; y < NW; ++y) {
+      const float *of = (const float *)(smem + y * PA_WAVE_LDS);
+      const float f = fast_exp2(of[2 * g] - (mm == pa_ninf() ? 0.f : mm));
+      ll = __builtin_fmaf(of[2 * g + 1], f, ll);
+      a = __builtin_fmaf(of[32 + g * (D + 4) + dim], f, a);
+    }
+    // (with scores that are not numbers, l is not, and the row stands)
+    if (!(fabsf(a) < __int_as_float(0x7f800000)) && ll > 0.f && ll < __int_as_float(0x7f800000)) atomicOr(s_bad, 1u << g);
+    if (ll == 0.f) a = 0.f;  // (no key seen)
+    const int t = g / p.G, h = x.kvh * p.G + g % p.G;
+    if (x.part >= 0) {
+      p.ws_acc[(x.part + g) * D + dim] = a;
+      if (dim == 0) {
+        p.ws_ml[2 * (x.part + g)] = mm;
+        p.ws_ml[2 * (x.part + g) + 1] = ll;
+      }
+    } else {
+      store_from_f32(p.out, pa_out_at(p, x.b, x.sq, t, h) + dim, p.out_dt, ll == 0.f ? 0.f : a / ll);
+      if (p.lse && dim == 0) p.lse[pa_lse_at(p, x.b, x.sq, t, h)] = ll == 0.f ? pa_ninf() : (mm + __log2f(ll)) * PA_LN2;
+    }
+  }
+  __syncthreads();
+  // (an infinity that a row sees meets weights of both signs in the second terms, so all are done
+  // again; every wave's stores are done, which those replace)
+  if (*s_bad != 0u) {
+    const uint32_t bad = *s_bad;
+    wait_vmcnt<0>();
+    __syncthreads();
+    for (int g = w; g < nrow; g += NW)
+      pa_again<elem, D, 16, KV8, true, false>(p, x.b, x.sq, x.kvh, x.part, 0, 0, bad & (1u << g), x.j0 * DA_BS, x.j1 * DA_BS);
+  }
+}
 
 // bf16 / fp16 rows: four waves of 32 rows, three workgroups a CU, and the products and registers of
 // dense_attn_kernel (S^T by 32x32x16 products leaves a lane 16 scores of one row; P goes into its
 // product with V from the same registers, rounded to the inputs' type (bf16 with an fp8 cache);
 // l is of the fp32 weights).
 //
-// A wave stages 16 keys of each block of 64.  Pages of whole sixteens (`EVEN`): these lie in one
-// page, whose place for 64 blocks ahead is looked up at once, a lane a block, and the rows go
-// global -> LDS from a scalar base.  Any other page size: a lane a key, four blocks ahead.  K is
-// staged a block ahead into the other of two slots, V while its block is scored.
-//
-// fp8 caches (KV8) are loaded a block ahead into registers and widened on their way into LDS, once
-// a workgroup (e4m3 is exact in bf16 and fp16); the scale of a key multiplies its scores, that of its
-// value its weights, both in fp32.
+// A wave stages 16 keys of each block of 64 (PaRows).  K is staged a block ahead into the other of
+// two slots, V while its block is scored.  fp8 caches (KV8): codes of K and V go into LDS a block
+// ahead, and are widened there once a workgroup (e4m3 is exact in bf16 and fp16); the scale of
+// a key multiplies its scores, that of its value its weights, both in fp32.
 template <class T, int D, bool KV8, bool EVEN>
-__global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP p) {
+__device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_scale) {
   typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V
-  constexpr int NW = 4, R = 32 * NW, BLK = DA_BS * D, CH = D / 8, RP = 64 / CH, NX = 16 / RP;
-  constexpr int NS = D / 16, ND = D / 32, SPAN = EVEN ? 64 : 4;
+  constexpr int NW = 4, R = 32 * NW, BLK = DA_BS * D, NX = D / 32;
+  constexpr int NS = D / 16, ND = D / 32;
+  constexpr int VSLOT = KV8 ? 1 : 2;  // K slots 0, 1, then V; KV8: K, V, then codes of K and of V
   typedef typename T::x8 x8;
   typedef typename TP::x8 px8;
   typedef typename T::elem elem;
   typedef typename TP::elem pelem;
-  __shared__ __align__(16) uint16_t smem[3 * BLK];  // K slots 0, 1, then V
-  __shared__ __align__(16) float s_scale[KV8 ? 3 * DA_BS : 1];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = pa_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hf = lane >> 5, r32 = lane & 31;
-  const int G = p.G;
-  PaWalk walk;
-  pa_rest<D>(p, blockIdx.x % (uint32_t)p.Hkv);
-  if (!walk.begin<R>(p)) return;
-  const int kvh = walk.kvh;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void_t *)smem);
-  // LDS-DMA: instruction x of wave w fills rows 16 w + RP x + lane / CH
-  uint32_t ko[NX], vo[NX];
-#pragma unroll
-  for (int x = 0; x < NX; ++x) {
-    const int rr = RP * x + lane / CH;
-    ko[x] = (uint32_t)((rr * D + 8 * ((lane % CH) ^ da_swz_k<D>(16 * w + rr))) * 2);
-    vo[x] = (uint32_t)((rr * D + 8 * ((lane % CH) ^ da_swz_v<D>(16 * w + rr))) * 2);
-  }
   // Byte offsets of this lane's first reads of a slot (as in dense_attn_kernel).
   const uint32_t k_at = 2 * (r32 * D + 8 * (hf ^ da_swz_k<D>(r32)));
   const int v_row = 4 * hf + ((lane & 15) >> 2);
-  const uint32_t v_at = 2 * (2 * BLK + v_row * D + 8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ da_swz_v<D>(v_row)) +
+  const uint32_t v_at = 2 * (VSLOT * BLK + v_row * D + 8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ da_swz_v<D>(v_row)) +
                              4 * (lane & 1));
   const char *lds = (const char *)smem;
-
-  while (true) {
-    const PaSeq sq = walk.seq;
-    const int b = walk.s.b, r0 = walk.s.i * R;
-    const int nrow = sq.lq * G, diag = sq.lk - sq.lq;
-    auto limit = [&](int t) { return p.causal ? diag + t : sq.lk - 1; };  // last key seen
-    const int r_first = r0 + 32 * w;
-    const int r_mine = min(r_first + r32, nrow - 1);
-    const bool live = r_first + r32 < nrow, wave_live = r_first < nrow;
-    const int t = r_mine / G, h = kvh * G + r_mine % G;
-    const int lim = limit(t);
+  float m = pa_ninf(), thr = pa_ninf(), l = 0.f, nmu = 0.f;
+  f32x16 acc[ND];
+  {
+    const PaKP &p = pa_args();
+    const PaPiece x = pa_piece<R, DA_BS>(p, walk);
+    const int G = p.G, nrow = x.sq.lq * G, diag = x.sq.lk - x.sq.lq, causal = p.causal;
+    auto limit = [&](int t) { return causal ? diag + t : x.sq.lk - 1; };  // last key seen
+    const int r_first = x.r0 + 32 * w, r_mine = min(r_first + r32, nrow - 1);
+    const int t = r_mine / G, lim = limit(t);
     const int lim_lo = __builtin_amdgcn_readfirstlane(limit(min(r_first, nrow - 1) / G));
     const int lim_hi = __builtin_amdgcn_readfirstlane(limit(min(r_first + 31, nrow - 1) / G));
-    const int lim_tile = __builtin_amdgcn_readfirstlane(limit((min(r0 + R, nrow) - 1) / G));
-    const int n_all = lim_tile < 0 ? 0 : lim_tile / DA_BS + 1;
-    const int64_t cost = walk.tiles.cost(walk.s.i), upto = min(cost, walk.s.off + walk.s.left);
-    const int j0 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, walk.s.off, cost));
-    const int j1 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, upto, cost));
-    const bool whole = walk.s.off == 0 && upto == cost;
-    const int64_t part = whole ? -1 : pa_part(p, walk.wg, walk.s.off == 0);
-    const int32_t *pages = p.page_table + b * p.pt_sb;
-
-    // The cache's rows of this wave's keys: EVEN: of block jb + lane, the first of its sixteen;
-    // else of block jb + lane / 16, key lane % 16 of them.
-    uint32_t rows = 0;
-    int jb = j0;
-    auto look = [&](int j) __attribute__((always_inline)) {
-      jb = j;
-      const int key = EVEN ? (j + lane) * DA_BS + 16 * w : (j + lane / 16) * DA_BS + 16 * w + lane % 16;
-      rows = pa_row(p, pages, min(key, sq.lk - 1), kvh);
+    const int j0 = x.j0, j1 = x.j1;
+    const float qscale = p.qscale, thr_gap = p.thr_gap;
+    const void *kp = p.k, *vp = p.v;
+    const float *k_scale = p.k_scale, *v_scale = p.v_scale;
+    const int64_t s_stride = p.s_stride;
+    PaRows<EVEN> rows;
+    rows.pages = p.page_table + x.b * p.pt_sb;
+    rows.key0 = 16 * w;
+    rows.last = x.sq.lk - 1;
+    const int sw = 16 * w;
+    auto dma_k = [&](int j) __attribute__((always_inline)) {
+      rows.template load<2 * D, 8>(kp, j, lds0 + 2 * (((j - j0) & 1) * BLK + sw * D), lane, [&](int r) { return da_swz_k<D>(sw + r); });
     };
-    // this lane's row for key `rr` of the wave's sixteen of block j
-    auto row_of = [&](int j, int rr) __attribute__((always_inline)) -> uint32_t {
-      if constexpr (EVEN) {
-        const int past = sq.lk - 1 - min(j * DA_BS + 16 * w, sq.lk - 1);  // keys behind the first
-        return (uint32_t)__builtin_amdgcn_readlane((int)rows, j - jb) + min(rr, past);
-      } else {
-        return (uint32_t)__shfl((int)rows, (j - jb) * 16 + rr, 64);
-      }
+    auto dma_v = [&](int j) __attribute__((always_inline)) {
+      rows.template load<2 * D, 4>(vp, j, lds0 + 2 * (VSLOT * BLK + sw * D), lane, [&](int r) { return da_swz_v<D>(sw + r); });
     };
-    auto dma = [&](const void *pool, const uint32_t (&off)[NX], int j, int slot) __attribute__((always_inline)) {
-      if constexpr (EVEN) {
-        const uint32_t row = (uint32_t)__builtin_amdgcn_readlane((int)rows, j - jb);
-        const uint16_t *base = (const uint16_t *)pool + (uint64_t)row * D;
-        const int last = sq.lk - 1 - min(j * DA_BS + 16 * w, sq.lk - 1);
-        if (last >= 15) {
-#pragma unroll
-          for (int x = 0; x < NX; ++x)
-            asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off[x]), "s"(base),
-                         "{m0}"(lds0 + 2 * (slot * BLK + 16 * w * D + x * 512)) : "memory");
-        } else {
-#pragma unroll
-          for (int x = 0; x < NX; ++x) {
-            const int past = max(RP * x + lane / CH - last, 0);  // rows back to the last key
-            asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off[x] - past * (uint32_t)(2 * D)), "s"(base),
-                         "{m0}"(lds0 + 2 * (slot * BLK + 16 * w * D + x * 512)) : "memory");
-          }
-        }
-      } else {
-#pragma unroll
-        for (int x = 0; x < NX; ++x) {
-          const int rr = RP * x + lane / CH;
-          const char *src = (const char *)pool + (uint64_t)row_of(j, rr) * (2 * D) + (off[x] - (uint32_t)(rr * 2 * D));
-          asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(src),
-                       "{m0}"(lds0 + 2 * (slot * BLK + 16 * w * D + x * 512)) : "memory");
-        }
-      }
-    };
-    auto dma_k = [&](int j) __attribute__((always_inline)) { dma(p.k, ko, j, (j - j0) & 1); };
-    auto dma_v = [&](int j) __attribute__((always_inline)) { dma(p.v, vo, j, 2); };
-
-    // fp8: 16 codes a lane and load, and (lanes below 16) the keys' scales
-    constexpr int N8 = D / 64, R8 = 64 / (D / 16);  // loads, rows of a load
-    uint4 kr[N8], vr[N8];
+    // fp8: codes of a block, a wave's own rows, and (lanes below 16) the keys' scales
     float ks = 0.f, vs = 0.f;
-    auto fetch = [&](const void *pool, const float *scale, uint4 (&to)[N8], float &sc, int j) __attribute__((always_inline)) {
-#pragma unroll
-      for (int x = 0; x < N8; ++x)
-        to[x] = *(const uint4 *)((const uint8_t *)pool + (uint64_t)row_of(j, R8 * x + lane / (D / 16)) * D + 16 * (lane % (D / 16)));
-      sc = scale[row_of(j, lane & 15) * p.s_stride];
+    auto dma_codes = [&](int j) __attribute__((always_inline)) {
+      rows.template load<D, 1>(kp, j, lds0 + 4 * BLK + sw * D, lane, [](int) { return 0; });
+      rows.template load<D, 1>(vp, j, lds0 + 5 * BLK + sw * D, lane, [](int) { return 0; });
+      const uint64_t at = (uint64_t)rows.of(j, lane & 15) * s_stride;
+      ks = k_scale[at];
+      vs = v_scale[at];
     };
-    auto put = [&](const uint4 (&from)[N8], float sc, bool is_v, int slot) __attribute__((always_inline)) {
+    auto widen = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < N8; ++x) {
-        const int row = 16 * w + R8 * x + lane / (D / 16), c = 2 * (lane % (D / 16));
-        const int swz = is_v ? da_swz_v<D>(row) : da_swz_k<D>(row);
-        const uint32_t word[4] = {from[x].x, from[x].y, from[x].z, from[x].w};
+      for (int v = 0; v < 2; ++v)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint32_t u[4];
+        for (int y = 0; y < D / 64; ++y) {
+          const int at = 64 * y + lane, row = sw + at / (D / 16), ch = 2 * (at % (D / 16));
+          const uint4 u = *(const uint4 *)(lds + (4 + v) * BLK + sw * D + 16 * at);
+          const int swz = v ? da_swz_v<D>(row) : da_swz_k<D>(row);
+          uint2 z[4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (is_v || std::is_same<T, DaBf16>::value) {
-              u[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word[2 * y + i], 1.f, false));
-              u[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word[2 * y + i], 1.f, true));
-            } else {
-              u[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word[2 * y + i], 1.f, false));
-              u[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word[2 * y + i], 1.f, true));
-            }
-          }
-          *(uint4 *)(smem + slot * BLK + row * D + 8 * ((c + y) ^ swz)) = uint4{u[0], u[1], u[2], u[3]};
+          for (int i = 0; i < 4; ++i) z[i] = v ? pa_widen<TP>((&u.x)[i]) : pa_widen<T>((&u.x)[i]);
+          char *to = (char *)smem + 2 * (v * BLK + row * D);
+          *(uint4 *)(to + 16 * (ch ^ swz)) = uint4{z[0].x, z[0].y, z[1].x, z[1].y};
+          *(uint4 *)(to + 16 * ((ch + 1) ^ swz)) = uint4{z[2].x, z[2].y, z[3].x, z[3].y};
         }
+      if (lane < 16) {
+        s_scale[sw + lane] = ks;
+        s_scale[DA_BS + sw + lane] = vs;
       }
-      if (lane < 16) s_scale[(slot == 2 ? 2 : slot) * DA_BS + 16 * w + lane] = sc;
     };
-
-    lds_barrier();  // (the piece before is read out of LDS)
     if (j0 < j1) {
-      look(j0);
+      rows.look(p, x.kvh, j0);
       if constexpr (KV8) {
-        fetch(p.k, p.k_scale, kr, ks, j0);
-        fetch(p.v, p.v_scale, vr, vs, j0);
-        put(kr, ks, false, 0);
-        if (j0 + 1 < j1) fetch(p.k, p.k_scale, kr, ks, j0 + 1);
+        dma_codes(j0);
       } else {
-        settle(rows);
         dma_k(j0);
         dma_v(j0);
       }
     }
     x8 qf[NS];  // B operand: dims 16 s + 8 hf ..
     {
-      const elem *qp = (const elem *)p.q + pa_q_at(p, b, sq, t, h) + 8 * hf;
+      const elem *qp = (const elem *)p.q + pa_q_at(p, x.b, x.sq, t, x.kvh * G + r_mine % G) + 8 * hf;
 #pragma unroll
       for (int s = 0; s < NS; ++s) qf[s] = *(const x8 *)(qp + 16 * s);
     }
 #pragma unroll
     for (int s = 0; s < NS; ++s) settle(qf[s]);
-
-    float m = pa_ninf(), thr = pa_ninf(), l = 0.f, nmu = 0.f;
-    f32x16 acc[ND];
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
@@ -357,7 +631,7 @@ __global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP p) {
 
     // scores of block j; register i of a half holds key 8 (i / 4) + 4 hf + i % 4
     auto scores = [&](int j, f32x16 (&st)[2]) __attribute__((always_inline)) {
-      const uint32_t at = k_at + 2 * ((j - j0) & 1) * BLK;
+      const uint32_t at = k_at + (KV8 ? 0 : 2 * ((j - j0) & 1) * BLK);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -372,7 +646,7 @@ __global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP p) {
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const f32x4 sc = *(const f32x4 *)(s_scale + ((j - j0) & 1) * DA_BS + 32 * kt + 8 * g + 4 * hf);
+            const f32x4 sc = *(const f32x4 *)(s_scale + 32 * kt + 8 * g + 4 * hf);
 #pragma unroll
             for (int i = 0; i < 4; ++i) st[kt][4 * g + i] *= sc[i];
           }
@@ -398,10 +672,10 @@ __global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP p) {
         mx = largest(st);
       }
       if (__ballot(mx > thr) != 0) {
-        const float mn = fmaxf(m, pair32_max(mx)), to = da_ref<TP>(mn, p.qscale);
+        const float mn = fmaxf(m, pair32_max(mx)), to = da_ref<TP>(mn, qscale);
         const float alpha = m == pa_ninf() ? 0.f : fast_exp2(to - nmu);  // (both as rounded in the weights)
         m = mn;
-        thr = mn + p.thr_gap;
+        thr = mn + thr_gap;
         nmu = to;
         l *= alpha;
 #pragma unroll
@@ -415,137 +689,153 @@ __global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP p) {
       float sum[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        st[i] = fast_exp2(__builtin_fmaf(st[i], p.qscale, nmu));
+        st[i] = fast_exp2(__builtin_fmaf(st[i], qscale, nmu));
         sum[i & 1] = i < 2 ? st[i] : sum[i & 1] + st[i];
+        if constexpr (!KV8) pw[i >> 3][i & 7] = (pelem)st[i];
       }
       l += sum[0] + sum[1];
-      if constexpr (!KV8) {
+      if constexpr (KV8) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) pw[i >> 3][i & 7] = (pelem)st[i];
-      }
-    };
-    auto scaled = [&](int kt, const f32x16 &st, px8 (&pw)[2]) __attribute__((always_inline)) {  // (KV8)
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 sc = *(const f32x4 *)(s_scale + DA_BS + 32 * kt + 8 * g + 4 * hf);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 sc = *(const f32x4 *)(s_scale + 2 * DA_BS + 32 * kt + 8 * g + 4 * hf);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pw[g >> 1][4 * (g & 1) + i] = (pelem)(st[4 * g + i] * sc[i]);
+          for (int i = 0; i < 4; ++i) pw[g >> 1][4 * (g & 1) + i] = (pelem)(st[4 * g + i] * sc[i]);
+        }
       }
     };
     auto values = [&](int kt, const px8 (&pw)[2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int ks_ = 0; ks_ < 2; ++ks_)
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) {
-          const char *v = lds + (v_at ^ (64 * dt)) + 2 * (32 * kt + 16 * ks_) * D;
+          const char *v = lds + (v_at ^ (64 * dt)) + 2 * (32 * kt + 16 * y) * D;
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v);
           const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 16 * D));
-          acc[dt] = TP::mfma(__builtin_bit_cast(px8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pw[ks_], acc[dt]);
+          acc[dt] = TP::mfma(__builtin_bit_cast(px8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pw[y], acc[dt]);
         }
     };
 
-    const int jw = wave_live && lim_hi >= 0 ? min(lim_hi / DA_BS, j1 - 1) : -1;  // this wave's last block
+    const int jw = r_first < nrow && lim_hi >= 0 ? min(lim_hi / DA_BS, j1 - 1) : -1;  // this wave's last block
     for (int j = j0; j < j1; ++j) {
+      wait_vmcnt<0>();
+      f32x16 st[2];
+      px8 pw[2];
       if constexpr (KV8) {
-        lds_barrier();  // K of block j is there for every wave, block j - 1 is read
-        put(vr, vs, true, 2);
+        lds_barrier();  // block j - 1 is read
+        widen();
+        lds_barrier();  // block j is there, and its codes are read
         if (j + 1 < j1) {
-          put(kr, ks, false, (j + 1 - j0) & 1);
-          fetch(p.v, p.v_scale, vr, vs, j + 1);
-          if (j + 2 < j1) {
-            if (j + 2 - jb == SPAN) look(j + 2);
-            fetch(p.k, p.k_scale, kr, ks, j + 2);
-          }
+          if (j + 1 - rows.jb == PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j + 1);
+          dma_codes(j + 1);
+        }
+        if (j <= jw) {
+          scores(j, st);
+          settle_max(j, st, largest(st));
+          weigh(0, st[0], pw);
         }
       } else {
-        wait_vmcnt<0>();
         lds_barrier();  // K of block j has landed for every wave, block j - 1 is read
         if (j > j0) dma_v(j);
         if (j + 1 < j1) {
-          if (j + 1 - jb == SPAN) {
-            look(j + 1);
-            settle(rows);
-          }
+          if (j + 1 - rows.jb == PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j + 1);
           dma_k(j + 1);
         }
-      }
-      f32x16 st[2];
-      px8 pw[2];
-      if (j <= jw) {
-        scores(j, st);
-        settle_max(j, st, largest(st));
-        weigh(0, st[0], pw);
-      }
-      if constexpr (!KV8) {
+        if (j <= jw) {
+          scores(j, st);
+          settle_max(j, st, largest(st));
+          weigh(0, st[0], pw);
+        }
         if (j + 1 < j1) wait_vmcnt<NX>();
         else wait_vmcnt<0>();
+        lds_barrier();  // V of block j has landed
       }
-      lds_barrier();  // V of block j has landed
       if (j <= jw) {
-        if constexpr (KV8) scaled(0, st[0], pw);
         values(0, pw);
         weigh(1, st[1], pw);
-        if constexpr (KV8) scaled(1, st[1], pw);
         values(1, pw);
       }
     }
-    if (wave_live) {
-      l = pair32_sum(l);
-      // results that are not finite (with scores that are not numbers, l is not, and the row stands)
-      float sum = 0.f;
+  }
+  const PaKP &p = pa_args();
+  const PaPiece x = pa_piece<R, DA_BS>(p, walk);
+  const int G = p.G, nrow = x.sq.lq * G, r_first = x.r0 + 32 * w, r_mine = min(r_first + r32, nrow - 1);
+  if (r_first >= nrow) return;
+  const bool live = r_first + r32 < nrow;
+  const int t = r_mine / G, h = x.kvh * G + r_mine % G;
+  l = pair32_sum(l);
+  // results that are not finite (with scores that are not numbers, l is not, and the row stands)
+  float sum = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[dt][i], 0.f, sum);
+  const uint64_t bad = __ballot(sum != 0.f && l < __int_as_float(0x7f800000));  // (sum: NaN)
+  // register i of dim tile dt holds dim 32 dt + 8 (i / 4) + 4 hf + i % 4
+  if (live && x.part >= 0) {
+    const int64_t pi = x.part + r_mine - x.r0;
+    if (hf == 0) {
+      p.ws_ml[2 * pi] = m == pa_ninf() ? m : -nmu;
+      p.ws_ml[2 * pi + 1] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(float4 *)(p.ws_acc + pi * D + 32 * dt + 8 * i + 4 * hf) =
+            float4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
+  } else if (live) {
+    const bool none = l == 0.f;  // no key seen
+    const float inv = none ? 0.f : 1.f / l;
+    const int64_t o = pa_out_at(p, x.b, x.sq, t, h);
+    if (p.out_dt == LA_F32) {
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[dt][i], 0.f, sum);
-      const uint64_t bad = __ballot(sum != 0.f && l < __int_as_float(0x7f800000));  // (sum: NaN)
-      // register i of dim tile dt holds dim 32 dt + 8 (i / 4) + 4 hf + i % 4
-      if (live && part >= 0) {
-        const int64_t pi = part + r_mine - r0;
-        if (hf == 0) {
-          p.ws_ml[2 * pi] = m == pa_ninf() ? m : -nmu;
-          p.ws_ml[2 * pi + 1] = l;
+        for (int i = 0; i < 4; ++i)
+          *(float4 *)((float *)p.out + o + 32 * dt + 8 * i + 4 * hf) =
+              float4{acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv, acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv};
+    } else {  // the halves of a row trade fours, so that a lane stores eight values
+      typedef elem x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          uint2 y[2];
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+            y[z] = __builtin_bit_cast(uint2, x4{(elem)(acc[dt][4 * (i + z)] * inv), (elem)(acc[dt][4 * (i + z) + 1] * inv),
+                                                (elem)(acc[dt][4 * (i + z) + 2] * inv), (elem)(acc[dt][4 * (i + z) + 3] * inv)});
+          const auto a = __builtin_amdgcn_permlane32_swap(y[0].x, y[1].x, false, false);
+          const auto c = __builtin_amdgcn_permlane32_swap(y[0].y, y[1].y, false, false);
+          *(uint4 *)((elem *)p.out + o + 32 * dt + 8 * (i + hf)) = uint4{a[0], c[0], a[1], c[1]};
         }
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *(float4 *)(p.ws_acc + pi * D + 32 * dt + 8 * i + 4 * hf) =
-                float4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
-      } else if (live) {
-        const bool none = l == 0.f;  // no key seen
-        const float inv = none ? 0.f : 1.f / l;
-        const int64_t o = pa_out_at(p, b, sq, t, h);
-        if (p.out_dt == LA_F32) {
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *(float4 *)((float *)p.out + o + 32 * dt + 8 * i + 4 * hf) =
-                  float4{acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv, acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv};
-        } else {  // the halves of a row trade fours, so that a lane stores eight values
-          typedef elem x4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-              uint2 y[2];
-#pragma unroll
-              for (int x = 0; x < 2; ++x)
-                y[x] = __builtin_bit_cast(uint2, x4{(elem)(acc[dt][4 * (i + x)] * inv), (elem)(acc[dt][4 * (i + x) + 1] * inv),
-                                                    (elem)(acc[dt][4 * (i + x) + 2] * inv), (elem)(acc[dt][4 * (i + x) + 3] * inv)});
-              const auto a = __builtin_amdgcn_permlane32_swap(y[0].x, y[1].x, false, false);
-              const auto c = __builtin_amdgcn_permlane32_swap(y[0].y, y[1].y, false, false);
-              *(uint4 *)((elem *)p.out + o + 32 * dt + 8 * (i + hf)) = uint4{a[0], c[0], a[1], c[1]};
-            }
-        }
-        if (p.lse && hf == 0) p.lse[pa_lse_at(p, b, sq, t, h)] = none ? pa_ninf() : (__log2f(l) - nmu) * PA_LN2;  // (as rounded in the weights)
-      }
-      if (bad != 0)
-        pa_again<elem, D, 32, KV8, (!KV8 && T::BIAS > 0.f)>(p, b, sq, kvh, part, r0, r_first, (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
-                                                           j0 * DA_BS, min(j1, lim_hi / DA_BS + 1) * DA_BS);
     }
-    if (!walk.next<R>(p, cost, upto)) break;
+    if (p.lse && hf == 0) p.lse[pa_lse_at(p, x.b, x.sq, t, h)] = none ? pa_ninf() : (__log2f(l) - nmu) * PA_LN2;  // (as rounded in the weights)
   }
+  if (bad != 0) {
+    const int lim_hi = p.causal ? x.sq.lk - x.sq.lq + min(r_first + 31, nrow - 1) / G : x.sq.lk - 1;
+    pa_again<elem, D, 32, KV8, false, (!KV8 && T::BIAS > 0.f)>(p, x.b, x.sq, x.kvh, x.part, x.r0, r_first,
+                                                              (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
+                                                              x.j0 * DA_BS, min(x.j1, lim_hi / DA_BS + 1) * DA_BS);
+  }
+}
+
+template <class T, int D, bool KV8, bool EVEN>
+__global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP) {
+  __shared__ __align__(16) uint16_t smem[PA_WAVE_LDS * 4 / 2];
+  __shared__ __align__(16) float s_scale[KV8 ? 768 : 4];  // few: 3 blocks' of each wave; many: a block's
+  __shared__ PaWalk s_walk;
+  __shared__ uint32_t s_bad;
+  static_assert(sizeof(uint16_t) * 3 * DA_BS * D <= sizeof(smem), "K and V");
+  {
+    const PaKP &p = pa_args();
+    pa_rest<D>(p, (int)(blockIdx.x % (uint32_t)p.Hkv));
+  }
+  if (!pa_begin<128>(&s_walk)) return;
+  do {
+    if (__builtin_amdgcn_readfirstlane(s_walk.seq.lq) * pa_args().G <= 16) pa_few<T, D, KV8, EVEN>(&s_walk, (char *)smem, s_scale, &s_bad);
+    else pa_many<T, D, KV8, EVEN>(&s_walk, smem, s_scale);
+  } while (pa_next<128>(&s_walk));
 }
 
 // fp32 rows: four waves of 16 rows on 16x16x4 products, blocks of 32 keys (dense_attn_f32_kernel's),
@@ -555,18 +845,19 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
   constexpr int NW = 4, R = 16 * NW, BS = 32, BLK = BS * D, CH = D / 4, RP = 64 / CH, NX = BS / RP / NW;
   constexpr int NS = D / 16;
   __shared__ __align__(16) float smem[4 * BLK];
+  __shared__ PaWalk s_walk;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane >> 4, ri = lane & 15;
   const int G = p.G;
-  PaWalk walk;
   pa_rest<D>(p, blockIdx.x % (uint32_t)p.Hkv);
-  if (!walk.begin<R>(p)) return;
-  const int kvh = walk.kvh;
+  if (!pa_begin<R>(&s_walk)) return;
   auto swz_k = [](int r) { return 2 * (r & 7); };
   auto swz_v = [](int r) { return 4 * ((r >> 2) & 3); };
-  while (true) {
-    const PaSeq sq = walk.seq;
-    const int b = walk.s.b, r0 = walk.s.i * R;
+  do {
+    const PaPiece x = pa_piece<R, BS>(p, &s_walk);
+    const PaSeq sq = x.sq;
+    const int b = x.b, r0 = x.r0, kvh = x.kvh, j0 = x.j0, j1 = x.j1;
+    const int64_t part = x.part;
     const int nrow = sq.lq * G, diag = sq.lk - sq.lq;
     auto limit = [&](int t) { return p.causal ? diag + t : sq.lk - 1; };
     const int r_first = r0 + 16 * w;
@@ -576,13 +867,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
     const int lim = limit(t);
     const int lim_lo = __builtin_amdgcn_readfirstlane(limit(min(r_first, nrow - 1) / G));
     const int lim_hi = __builtin_amdgcn_readfirstlane(limit(min(r_first + 15, nrow - 1) / G));
-    const int lim_tile = __builtin_amdgcn_readfirstlane(limit((min(r0 + R, nrow) - 1) / G));
-    const int n_all = lim_tile < 0 ? 0 : lim_tile / BS + 1;
-    const int64_t cost = walk.tiles.cost(walk.s.i), upto = min(cost, walk.s.off + walk.s.left);
-    const int j0 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, walk.s.off, cost));
-    const int j1 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, upto, cost));
-    const bool whole = walk.s.off == 0 && upto == cost;
-    const int64_t part = whole ? -1 : pa_part(p, walk.wg, walk.s.off == 0);
     const int32_t *pages = p.page_table + b * p.pt_sb;
     // the cache's row of key lane % 32 of a block
     uint32_t rows = 0, rows_next = 0;
@@ -596,7 +880,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
         dma16((const float *)p.v + row * D + 4 * ((lane % CH) ^ swz_v(rr)), smem + (2 + slot) * BLK + u * 256);
       }
     };
-    lds_barrier();
     if (j0 < j1) {
       rows = look(j0);
       rows_next = look(j0 + 1);
@@ -720,12 +1003,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
       }
       if (bad != 0) {
         bad |= bad >> 32;
-        pa_again<float, D, 16, false, false>(p, b, sq, kvh, part, r0, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
+        pa_again<float, D, 16, false, false, false>(p, b, sq, kvh, part, r0, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
                                             j0 * BS, min(j1, lim_hi / BS + 1) * BS);
       }
     }
-    if (!walk.next<R>(p, cost, upto)) break;
-  }
+  } while (pa_next<R>(&s_walk));
 }
 
 // Joins the parts of the tile that began last in a workgroup's stretch: a row by D / 4 lanes.
