@@ -31,13 +31,25 @@ struct PaCache {
 // A part of a row: where it is kept until the parts are joined.
 __device__ __forceinline__ int64_t pa_part(const PaKP &p, int wg, bool last) { return ((int64_t)wg * 2 + (last ? 1 : 0)) * p.part_rows; }
 
+// The blocks of a piece: number i of j0 .. j1 - 1 is block i + turn of the tile, and behind its last of
+// n_all comes its first.  A tile's blocks begin where the workgroups of its KV head are at that time, if
+// all take equally long for a block: they read the same keys at about the same time, of which
+// L2 then has what another has read (8192 tokens behind 24576: 28 % of the reads without turning
+// TURNED, 3.87 ms; with it TURNED).
+struct PaBlocks {
+  int32_t j0, j1, turn, n_all;
+  __device__ __forceinline__ int at(int i) const { return i + turn < n_all ? i + turn : i + turn - n_all; }
+};
+
 // Rows r_first + i of which bit i of `bad` is set, whose results are not finite: those with an
-// infinity or NaN of V among what their blocks (keys a .. end - 1) held and they do not see are done
-// again, key by key, in fp32 (ALL: and the others); the others stand, but in fp16 (LOST), where a weight below 2^-40 of the
-// row's largest is 0 and its product with an infinity NaN: a dim's first keys with NaN and either
-// infinity say what it is for each row.  (What a block holds past the last key is that key again.)
-template <class E, int D, int NR, bool KV8, bool ALL, bool LOST>
-__device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t part, int r_tile, int r_first, uint32_t bad, int a, int end) {
+// infinity or NaN of V among what their blocks of BS keys (up to the tile's block `top`) held and they do
+// not see are done again, key by key, in fp32 (ALL: and the others); the others stand, but in
+// fp16 (LOST), where a weight below 2^-40 of the row's largest is 0 and its product with an
+// infinity NaN: a dim's first keys with NaN and either infinity say what it is for each row.
+// (What a block holds past the last key is that key again.)
+template <class E, int D, int BS, int NR, bool KV8, bool ALL, bool LOST>
+__device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t part, int r_tile, int r_first, uint32_t bad,
+                         const PaBlocks &blocks, int top) {
   const int lane = threadIdx.x & 63, G = p.G;
   const int32_t *pages = p.page_table + b * p.pt_sb;
   const PaCache<E, KV8> K{p.k, p.k_scale, p.s_stride, D}, V{p.v, p.v_scale, p.s_stride, D};
@@ -48,27 +60,34 @@ __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t
 #pragma unroll
   for (int x = 0; x < N; ++x) at[0][x] = at[1][x] = at[2][x] = INT32_MAX;
   if constexpr (LOST) {
-    const int e = min(end, sq.lk);
-    for (int key = a; key < e; ++key) {
-      const uint32_t kr = row(key);
+    for (int i = blocks.j0; i < blocks.j1; ++i) {
+      const int j = blocks.at(i);
+      if (j > top) continue;
+      for (int key = j * BS; key < min(j * BS + BS, sq.lk); ++key) {
+        const uint32_t kr = row(key);
 #pragma unroll
-      for (int x = 0; x < N; ++x) {
-        const float v = V.at(kr, lane + 64 * x);
-        at[0][x] = min(at[0][x], v != v ? key : INT32_MAX);
-        at[1][x] = min(at[1][x], v == inf ? key : INT32_MAX);
-        at[2][x] = min(at[2][x], v == -inf ? key : INT32_MAX);
+        for (int x = 0; x < N; ++x) {
+          const float v = V.at(kr, lane + 64 * x);
+          at[0][x] = min(at[0][x], v != v ? key : INT32_MAX);
+          at[1][x] = min(at[1][x], v == inf ? key : INT32_MAX);
+          at[2][x] = min(at[2][x], v == -inf ? key : INT32_MAX);
+        }
       }
     }
   }
   wait_vmcnt<0>();  // (stores over those)
 #pragma unroll 1
-  for (int i = 0; i < NR; ++i) {
-    if (!((bad >> i) & 1u)) continue;
-    const int r = r_first + i, t = r / G, h = kvh * G + r % G;
+  for (int r = r_first; r < r_first + NR; ++r) {
+    if (!((bad >> (r - r_first)) & 1u)) continue;
+    const int t = r / G, h = kvh * G + r % G;
     const int lim = p.causal ? min(sq.lk - 1, sq.lk - sq.lq + t) : sq.lk - 1;
     bool met = ALL;
-    for (int key = max(max(lim + 1, a), 0); key < end && !ALL; ++key)
-      for (int d = lane; d < D; d += 64) met = met || !(fabsf(V.at(row(key), d)) < inf);
+    for (int i = blocks.j0; i < blocks.j1 && !ALL; ++i) {
+      const int j = blocks.at(i);
+      if (j > top || j * BS + BS - 1 <= lim) continue;
+      for (int key = max(j * BS, lim + 1); key < j * BS + BS; ++key)
+        for (int d = lane; d < D; d += 64) met = met || !(fabsf(V.at(row(key), d)) < inf);
+    }
     if (__ballot(met) == 0) {
 #pragma unroll
       for (int x = 0; x < N; ++x) {
@@ -81,15 +100,16 @@ __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t
       continue;
     }
     const E *q = (const E *)p.q + pa_q_at(p, b, sq, t, h);
-    const int e = min(end, lim + 1);
     float m = pa_ninf(), l = 0.f, acc[N];
 #pragma unroll
     for (int x = 0; x < N; ++x) acc[x] = 0.f;
-    for (int key0 = a; key0 < e; key0 += 64) {
-      const uint32_t kr = row(min(key0 + lane, e - 1));
+    for (int i = blocks.j0; i < blocks.j1; ++i) {
+      const int key0 = blocks.at(i) * BS, n = min(BS, lim + 1 - key0);  // keys of the block that it sees
+      if (n <= 0) continue;
+      const uint32_t kr = row(key0 + min(lane, n - 1));
       float s = 0.f;
       for (int d = 0; d < D; ++d) s = __builtin_fmaf((float)q[d], K.at(kr, d), s);
-      s = key0 + lane < e ? s * p.qscale : pa_ninf();
+      s = lane < n ? s * p.qscale : pa_ninf();
       float mx = s;
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
@@ -100,10 +120,9 @@ __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t
       l = l * alpha + group_sum<64>(pr);
 #pragma unroll
       for (int x = 0; x < N; ++x) acc[x] *= alpha;
-      const int n = min(64, e - key0);
-      for (int j = 0; j < n; ++j) {
-        const float w = __shfl(pr, j, 64);
-        const uint32_t vr = __shfl((int)kr, j, 64);
+      for (int y = 0; y < n; ++y) {
+        const float w = __shfl(pr, y, 64);
+        const uint32_t vr = __shfl((int)kr, y, 64);
 #pragma unroll
         for (int x = 0; x < N; ++x) acc[x] = __builtin_fmaf(w, V.at(vr, lane + 64 * x), acc[x]);
       }
@@ -131,6 +150,7 @@ struct PaWalk {
   PaStretch s;
   PaSeq seq;
   int64_t a, step;  // (of the sequence's tiles)
+  int64_t since;    // where the tile begins, from where its first workgroup's stretch does
   int32_t n;
 };
 
@@ -169,6 +189,7 @@ __device__ __forceinline__ bool pa_begin(PaWalk *walk) {
     return false;
   }
   pa_load<R>(p, w);
+  w.since = w.s.off == 0 ? 0 : w.s.quota - 1 - (w.s.off - 1) % w.s.quota;
   if (threadIdx.x == 0) *walk = w;
   __syncthreads();
   return true;
@@ -190,6 +211,7 @@ __device__ __forceinline__ bool pa_next(PaWalk *walk) {
       p.ws_join[blockIdx.x] = int4{w.s.b, w.s.i, parts, 0};
     } else {
       w.s.off = 0;
+      w.since = w.s.quota - w.s.left;  // (but of the line's last stretch)
       if (++w.s.i >= w.n) {
         w.s.i = 0;
         do {
@@ -208,10 +230,11 @@ __device__ __forceinline__ bool pa_next(PaWalk *walk) {
 // blocks of BS keys.
 struct PaPiece {
   PaSeq sq;
-  int32_t b, r0, kvh, j0, j1;
+  int32_t b, r0, kvh;
+  PaBlocks blocks;
   int64_t part;  // (-1: the whole tile)
 };
-template <int R, int BS>
+template <int R, int BS, bool TURN>
 __device__ __forceinline__ PaPiece pa_piece(const PaKP &p, const PaWalk *walk) {
   asm volatile("" ::: "memory");
   PaWalk w = *walk;
@@ -226,8 +249,11 @@ __device__ __forceinline__ PaPiece pa_piece(const PaKP &p, const PaWalk *walk) {
   const int lim = p.causal ? x.sq.lk - x.sq.lq + last : x.sq.lk - 1;
   const int n_all = lim < 0 ? 0 : lim / BS + 1;
   const int64_t cost = w.a + w.step * (w.s.i + 1), upto = min(cost, w.s.off + w.s.left);
-  x.j0 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, w.s.off, cost));
-  x.j1 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, upto, cost));
+  x.blocks.n_all = __builtin_amdgcn_readfirstlane(n_all);
+  x.blocks.j0 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, w.s.off, cost));
+  x.blocks.j1 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, upto, cost));
+  const double turns = (double)w.since / (double)cost;
+  x.blocks.turn = TURN ? __builtin_amdgcn_readfirstlane(max(0, min((int)((turns - floor(turns)) * n_all), n_all - 1))) : 0;
   x.part = pa_uniform(w.s.off == 0 && upto == cost ? -1 : pa_part(p, blockIdx.x, w.s.off == 0));
   return x;
 }
@@ -339,7 +365,7 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
   float m = pa_ninf(), thr = pa_ninf(), l = 0.f, nmu = 0.f;
   {
     const PaKP &p = pa_args();
-    const PaPiece x = pa_piece<128, DA_BS>(p, walk);
+    const PaPiece x = pa_piece<128, DA_BS, false>(p, walk);
     const int nrow = x.sq.lq * p.G, row = min(ri, nrow - 1), t = row / p.G;
     const int lim = p.causal ? x.sq.lk - x.sq.lq + t : x.sq.lk - 1;  // last key seen
     const float qscale = p.qscale, thr_gap = p.thr_gap;
@@ -350,10 +376,10 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
     rows.pages = p.page_table + x.b * p.pt_sb;
     rows.key0 = 16 * w;
     rows.last = x.sq.lk - 1;
-    const int n = x.j1 - x.j0;
+    const int n = x.blocks.j1 - x.blocks.j0;
     // piece u of K or V rows: K of block j0 + u / 2, then V
     auto load = [&](int u) {
-      const int j = x.j0 + (u >> 1);
+      const int j = x.blocks.j0 + (u >> 1);
       if ((u & 1) == 0 && j - rows.jb == PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j);
       const uint32_t to = lds0 + (uint32_t)(u % NU) * UNIT;
       if (u & 1) {
@@ -374,7 +400,7 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (n > 0) {
-      rows.look(p, x.kvh, x.j0);
+      rows.look(p, x.kvh, x.blocks.j0);
 #pragma unroll
       for (int u = 0; u < NU; ++u)
         if (u < 2 * n) load(u);
@@ -382,7 +408,7 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
 #pragma unroll
     for (int s = 0; s < NK; ++s) settle(qf[s]);
     for (int i = 0; i < n; ++i) {
-      const int j = x.j0 + i;
+      const int j = x.blocks.j0 + i;
       // newer pieces on their way: V of this block, and K (fp8: and V) of the next
       if (i + 1 < n) wait_vmcnt<(NU - 1) * NX + (KV8 ? 1 : 0)>();
       else wait_vmcnt<NX>();
@@ -481,7 +507,7 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
   if (threadIdx.x == 0) *s_bad = 0u;
   lds_barrier();
   const PaKP &p = pa_args();
-  const PaPiece x = pa_piece<128, DA_BS>(p, walk);
+  const PaPiece x = pa_piece<128, DA_BS, false>(p, walk);
   const int nrow = x.sq.lq * p.G;
   for (int e = threadIdx.x; e < nrow * D; e += 64 * NW) {
     const int g = e / D, dim = e % D;
@@ -519,7 +545,7 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
     wait_vmcnt<0>();
     __syncthreads();
     for (int g = w; g < nrow; g += NW)
-      pa_again<elem, D, 16, KV8, true, false>(p, x.b, x.sq, x.kvh, x.part, 0, 0, bad & (1u << g), x.j0 * DA_BS, x.j1 * DA_BS);
+      pa_again<elem, D, DA_BS, 16, KV8, true, false>(p, x.b, x.sq, x.kvh, x.part, 0, 0, bad & (1u << g), x.blocks, x.blocks.n_all);
   }
 }
 
@@ -555,14 +581,15 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
   f32x16 acc[ND];
   {
     const PaKP &p = pa_args();
-    const PaPiece x = pa_piece<R, DA_BS>(p, walk);
+    const PaPiece x = pa_piece<R, DA_BS, true>(p, walk);
     const int G = p.G, nrow = x.sq.lq * G, diag = x.sq.lk - x.sq.lq, causal = p.causal;
     auto limit = [&](int t) { return causal ? diag + t : x.sq.lk - 1; };  // last key seen
     const int r_first = x.r0 + 32 * w, r_mine = min(r_first + r32, nrow - 1);
     const int t = r_mine / G, lim = limit(t);
     const int lim_lo = __builtin_amdgcn_readfirstlane(limit(min(r_first, nrow - 1) / G));
     const int lim_hi = __builtin_amdgcn_readfirstlane(limit(min(r_first + 31, nrow - 1) / G));
-    const int j0 = x.j0, j1 = x.j1;
+    const PaBlocks blocks = x.blocks;
+    const int j0 = blocks.j0, j1 = blocks.j1;
     const float qscale = p.qscale, thr_gap = p.thr_gap;
     const void *kp = p.k, *vp = p.v;
     const float *k_scale = p.k_scale, *v_scale = p.v_scale;
@@ -572,8 +599,10 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
     rows.key0 = 16 * w;
     rows.last = x.sq.lk - 1;
     const int sw = 16 * w;
-    auto dma_k = [&](int j) __attribute__((always_inline)) {
-      rows.template load<2 * D, 8>(kp, j, lds0 + 2 * (((j - j0) & 1) * BLK + sw * D), lane, [&](int r) { return da_swz_k<D>(sw + r); });
+    // (i: number in the piece; j: the tile's block)
+    auto dma_k = [&](int i, int j) __attribute__((always_inline)) {
+      if ((uint32_t)(j - rows.jb) >= (uint32_t)PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j);
+      rows.template load<2 * D, 8>(kp, j, lds0 + 2 * ((i & 1) * BLK + sw * D), lane, [&](int r) { return da_swz_k<D>(sw + r); });
     };
     auto dma_v = [&](int j) __attribute__((always_inline)) {
       rows.template load<2 * D, 4>(vp, j, lds0 + 2 * (VSLOT * BLK + sw * D), lane, [&](int r) { return da_swz_v<D>(sw + r); });
@@ -581,6 +610,7 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
     // fp8: codes of a block, a wave's own rows, and (lanes below 16) the keys' scales
     float ks = 0.f, vs = 0.f;
     auto dma_codes = [&](int j) __attribute__((always_inline)) {
+      if ((uint32_t)(j - rows.jb) >= (uint32_t)PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j);
       rows.template load<D, 1>(kp, j, lds0 + 4 * BLK + sw * D, lane, [](int) { return 0; });
       rows.template load<D, 1>(vp, j, lds0 + 5 * BLK + sw * D, lane, [](int) { return 0; });
       const uint64_t at = (uint64_t)rows.of(j, lane & 15) * s_stride;
@@ -607,13 +637,14 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
         s_scale[DA_BS + sw + lane] = vs;
       }
     };
+    int j = blocks.at(j0);
     if (j0 < j1) {
-      rows.look(p, x.kvh, j0);
+      rows.look(p, x.kvh, j);
       if constexpr (KV8) {
-        dma_codes(j0);
+        dma_codes(j);
       } else {
-        dma_k(j0);
-        dma_v(j0);
+        dma_k(j0, j);
+        dma_v(j);
       }
     }
     x8 qf[NS];  // B operand: dims 16 s + 8 hf ..
@@ -630,8 +661,8 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
       for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
     // scores of block j; register i of a half holds key 8 (i / 4) + 4 hf + i % 4
-    auto scores = [&](int j, f32x16 (&st)[2]) __attribute__((always_inline)) {
-      const uint32_t at = k_at + (KV8 ? 0 : 2 * ((j - j0) & 1) * BLK);
+    auto scores = [&](int i_, f32x16 (&st)[2]) __attribute__((always_inline)) {
+      const uint32_t at = k_at + (KV8 ? 0 : 2 * (i_ & 1) * BLK);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -715,49 +746,45 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
         }
     };
 
-    const int jw = r_first < nrow && lim_hi >= 0 ? min(lim_hi / DA_BS, j1 - 1) : -1;  // this wave's last block
-    for (int j = j0; j < j1; ++j) {
+    const int jw = r_first < nrow && lim_hi >= 0 ? lim_hi / DA_BS : -1;  // this wave's last block
+    for (int i = j0; i < j1; ++i) {
+      const int next = j + 1 < blocks.n_all ? j + 1 : 0;
       wait_vmcnt<0>();
       f32x16 st[2];
       px8 pw[2];
       if constexpr (KV8) {
-        lds_barrier();  // block j - 1 is read
+        lds_barrier();  // the block before is read
         widen();
-        lds_barrier();  // block j is there, and its codes are read
-        if (j + 1 < j1) {
-          if (j + 1 - rows.jb == PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j + 1);
-          dma_codes(j + 1);
-        }
+        lds_barrier();  // this one is there, and its codes are read
+        if (i + 1 < j1) dma_codes(next);
         if (j <= jw) {
-          scores(j, st);
+          scores(i, st);
           settle_max(j, st, largest(st));
           weigh(0, st[0], pw);
         }
       } else {
-        lds_barrier();  // K of block j has landed for every wave, block j - 1 is read
-        if (j > j0) dma_v(j);
-        if (j + 1 < j1) {
-          if (j + 1 - rows.jb == PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j + 1);
-          dma_k(j + 1);
-        }
+        lds_barrier();  // K of this block has landed for every wave, the one before is read
+        if (i > j0) dma_v(j);
+        if (i + 1 < j1) dma_k(i + 1, next);
         if (j <= jw) {
-          scores(j, st);
+          scores(i, st);
           settle_max(j, st, largest(st));
           weigh(0, st[0], pw);
         }
-        if (j + 1 < j1) wait_vmcnt<NX>();
+        if (i + 1 < j1) wait_vmcnt<NX>();
         else wait_vmcnt<0>();
-        lds_barrier();  // V of block j has landed
+        lds_barrier();  // V of this block has landed
       }
       if (j <= jw) {
         values(0, pw);
         weigh(1, st[1], pw);
         values(1, pw);
       }
+      j = next;
     }
   }
   const PaKP &p = pa_args();
-  const PaPiece x = pa_piece<R, DA_BS>(p, walk);
+  const PaPiece x = pa_piece<R, DA_BS, true>(p, walk);
   const int G = p.G, nrow = x.sq.lq * G, r_first = x.r0 + 32 * w, r_mine = min(r_first + r32, nrow - 1);
   if (r_first >= nrow) return;
   const bool live = r_first + r32 < nrow;
@@ -814,9 +841,9 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
   }
   if (bad != 0) {
     const int lim_hi = p.causal ? x.sq.lk - x.sq.lq + min(r_first + 31, nrow - 1) / G : x.sq.lk - 1;
-    pa_again<elem, D, 32, KV8, false, (!KV8 && T::BIAS > 0.f)>(p, x.b, x.sq, x.kvh, x.part, x.r0, r_first,
-                                                              (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
-                                                              x.j0 * DA_BS, min(x.j1, lim_hi / DA_BS + 1) * DA_BS);
+    pa_again<elem, D, DA_BS, 32, KV8, false, (!KV8 && T::BIAS > 0.f)>(p, x.b, x.sq, x.kvh, x.part, x.r0, r_first,
+                                                                     (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
+                                                                     x.blocks, lim_hi / DA_BS);
   }
 }
 
@@ -854,9 +881,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
   auto swz_k = [](int r) { return 2 * (r & 7); };
   auto swz_v = [](int r) { return 4 * ((r >> 2) & 3); };
   do {
-    const PaPiece x = pa_piece<R, BS>(p, &s_walk);
+    const PaPiece x = pa_piece<R, BS, true>(p, &s_walk);
     const PaSeq sq = x.sq;
-    const int b = x.b, r0 = x.r0, kvh = x.kvh, j0 = x.j0, j1 = x.j1;
+    const PaBlocks blocks = x.blocks;
+    const int b = x.b, r0 = x.r0, kvh = x.kvh, j0 = blocks.j0, j1 = blocks.j1;
     const int64_t part = x.part;
     const int nrow = sq.lq * G, diag = sq.lk - sq.lq;
     auto limit = [&](int t) { return p.causal ? diag + t : sq.lk - 1; };
@@ -881,8 +909,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
       }
     };
     if (j0 < j1) {
-      rows = look(j0);
-      rows_next = look(j0 + 1);
+      rows = look(blocks.at(j0));
+      rows_next = look(blocks.at(min(j0 + 1, j1 - 1)));
       settle(rows);
       settle(rows_next);
       dma(rows, 0);
@@ -901,14 +929,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
     f32x4 acc[NS], total[NS];
 #pragma unroll
     for (int dt = 0; dt < NS; ++dt) acc[dt] = total[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int j = j0; j < j1; ++j) {
-      const int par = (j - j0) & 1;
+    for (int i = j0; i < j1; ++i) {
+      const int par = (i - j0) & 1, j = blocks.at(i);
       wait_vmcnt<0>();
       settle(rows_next);
       lds_barrier();
-      if (j + 1 < j1) {
+      if (i + 1 < j1) {
         dma(rows_next, par ^ 1);
-        rows_next = look(j + 2);
+        rows_next = look(blocks.at(min(i + 2, j1 - 1)));
       }
       if (!wave_live || j * BS > lim_hi) continue;
       const float *sk = smem + par * BLK, *sv = smem + (2 + par) * BLK;
@@ -964,7 +992,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
                 sv[kr * D + 4 * ((4 * dt + (ri >> 2)) ^ swz_v(kr)) + (ri & 3)], pr, acc[dt], 0, 0, 0);
         }
       l += sum;
-      if ((j - j0) % 16 == 15) {
+      if ((i - j0) % 16 == 15) {
 #pragma unroll
         for (int dt = 0; dt < NS; ++dt) {
           total[dt] += acc[dt];
@@ -1003,8 +1031,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
       }
       if (bad != 0) {
         bad |= bad >> 32;
-        pa_again<float, D, 16, false, false, false>(p, b, sq, kvh, part, r0, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
-                                            j0 * BS, min(j1, lim_hi / BS + 1) * BS);
+        pa_again<float, D, BS, 16, false, false, false>(p, b, sq, kvh, part, r0, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
+                                                       blocks, lim_hi / BS);
       }
     }
   } while (pa_next<R>(&s_walk));
