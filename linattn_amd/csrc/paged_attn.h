@@ -7,10 +7,14 @@
 // The lengths are known on the device only, and a batch holds single tokens beside long chunks, so
 // the work is shared out there: all tiles of a KV head in a line, sequence after sequence, each
 // as long as its keys (and a little, for its beginning and end); of that line every workgroup
-// takes an equal stretch, from its place on, across the ends of tiles.  A tile that
-// lies in one stretch is finished by its workgroup; of one that does not, each workgroup
-// leaves its part (unnormalised sums, reference and weight sum of each row) and the join, a
-// second launch, adds them up.
+// takes a stretch, across the ends of tiles.  A tile that lies in one stretch is finished by
+// its workgroup; of one that does not, each workgroup leaves its part (unnormalised sums,
+// reference and weight sum of each row) and the join, a second launch, adds them up.
+// Sequences of few rows (at most 16: single tokens, bound by the reads) have a line of their own.
+// There are as many stretches as there are places for workgroups: with three times as many, the
+// last of which would fill the places of workgroups that are done early, beginnings and ends
+// cost more than that gains (tokens of 48 sequences 333 us in place of 312, tokens and chunks
+// together 293 in place of 254).
 #pragma once
 
 #include "few_rows.h"
@@ -23,10 +27,11 @@ struct PaKP {
   float *lse;
   const float *k_scale, *v_scale;
   const int32_t *page_table, *lengths, *cu_q, *q_len;
-  float *ws_ml, *ws_acc;  // parts: [workgroup][first, last][row] (reference, sum) and D values
-  int4 *ws_join;          // [workgroup]: sequence, tile, parts (0: none), of the tile that begins last there
+  float *ws_ml, *ws_acc;  // parts (pa_part): (reference, sum) and D values of each row
+  int4 *ws_join;          // [workgroup]: of the tile that begins last there: sequence, tile, parts (0: none), and
+                          // 1 + the stretch's number where rows are few, else 0
   int64_t Tq, q_sb, q_sh, q_st, o_sb, o_sh, o_st, l_sb, l_sh, pt_sb, s_stride, n_phys;
-  int64_t least;  // of a stretch
+  int64_t least, few_parts;  // of a stretch; where the parts of few rows begin
   int32_t B, G, Hq, Hkv, D, W, part_rows;  // W: workgroups of a KV head
   int32_t page, pt_pages, causal, out_dt, zero_rest;
   float qscale, thr_gap;
@@ -60,10 +65,13 @@ struct PaTiles {
   __device__ __forceinline__ int64_t upto(int64_t i) const { return i * a + step * (i * (i + 1) / 2); }
   __device__ __forceinline__ int64_t cost(int64_t i) const { return a + step * (i + 1); }
 };
-template <int R>
-__device__ __forceinline__ PaTiles pa_tiles(const PaKP &p, const PaSeq &s) {
+constexpr int PA_FEW = 16;  // rows of a sequence that are few
+// (n 0: no tiles in that line; FEW: whether there are two)
+template <int R, bool FEW>
+__device__ __forceinline__ PaTiles pa_tiles(const PaKP &p, const PaSeq &s, bool few) {
   PaTiles t;
-  t.n = (int32_t)(((int64_t)s.lq * p.G + R - 1) / R);
+  const int64_t rows = (int64_t)s.lq * p.G;
+  t.n = FEW && (rows <= PA_FEW) != few ? 0 : (int32_t)((rows + R - 1) / R);
   t.a = (int64_t)p.G * ((p.causal ? max(s.lk - s.lq, 0) : s.lk) + PA_AHEAD);
   t.step = p.causal ? R : 0;
   return t;
@@ -75,37 +83,57 @@ __device__ __forceinline__ int64_t pa_uniform(int64_t x) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
-// Where stretch w of a KV head's line begins: sequence b, tile i, `off` into the tile; `left` is
-// the stretch's length (0: none) and `quota` that of every full one.
-struct PaStretch {
-  int32_t b, i;
-  int64_t off, left, quota;
+// A line: its length, that of a stretch (but of the last), its first workgroup.
+struct PaLine {
+  int64_t all, quota;
+  int32_t first;
 };
-template <int R>
+
+// The stretch of workgroup w of a KV head: sequence b, tile i, `off` into the tile, which begins at
+// `pos` of the line; `left` is the stretch's length (0: none).
+struct PaStretch {
+  PaLine line;
+  int64_t off, left, pos;
+  int32_t b, i, few;
+};
+template <int R, bool FEW>
 __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w) {
   const int lane = threadIdx.x & 63;
-  auto cost = [&](int b) -> int64_t {
+  auto cost = [&](int b, bool few) -> int64_t {
     if (b >= p.B) return 0;
-    const PaTiles t = pa_tiles<R>(p, pa_seq(p, b));
+    const PaTiles t = pa_tiles<R, FEW>(p, pa_seq(p, b), few);
     return t.upto(t.n);
   };
-  const int64_t mine = cost(lane);
-  int64_t all = mine;
-  for (int b = 64 + lane; b < p.B; b += 64) all += cost(b);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) all += __shfl_xor((long long)all, o, 64);
-  PaStretch s;
-  all = pa_uniform(all);
-  s.quota = max((all + p.W - 1) / p.W, p.least);
-  s.off = s.quota * w;
-  s.left = min(s.quota, all - s.off);
-  s.b = s.i = 0;
-  if (s.left <= 0) {
-    s.left = 0;
-    return s;
+  const int64_t mine_many = cost(lane, false), mine_few = FEW ? cost(lane, true) : 0;
+  int64_t many = mine_many, few = mine_few;
+  for (int b = 64 + lane; b < p.B; b += 64) {
+    many += cost(b, false);
+    if (FEW) few += cost(b, true);
   }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    many += __shfl_xor((long long)many, o, 64);
+    if (FEW) few += __shfl_xor((long long)few, o, 64);
+  }
+  many = pa_uniform(many);
+  few = pa_uniform(few);
+  PaStretch s;
+  s.left = 0;
+  s.b = s.i = 0;
+  // places for tiles of many rows, by the share of the time (beside them, a block of few rows takes a
+  // little less than one of many: chunks and tokens together 261, 253 and 255 us at 0.5, 0.7 and 1)
+  const int wm = few == 0 ? p.W : many == 0 ? 0 : max(1, min(p.W - 1, (int)((double)p.W * (double)many / ((double)many + 0.8 * (double)few) + 0.5)));
+  s.few = w >= wm && few > 0;
+  s.line.all = s.few ? few : many;
+  s.line.first = s.few ? wm : 0;
+  const int places = s.few ? p.W - wm : max(wm, 1);
+  s.line.quota = max((s.line.all + places - 1) / places, p.least);
+  s.off = (w - s.line.first) * s.line.quota;
+  if (s.off >= s.line.all) return s;
+  s.left = min(s.line.quota, s.line.all - s.off);
+  s.pos = s.off;
   for (int b0 = 0;; b0 += 64) {
-    const int64_t c = b0 == 0 ? mine : cost(b0 + lane);
+    const int64_t c = b0 == 0 ? (s.few ? mine_few : mine_many) : cost(b0 + lane, s.few);
     int64_t sum = c;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -122,7 +150,7 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w) {
     s.off -= pa_uniform(pa_shfl(sum - c, at));
     break;
   }
-  const PaTiles t = pa_tiles<R>(p, pa_seq(p, s.b));
+  const PaTiles t = pa_tiles<R, FEW>(p, pa_seq(p, s.b), s.few);
   // upto(i) <= off < upto(i + 1): the quadratic's root, and what its rounding may have missed
   int64_t i;
   if (t.step == 0) {
@@ -137,7 +165,14 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w) {
   s.i = __builtin_amdgcn_readfirstlane((int32_t)i);
   s.off = pa_uniform(s.off - t.upto(i));
   s.left = pa_uniform(s.left);
+  s.pos -= s.off;
   return s;
+}
+
+// A part of a row of stretch x of a KV head: where it is kept until the parts are joined.
+__device__ __forceinline__ int64_t pa_part(const PaKP &p, int64_t x, int kvh, bool last, bool few) {
+  const int64_t at = (x * p.Hkv + kvh) * 2 + (last ? 1 : 0);
+  return few ? p.few_parts + at * PA_FEW : at * p.part_rows;
 }
 
 // Of a tile of `n` staged blocks of keys and cost C, those before place c.

@@ -28,9 +28,6 @@ struct PaCache {
   }
 };
 
-// A part of a row: where it is kept until the parts are joined.
-__device__ __forceinline__ int64_t pa_part(const PaKP &p, int wg, bool last) { return ((int64_t)wg * 2 + (last ? 1 : 0)) * p.part_rows; }
-
 // The blocks of a piece: number i of j0 .. j1 - 1 is block i + turn of the tile, and behind its last of
 // n_all comes its first.  A tile's blocks begin where the workgroups of its KV head are at that time, if
 // all take equally long for a block: they read the same keys at about the same time, of which
@@ -169,27 +166,27 @@ __device__ __forceinline__ const PaKP &pa_args() {
   return *(const PaKP *)x;
 }
 
-template <int R>
+template <int R, bool FEW>
 __device__ __forceinline__ void pa_load(const PaKP &p, PaWalk &w) {
   w.seq = pa_seq(p, w.s.b);
-  const PaTiles t = pa_tiles<R>(p, w.seq);
+  const PaTiles t = pa_tiles<R, FEW>(p, w.seq, w.s.few);
   w.a = t.a;
   w.step = t.step;
   w.n = t.n;
 }
 
 // The stretch's beginning, by every wave; false: there is none.
-template <int R>
+template <int R, bool FEW>
 __device__ __forceinline__ bool pa_begin(PaWalk *walk) {
   const PaKP &p = pa_args();
   PaWalk w;
-  w.s = pa_stretch<R>(p, blockIdx.x / (uint32_t)p.Hkv);
+  w.s = pa_stretch<R, FEW>(p, blockIdx.x / (uint32_t)p.Hkv);
   if (w.s.left == 0) {
     if (threadIdx.x == 0) p.ws_join[blockIdx.x] = int4{0, 0, 0, 0};
     return false;
   }
-  pa_load<R>(p, w);
-  w.since = w.s.off == 0 ? 0 : w.s.quota - 1 - (w.s.off - 1) % w.s.quota;
+  pa_load<R, FEW>(p, w);
+  w.since = w.s.pos % w.s.line.quota;
   if (threadIdx.x == 0) *walk = w;
   __syncthreads();
   return true;
@@ -197,7 +194,7 @@ __device__ __forceinline__ bool pa_begin(PaWalk *walk) {
 
 // The next tile of the stretch, or the join's note of the tile that is left open (false: the stretch
 // is done).  By every wave.
-template <int R>
+template <int R, bool FEW>
 __device__ __forceinline__ bool pa_next(PaWalk *walk) {
   const PaKP &p = pa_args();
   PaWalk w = *walk;
@@ -206,17 +203,19 @@ __device__ __forceinline__ bool pa_next(PaWalk *walk) {
   w.s.left -= upto - w.s.off;
   const bool more = __builtin_amdgcn_readfirstlane(w.s.left > 0);
   if (threadIdx.x == 0) {
+    const int64_t own = blockIdx.x / (uint32_t)p.Hkv - w.s.line.first;
     if (!more) {
-      const int parts = w.s.off == 0 && upto < cost ? 1 + (int)((cost - upto + w.s.quota - 1) / w.s.quota) : 0;
-      p.ws_join[blockIdx.x] = int4{w.s.b, w.s.i, parts, 0};
+      const int parts = w.s.off == 0 && upto < cost ? (int)((w.s.pos + cost - 1) / w.s.line.quota - own) + 1 : 0;
+      p.ws_join[blockIdx.x] = int4{w.s.b, w.s.i, parts, w.s.few ? 1 + (int)own : 0};
     } else {
       w.s.off = 0;
-      w.since = w.s.quota - w.s.left;  // (but of the line's last stretch)
+      w.s.pos += cost;
+      w.since = w.s.pos - own * w.s.line.quota;
       if (++w.s.i >= w.n) {
         w.s.i = 0;
         do {
           ++w.s.b;
-          pa_load<R>(p, w);
+          pa_load<R, FEW>(p, w);
         } while (w.n == 0 && w.s.b + 1 < p.B);
       }
       *walk = w;
@@ -254,7 +253,7 @@ __device__ __forceinline__ PaPiece pa_piece(const PaKP &p, const PaWalk *walk) {
   x.blocks.j1 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, upto, cost));
   const double turns = (double)w.since / (double)cost;
   x.blocks.turn = TURN ? __builtin_amdgcn_readfirstlane(max(0, min((int)((turns - floor(turns)) * n_all), n_all - 1))) : 0;
-  x.part = pa_uniform(w.s.off == 0 && upto == cost ? -1 : pa_part(p, blockIdx.x, w.s.off == 0));
+  x.part = pa_uniform(w.s.off == 0 && upto == cost ? -1 : pa_part(p, blockIdx.x / (uint32_t)p.Hkv - w.s.line.first, x.kvh, w.s.off == 0, w.s.few));
   return x;
 }
 
@@ -336,6 +335,16 @@ __device__ __forceinline__ f32x4 pa_mfma16(s16x4 a, s16x4 b, f32x4 c) {
   else return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
 }
 
+// Of a CU's three workgroups each is preferred for a block in turn: else the one that came first is, and
+// they end one after the other (8192 tokens behind 24576, equal stretches: after 2.87, 3.23 and
+// 3.81 ms; in turn 3.50, 3.59, 3.65).
+__device__ __forceinline__ void pa_prefer(int turn) {
+  turn %= 3;
+  if (turn == 0) __builtin_amdgcn_s_setprio(0);
+  else if (turn == 1) __builtin_amdgcn_s_setprio(1);
+  else __builtin_amdgcn_s_setprio(2);
+}
+
 constexpr int PA_WAVE_LDS = 12288;  // of a wave, where the waves of a workgroup go their own ways
 
 // At most 16 rows of a sequence and KV head (single tokens): the waves take a quarter of each block's
@@ -407,8 +416,10 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
     }
 #pragma unroll
     for (int s = 0; s < NK; ++s) settle(qf[s]);
+    const int third = (int)(blockIdx.x / (uint32_t)(p.W * p.Hkv / 3 + 1));
     for (int i = 0; i < n; ++i) {
       const int j = x.blocks.j0 + i;
+      pa_prefer(i + third);
       // newer pieces on their way: V of this block, and K (fp8: and V) of the next
       if (i + 1 < n) wait_vmcnt<(NU - 1) * NX + (KV8 ? 1 : 0)>();
       else wait_vmcnt<NX>();
@@ -554,8 +565,8 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
 // product with V from the same registers, rounded to the inputs' type (bf16 with an fp8 cache);
 // l is of the fp32 weights).
 //
-// A wave stages 16 keys of each block of 64 (PaRows).  K is staged a block ahead into the other of
-// two slots, V while its block is scored.  fp8 caches (KV8): codes of K and V go into LDS a block
+// A wave stages 16 keys of each block of 64 (PaRows).  K and V of the blocks take three slots in turn,
+// so that each is on its way while the block before is scored and weighed.  fp8 caches (KV8): codes of K and V go into LDS a block
 // ahead, and are widened there once a workgroup (e4m3 is exact in bf16 and fp16); the scale of
 // a key multiplies its scores, that of its value its weights, both in fp32.
 template <class T, int D, bool KV8, bool EVEN>
@@ -563,7 +574,7 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
   typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V
   constexpr int NW = 4, R = 32 * NW, BLK = DA_BS * D, NX = D / 32;
   constexpr int NS = D / 16, ND = D / 32;
-  constexpr int VSLOT = KV8 ? 1 : 2;  // K slots 0, 1, then V; KV8: K, V, then codes of K and of V
+  constexpr int SLOT = 2 * BLK;  // bytes; KV8: K, V, then codes of K and of V
   typedef typename T::x8 x8;
   typedef typename TP::x8 px8;
   typedef typename T::elem elem;
@@ -574,7 +585,7 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
   // Byte offsets of this lane's first reads of a slot (as in dense_attn_kernel).
   const uint32_t k_at = 2 * (r32 * D + 8 * (hf ^ da_swz_k<D>(r32)));
   const int v_row = 4 * hf + ((lane & 15) >> 2);
-  const uint32_t v_at = 2 * (VSLOT * BLK + v_row * D + 8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ da_swz_v<D>(v_row)) +
+  const uint32_t v_at = 2 * (v_row * D + 8 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ da_swz_v<D>(v_row)) +
                              4 * (lane & 1));
   const char *lds = (const char *)smem;
   float m = pa_ninf(), thr = pa_ninf(), l = 0.f, nmu = 0.f;
@@ -599,13 +610,12 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
     rows.key0 = 16 * w;
     rows.last = x.sq.lk - 1;
     const int sw = 16 * w;
-    // (i: number in the piece; j: the tile's block)
-    auto dma_k = [&](int i, int j) __attribute__((always_inline)) {
+    auto dma_k = [&](int j, int slot) __attribute__((always_inline)) {
       if ((uint32_t)(j - rows.jb) >= (uint32_t)PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j);
-      rows.template load<2 * D, 8>(kp, j, lds0 + 2 * ((i & 1) * BLK + sw * D), lane, [&](int r) { return da_swz_k<D>(sw + r); });
+      rows.template load<2 * D, 8>(kp, j, lds0 + (uint32_t)(slot * SLOT + 2 * sw * D), lane, [&](int r) { return da_swz_k<D>(sw + r); });
     };
-    auto dma_v = [&](int j) __attribute__((always_inline)) {
-      rows.template load<2 * D, 4>(vp, j, lds0 + 2 * (VSLOT * BLK + sw * D), lane, [&](int r) { return da_swz_v<D>(sw + r); });
+    auto dma_v = [&](int j, int slot) __attribute__((always_inline)) {
+      rows.template load<2 * D, 4>(vp, j, lds0 + (uint32_t)(slot * SLOT + 2 * sw * D), lane, [&](int r) { return da_swz_v<D>(sw + r); });
     };
     // fp8: codes of a block, a wave's own rows, and (lanes below 16) the keys' scales
     float ks = 0.f, vs = 0.f;
@@ -643,8 +653,8 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
       if constexpr (KV8) {
         dma_codes(j);
       } else {
-        dma_k(j0, j);
-        dma_v(j);
+        dma_k(j, 0);
+        dma_v(j, 1);
       }
     }
     x8 qf[NS];  // B operand: dims 16 s + 8 hf ..
@@ -661,8 +671,8 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
       for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
     // scores of block j; register i of a half holds key 8 (i / 4) + 4 hf + i % 4
-    auto scores = [&](int i_, f32x16 (&st)[2]) __attribute__((always_inline)) {
-      const uint32_t at = k_at + (KV8 ? 0 : 2 * (i_ & 1) * BLK);
+    auto scores = [&](int slot, f32x16 (&st)[2]) __attribute__((always_inline)) {
+      const uint32_t at = k_at + slot * SLOT;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -734,12 +744,13 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
         }
       }
     };
-    auto values = [&](int kt, const px8 (&pw)[2]) __attribute__((always_inline)) {
+    auto values = [&](int slot, int kt, const px8 (&pw)[2]) __attribute__((always_inline)) {
+      const uint32_t at = v_at + slot * SLOT;
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) {
-          const char *v = lds + (v_at ^ (64 * dt)) + 2 * (32 * kt + 16 * y) * D;
+          const char *v = lds + (at ^ (64 * dt)) + 2 * (32 * kt + 16 * y) * D;
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v);
           const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 16 * D));
           acc[dt] = TP::mfma(__builtin_bit_cast(px8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pw[y], acc[dt]);
@@ -747,46 +758,43 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
     };
 
     const int jw = r_first < nrow && lim_hi >= 0 ? lim_hi / DA_BS : -1;  // this wave's last block
-    const int third = (int)(blockIdx.x / (gridDim.x / 3 + 1));
+    const int third = (int)(blockIdx.x / (uint32_t)(p.W * p.Hkv / 3 + 1));
+    int sk = 0, sv = 1;  // this block's slots
     for (int i = j0; i < j1; ++i) {
-      const int next = j + 1 < blocks.n_all ? j + 1 : 0;
-      // of a CU's three workgroups each is preferred for a block in turn: else the one that came first
-      // is, and they end one after the other (8192 tokens behind 24576, equal stretches: after 2.87,
-      // 3.23 and 3.81 ms; in turn 3.50, 3.59, 3.65)
-      const int turn = (i + third) % 3;
-      if (turn == 0) __builtin_amdgcn_s_setprio(0);
-      else if (turn == 1) __builtin_amdgcn_s_setprio(1);
-      else __builtin_amdgcn_s_setprio(2);
-      wait_vmcnt<0>();
+      const int next = j + 1 < blocks.n_all ? j + 1 : 0, free = 3 - sk - sv;
+      pa_prefer(i + third);
       f32x16 st[2];
       px8 pw[2];
       if constexpr (KV8) {
+        wait_vmcnt<0>();
         lds_barrier();  // the block before is read
         widen();
         lds_barrier();  // this one is there, and its codes are read
         if (i + 1 < j1) dma_codes(next);
-        if (j <= jw) {
-          scores(i, st);
-          settle_max(j, st, largest(st));
-          weigh(0, st[0], pw);
-        }
       } else {
-        lds_barrier();  // K of this block has landed for every wave, the one before is read
-        if (i > j0) dma_v(j);
-        if (i + 1 < j1) dma_k(i + 1, next);
-        if (j <= jw) {
-          scores(i, st);
-          settle_max(j, st, largest(st));
-          weigh(0, st[0], pw);
-        }
-        if (i + 1 < j1) wait_vmcnt<NX>();
-        else wait_vmcnt<0>();
-        lds_barrier();  // V of this block has landed
+        wait_vmcnt<NX>();
+        lds_barrier();  // K of this block has landed for every wave, V of the one before is read
+        if (i + 1 < j1) dma_k(next, free);
       }
       if (j <= jw) {
-        values(0, pw);
+        scores(sk, st);
+        settle_max(j, st, largest(st));
+        weigh(0, st[0], pw);
+      }
+      if constexpr (!KV8) {
+        if (i + 1 < j1) wait_vmcnt<NX>();
+        else wait_vmcnt<0>();
+        lds_barrier();  // V of this block has landed, its K is read
+        if (i + 1 < j1) dma_v(next, sk);
+      }
+      if (j <= jw) {
+        values(sv, 0, pw);
         weigh(1, st[1], pw);
-        values(1, pw);
+        values(sv, 1, pw);
+      }
+      if constexpr (!KV8) {
+        sv = sk;
+        sk = free;
       }
       j = next;
     }
@@ -866,11 +874,11 @@ __global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP) {
     const PaKP &p = pa_args();
     pa_rest<D>(p, (int)(blockIdx.x % (uint32_t)p.Hkv));
   }
-  if (!pa_begin<128>(&s_walk)) return;
+  if (!pa_begin<128, true>(&s_walk)) return;
   do {
-    if (__builtin_amdgcn_readfirstlane(s_walk.seq.lq) * pa_args().G <= 16) pa_few<T, D, KV8, EVEN>(&s_walk, (char *)smem, s_scale, &s_bad);
+    if (__builtin_amdgcn_readfirstlane(s_walk.s.few)) pa_few<T, D, KV8, EVEN>(&s_walk, (char *)smem, s_scale, &s_bad);
     else pa_many<T, D, KV8, EVEN>(&s_walk, smem, s_scale);
-  } while (pa_next<128>(&s_walk));
+  } while (pa_next<128, true>(&s_walk));
 }
 
 // fp32 rows: four waves of 16 rows on 16x16x4 products, blocks of 32 keys (dense_attn_f32_kernel's),
@@ -885,7 +893,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
   const int c = lane >> 4, ri = lane & 15;
   const int G = p.G;
   pa_rest<D>(p, blockIdx.x % (uint32_t)p.Hkv);
-  if (!pa_begin<R>(&s_walk)) return;
+  if (!pa_begin<R, false>(&s_walk)) return;
   auto swz_k = [](int r) { return 2 * (r & 7); };
   auto swz_v = [](int r) { return 4 * ((r >> 2) & 3); };
   do {
@@ -1043,7 +1051,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
                                                        blocks, lim_hi / BS);
       }
     }
-  } while (pa_next<R>(&s_walk));
+  } while (pa_next<R, false>(&s_walk));
 }
 
 // Joins the parts of the tile that began last in a workgroup's stretch: a row by D / 4 lanes.
@@ -1053,7 +1061,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaKP p) {
   const int wg = blockIdx.x;
   const int4 note = p.ws_join[wg];
   if (note.z == 0) return;
-  const int kvh = wg % p.Hkv, b = note.x, G = p.G;
+  const int kvh = wg % p.Hkv, b = note.x, G = p.G, own = note.w ? note.w - 1 : wg / p.Hkv;
   const PaSeq sq = pa_seq(p, b);
   const int nrow = sq.lq * G, r0 = note.y * R, lane = threadIdx.x % LR;
   for (int r = r0 + blockIdx.y * RW + threadIdx.x / LR; r < min(nrow, r0 + R); r += gridDim.y * RW) {
@@ -1066,7 +1074,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaKP p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int x = min(i0 + i, note.z - 1);
-        const int64_t pi = pa_part(p, wg + x * p.Hkv, x == 0) + r - r0;
+        const int64_t pi = pa_part(p, own + x, kvh, x == 0, note.w != 0) + r - r0;
         ml[i] = *(const float2 *)(p.ws_ml + 2 * pi);
         v[i] = *(const float4 *)(p.ws_acc + pi * D + 4 * lane);
       }
@@ -1103,27 +1111,34 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaKP p) {
 
 // ------------------------------------------------------------------ host ----
 struct PaPlan {
-  int64_t W = 1, rows = 128, least = 0;
-  size_t ml = 0, join = 0, bytes = 0;
+  int64_t W = 1, rows = 128, least = 0, few_parts = 0;
+  bool join = true;
+  size_t ml = 0, notes = 0, bytes = 0;
 };
 
 static PaPlan pa_plan(const la_paged_attn_args *a) {
   PaPlan pl;
   const bool f32 = a->dtype == LA_F32;
   const int64_t G = a->Hq / a->Hkv, R = f32 ? 64 : 128;
-  // workgroups that are there at once, shared among the KV heads; no stretch is shorter than four
-  // blocks of keys and a tile's beginning and end
+  // workgroups that are there at once, shared among the KV heads (one at least for either line); no
+  // stretch is shorter than four blocks of keys and a tile's beginning and end
   pl.least = G * (4 * (f32 ? 32 : DA_BS) + PA_AHEAD);
   const int64_t rows = a->Tq * G, keys = a->pt_pages * a->page;  // (rows: of a sequence, at most)
   const int64_t tiles = a->cu_q ? std::min(rows, rows / R + a->B) : a->B * ceil_div(rows, R);  // at most
   const double most = (double)tiles * ((double)G * (keys + PA_AHEAD) + (a->causal ? R + 0.0 : 0.0));
-  pl.W = std::max<int64_t>(1, (f32 ? 2 : 3) * num_cus() / a->Hkv);
-  if (most / pl.least < (double)pl.W) pl.W = (int64_t)(most / pl.least) + 1;
+  pl.W = std::max<int64_t>(f32 ? 1 : 2, (f32 ? 2 : 3) * num_cus() / a->Hkv);
+  if (most / pl.least + 2 < (double)pl.W) pl.W = (int64_t)(most / pl.least) + 2;
+  if (most <= 2.0 * pl.least) {  // a stretch for each line, nothing to join: a launch less (4 us)
+    pl.least = (int64_t)1 << 60;
+    pl.W = 2;
+    pl.join = false;
+  }
   pl.rows = std::min(R, rows);
-  const int64_t parts = pl.W * a->Hkv * 2 * pl.rows;
+  pl.few_parts = pl.W * a->Hkv * 2 * pl.rows;
+  const int64_t parts = pl.join ? pl.few_parts + (f32 ? 0 : pl.W * a->Hkv * 2 * PA_FEW) : 0;
   pl.ml = ((size_t)parts * 2 * sizeof(float) + 255) / 256 * 256;
-  pl.join = pl.ml + ((size_t)parts * a->D * sizeof(float) + 255) / 256 * 256;
-  pl.bytes = pl.join + (size_t)(pl.W * a->Hkv) * sizeof(int4);
+  pl.notes = pl.ml + ((size_t)parts * a->D * sizeof(float) + 255) / 256 * 256;
+  pl.bytes = pl.notes + (size_t)(pl.W * a->Hkv) * sizeof(int4);
   return pl;
 }
 
@@ -1205,13 +1220,13 @@ extern "C" int la_paged_attention(const la_paged_attn_args *args, void *stream) 
   p.page_table = a->page_table; p.lengths = a->lengths; p.cu_q = a->cu_q; p.q_len = a->q_len;
   p.ws_ml = (float *)a->workspace;
   p.ws_acc = (float *)((char *)a->workspace + pl.ml);
-  p.ws_join = (int4 *)((char *)a->workspace + pl.join);
+  p.ws_join = (int4 *)((char *)a->workspace + pl.notes);
   p.Tq = a->Tq;
   p.q_sb = a->q_sb; p.q_sh = a->q_sh; p.q_st = a->q_st;
   p.o_sb = a->o_sb; p.o_sh = a->o_sh; p.o_st = a->o_st;
   p.l_sb = a->l_sb; p.l_sh = a->l_sh;
   p.pt_sb = a->pt_sb; p.s_stride = a->s_stride; p.n_phys = a->n_phys;
-  p.least = pl.least;
+  p.least = pl.least; p.few_parts = pl.few_parts;
   p.B = (int32_t)a->B; p.G = (int32_t)(a->Hq / a->Hkv); p.Hq = (int32_t)a->Hq; p.Hkv = (int32_t)a->Hkv;
   p.D = (int32_t)a->D; p.W = (int32_t)pl.W; p.part_rows = (int32_t)pl.rows;
   p.page = (int32_t)a->page; p.pt_pages = (int32_t)a->pt_pages;
@@ -1225,7 +1240,7 @@ extern "C" int la_paged_attention(const la_paged_attn_args *args, void *stream) 
   if (a->dtype == LA_F32) rc = d128 ? pa_launch(paged_attn_f32_kernel<128>, wgs, p, st) : pa_launch(paged_attn_f32_kernel<64>, wgs, p, st);
   else if (a->dtype == LA_BF16) rc = d128 ? pa_launch16<DaBf16, 128>(kv8, even, wgs, p, st) : pa_launch16<DaBf16, 64>(kv8, even, wgs, p, st);
   else rc = d128 ? pa_launch16<DaF16, 128>(kv8, even, wgs, p, st) : pa_launch16<DaF16, 64>(kv8, even, wgs, p, st);
-  if (rc != LA_OK) return rc;
+  if (rc != LA_OK || !pl.join) return rc;
   const dim3 grid((uint32_t)wgs, pl.rows > 32 ? 4 : 1);
   if (a->dtype == LA_F32) {
     if (d128) paged_join_kernel<128, 64><<<grid, 256, 0, st>>>(p);
