@@ -37,7 +37,7 @@ struct PaKP {
   float qscale, thr_gap;
 };
 
-constexpr int PA_AHEAD = 160;  // what a tile's beginning and end cost, in keys
+constexpr int PA_AHEAD = 256;  // what a tile's beginning and end cost, in keys (twelve prompts 264, 256 and 263 us at 160, 256, 600)
 
 struct PaSeq {
   int32_t lq, lk;
@@ -121,8 +121,8 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w) {
   s.left = 0;
   s.b = s.i = 0;
   // places for tiles of many rows, by the share of the time (beside them, a block of few rows takes a
-  // little less than one of many: chunks and tokens together 261, 253 and 255 us at 0.5, 0.7 and 1)
-  const int wm = few == 0 ? p.W : many == 0 ? 0 : max(1, min(p.W - 1, (int)((double)p.W * (double)many / ((double)many + 0.8 * (double)few) + 0.5)));
+  // little less than one of many: four such batches 587, 568 and 584 us together at 0.5, 0.7 and 1)
+  const int wm = few == 0 ? p.W : many == 0 ? 0 : max(1, min(p.W - 1, (int)((double)p.W * (double)many / ((double)many + 0.7 * (double)few) + 0.5)));
   s.few = w >= wm && few > 0;
   s.line.all = s.few ? few : many;
   s.line.first = s.few ? wm : 0;

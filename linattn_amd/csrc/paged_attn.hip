@@ -31,8 +31,8 @@ struct PaCache {
 // The blocks of a piece: number i of j0 .. j1 - 1 is block i + turn of the tile, and behind its last of
 // n_all comes its first.  A tile's blocks begin where the workgroups of its KV head are at that time, if
 // all take equally long for a block: they read the same keys at about the same time, of which
-// L2 then has what another has read (8192 tokens behind 24576: 28 % of the reads without turning
-// TURNED, 3.87 ms; with it TURNED).
+// L2 then has what another has read (8192 tokens behind 24576: 67 % of the reads in place of 28,
+// 3.67 ms in place of 3.87).
 struct PaBlocks {
   int32_t j0, j1, turn, n_all;
   __device__ __forceinline__ int at(int i) const { return i + turn < n_all ? i + turn : i + turn - n_all; }

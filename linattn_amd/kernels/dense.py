@@ -22,6 +22,7 @@ from linattn_amd.kernels.block_sparse import _paged_scale_stride
 __all__ = ["dense_attention", "packed_attention", "paged_attention"]
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_pack, _library = N.by_bytes(N.LaPagedAttnArgs, "la_paged_attention_workspace", "la_paged_attention")
 
 
 def _rows(t: torch.Tensor, token: int = -2) -> torch.Tensor:
@@ -198,32 +199,35 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
 
 def _pools(what: str, k_pool: torch.Tensor, v_pool: torch.Tensor, dtype: torch.dtype, Hkv: int, D: int,
-           k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor]) -> Tuple[bool, int]:
-    """(whether the pools hold fp8 codes, the stride of their scales), checked."""
-    if k_pool.dim() != 4 or v_pool.shape != k_pool.shape or k_pool.shape[1] != Hkv or k_pool.shape[3] != D \
-            or k_pool.numel() == 0:
+           k_scale: Optional[torch.Tensor], v_scale: Optional[torch.Tensor]) -> Tuple[torch.Size, bool, int]:
+    """(the pools' shape, whether they hold fp8 codes, the stride of their scales), checked."""
+    shape, held = k_pool.shape, k_pool.dtype
+    if len(shape) != 4 or v_pool.shape != shape or shape[1] != Hkv or shape[3] != D or shape[0] * shape[1] * shape[2] == 0:
         raise ValueError(f"{what}: pools must be (n_phys, {Hkv}, page_size, {D}), and not empty")
     if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError(f"{what}: pools must be contiguous")
-    fp8 = k_pool.dtype == torch.float8_e4m3fn
-    if k_pool.dtype != v_pool.dtype or not (fp8 or k_pool.dtype == dtype):
+    fp8 = held == torch.float8_e4m3fn
+    if held != v_pool.dtype or not (fp8 or held == dtype):
         raise ValueError(f"{what}: the pools hold the queries' dtype, or float8_e4m3fn codes")
     if not fp8:
         if k_scale is not None or v_scale is not None:
             raise ValueError(f"{what}: scales are for fp8 pools")
-        return False, 1
+        return shape, False, 1
     for s in (k_scale, v_scale):
-        if s is None or s.dtype != torch.float32 or s.shape != k_pool.shape[:3]:
+        if s is None or s.dtype != torch.float32 or s.shape != shape[:3]:
             raise ValueError(f"{what}: fp8 pools need fp32 k_scale / v_scale (n_phys, Hkv, page_size)")
     if k_scale.stride() != v_scale.stride():
         raise ValueError(f"{what}: k_scale / v_scale must share strides")
-    return True, _paged_scale_stride(k_scale, k_pool)
+    return shape, True, _paged_scale_stride(k_scale, k_pool)
 
 
-def _table(what: str, page_table: torch.Tensor, B: int) -> None:
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B \
-            or page_table.shape[1] == 0 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+def _table(what: str, page_table: torch.Tensor, B: int) -> Tuple[int, int]:
+    """(row stride, pages), checked."""
+    shape = page_table.shape
+    if page_table.dtype != torch.int32 or len(shape) != 2 or shape[0] != B or shape[1] == 0 \
+            or (shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError(f"{what}: page_table must be int32 ({B}, pages) with unit column stride")
+    return page_table.stride()[0], shape[1]
 
 
 def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, page_table: torch.Tensor,
@@ -252,53 +256,54 @@ def paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     shared out there, so a captured call may be replayed with others.  Forward only."""
     what = "paged_attention"
     dev = N.require_gpu(q, k_pool, v_pool, page_table, lengths, cu_seqlens, q_lengths, k_scale, v_scale, out, what=what)
-    packed = cu_seqlens is not None
-    if q.dim() != (3 if packed else 4):
+    packed, shape, dtype = cu_seqlens is not None, q.shape, q.dtype
+    if len(shape) != (3 if packed else 4):
         raise ValueError(f"{what}: q must be (N, Hq, D) with cu_seqlens, or (B, Hq, Tq, D)")
-    if q.dtype not in _TYPES:
+    if dtype not in _TYPES:
         raise ValueError(f"{what}: q must be bfloat16, float16 or float32")
-    Hq, D = q.shape[1], q.shape[-1]
+    Hq, D = shape[1], shape[-1]
     if D not in (64, 128):
         raise ValueError(f"{what}: head_dim must be 64 or 128")
     Hkv = k_pool.shape[1] if k_pool.dim() == 4 else 0
-    fp8, s_stride = _pools(what, k_pool, v_pool, q.dtype, Hkv, D, k_scale, v_scale)
-    if fp8 and q.dtype == torch.float32:
+    pool, fp8, s_stride = _pools(what, k_pool, v_pool, dtype, Hkv, D, k_scale, v_scale)
+    if fp8 and dtype == torch.float32:
         raise ValueError(f"{what}: fp8 pools take bfloat16 or float16 queries")
     if Hq == 0 or Hq % Hkv:
         raise ValueError(f"{what}: the query heads must be a multiple of the KV heads")
+    cp = qp = 0
     if packed:
         cu_seqlens = _cu(cu_seqlens, "cu_seqlens")
         if q_lengths is not None:
             raise ValueError(f"{what}: q_lengths are for batched queries")
-        B, Tq = cu_seqlens.shape[0] - 1, q.shape[0]
+        B, Tq, cp = cu_seqlens.shape[0] - 1, shape[0], cu_seqlens.data_ptr()
     else:
-        B, Tq = q.shape[0], q.shape[2]
-        q_lengths = _int32(q_lengths, (B,), "q_lengths")
-    _table(what, page_table, B)
-    lengths = _int32(lengths, (B,), "lengths")
+        B, Tq = shape[0], shape[2]
+        if q_lengths is not None:
+            q_lengths = _int32(q_lengths, (B,), "q_lengths")
+            qp = q_lengths.data_ptr()
+    pt_stride, pt_pages = _table(what, page_table, B)
     if lengths is None:
         raise ValueError(f"{what}: lengths must be int32 ({B},)")
+    lengths = _int32(lengths, (B,), "lengths")
     zero_rest = out is None
     out = _out(what, out, q, out_dtype, k_pool, v_pool)
-    lse, l_s = None, (0, 0)
+    lse, lp, l_s = None, 0, (0, 0)
     if return_lse:
-        lse = torch.empty((Hq, Tq) if packed else (B, Hq, Tq), dtype=torch.float32, device=dev) if zero_rest or not packed \
-            else torch.full((Hq, Tq), float("-inf"), dtype=torch.float32, device=dev)
-        l_s = (0, Tq) if packed else (Hq * Tq, Tq)
+        ls = (Hq, Tq) if packed else (B, Hq, Tq)
+        lse = torch.empty(ls, dtype=torch.float32, device=dev) if zero_rest or not packed \
+            else torch.full(ls, float("-inf"), dtype=torch.float32, device=dev)
+        lp, l_s = lse.data_ptr(), (0, Tq) if packed else (Hq * Tq, Tq)
     if B > 0 and Tq > 0:
         q = _rows(q, 0 if packed else -2)
-        q_s, o_s = (((0, t.stride(1), t.stride(0)) if packed else t.stride()[:3]) for t in (q, out))
-        a = N.LaPagedAttnArgs(
-            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), N.ptr(lse), N.ptr(k_scale),
-            N.ptr(v_scale), page_table.data_ptr(), lengths.data_ptr(), N.ptr(cu_seqlens), N.ptr(q_lengths), None, 0,
-            B, Hq, Hkv, Tq, D, *q_s, *o_s, *l_s, k_pool.shape[0], k_pool.shape[2], page_table.stride(0),
-            page_table.shape[1], s_stride, _scale(scale, D), 1 if causal else 0, N.dtype_code(q.dtype),
-            N.dtype_code(k_pool.dtype), N.dtype_code(out.dtype), 1 if zero_rest else 0)
-        L, ref = N.load(), ctypes.byref(a)
+        q_s, o_s = q.stride(), out.stride()
+        q_s, o_s = ((0, q_s[1], q_s[0]), (0, o_s[1], o_s[0])) if packed else (q_s[:3], o_s[:3])
+        head = (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), lp, k_scale.data_ptr() if fp8 else 0,
+                v_scale.data_ptr() if fp8 else 0, page_table.data_ptr(), lengths.data_ptr(), cp, qp)
+        tail = (B, Hq, Hkv, Tq, D, *q_s, *o_s, *l_s, pool[0], pool[2], pt_stride, pt_pages, s_stride, _scale(scale, D),
+                bool(causal), N.dtype_code(dtype), N.dtype_code(k_pool.dtype), N.dtype_code(out.dtype), zero_rest)
+        room, run = _library()
         with N.on_device(dev):
-            nbytes = L.la_paged_attention_workspace(ref)
-            if nbytes:
-                ws = N.workspace(nbytes, dev)
-                a.workspace, a.ws_bytes = ws.data_ptr(), nbytes
-            N.check(L.la_paged_attention(ref, N.stream_handle(dev)), what)
+            nbytes = room(_pack(*head, 0, 0, *tail))
+            ws = N.workspace(nbytes, dev)
+            N.check(run(_pack(*head, 0 if ws is None else ws.data_ptr(), nbytes, *tail), N.stream_handle(dev)), what)
     return (out, lse) if return_lse else out

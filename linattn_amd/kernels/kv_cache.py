@@ -16,16 +16,18 @@ turns the new queries and keys by their rotary positions on the way.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import Optional
 
 import torch
 
 from linattn_amd import _native as N
 from linattn_amd.kernels.block_sparse import _paged_scale_stride
-from linattn_amd.kernels.dense import _pools, _table
+from linattn_amd.kernels.dense import _cu, _pools, _table
 from linattn_amd.kernels.rotary import _TYPES, _frequencies, _out_rows, _positions, _strides, _unit_rows
 
 __all__ = ["paged_kv_append", "rotary_kv_append"]
+
+_pack, _library = N.by_bytes(N.LaRotaryAppendArgs, "la_rotary_append")
 
 
 def paged_kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
@@ -138,75 +140,74 @@ def rotary_kv_append(q: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torc
     what = "rotary_kv_append"
     dev = N.require_gpu(k_new, v_new, q, k_pool, v_pool, page_table, positions, inv_freq, cu_seqlens,
                         rotary_positions, axes, q_out, page_min, page_max, k_scale, v_scale, what=what)
-    packed = cu_seqlens is not None
-    if k_new.dim() != (3 if packed else 4) or v_new.shape != k_new.shape:
+    packed, shape, dtype = cu_seqlens is not None, k_new.shape, k_new.dtype
+    if len(shape) != (3 if packed else 4) or v_new.shape != shape:
         raise ValueError(f"{what}: k_new / v_new must be (B, Hkv, Tn, D), or with cu_seqlens (N, Hkv, D)")
-    if k_new.dtype not in _TYPES or v_new.dtype != k_new.dtype:
+    if dtype not in _TYPES or v_new.dtype != dtype:
         raise ValueError(f"{what}: k_new / v_new must both be bfloat16, float16 or float32")
-    Hkv, D = k_new.shape[1], k_new.shape[-1]
+    Hkv, D, Hq = shape[1], shape[-1], 0
     if Hkv == 0:
         raise ValueError(f"{what}: no KV heads")
-    if q is not None and (q.dim() != k_new.dim() or q.dtype != k_new.dtype or q.shape[0] != k_new.shape[0]
-                          or q.shape[2:] != k_new.shape[2:] or q.shape[1] % Hkv):
-        raise ValueError(f"{what}: q must have k_new's dtype, tokens and head_dim, and a multiple of its heads")
+    if q is not None:
+        qs = q.shape
+        if len(qs) != len(shape) or q.dtype != dtype or qs[0] != shape[0] or qs[2:] != shape[2:] or qs[1] % Hkv:
+            raise ValueError(f"{what}: q must have k_new's dtype, tokens and head_dim, and a multiple of its heads")
+        Hq = qs[1]
+    elif q_out is not None:
+        raise ValueError(f"{what}: q_out without q")
     if packed:
-        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
-            raise ValueError(f"{what}: cu_seqlens must be int32 (B + 1,)")
-        cu_seqlens = cu_seqlens.contiguous()
-        B, T = cu_seqlens.shape[0] - 1, k_new.shape[0]
+        cu_seqlens = _cu(cu_seqlens, "cu_seqlens")
+        B, T = cu_seqlens.shape[0] - 1, shape[0]
     else:
-        B, T = k_new.shape[0], k_new.shape[2]
-    fp8, s_stride = _pools(what, k_pool, v_pool, k_new.dtype, Hkv, D, k_scale, v_scale)
-    _table(what, page_table, B)
+        B, T = shape[0], shape[2]
+    pool, fp8, s_stride = _pools(what, k_pool, v_pool, dtype, Hkv, D, k_scale, v_scale)
+    pt_stride, pt_pages = _table(what, page_table, B)
     if positions.dtype != torch.int32 or positions.shape != (B,):
         raise ValueError(f"{what}: positions must be int32 ({B},)")
-    positions = positions.contiguous()
-    _frequencies(what, inv_freq, axes, D)
-    A, p_s = 1, (0, 0, 0)
+    n = _frequencies(what, inv_freq, axes, D)
+    A, p_s, rp = 1, (0, 0, 0), 0
     if rotary_positions is not None:
         A, p_s = _positions(what, rotary_positions, axes, (T,) if packed else (B, T))
+        rp = rotary_positions.data_ptr()
     elif axes is not None:
         raise ValueError(f"{what}: axes need rotary_positions")
-    if (page_min is None) != (page_max is None):
-        raise ValueError(f"{what}: pass both page_min and page_max, or neither")
+    mn = mx = 0
     meta = (0, 0, 0, 0, 0, 0)
-    if page_min is not None:
+    if page_min is not None and page_max is not None:
         if fp8:
             raise ValueError(f"{what}: fp8 pools take no page bounds")
         if page_size is None or not 0 < int(page_size) < 1 << 30:
             raise ValueError(f"{what}: page bounds need page_size")
-        if page_min.dim() != 4 or page_min.shape[:2] != (B, Hkv) or page_min.shape[3] != D \
-                or page_max.shape != page_min.shape or page_min.stride() != page_max.stride():
+        ms, m_s = page_min.shape, page_min.stride()
+        if len(ms) != 4 or ms[0] != B or ms[1] != Hkv or ms[3] != D or page_max.shape != ms or page_max.stride() != m_s:
             raise ValueError(f"{what}: page_min / page_max must be (B, Hkv, n_pages, D) with equal strides")
-        if page_min.dtype != k_new.dtype or page_max.dtype != k_new.dtype:
+        if page_min.dtype != dtype or page_max.dtype != dtype:
             raise ValueError(f"{what}: page bounds are stored in the key dtype")
-        meta = (int(page_size), page_min.shape[2], *page_min.stride())
-        if page_min.numel() == 0:
-            page_min = page_max = None
+        if ms[2] > 0:
+            mn, mx, meta = page_min.data_ptr(), page_max.data_ptr(), (int(page_size), ms[2], *m_s)
+    elif page_min is not None or page_max is not None:
+        raise ValueError(f"{what}: pass both page_min and page_max, or neither")
     elif page_size is not None:
         raise ValueError(f"{what}: page_size is for page bounds")
     zero_rest = q_out is None
-    if q is None:
-        if q_out is not None:
-            raise ValueError(f"{what}: q_out without q")
-    else:
+    if q is not None:
         q_out = _out_rows(what, "q_out", q_out, q)
     if B == 0 or T == 0:
         return q_out
-    q = None if q is None else _unit_rows(what, "q", q)
-    k_new, v_new = _unit_rows(what, "k_new", k_new), _unit_rows(what, "v_new", v_new)
-    inv_freq = inv_freq.contiguous()
+    k_new, v_new, inv_freq, positions = _unit_rows(k_new), _unit_rows(v_new), inv_freq.contiguous(), positions.contiguous()
     axes = None if axes is None else axes.contiguous()
-    Hq = 0 if q is None else q.shape[1]
-    none = (0, 0, 0)
-    a = N.LaRotaryAppendArgs(
-        N.ptr(q), k_new.data_ptr(), v_new.data_ptr(), N.ptr(q_out), k_pool.data_ptr(), v_pool.data_ptr(),
-        N.ptr(k_scale), N.ptr(v_scale), page_table.data_ptr(), positions.data_ptr(), N.ptr(cu_seqlens),
-        N.ptr(rotary_positions), inv_freq.data_ptr(), N.ptr(axes), N.ptr(page_min), N.ptr(page_max),
-        B, T, Hq, Hkv, D, inv_freq.shape[0], A, *(_strides(q) if Hq else none), *_strides(k_new), *_strides(v_new),
-        *(_strides(q_out) if Hq else none), *p_s, k_pool.shape[0], k_pool.shape[2], page_table.stride(0),
-        page_table.shape[1], s_stride, *meta, N.dtype_code(k_new.dtype), N.dtype_code(k_pool.dtype),
-        1 if interleaved else 0, 1 if zero_rest else 0)
+    qp = qo = 0
+    q_s = o_s = (0, 0, 0)
+    if Hq:
+        q = _unit_rows(q)
+        qp, qo, q_s, o_s = q.data_ptr(), q_out.data_ptr(), _strides(q), _strides(q_out)
+    a = _pack(qp, k_new.data_ptr(), v_new.data_ptr(), qo, k_pool.data_ptr(), v_pool.data_ptr(),
+              k_scale.data_ptr() if fp8 else 0, v_scale.data_ptr() if fp8 else 0, page_table.data_ptr(),
+              positions.data_ptr(), cu_seqlens.data_ptr() if packed else 0, rp, inv_freq.data_ptr(),
+              0 if axes is None else axes.data_ptr(), mn, mx, B, T, Hq, Hkv, D, n, A, *q_s, *_strides(k_new),
+              *_strides(v_new), *o_s, *p_s, pool[0], pool[2], pt_stride, pt_pages, s_stride, *meta,
+              N.dtype_code(dtype), N.dtype_code(k_pool.dtype), interleaved, zero_rest)
+    run, = _library()
     with N.on_device(dev):
-        N.check(N.load().la_rotary_append(ctypes.byref(a), N.stream_handle(dev)), what)
+        N.check(run(a, N.stream_handle(dev)), what)
     return q_out

@@ -7,7 +7,6 @@
 
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -33,17 +32,21 @@ def rotary_axes(sections: Sequence[int], interleaved: bool = False,
     return torch.tensor(axes, dtype=torch.int32, device=device)
 
 
-def _unit_rows(what: str, name: str, t: torch.Tensor) -> torch.Tensor:
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        return t.contiguous()
-    return t
+_pack, _library = N.by_bytes(N.LaRotaryArgs, "la_rotary")
 
 
-def _frequencies(what: str, inv_freq: torch.Tensor, axes: Optional[torch.Tensor], D: int) -> None:
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= D <= 512:
+def _unit_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride()[-1] == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _frequencies(what: str, inv_freq: torch.Tensor, axes: Optional[torch.Tensor], D: int) -> int:
+    """How many there are, checked."""
+    shape = inv_freq.shape
+    if inv_freq.dtype != torch.float32 or len(shape) != 1 or not 0 < 2 * shape[0] <= D <= 512:
         raise ValueError(f"{what}: inv_freq must be float32 (n,) with 2 n <= head_dim <= 512")
-    if axes is not None and (axes.dtype != torch.int32 or axes.shape != inv_freq.shape):
+    if axes is not None and (axes.dtype != torch.int32 or axes.shape != shape):
         raise ValueError(f"{what}: axes must be int32 with an entry for each frequency")
+    return shape[0]
 
 
 def _positions(what: str, positions: torch.Tensor, axes: Optional[torch.Tensor],
@@ -51,26 +54,26 @@ def _positions(what: str, positions: torch.Tensor, axes: Optional[torch.Tensor],
     """(axes, strides by axis, sequence and token) of positions (*tokens) or (A, *tokens)."""
     if positions.dtype != torch.int32:
         raise ValueError(f"{what}: positions must be int32")
-    shape, st = tuple(positions.shape), positions.stride()
+    shape, st = positions.shape, positions.stride()
     if axes is None:
         if shape != tokens:
-            raise ValueError(f"{what}: positions must be {tokens} (with several axes, pass `axes`), got {shape}")
-        A, st = 1, (0, *st)
-    else:
-        if len(shape) != len(tokens) + 1 or shape[1:] != tokens or shape[0] == 0:
-            raise ValueError(f"{what}: positions must be (axes, {', '.join(map(str, tokens))}), got {shape}")
-        A = shape[0]
-    return A, (st if len(tokens) == 2 else (st[0], 0, st[1]))
+            raise ValueError(f"{what}: positions must be {tokens} (with several axes, pass `axes`), got {tuple(shape)}")
+        return 1, (0, *st) if len(st) == 2 else (0, 0, st[0])
+    if len(shape) != len(tokens) + 1 or shape[1:] != tokens or shape[0] == 0:
+        raise ValueError(f"{what}: positions must be (axes, {', '.join(map(str, tokens))}), got {tuple(shape)}")
+    return shape[0], st if len(st) == 3 else (st[0], 0, st[1])
 
 
 def _out_rows(what: str, name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty_like(x, memory_format=torch.contiguous_format)
+    if out is x:
+        return out
     if out.shape != x.shape or out.dtype != x.dtype or (out.shape[-1] > 1 and out.stride(-1) != 1):
         raise ValueError(f"{what}: {name} must have its input's shape and dtype, and contiguous rows")
-    if out is not x and out.data_ptr() != x.data_ptr():
+    if out.data_ptr() != x.data_ptr():
         _apart(what, out, x)
-    elif out is not x and out.numel() and any(a != b for a, b, d in zip(out.stride(), x.stride(), x.shape) if d > 1):
+    elif out.numel() and any(a != b for a, b, d in zip(out.stride(), x.stride(), x.shape) if d > 1):
         raise ValueError(f"{what}: {name} shares memory with its input, but does not hold the same rows")
     return out
 
@@ -78,7 +81,7 @@ def _out_rows(what: str, name: str, out: Optional[torch.Tensor], x: torch.Tensor
 def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
     """(sequence, head, token) of (B, H, T, D), or packed (T, H, D)."""
     s = t.stride()
-    return (s[0], s[1], s[2]) if len(s) == 4 else (0, s[1], s[0])
+    return s[:3] if len(s) == 4 else (0, s[1], s[0])
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor, *,
@@ -99,38 +102,39 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     may be q and k themselves (in place)."""
     what = "rotary"
     dev = N.require_gpu(q, k, positions, inv_freq, axes, q_out, k_out, what=what)
-    if q.dim() not in (3, 4) or q.dtype not in _TYPES:
+    shape, dtype = q.shape, q.dtype
+    batched = len(shape) == 4
+    if not (batched or len(shape) == 3) or dtype not in _TYPES:
         raise ValueError(f"{what}: q must be (B, Hq, T, D) or (N, Hq, D) in bfloat16, float16 or float32")
-    batched = q.dim() == 4
-    if k is not None and (k.dim() != q.dim() or k.dtype != q.dtype or k.shape[0] != q.shape[0]
-                          or k.shape[2:] != q.shape[2:]):
-        raise ValueError(f"{what}: k must have q's dtype, tokens and head_dim")
-    D, Hq = q.shape[-1], q.shape[1]
-    Hkv = 0 if k is None else k.shape[1]
-    B, T = (q.shape[0], q.shape[2]) if batched else (1, q.shape[0])
-    _frequencies(what, inv_freq, axes, D)
-    A, p_s = _positions(what, positions, axes, (B, T) if batched else (T,))
-    if k is None and k_out is not None:
+    B, Hq, T, D = shape if batched else (1, shape[1], shape[0], shape[2])
+    Hkv = 0
+    if k is not None:
+        ks = k.shape
+        if len(ks) != len(shape) or k.dtype != dtype or ks[0] != shape[0] or ks[2:] != shape[2:]:
+            raise ValueError(f"{what}: k must have q's dtype, tokens and head_dim")
+        Hkv = ks[1]
+    elif k_out is not None:
         raise ValueError(f"{what}: k_out without k")
+    n = _frequencies(what, inv_freq, axes, D)
+    A, p_s = _positions(what, positions, axes, (B, T) if batched else (T,))
     q_out = _out_rows(what, "q_out", q_out, q)
     if k is not None:
         k_out = _out_rows(what, "k_out", k_out, k)
-    if q_out.numel() or (k is not None and k_out.numel()):
-        inv_freq = inv_freq.contiguous()
+    if B * T * (Hq + Hkv) * D > 0:
+        q, inv_freq = _unit_rows(q), inv_freq.contiguous()
         axes = None if axes is None else axes.contiguous()
-        q = _unit_rows(what, "q", q)
-        k = None if k is None else _unit_rows(what, "k", k)
-        none = (0, 0, 0)
-        kv = k is not None and Hkv > 0
+        kp = ko = 0
+        k_s = ko_s = (0, 0, 0)
+        if Hkv:
+            k = _unit_rows(k)
+            kp, ko, k_s, ko_s = k.data_ptr(), k_out.data_ptr(), _strides(k), _strides(k_out)
         if Hq == 0:  # (the rows of k alone)
-            if kv:
-                rotary(k, None, positions, inv_freq, axes=axes, interleaved=interleaved, inverse=inverse, q_out=k_out)
+            rotary(k, None, positions, inv_freq, axes=axes, interleaved=interleaved, inverse=inverse, q_out=k_out)
             return q_out, k_out
-        a = N.LaRotaryArgs(
-            q.data_ptr(), k.data_ptr() if kv else None, q_out.data_ptr(), k_out.data_ptr() if kv else None,
-            positions.data_ptr(), inv_freq.data_ptr(), N.ptr(axes), B, T, Hq, Hkv, D, inv_freq.shape[0], A,
-            *_strides(q), *(_strides(k) if kv else none), *_strides(q_out), *(_strides(k_out) if kv else none),
-            *p_s, N.dtype_code(q.dtype), 1 if interleaved else 0, 1 if inverse else 0, 0)
+        a = _pack(q.data_ptr(), kp, q_out.data_ptr(), ko, positions.data_ptr(), inv_freq.data_ptr(),
+                  0 if axes is None else axes.data_ptr(), B, T, Hq, Hkv, D, n, A, *_strides(q), *k_s, *_strides(q_out),
+                  *ko_s, *p_s, N.dtype_code(dtype), interleaved, inverse, 0)
+        run, = _library()
         with N.on_device(dev):
-            N.check(N.load().la_rotary(ctypes.byref(a), N.stream_handle(dev)), what)
+            N.check(run(a, N.stream_handle(dev)), what)
     return q_out if k is None else (q_out, k_out)
