@@ -27,7 +27,7 @@ struct PaKP {
   float *lse;
   const float *k_scale, *v_scale;
   const int32_t *page_table, *lengths, *cu_q, *q_len;
-  float *ws_ml, *ws_acc;  // parts (pa_part): (reference, sum) and D values of each row
+  float *ws_ml, *ws_acc;  // parts (pa_part): (reference, sum) and D values (pa_in_part) of each row
   int4 *ws_join;          // [workgroup]: of the tile that begins last there: sequence, tile, parts (0: none), and
                           // 1 + the stretch's number where rows are few, else 0
   int64_t Tq, q_sb, q_sh, q_st, o_sb, o_sh, o_st, l_sb, l_sh, pt_sb, s_stride, n_phys;
@@ -173,6 +173,14 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w) {
 __device__ __forceinline__ int64_t pa_part(const PaKP &p, int64_t x, int kvh, bool last, bool few) {
   const int64_t at = (x * p.Hkv + kvh) * 2 + (last ? 1 : 0);
   return few ? p.few_parts + at * PA_FEW : at * p.part_rows;
+}
+
+// Where value d of row r of a tile of D-value rows lies in its part, in 16-bit types: the 32 rows of a wave as
+// its lanes hold them (register i of dim tile dt of lane l: dim 32 dt + 8 (i / 4) + 4 (l / 32) + i % 4 of row
+// l % 32), so that a wave writes and reads 1 KB at a time.
+template <int D>
+__device__ __forceinline__ int64_t pa_in_part(int r, int d) {
+  return (int64_t)(r >> 5) * 32 * D + ((d >> 5) * 4 + ((d >> 3) & 3)) * 256 + ((((d >> 2) & 1) << 5) | (r & 31)) * 4 + (d & 3);
 }
 
 // Of a tile of `n` staged blocks of keys and cost C, those before place c.

@@ -44,7 +44,7 @@ struct PaBlocks {
 // fp16 (LOST), where a weight below 2^-40 of the row's largest is 0 and its product with an
 // infinity NaN: a dim's first keys with NaN and either infinity say what it is for each row.
 // (What a block holds past the last key is that key again.)
-template <class E, int D, int BS, int NR, bool KV8, bool ALL, bool LOST>
+template <class E, int D, int BS, int NR, bool KV8, bool ALL, bool LOST, bool WAVES>
 __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t part, int r_tile, int r_first, uint32_t bad,
                          const PaBlocks &blocks, int top) {
   const int lane = threadIdx.x & 63, G = p.G;
@@ -53,6 +53,7 @@ __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t
   auto row = [&](int key) { return pa_row(p, pages, min(key, sq.lk - 1), kvh); };
   constexpr int N = D / 64;
   const float inf = __int_as_float(0x7f800000);
+  auto in_part = [&](int r, int d) { return part * D + (WAVES ? pa_in_part<D>(r - r_tile, d) : (int64_t)(r - r_tile) * D + d); };
   int32_t at[3][N];  // of dim lane + 64 x
 #pragma unroll
   for (int x = 0; x < N; ++x) at[0][x] = at[1][x] = at[2][x] = INT32_MAX;
@@ -91,7 +92,7 @@ __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t
         const bool up = at[1][x] <= lim, down = at[2][x] <= lim, nan = at[0][x] <= lim || (up && down);
         if (!nan && !up && !down) continue;
         const float y = nan ? __int_as_float(0x7fc00000) : up ? inf : -inf;
-        if (part >= 0) p.ws_acc[(part + r - r_tile) * D + lane + 64 * x] = y;
+        if (part >= 0) p.ws_acc[in_part(r, lane + 64 * x)] = y;
         else store_from_f32(p.out, pa_out_at(p, b, sq, t, h) + lane + 64 * x, p.out_dt, y);
       }
       continue;
@@ -131,7 +132,7 @@ __device__ void pa_again(const PaKP &p, int b, const PaSeq &sq, int kvh, int64_t
         p.ws_ml[2 * pi + 1] = l;
       }
 #pragma unroll
-      for (int x = 0; x < N; ++x) p.ws_acc[pi * D + lane + 64 * x] = acc[x];
+      for (int x = 0; x < N; ++x) p.ws_acc[in_part(r, lane + 64 * x)] = acc[x];
       continue;
     }
     const int64_t o = pa_out_at(p, b, sq, t, h);
@@ -556,8 +557,37 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
     wait_vmcnt<0>();
     __syncthreads();
     for (int g = w; g < nrow; g += NW)
-      pa_again<elem, D, DA_BS, 16, KV8, true, false>(p, x.b, x.sq, x.kvh, x.part, 0, 0, bad & (1u << g), x.blocks, x.blocks.n_all);
+      pa_again<elem, D, DA_BS, 16, KV8, true, false, false>(p, x.b, x.sq, x.kvh, x.part, 0, 0, bad & (1u << g), x.blocks, x.blocks.n_all);
   }
+}
+
+// A row as two lanes hold it (pa_in_part), times inv, to out; the two (hf 0 and 1) trade fours, so that each
+// stores eight values of 16 bits.
+template <class E, int D>
+__device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x16 (&acc)[D / 32], float inv, int hf) {
+  if (p.out_dt == LA_F32) {
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(float4 *)((float *)p.out + o + 32 * dt + 8 * i + 4 * hf) =
+            float4{acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv, acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv};
+    return;
+  }
+  typedef E x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      uint2 y[2];
+#pragma unroll
+      for (int z = 0; z < 2; ++z)
+        y[z] = __builtin_bit_cast(uint2, x4{(E)(acc[dt][4 * (i + z)] * inv), (E)(acc[dt][4 * (i + z) + 1] * inv),
+                                            (E)(acc[dt][4 * (i + z) + 2] * inv), (E)(acc[dt][4 * (i + z) + 3] * inv)});
+      const auto a = __builtin_amdgcn_permlane32_swap(y[0].x, y[1].x, false, false);
+      const auto c = __builtin_amdgcn_permlane32_swap(y[0].y, y[1].y, false, false);
+      *(uint4 *)((E *)p.out + o + 32 * dt + 8 * (i + hf)) = uint4{a[0], c[0], a[1], c[1]};
+    }
 }
 
 // bf16 / fp16 rows: four waves of 32 rows, three workgroups a CU, and the products and registers of
@@ -620,6 +650,7 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
     // fp8: codes of a block, a wave's own rows, and (lanes below 16) the keys' scales
     float ks = 0.f, vs = 0.f;
     auto dma_codes = [&](int j) __attribute__((always_inline)) {
+      const int lane = pa_lane();
       if ((uint32_t)(j - rows.jb) >= (uint32_t)PaRows<EVEN>::SPAN) rows.look(p, x.kvh, j);
       rows.template load<D, 1>(kp, j, lds0 + 4 * BLK + sw * D, lane, [](int) { return 0; });
       rows.template load<D, 1>(vp, j, lds0 + 5 * BLK + sw * D, lane, [](int) { return 0; });
@@ -628,6 +659,7 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
       vs = v_scale[at];
     };
     auto widen = [&]() __attribute__((always_inline)) {
+      const int lane = pa_lane();
 #pragma unroll
       for (int v = 0; v < 2; ++v)
 #pragma unroll
@@ -770,7 +802,6 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
         lds_barrier();  // the block before is read
         widen();
         lds_barrier();  // this one is there, and its codes are read
-        if (i + 1 < j1) dma_codes(next);
       } else {
         wait_vmcnt<NX>();
         lds_barrier();  // K of this block has landed for every wave, V of the one before is read
@@ -781,7 +812,11 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
         settle_max(j, st, largest(st));
         weigh(0, st[0], pw);
       }
-      if constexpr (!KV8) {
+      if constexpr (KV8) {
+        // (here: registers are short before, and a reload of one waits for loads issued before it: chunks of
+        // four prompts over fp8 caches take 260 us, and 290 with these at the block's beginning)
+        if (i + 1 < j1) dma_codes(next);
+      } else {
         if (i + 1 < j1) wait_vmcnt<NX>();
         else wait_vmcnt<0>();
         lds_barrier();  // V of this block has landed, its K is read
@@ -814,50 +849,26 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
     for (int i = 0; i < 16; ++i) sum = __builtin_fmaf(acc[dt][i], 0.f, sum);
   const uint64_t bad = __ballot(sum != 0.f && l < __int_as_float(0x7f800000));  // (sum: NaN)
   // register i of dim tile dt holds dim 32 dt + 8 (i / 4) + 4 hf + i % 4
-  if (live && x.part >= 0) {
-    const int64_t pi = x.part + r_mine - x.r0;
+  if (x.part >= 0) {
+    const int64_t pi = x.part + r_first - x.r0;  // (room for whole waves)
     if (hf == 0) {
-      p.ws_ml[2 * pi] = m == pa_ninf() ? m : -nmu;
-      p.ws_ml[2 * pi + 1] = l;
+      p.ws_ml[2 * (pi + r32)] = m == pa_ninf() ? m : -nmu;
+      p.ws_ml[2 * (pi + r32) + 1] = l;
     }
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *(float4 *)(p.ws_acc + pi * D + 32 * dt + 8 * i + 4 * hf) =
+        *(float4 *)(p.ws_acc + pi * D + (dt * 4 + i) * 256 + 4 * lane) =
             float4{acc[dt][4 * i], acc[dt][4 * i + 1], acc[dt][4 * i + 2], acc[dt][4 * i + 3]};
   } else if (live) {
     const bool none = l == 0.f;  // no key seen
-    const float inv = none ? 0.f : 1.f / l;
-    const int64_t o = pa_out_at(p, x.b, x.sq, t, h);
-    if (p.out_dt == LA_F32) {
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(float4 *)((float *)p.out + o + 32 * dt + 8 * i + 4 * hf) =
-              float4{acc[dt][4 * i] * inv, acc[dt][4 * i + 1] * inv, acc[dt][4 * i + 2] * inv, acc[dt][4 * i + 3] * inv};
-    } else {  // the halves of a row trade fours, so that a lane stores eight values
-      typedef elem x4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          uint2 y[2];
-#pragma unroll
-          for (int z = 0; z < 2; ++z)
-            y[z] = __builtin_bit_cast(uint2, x4{(elem)(acc[dt][4 * (i + z)] * inv), (elem)(acc[dt][4 * (i + z) + 1] * inv),
-                                                (elem)(acc[dt][4 * (i + z) + 2] * inv), (elem)(acc[dt][4 * (i + z) + 3] * inv)});
-          const auto a = __builtin_amdgcn_permlane32_swap(y[0].x, y[1].x, false, false);
-          const auto c = __builtin_amdgcn_permlane32_swap(y[0].y, y[1].y, false, false);
-          *(uint4 *)((elem *)p.out + o + 32 * dt + 8 * (i + hf)) = uint4{a[0], c[0], a[1], c[1]};
-        }
-    }
+    pa_rows_out<elem, D>(p, pa_out_at(p, x.b, x.sq, t, h), acc, none ? 0.f : 1.f / l, hf);
     if (p.lse && hf == 0) p.lse[pa_lse_at(p, x.b, x.sq, t, h)] = none ? pa_ninf() : (__log2f(l) - nmu) * PA_LN2;  // (as rounded in the weights)
   }
   if (bad != 0) {
     const int lim_hi = p.causal ? x.sq.lk - x.sq.lq + min(r_first + 31, nrow - 1) / G : x.sq.lk - 1;
-    pa_again<elem, D, DA_BS, 32, KV8, false, (!KV8 && T::BIAS > 0.f)>(p, x.b, x.sq, x.kvh, x.part, x.r0, r_first,
+    pa_again<elem, D, DA_BS, 32, KV8, false, (!KV8 && T::BIAS > 0.f), true>(p, x.b, x.sq, x.kvh, x.part, x.r0, r_first,
                                                                      (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
                                                                      x.blocks, lim_hi / DA_BS);
   }
@@ -1047,21 +1058,18 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
       }
       if (bad != 0) {
         bad |= bad >> 32;
-        pa_again<float, D, BS, 16, false, false, false>(p, b, sq, kvh, part, r0, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
+        pa_again<float, D, BS, 16, false, false, false, false>(p, b, sq, kvh, part, r0, r_first, (uint32_t)((bad | (bad >> 16)) & __ballot(live) & 0xffffu),
                                                        blocks, lim_hi / BS);
       }
     }
   } while (pa_next<R, false>(&s_walk));
 }
 
-// Joins the parts of the tile that began last in a workgroup's stretch: a row by D / 4 lanes.
+// Joins the parts of tiles that lie row by row: a row by D / 4 lanes.
 template <int D, int R>
-__global__ __launch_bounds__(256) void paged_join_kernel(PaKP p) {
+__device__ __forceinline__ void pa_join_rows(const PaKP &p, const int4 &note, int own, int kvh) {
   constexpr int LR = D / 4, RW = 256 / LR;  // lanes of a row, rows at a time
-  const int wg = blockIdx.x;
-  const int4 note = p.ws_join[wg];
-  if (note.z == 0) return;
-  const int kvh = wg % p.Hkv, b = note.x, G = p.G, own = note.w ? note.w - 1 : wg / p.Hkv;
+  const int b = note.x, G = p.G;
   const PaSeq sq = pa_seq(p, b);
   const int nrow = sq.lq * G, r0 = note.y * R, lane = threadIdx.x % LR;
   for (int r = r0 + blockIdx.y * RW + threadIdx.x / LR; r < min(nrow, r0 + R); r += gridDim.y * RW) {
@@ -1109,6 +1117,64 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaKP p) {
   }
 }
 
+// The same where parts lie as waves hold them: four waves of 32 rows.
+template <class E, int D>
+__device__ __forceinline__ void pa_join_many(const PaKP &p, const int4 &note, int own, int kvh) {
+  constexpr int ND = D / 32;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5, r32 = lane & 31;
+  const PaSeq sq = pa_seq(p, note.x);
+  const int nrow = sq.lq * p.G, r_first = note.y * 128 + 32 * w;
+  if (r_first >= nrow) return;
+  const int r = min(r_first + r32, nrow - 1);
+  f32x16 acc[ND];
+  float m = pa_ninf(), l = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+  for (int x = 0; x < note.z; ++x) {  // (parts in their order)
+    const int64_t pi = pa_part(p, own + x, kvh, x == 0, false) + 32 * w;
+    const float2 ml = *(const float2 *)(p.ws_ml + 2 * (pi + r32));
+    float4 v[ND * 4];
+#pragma unroll
+    for (int i = 0; i < ND * 4; ++i) v[i] = *(const float4 *)(p.ws_acc + pi * D + i * 256 + 4 * lane);
+    const bool empty = ml.x == pa_ninf() && ml.y == 0.f;  // (no key seen)
+    const float mn = fmaxf(m, ml.x), from = mn == pa_ninf() ? 0.f : mn;
+    const float f = m == pa_ninf() && l == 0.f ? 0.f : fast_exp2(m - from), g = empty ? 0.f : fast_exp2(ml.x - from);
+    m = mn;
+    l = l * f + (empty ? 0.f : ml.y * g);
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y[4] = {v[4 * dt + i].x, v[4 * dt + i].y, v[4 * dt + i].z, v[4 * dt + i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[dt][4 * i + e] = acc[dt][4 * i + e] * f + (empty ? 0.f : y[e] * g);
+      }
+  }
+  const int t = r / p.G, h = kvh * p.G + r % p.G;
+  const bool none = l == 0.f;
+  const int64_t o = pa_out_at(p, note.x, sq, t, h);
+  if (r_first + r32 >= nrow) return;
+  pa_rows_out<E, D>(p, o, acc, none ? 0.f : 1.f / l, hf);
+  if (p.lse && hf == 0) p.lse[pa_lse_at(p, note.x, sq, t, h)] = none ? pa_ninf() : (m + __log2f(l)) * PA_LN2;
+}
+
+// Joins the tile that began last in a workgroup's stretch, if others have parts of it.
+template <class E, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(PaKP p) {
+  const int wg = blockIdx.x;
+  const int4 note = p.ws_join[wg];
+  if (note.z == 0) return;
+  const int kvh = wg % p.Hkv, own = note.w ? note.w - 1 : wg / p.Hkv;
+  if constexpr (sizeof(E) == 4) {
+    pa_join_rows<D, 64>(p, note, own, kvh);
+  } else {
+    if (note.w) pa_join_rows<D, PA_FEW>(p, note, own, kvh);
+    else pa_join_many<E, D>(p, note, own, kvh);
+  }
+}
+
 // ------------------------------------------------------------------ host ----
 struct PaPlan {
   int64_t W = 1, rows = 128, least = 0, few_parts = 0;
@@ -1133,7 +1199,7 @@ static PaPlan pa_plan(const la_paged_attn_args *a) {
     pl.W = 2;
     pl.join = false;
   }
-  pl.rows = std::min(R, rows);
+  pl.rows = std::min(R, ceil_div(rows, 32) * 32);  // (whole waves)
   pl.few_parts = pl.W * a->Hkv * 2 * pl.rows;
   const int64_t parts = pl.join ? pl.few_parts + (f32 ? 0 : pl.W * a->Hkv * 2 * PA_FEW) : 0;
   pl.ml = ((size_t)parts * 2 * sizeof(float) + 255) / 256 * 256;
@@ -1163,8 +1229,8 @@ static int pa_check(const la_paged_attn_args *a) {
 }
 
 template <class K>
-static int pa_launch(K kernel, int64_t wgs, const PaKP &p, hipStream_t st) {
-  kernel<<<dim3((uint32_t)wgs), dim3(256), 0, st>>>(p);
+static int pa_launch(K kernel, int64_t wgs, const PaKP &p, hipStream_t st, int y = 1) {
+  kernel<<<dim3((uint32_t)wgs, y), dim3(256), 0, st>>>(p);
   LA_LAUNCHED();
   return LA_OK;
 }
@@ -1241,14 +1307,8 @@ extern "C" int la_paged_attention(const la_paged_attn_args *args, void *stream) 
   else if (a->dtype == LA_BF16) rc = d128 ? pa_launch16<DaBf16, 128>(kv8, even, wgs, p, st) : pa_launch16<DaBf16, 64>(kv8, even, wgs, p, st);
   else rc = d128 ? pa_launch16<DaF16, 128>(kv8, even, wgs, p, st) : pa_launch16<DaF16, 64>(kv8, even, wgs, p, st);
   if (rc != LA_OK || !pl.join) return rc;
-  const dim3 grid((uint32_t)wgs, pl.rows > 32 ? 4 : 1);
-  if (a->dtype == LA_F32) {
-    if (d128) paged_join_kernel<128, 64><<<grid, 256, 0, st>>>(p);
-    else paged_join_kernel<64, 64><<<grid, 256, 0, st>>>(p);
-  } else {
-    if (d128) paged_join_kernel<128, 128><<<grid, 256, 0, st>>>(p);
-    else paged_join_kernel<64, 128><<<grid, 256, 0, st>>>(p);
-  }
-  LA_LAUNCHED();
-  return LA_OK;
+  if (a->dtype == LA_F32) return d128 ? pa_launch(paged_join_kernel<float, 128>, wgs, p, st, 4) : pa_launch(paged_join_kernel<float, 64>, wgs, p, st, 4);
+  if (a->dtype == LA_BF16) return d128 ? pa_launch(paged_join_kernel<__bf16, 128>, wgs, p, st) : pa_launch(paged_join_kernel<__bf16, 64>, wgs, p, st);
+  return d128 ? pa_launch(paged_join_kernel<_Float16, 128>, wgs, p, st) : pa_launch(paged_join_kernel<_Float16, 64>, wgs, p, st);
 }
+
