@@ -77,10 +77,36 @@ __device__ __forceinline__ PaTiles pa_tiles(const PaKP &p, const PaSeq &s, bool 
   return t;
 }
 
-__device__ __forceinline__ int64_t pa_shfl(int64_t x, int lane) { return __shfl((long long)x, lane, 64); }
 __device__ __forceinline__ int64_t pa_uniform(int64_t x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
   return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t pa_lane_value(int64_t x, int lane) {  // (the same lane for all)
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)x >> 32), lane);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+// Sum over the lanes up to this one, on the vector unit (shuffles go through LDS: a call's first
+// microsecond is such sums).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t pa_dpp(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)((uint64_t)x >> 32), CTRL, ROWS, 0xf, false);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int64_t pa_scan(int64_t x) {
+  x += pa_dpp<0x111, 0xf>(x);  // 1, 2, 4, 8 lanes up within rows of 16
+  x += pa_dpp<0x112, 0xf>(x);
+  x += pa_dpp<0x114, 0xf>(x);
+  x += pa_dpp<0x118, 0xf>(x);
+  x += pa_dpp<0x142, 0xa>(x);  // lane 15 of a row to the next, then lane 31 to the upper half
+  x += pa_dpp<0x143, 0xc>(x);
+  return x;
+}
+// a / b, both below 2^53, a >= 0, b > 0
+__device__ __forceinline__ int64_t pa_div(int64_t a, int64_t b) {
+  int64_t q = (int64_t)((double)a / (double)b);
+  const int64_t r = a - q * b;
+  return r < 0 ? q - 1 : r >= b ? q + 1 : q;
 }
 
 // A line: its length, that of a stretch (but of the last), its first workgroup.
@@ -97,26 +123,20 @@ struct PaStretch {
   int32_t b, i, few;
 };
 template <int R, bool FEW>
-__device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w) {
+__device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w, PaSeq &seq, PaTiles &tiles) {
   const int lane = threadIdx.x & 63;
-  auto cost = [&](int b, bool few) -> int64_t {
-    if (b >= p.B) return 0;
-    const PaTiles t = pa_tiles<R, FEW>(p, pa_seq(p, b), few);
-    return t.upto(t.n);
+  auto cost = [&](const PaSeq &q, int b, bool few) -> int64_t {
+    const PaTiles t = pa_tiles<R, FEW>(p, q, few);
+    return b < p.B ? t.upto(t.n) : 0;
   };
-  const int64_t mine_many = cost(lane, false), mine_few = FEW ? cost(lane, true) : 0;
-  int64_t many = mine_many, few = mine_few;
-  for (int b = 64 + lane; b < p.B; b += 64) {
-    many += cost(b, false);
-    if (FEW) few += cost(b, true);
+  PaSeq mine = pa_seq(p, min(lane, p.B - 1));
+  int64_t sum_many = pa_scan(cost(mine, lane, false)), sum_few = FEW ? pa_scan(cost(mine, lane, true)) : 0;
+  int64_t many = pa_lane_value(sum_many, 63), few = pa_lane_value(sum_few, 63);
+  for (int b0 = 64; b0 < p.B; b0 += 64) {
+    const PaSeq q = pa_seq(p, min(b0 + lane, p.B - 1));
+    many += pa_lane_value(pa_scan(cost(q, b0 + lane, false)), 63);
+    if (FEW) few += pa_lane_value(pa_scan(cost(q, b0 + lane, true)), 63);
   }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    many += __shfl_xor((long long)many, o, 64);
-    if (FEW) few += __shfl_xor((long long)few, o, 64);
-  }
-  many = pa_uniform(many);
-  few = pa_uniform(few);
   PaStretch s;
   s.left = 0;
   s.b = s.i = 0;
@@ -127,43 +147,46 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w) {
   s.line.all = s.few ? few : many;
   s.line.first = s.few ? wm : 0;
   const int places = s.few ? p.W - wm : max(wm, 1);
-  s.line.quota = max((s.line.all + places - 1) / places, p.least);
+  s.line.quota = max(pa_div(s.line.all + places - 1, places), p.least);
   s.off = (w - s.line.first) * s.line.quota;
   if (s.off >= s.line.all) return s;
   s.left = min(s.line.quota, s.line.all - s.off);
   s.pos = s.off;
+  int64_t sum = s.few ? sum_few : sum_many;
   for (int b0 = 0;; b0 += 64) {
-    const int64_t c = b0 == 0 ? (s.few ? mine_few : mine_many) : cost(b0 + lane, s.few);
-    int64_t sum = c;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t y = __shfl_up((long long)sum, o, 64);
-      if (lane >= o) sum += y;
+    if (b0 > 0) {
+      mine = pa_seq(p, min(b0 + lane, p.B - 1));
+      sum = pa_scan(cost(mine, b0 + lane, s.few));
     }
-    const int64_t here = pa_uniform(pa_shfl(sum, 63));
+    const int64_t here = pa_lane_value(sum, 63);
     if (s.off >= here && b0 + 64 < p.B) {
       s.off -= here;
       continue;
     }
     const int at = __ffsll((unsigned long long)__ballot(sum > s.off)) - 1;  // (off is below the line's end)
     s.b = __builtin_amdgcn_readfirstlane(b0 + at);
-    s.off -= pa_uniform(pa_shfl(sum - c, at));
+    if (at > 0) s.off -= pa_lane_value(sum, at - 1);
+    seq.lq = __builtin_amdgcn_readlane(mine.lq, at);
+    seq.lk = __builtin_amdgcn_readlane(mine.lk, at);
+    seq.q0 = pa_lane_value(mine.q0, at);
     break;
   }
-  const PaTiles t = pa_tiles<R, FEW>(p, pa_seq(p, s.b), s.few);
-  // upto(i) <= off < upto(i + 1): the quadratic's root, and what its rounding may have missed
-  int64_t i;
-  if (t.step == 0) {
-    i = s.off / t.a;
-  } else {
-    const double h = (double)t.a + 0.5 * (double)t.step;
-    i = (int64_t)((sqrt(h * h + 2.0 * (double)t.step * (double)s.off) - h) / (double)t.step);
+  tiles = pa_tiles<R, FEW>(p, seq, s.few);
+  if (tiles.n > 1) {
+    // upto(i) <= off < upto(i + 1): the quadratic's root, and what its rounding may have missed
+    int64_t i;
+    if (tiles.step == 0) {
+      i = pa_div(s.off, tiles.a);
+    } else {
+      const double h = (double)tiles.a + 0.5 * (double)tiles.step;
+      i = (int64_t)((sqrt(h * h + 2.0 * (double)tiles.step * (double)s.off) - h) / (double)tiles.step);
+    }
+    i = min(max(i, (int64_t)0), (int64_t)tiles.n - 1);
+    while (i > 0 && tiles.upto(i) > s.off) --i;
+    while (i + 1 < tiles.n && tiles.upto(i + 1) <= s.off) ++i;
+    s.i = __builtin_amdgcn_readfirstlane((int32_t)i);
+    s.off = pa_uniform(s.off - tiles.upto(i));
   }
-  i = min(max(i, (int64_t)0), (int64_t)t.n - 1);
-  while (i > 0 && t.upto(i) > s.off) --i;
-  while (i + 1 < t.n && t.upto(i + 1) <= s.off) ++i;
-  s.i = __builtin_amdgcn_readfirstlane((int32_t)i);
-  s.off = pa_uniform(s.off - t.upto(i));
   s.left = pa_uniform(s.left);
   s.pos -= s.off;
   return s;

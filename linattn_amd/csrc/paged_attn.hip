@@ -181,13 +181,16 @@ template <int R, bool FEW>
 __device__ __forceinline__ bool pa_begin(PaWalk *walk) {
   const PaKP &p = pa_args();
   PaWalk w;
-  w.s = pa_stretch<R, FEW>(p, blockIdx.x / (uint32_t)p.Hkv);
+  PaTiles t;
+  w.s = pa_stretch<R, FEW>(p, blockIdx.x / (uint32_t)p.Hkv, w.seq, t);
   if (w.s.left == 0) {
     if (threadIdx.x == 0) p.ws_join[blockIdx.x] = int4{0, 0, 0, 0};
     return false;
   }
-  pa_load<R, FEW>(p, w);
-  w.since = w.s.pos % w.s.line.quota;
+  w.a = t.a;
+  w.step = t.step;
+  w.n = t.n;
+  w.since = w.s.off == 0 ? 0 : w.s.pos - pa_div(w.s.pos, w.s.line.quota) * w.s.line.quota;
   if (threadIdx.x == 0) *walk = w;
   __syncthreads();
   return true;
@@ -206,7 +209,7 @@ __device__ __forceinline__ bool pa_next(PaWalk *walk) {
   if (threadIdx.x == 0) {
     const int64_t own = blockIdx.x / (uint32_t)p.Hkv - w.s.line.first;
     if (!more) {
-      const int parts = w.s.off == 0 && upto < cost ? (int)((w.s.pos + cost - 1) / w.s.line.quota - own) + 1 : 0;
+      const int parts = w.s.off == 0 && upto < cost ? (int)(pa_div(w.s.pos + cost - 1, w.s.line.quota) - own) + 1 : 0;
       p.ws_join[blockIdx.x] = int4{w.s.b, w.s.i, parts, w.s.few ? 1 + (int)own : 0};
     } else {
       w.s.off = 0;
@@ -250,10 +253,14 @@ __device__ __forceinline__ PaPiece pa_piece(const PaKP &p, const PaWalk *walk) {
   const int n_all = lim < 0 ? 0 : lim / BS + 1;
   const int64_t cost = w.a + w.step * (w.s.i + 1), upto = min(cost, w.s.off + w.s.left);
   x.blocks.n_all = __builtin_amdgcn_readfirstlane(n_all);
-  x.blocks.j0 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, w.s.off, cost));
-  x.blocks.j1 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, upto, cost));
-  const double turns = (double)w.since / (double)cost;
-  x.blocks.turn = TURN ? __builtin_amdgcn_readfirstlane(max(0, min((int)((turns - floor(turns)) * n_all), n_all - 1))) : 0;
+  x.blocks.j0 = x.blocks.turn = 0;
+  x.blocks.j1 = x.blocks.n_all;
+  if (w.s.off > 0) x.blocks.j0 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, w.s.off, cost));
+  if (upto < cost) x.blocks.j1 = __builtin_amdgcn_readfirstlane(pa_blocks(n_all, upto, cost));
+  if (TURN && w.since > 0) {
+    const double turns = (double)w.since / (double)cost;
+    x.blocks.turn = __builtin_amdgcn_readfirstlane(max(0, min((int)((turns - floor(turns)) * n_all), n_all - 1)));
+  }
   x.part = pa_uniform(w.s.off == 0 && upto == cost ? -1 : pa_part(p, blockIdx.x / (uint32_t)p.Hkv - w.s.line.first, x.kvh, w.s.off == 0, w.s.few));
   return x;
 }
@@ -881,15 +888,14 @@ __global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP) {
   __shared__ PaWalk s_walk;
   __shared__ uint32_t s_bad;
   static_assert(sizeof(uint16_t) * 3 * DA_BS * D <= sizeof(smem), "K and V");
-  {
-    const PaKP &p = pa_args();
-    pa_rest<D>(p, (int)(blockIdx.x % (uint32_t)p.Hkv));
+  if (pa_begin<128, true>(&s_walk)) {
+    do {
+      if (__builtin_amdgcn_readfirstlane(s_walk.s.few)) pa_few<T, D, KV8, EVEN>(&s_walk, (char *)smem, s_scale, &s_bad);
+      else pa_many<T, D, KV8, EVEN>(&s_walk, smem, s_scale);
+    } while (pa_next<128, true>(&s_walk));
   }
-  if (!pa_begin<128, true>(&s_walk)) return;
-  do {
-    if (__builtin_amdgcn_readfirstlane(s_walk.s.few)) pa_few<T, D, KV8, EVEN>(&s_walk, (char *)smem, s_scale, &s_bad);
-    else pa_many<T, D, KV8, EVEN>(&s_walk, smem, s_scale);
-  } while (pa_next<128, true>(&s_walk));
+  const PaKP &p = pa_args();
+  pa_rest<D>(p, (int)(blockIdx.x % (uint32_t)p.Hkv));
 }
 
 // fp32 rows: four waves of 16 rows on 16x16x4 products, blocks of 32 keys (dense_attn_f32_kernel's),
@@ -903,11 +909,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane >> 4, ri = lane & 15;
   const int G = p.G;
-  pa_rest<D>(p, blockIdx.x % (uint32_t)p.Hkv);
-  if (!pa_begin<R, false>(&s_walk)) return;
+  bool more = pa_begin<R, false>(&s_walk);
   auto swz_k = [](int r) { return 2 * (r & 7); };
   auto swz_v = [](int r) { return 4 * ((r >> 2) & 3); };
-  do {
+  for (; more; more = pa_next<R, false>(&s_walk)) {
     const PaPiece x = pa_piece<R, BS, true>(p, &s_walk);
     const PaSeq sq = x.sq;
     const PaBlocks blocks = x.blocks;
@@ -1062,7 +1067,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
                                                        blocks, lim_hi / BS);
       }
     }
-  } while (pa_next<R, false>(&s_walk));
+  }
+  pa_rest<D>(p, (int)(blockIdx.x % (uint32_t)p.Hkv));
 }
 
 // Joins the parts of tiles that lie row by row: a row by D / 4 lanes.
@@ -1075,19 +1081,20 @@ __device__ __forceinline__ void pa_join_rows(const PaKP &p, const int4 &note, in
   for (int r = r0 + blockIdx.y * RW + threadIdx.x / LR; r < min(nrow, r0 + R); r += gridDim.y * RW) {
     float m = pa_ninf(), l = 0.f;
     float4 acc{0.f, 0.f, 0.f, 0.f};
-    // (parts in their order, four on their way at a time)
-    for (int i0 = 0; i0 < note.z; i0 += 4) {
-      float2 ml[4];
-      float4 v[4];
+    // (parts in their order, as many on their way at a time as there may be: a row is bound by this)
+    constexpr int AHEAD = 8;
+    for (int i0 = 0; i0 < note.z; i0 += AHEAD) {
+      float2 ml[AHEAD];
+      float4 v[AHEAD];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < AHEAD; ++i) {
         const int x = min(i0 + i, note.z - 1);
         const int64_t pi = pa_part(p, own + x, kvh, x == 0, note.w != 0) + r - r0;
         ml[i] = *(const float2 *)(p.ws_ml + 2 * pi);
         v[i] = *(const float4 *)(p.ws_acc + pi * D + 4 * lane);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < AHEAD; ++i) {
         if (i0 + i >= note.z || (ml[i].x == pa_ninf() && ml[i].y == 0.f)) continue;  // (empty: no key seen)
         const float mn = fmaxf(m, ml[i].x), from = mn == pa_ninf() ? 0.f : mn;
         const float f = m == pa_ninf() && l == 0.f ? 0.f : fast_exp2(m - from), g = fast_exp2(ml[i].x - from);
