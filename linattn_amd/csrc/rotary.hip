@@ -15,7 +15,7 @@ struct RoKP {
   void *q_out, *k_out;
   int64_t tokens, T;
   int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, qo_sb, qo_sh, qo_st, ko_sb, ko_sh, ko_st;
-  int32_t Hq, Hkv, D, units, ts, hs, per;  // per: heads of a workgroup
+  int32_t Hq, Hkv, D, units, ts, hs;
 };
 
 template <class E, int V>
@@ -25,8 +25,7 @@ __global__ __launch_bounds__(RO_NT) void rotary_kernel(RoKP p) {
   const int tid = threadIdx.x, n = p.an.n;
   const int64_t tok0 = (int64_t)blockIdx.x * p.ts;
   const int slot = tid / p.units, u = tid - slot * p.units;
-  const int ti = slot / p.hs, h0 = (int)blockIdx.y * p.per + slot % p.hs;
-  const int H = min((int)(blockIdx.y + 1) * p.per, p.Hq + p.Hkv);
+  const int ti = slot / p.hs, h0 = slot % p.hs, H = p.Hq + p.Hkv;
   const int64_t tok = tok0 + ti, b = tok / p.T, t = tok - b * p.T;
   const bool live = ti < p.ts && tok < p.tokens;
   const U unit(u, p.D, n, p.an.interleaved);
@@ -84,11 +83,10 @@ static int ro_launch(RoKP p, hipStream_t st) {
   p.ts = (int)std::min<int64_t>(std::max(1, 4 * slots / H), std::max<int64_t>(1, p.tokens / (2 * num_cus())));
   p.ts = std::min(p.ts, slots);
   p.hs = std::min(H, slots / p.ts);
-  p.per = H;
   const int64_t wgs = ceil_div(p.tokens, p.ts);
   LA_REQUIRE(grid_fits(wgs, RO_NT), "la_rotary: too many tokens");
   const size_t lds = (size_t)p.ts * p.an.n * sizeof(float2);
-  rotary_kernel<E, V><<<dim3((uint32_t)wgs, (uint32_t)ceil_div(H, p.per)), RO_NT, lds, st>>>(p);
+  rotary_kernel<E, V><<<dim3((uint32_t)wgs), RO_NT, lds, st>>>(p);
   LA_LAUNCHED();
   return LA_OK;
 }

@@ -21,7 +21,7 @@ struct RaKP {
   int64_t B, T;  // batched: T tokens of each sequence; packed: T rows
   int64_t q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, o_sb, o_sh, o_st;
   int64_t n_phys, pt_sb, m_sb, m_sh, m_sp, m_sd, n_pages, s_stride;
-  int32_t Hq, Hkv, D, units, lanes, ts, hs, per;
+  int32_t Hq, Hkv, D, units, lanes, ts, hs;
   int32_t pool_page, pt_pages, meta_page, zero_rest, fp8;
   int64_t blocks;  // (with bounds)
 };
@@ -105,8 +105,7 @@ __device__ __forceinline__ void ra_store(const RaKP &p, const RoUnit<E, V> &unit
   if (unit.oa == 0) scales[row * p.s_stride] = scale;
 }
 
-// Rows r0, r0 + step, .. below R of one token: heads of q, then of k, then of v.  `first` says which
-// head of q (and of k and v) row 0 (and the first after q's, ..) is, nq and nkv how many.
+// Row r of a token: heads of q, then of k, then of v.
 template <class E, int V>
 __device__ __forceinline__ const E *ra_source(const RaKP &p, int b, int t, int r) {
   if (r < p.Hq) return (const E *)p.q + b * p.q_sb + t * p.q_st + r * p.q_sh;
@@ -115,8 +114,8 @@ __device__ __forceinline__ const E *ra_source(const RaKP &p, int b, int t, int r
   return (const E *)p.v_new + b * p.v_sb + t * p.v_st + (r - p.Hkv) * p.v_sh;
 }
 
-// Without page bounds: a workgroup takes `ts` tokens, packed or batched, as they lie, and `per`
-// of each token's rows (heads of q, then of k, then of v), `hs` at a time.
+// Without page bounds: a workgroup takes `ts` tokens, packed or batched, as they lie, and each
+// token's rows (heads of q, then of k, then of v), `hs` at a time.
 template <class E, int V>
 __global__ __launch_bounds__(RO_NT) void rotary_append_kernel(RaKP p) {
   typedef RoUnit<E, V> U;
@@ -126,8 +125,7 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_kernel(RaKP p) {
   const int64_t tokens = p.cu ? p.T : p.B * p.T, tok0 = (int64_t)blockIdx.x * p.ts;
   const int count = (int)min((int64_t)p.ts, tokens - tok0);
   const int slot = tid / p.lanes, u = tid - slot * p.lanes;
-  const int ti = slot / p.hs, r0 = (int)blockIdx.y * p.per + slot % p.hs;
-  const int R = min((int)(blockIdx.y + 1) * p.per, p.Hq + 2 * p.Hkv);
+  const int ti = slot / p.hs, r0 = slot % p.hs, R = p.Hq + 2 * p.Hkv;
   const bool mine = u < p.units;
   const U unit(mine ? u : 0, p.D, n, p.an.interleaved);
   // (rows do not wait for what their tokens are)
@@ -351,10 +349,9 @@ static int ra_launch(RaKP p, hipStream_t st) {
   p.ts = (int)std::min<int64_t>(std::max(1, 4 * slots / R), std::max<int64_t>(1, tokens / (2 * num_cus())));
   p.ts = std::min(p.ts, slots);
   p.hs = std::min(R, slots / p.ts);
-  p.per = R;
   const int64_t wgs = ceil_div(tokens, p.ts);
   LA_REQUIRE(grid_fits(wgs, RO_NT), "la_rotary_append: too many tokens");
-  rotary_append_kernel<E, V><<<dim3((uint32_t)wgs, (uint32_t)ceil_div(R, p.per)), RO_NT, p.ts * turns, st>>>(p);
+  rotary_append_kernel<E, V><<<dim3((uint32_t)wgs), RO_NT, p.ts * turns, st>>>(p);
   LA_LAUNCHED();
   return LA_OK;
 }
@@ -409,10 +406,14 @@ extern "C" int la_rotary_append(const la_rotary_append_args *args, void *stream)
   const Cover kn = cover(a->k_new, a->kn_sb, a->kn_sh, a->kn_st, a->Hkv), vn = cover(a->v_new, a->vn_sb, a->vn_sh, a->vn_st, a->Hkv);
   const int64_t pool = a->n_phys * a->Hkv * a->pool_page;
   const Cover kp(a->k_pool, pool * a->D * psz), vp(a->v_pool, pool * a->D * psz);
+  const Cover::Dim each{a->s_stride * 4, pool};
+  const Cover ks(fp8 ? a->k_scale : nullptr, 4, each), vs(fp8 ? a->v_scale : nullptr, 4, each);
   const bool in = a->q_out == a->q && a->o_sb == a->q_sb && a->o_sh == a->q_sh && a->o_st == a->q_st;
   LA_REQUIRE((in || !overlap(out, q)) && !overlap(out, kn) && !overlap(out, vn) && !overlap(out, kp) && !overlap(out, vp) &&
                  !overlap(kp, vp) && !overlap(kp, q) && !overlap(kp, kn) && !overlap(kp, vn) && !overlap(vp, q) &&
-                 !overlap(vp, kn) && !overlap(vp, vn),
+                 !overlap(vp, kn) && !overlap(vp, vn) && !overlap(ks, vs) && !overlap(ks, kp) && !overlap(ks, vp) &&
+                 !overlap(vs, kp) && !overlap(vs, vp) && !overlap(ks, out) && !overlap(vs, out) && !overlap(ks, q) &&
+                 !overlap(vs, q) && !overlap(ks, kn) && !overlap(vs, kn) && !overlap(ks, vn) && !overlap(vs, vn),
              "la_rotary_append: what is written shares memory with another argument");
   RaKP p{};
   p.an = RoAngles{a->rot_positions, a->axes, a->inv_freq, a->p_sa, a->p_sb, a->p_st, (int32_t)a->n, (int32_t)a->A,

@@ -67,12 +67,14 @@ def _positions(what: str, positions: torch.Tensor, axes: Optional[torch.Tensor],
 def _out_rows(what: str, name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty_like(x, memory_format=torch.contiguous_format)
-    if out is x:
-        return out
     if out.shape != x.shape or out.dtype != x.dtype or (out.shape[-1] > 1 and out.stride(-1) != 1):
         raise ValueError(f"{what}: {name} must have its input's shape and dtype, and contiguous rows")
     if out.data_ptr() != x.data_ptr():
         _apart(what, out, x)
+    elif any(s == 0 and d > 1 for s, d in zip(out.stride(), out.shape)):
+        raise ValueError(f"{what}: {name} holds some of its rows twice")
+    elif out is x:
+        return out
     elif out.numel() and any(a != b for a, b, d in zip(out.stride(), x.stride(), x.shape) if d > 1):
         raise ValueError(f"{what}: {name} shares memory with its input, but does not hold the same rows")
     return out

@@ -380,3 +380,22 @@ def test_captured_and_replayed(dev):
         for a, b in zip(eager, held):
             assert torch.equal(a, b), i
         pos.add_(1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_bounds_of_the_widest_heads(dev, dtype):
+    """512 values, all of them turned: the angles of 32 tokens are 64 KB."""
+    lq, before, page, Hq, Hkv, D, n = [70, 1], [10, 31], 32, 2, 1, 512, 256
+    q, k, v, kp, vp, table = _case(38, lq, before, page, Hq, Hkv, D, dtype)
+    freq, kp, vp = _freq(n), kp.to(dtype), vp.to(dtype)
+    b, t, ok, phys, slot, (wq, tq), (wk, tk) = _expect(q, k, v, kp, vp, table, before, lq, freq)
+    mn, mx = (_rand(s, 2, Hkv, 3, D, dtype=dtype) for s in (39, 40))
+    gk, gv, gmn, gmx = (x.to(dev) for x in (kp, vp, mn, mx))
+    gq = rotary_kv_append(q.to(dev), k.to(dev), v.to(dev), gk, gv, table.to(dev), _i32(before, dev), freq.to(dev),
+                          cu_seqlens=_i32([0, 70, 71], dev), page_min=gmn, page_max=gmx, page_size=page)
+    close(gq, wq, rounded(wq, tq, dtype), "q")
+    stored = gk[phys, :, slot].cpu()
+    close(stored, wk, rounded(wk, tk, dtype), "k")
+    assert torch.equal(gv[phys, :, slot].cpu(), v)
+    emn, emx = bounds(mn, mx, stored, b, t, ok, before, page)
+    assert torch.equal(gmn.cpu(), emn) and torch.equal(gmx.cpu(), emx)

@@ -222,3 +222,31 @@ def test_the_reference_turns():
     a, b = turn(z, p, f)[0], turn(z.flip(0), p + 5, f)[0]
     c, d = turn(z, p - p, f)[0], turn(z.flip(0), p - p + 5, f)[0]
     assert torch.allclose((a * b).sum(-1), (c * d).sum(-1), atol=1e-9)
+
+
+def test_outputs_that_are_inputs_hold_their_rows_once(as_gpu):
+    """In place: rows of unit stride, each once."""
+    for x in (torch.zeros(5, 64, 4).transpose(1, 2), torch.zeros(5, 1, 64).expand(5, 4, 64)):
+        with pytest.raises(ValueError):
+            rotary(x, None, _i32(5), torch.zeros(32), q_out=x)
+        with pytest.raises(ValueError):
+            rotary(torch.zeros(5, 4, 64), x, _i32(5), torch.zeros(32), k_out=x)
+        with pytest.raises(ValueError):
+            rotary_kv_append(x, torch.zeros(5, 2, 64), torch.zeros(5, 2, 64), P.clone(), P.clone(), _i32(2, 4), _i32(2),
+                             torch.zeros(32), cu_seqlens=_i32(3), q_out=x)
+
+
+def test_the_library_refuses_scales_over_others():
+    def with_scales():
+        a, base, far = _append_args()
+        a.pool_dtype, a.k_scale, a.v_scale = N.LA_FP8_E4M3, base + 20 * far, base + 21 * far
+        return a, base, far
+
+    rows = 6 * 2 * 16
+    for change in (dict(k_scale=lambda b, f: b + 4 * f + rows * 64 - 4), dict(v_scale=lambda b, f: b + 5 * f),
+                   dict(v_scale=lambda b, f: b + 20 * f + rows * 4 - 4), dict(k_scale=lambda b, f: b + 3 * f + 64),
+                   dict(v_scale=lambda b, f: b + f), dict(k_scale=lambda b, f: b + 2 * f + 128), dict(k_scale=lambda b, f: b)):
+        a, base, far = with_scales()
+        for name, x in change.items():
+            setattr(a, name, x(base, far))
+        assert "shares memory" in _refused("la_rotary_append", a), change
