@@ -31,13 +31,14 @@ struct PaKP {
   int4 *ws_join;          // [workgroup]: of the tile that begins last there: sequence, tile, parts (0: none), and
                           // 1 + the stretch's number where rows are few, else 0
   int64_t Tq, q_sb, q_sh, q_st, o_sb, o_sh, o_st, l_sb, l_sh, pt_sb, s_stride, n_phys;
-  int64_t least, few_parts;  // of a stretch; where the parts of few rows begin
+  int64_t least, least_few, few_parts;  // of a stretch, of few rows; where the parts of few rows begin
   int32_t B, G, Hq, Hkv, D, W, part_rows;  // W: workgroups of a KV head
   int32_t page, pt_pages, causal, out_dt, zero_rest;
   float qscale, thr_gap;
 };
 
-constexpr int PA_AHEAD = 256;  // what a tile's beginning and end cost, in keys (twelve prompts 264, 256 and 263 us at 160, 256, 600)
+// What a tile's beginning and end cost, in keys (twelve prompts 264, 256 and 263 us at 160, 256, 600).
+constexpr int PA_AHEAD = 256;
 
 struct PaSeq {
   int32_t lq, lk;
@@ -141,13 +142,14 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w, PaSeq &seq
   s.left = 0;
   s.b = s.i = 0;
   // places for tiles of many rows, by the share of the time (beside them, a block of few rows takes a
-  // little less than one of many: four such batches 587, 568 and 584 us together at 0.5, 0.7 and 1)
+  // little less than one of many: three mixed batches 707, 697, 702, 709 and 747 us together at 0.5,
+  // 0.65, 0.8, 1 and 1.3)
   const int wm = few == 0 ? p.W : many == 0 ? 0 : max(1, min(p.W - 1, (int)((double)p.W * (double)many / ((double)many + 0.7 * (double)few) + 0.5)));
   s.few = w >= wm && few > 0;
   s.line.all = s.few ? few : many;
   s.line.first = s.few ? wm : 0;
   const int places = s.few ? p.W - wm : max(wm, 1);
-  s.line.quota = max(pa_div(s.line.all + places - 1, places), p.least);
+  s.line.quota = max(pa_div(s.line.all + places - 1, places), s.few ? p.least_few : p.least);
   s.off = (w - s.line.first) * s.line.quota;
   if (s.off >= s.line.all) return s;
   s.left = min(s.line.quota, s.line.all - s.off);

@@ -1071,46 +1071,57 @@ __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
   pa_rest<D>(p, (int)(blockIdx.x % (uint32_t)p.Hkv));
 }
 
-// Joins the parts of tiles that lie row by row: a row by D / 4 lanes.
+// What D / 4 lanes hold of a row: the reference, the weights' sum and four values each.
+struct PaState {
+  float m, l;
+  float4 acc;
+  __device__ __forceinline__ PaState() : m(pa_ninf()), l(0.f), acc{0.f, 0.f, 0.f, 0.f} {}
+  __device__ __forceinline__ void add(float2 ml, const float4 &v) {
+    if (ml.x == pa_ninf() && ml.y == 0.f) return;  // (empty: no key seen)
+    const float mn = fmaxf(m, ml.x), from = mn == pa_ninf() ? 0.f : mn;
+    const float f = m == pa_ninf() && l == 0.f ? 0.f : fast_exp2(m - from), g = fast_exp2(ml.x - from);
+    m = mn;
+    l = l * f + ml.y * g;
+    acc.x = acc.x * f + v.x * g;
+    acc.y = acc.y * f + v.y * g;
+    acc.z = acc.z * f + v.z * g;
+    acc.w = acc.w * f + v.w * g;
+  }
+};
+
+// Joins the parts of tiles that lie row by row: a row by D / 4 lanes, or, of more than 16 parts
+// (few tiles, each shared by many workgroups), by all, which take the parts in turn and join in LDS (with
+// more than 4 by all, fp32 chunks of 8 parts take 202 us, not 177).
 template <int D, int R>
 __device__ __forceinline__ void pa_join_rows(const PaKP &p, const int4 &note, int own, int kvh) {
-  constexpr int LR = D / 4, RW = 256 / LR;  // lanes of a row, rows at a time
+  constexpr int LR = D / 4, RW = 256 / LR, AHEAD = 8;  // lanes of a row, rows at a time, parts on their way
+  __shared__ float s_ml[2 * RW];
+  __shared__ float4 s_acc[256];
   const int b = note.x, G = p.G;
   const PaSeq sq = pa_seq(p, b);
-  const int nrow = sq.lq * G, r0 = note.y * R, lane = threadIdx.x % LR;
-  for (int r = r0 + blockIdx.y * RW + threadIdx.x / LR; r < min(nrow, r0 + R); r += gridDim.y * RW) {
-    float m = pa_ninf(), l = 0.f;
-    float4 acc{0.f, 0.f, 0.f, 0.f};
-    // (parts in their order, as many on their way at a time as there may be: a row is bound by this)
-    constexpr int AHEAD = 8;
-    for (int i0 = 0; i0 < note.z; i0 += AHEAD) {
+  const int nrow = sq.lq * G, r0 = note.y * R, lane = threadIdx.x % LR, group = threadIdx.x / LR;
+  auto parts = [&](PaState &x, int r, int first, int step) {
+    for (int i0 = first; i0 < note.z; i0 += AHEAD * step) {
       float2 ml[AHEAD];
       float4 v[AHEAD];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        const int x = min(i0 + i, note.z - 1);
-        const int64_t pi = pa_part(p, own + x, kvh, x == 0, note.w != 0) + r - r0;
+        const int y = min(i0 + i * step, note.z - 1);
+        const int64_t pi = pa_part(p, own + y, kvh, y == 0, note.w != 0) + r - r0;
         ml[i] = *(const float2 *)(p.ws_ml + 2 * pi);
         v[i] = *(const float4 *)(p.ws_acc + pi * D + 4 * lane);
       }
 #pragma unroll
-      for (int i = 0; i < AHEAD; ++i) {
-        if (i0 + i >= note.z || (ml[i].x == pa_ninf() && ml[i].y == 0.f)) continue;  // (empty: no key seen)
-        const float mn = fmaxf(m, ml[i].x), from = mn == pa_ninf() ? 0.f : mn;
-        const float f = m == pa_ninf() && l == 0.f ? 0.f : fast_exp2(m - from), g = fast_exp2(ml[i].x - from);
-        m = mn;
-        l = l * f + ml[i].y * g;
-        acc.x = acc.x * f + v[i].x * g;
-        acc.y = acc.y * f + v[i].y * g;
-        acc.z = acc.z * f + v[i].z * g;
-        acc.w = acc.w * f + v[i].w * g;
-      }
+      for (int i = 0; i < AHEAD; ++i)
+        if (i0 + i * step < note.z) x.add(ml[i], v[i]);
     }
+  };
+  auto store = [&](const PaState &x, int r) {
     const int t = r / G, h = kvh * G + r % G;
-    const bool none = l == 0.f;
-    const float inv = none ? 0.f : 1.f / l;
+    const bool none = x.l == 0.f;
+    const float inv = none ? 0.f : 1.f / x.l;
     const int64_t o = pa_out_at(p, b, sq, t, h) + 4 * lane;
-    const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+    const float y[4] = {x.acc.x * inv, x.acc.y * inv, x.acc.z * inv, x.acc.w * inv};
     if (p.out_dt == LA_F32) {
       *(float4 *)((float *)p.out + o) = float4{y[0], y[1], y[2], y[3]};
     } else if (p.out_dt == LA_BF16) {
@@ -1120,7 +1131,31 @@ __device__ __forceinline__ void pa_join_rows(const PaKP &p, const int4 &note, in
       typedef _Float16 x4 __attribute__((ext_vector_type(4)));
       *(x4 *)((_Float16 *)p.out + o) = x4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
     }
-    if (p.lse && lane == 0) p.lse[pa_lse_at(p, b, sq, t, h)] = none ? pa_ninf() : (m + __log2f(l)) * PA_LN2;
+    if (p.lse && lane == 0) p.lse[pa_lse_at(p, b, sq, t, h)] = none ? pa_ninf() : (x.m + __log2f(x.l)) * PA_LN2;
+  };
+  const int end = min(nrow, r0 + R);
+  if (note.z <= 2 * AHEAD) {
+    for (int r = r0 + blockIdx.y * RW + group; r < end; r += gridDim.y * RW) {
+      PaState x;
+      parts(x, r, 0, 1);
+      store(x, r);
+    }
+    return;
+  }
+  for (int r = r0 + blockIdx.y; r < end; r += gridDim.y) {
+    PaState x;
+    parts(x, r, group, RW);
+    if (lane == 0) {
+      s_ml[2 * group] = x.m;
+      s_ml[2 * group + 1] = x.l;
+    }
+    s_acc[threadIdx.x] = x.acc;
+    __syncthreads();
+    if (group == 0) {
+      for (int g = 1; g < RW; ++g) x.add(float2{s_ml[2 * g], s_ml[2 * g + 1]}, s_acc[g * LR + lane]);
+      store(x, r);
+    }
+    __syncthreads();
   }
 }
 
@@ -1178,14 +1213,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaKP p) {
     pa_join_rows<D, 64>(p, note, own, kvh);
   } else {
     if (note.w) pa_join_rows<D, PA_FEW>(p, note, own, kvh);
-    else pa_join_many<E, D>(p, note, own, kvh);
+    else if (blockIdx.y == 0) pa_join_many<E, D>(p, note, own, kvh);
   }
 }
 
 // ------------------------------------------------------------------ host ----
 struct PaPlan {
-  int64_t W = 1, rows = 128, least = 0, few_parts = 0;
-  bool join = true;
+  int64_t W = 1, rows = 128, least = 0, least_few = 0, few_parts = 0;
+  int join = 1;  // workgroups of the join for each of the first launch's
   size_t ml = 0, notes = 0, bytes = 0;
 };
 
@@ -1194,18 +1229,24 @@ static PaPlan pa_plan(const la_paged_attn_args *a) {
   const bool f32 = a->dtype == LA_F32;
   const int64_t G = a->Hq / a->Hkv, R = f32 ? 64 : 128;
   // workgroups that are there at once, shared among the KV heads (one at least for either line); no
-  // stretch is shorter than four blocks of keys and a tile's beginning and end
-  pl.least = G * (4 * (f32 ? 32 : DA_BS) + PA_AHEAD);
+  // stretch is shorter than four blocks of keys and a tile's beginning and end.  Of few rows four blocks
+  // are enough: four tokens behind 1000 keys each 17.2 us (two blocks 17.0, eight 19.1), eight behind
+  // 4000 25.1 (27.4, 23.9), one behind 16384 24.9 (24.6, 23.0), sixteen fp8 ones 19.5 (19.6, 20.3); in
+  // fp32, whose blocks take four times as long, two: three tokens behind 1000 keys 17.7 (four 21.4).
+  pl.least = G * (4 * DA_BS + PA_AHEAD);
+  pl.least_few = G * 4 * DA_BS;
+  if (f32) pl.least = pl.least_few = G * 2 * DA_BS;
   const int64_t rows = a->Tq * G, keys = a->pt_pages * a->page;  // (rows: of a sequence, at most)
   const int64_t tiles = a->cu_q ? std::min(rows, rows / R + a->B) : a->B * ceil_div(rows, R);  // at most
   const double most = (double)tiles * ((double)G * (keys + PA_AHEAD) + (a->causal ? R + 0.0 : 0.0));
   pl.W = std::max<int64_t>(f32 ? 1 : 2, (f32 ? 2 : 3) * num_cus() / a->Hkv);
-  if (most / pl.least + 2 < (double)pl.W) pl.W = (int64_t)(most / pl.least) + 2;
-  if (most <= 2.0 * pl.least) {  // a stretch for each line, nothing to join: a launch less (4 us)
-    pl.least = (int64_t)1 << 60;
+  if (most / pl.least_few + 2 < (double)pl.W) pl.W = (int64_t)(most / pl.least_few) + 2;
+  if (most <= 2.0 * G * (4 * DA_BS + PA_AHEAD)) {  // a stretch for each line, nothing to join: a launch less (4 us)
+    pl.least = pl.least_few = (int64_t)1 << 60;
     pl.W = 2;
-    pl.join = false;
+    pl.join = 0;
   }
+  if (pl.join && (f32 || tiles < pl.W / 4)) pl.join = 4;  // (fp32's rows, or a row's many parts: 2 us of 26 of one token behind 16384 keys)
   pl.rows = std::min(R, ceil_div(rows, 32) * 32);  // (whole waves)
   pl.few_parts = pl.W * a->Hkv * 2 * pl.rows;
   const int64_t parts = pl.join ? pl.few_parts + (f32 ? 0 : pl.W * a->Hkv * 2 * PA_FEW) : 0;
@@ -1232,6 +1273,11 @@ static int pa_check(const la_paged_attn_args *a) {
                  (a->cu_q ? 1 : a->B) * std::max<int64_t>(1, a->Tq) < ((int64_t)1 << 30) / (a->Hq / a->Hkv),
              "la_paged_attention: sizes past 2^30 rows");
   LA_REQUIRE(!(a->cu_q && a->q_len), "la_paged_attention: q_len is for batched calls");
+  // the line of all tiles is counted in 64 bits and shared out by quotients that are exact below 2^53 (a
+  // call of that size would take hours)
+  const double G = (double)(a->Hq / a->Hkv), span = (double)std::max(a->pt_pages * a->page, a->Tq) + PA_AHEAD;
+  LA_REQUIRE(((a->cu_q ? 1. : (double)a->B) * (double)a->Tq * G / 64 + (double)a->B) * (G * span + 128) < 4e15,
+             "la_paged_attention: more products than one call takes");
   return LA_OK;
 }
 
@@ -1299,7 +1345,7 @@ extern "C" int la_paged_attention(const la_paged_attn_args *args, void *stream) 
   p.o_sb = a->o_sb; p.o_sh = a->o_sh; p.o_st = a->o_st;
   p.l_sb = a->l_sb; p.l_sh = a->l_sh;
   p.pt_sb = a->pt_sb; p.s_stride = a->s_stride; p.n_phys = a->n_phys;
-  p.least = pl.least; p.few_parts = pl.few_parts;
+  p.least = pl.least; p.least_few = pl.least_few; p.few_parts = pl.few_parts;
   p.B = (int32_t)a->B; p.G = (int32_t)(a->Hq / a->Hkv); p.Hq = (int32_t)a->Hq; p.Hkv = (int32_t)a->Hkv;
   p.D = (int32_t)a->D; p.W = (int32_t)pl.W; p.part_rows = (int32_t)pl.rows;
   p.page = (int32_t)a->page; p.pt_pages = (int32_t)a->pt_pages;
@@ -1314,8 +1360,8 @@ extern "C" int la_paged_attention(const la_paged_attn_args *args, void *stream) 
   else if (a->dtype == LA_BF16) rc = d128 ? pa_launch16<DaBf16, 128>(kv8, even, wgs, p, st) : pa_launch16<DaBf16, 64>(kv8, even, wgs, p, st);
   else rc = d128 ? pa_launch16<DaF16, 128>(kv8, even, wgs, p, st) : pa_launch16<DaF16, 64>(kv8, even, wgs, p, st);
   if (rc != LA_OK || !pl.join) return rc;
-  if (a->dtype == LA_F32) return d128 ? pa_launch(paged_join_kernel<float, 128>, wgs, p, st, 4) : pa_launch(paged_join_kernel<float, 64>, wgs, p, st, 4);
-  if (a->dtype == LA_BF16) return d128 ? pa_launch(paged_join_kernel<__bf16, 128>, wgs, p, st) : pa_launch(paged_join_kernel<__bf16, 64>, wgs, p, st);
-  return d128 ? pa_launch(paged_join_kernel<_Float16, 128>, wgs, p, st) : pa_launch(paged_join_kernel<_Float16, 64>, wgs, p, st);
+  if (a->dtype == LA_F32) return d128 ? pa_launch(paged_join_kernel<float, 128>, wgs, p, st, pl.join) : pa_launch(paged_join_kernel<float, 64>, wgs, p, st, pl.join);
+  if (a->dtype == LA_BF16) return d128 ? pa_launch(paged_join_kernel<__bf16, 128>, wgs, p, st, pl.join) : pa_launch(paged_join_kernel<__bf16, 64>, wgs, p, st, pl.join);
+  return d128 ? pa_launch(paged_join_kernel<_Float16, 128>, wgs, p, st, pl.join) : pa_launch(paged_join_kernel<_Float16, 64>, wgs, p, st, pl.join);
 }
 

@@ -166,3 +166,14 @@ def test_struct_layouts_match_the_header(tmp_path):
         pack, _ = N.by_bytes(py)
         if f == "size":
             assert len(pack(*[0] * len(py._fields_))) == int(at)
+
+
+def test_more_work_than_can_be_counted():
+    """The lengths are on the device: sizes whose longest tiles would pass 64-bit places are refused."""
+    a, base, far = _args()
+    a.Hq, a.Tq, a.page, a.pt_pages = 2 * 1024, 1 << 19, 1 << 14, 1 << 15
+    a.q_sb, a.q_sh, a.q_st = a.o_sb, a.o_sh, a.o_st = 0, 64, 64 * a.Hq
+    a.cu_q = 1 << 50
+    rc, text = _call(a)
+    assert rc == N.LA_ERR_INVALID and "more products" in text, (rc, text)
+    assert N.load().la_paged_attention_workspace(ctypes.byref(a)) == 0
