@@ -1,8 +1,9 @@
 """linattn_amd -- MI355X (gfx950) HIP implementation of the sparse-attention hot
 path of tongxin/linattn: Quest page selection, the lightning indexer top-k,
-block-sparse prefill / paged sparse decode, dense attention of prompts
-(``kernels.dense``) and eviction of cached keys by gathered weight
-(``kernels.eviction``).
+block-sparse prefill / paged sparse decode, dense attention of prompts and over
+paged caches (``kernels.dense``), rotary positions (``kernels.rotary``) and their
+append to paged caches (``kernels.kv_cache``), and eviction of cached keys by
+gathered weight (``kernels.eviction``).
 
 Kernel-level entry points mirror the reference's kernel modules
 (src/linattn/kernels/triton/{block_sparse,quest_pages,fused_indexer}.py and

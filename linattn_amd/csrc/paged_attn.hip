@@ -611,7 +611,8 @@ __device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x
 // in bf16 and fp16); the scale of a key multiplies its scores, that of its value its weights, both in fp32.
 //
 // Bound by matrix and vector unit in turn: 8192 tokens behind 24576 3.33 to 3.47 ms, 1.11 to 1.16 PFLOP/s
-// (a large product has 1.36), the matrix unit busy for 57 % of the cycles.  Products of the next block
+// (a large product has 1.36), the matrix unit busy for 57 to 64 % of the cycles
+// at 1.75 to 1.55 GHz.  Products of the next block
 // beside a block's weights (32 keys at a time, for the registers) take 3.77 to 3.90 ms, two workgroups
 // a CU with them 4.16.
 template <class T, int D, bool KV8, bool EVEN>
