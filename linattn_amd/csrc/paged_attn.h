@@ -130,14 +130,20 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w, PaSeq &seq
     const PaTiles t = pa_tiles<R, FEW>(p, q, few);
     return b < p.B ? t.upto(t.n) : 0;
   };
-  PaSeq mine = pa_seq(p, min(lane, p.B - 1));
-  int64_t sum_many = pa_scan(cost(mine, lane, false)), sum_few = FEW ? pa_scan(cost(mine, lane, true)) : 0;
-  int64_t many = pa_lane_value(sum_many, 63), few = pa_lane_value(sum_few, 63);
-  for (int b0 = 64; b0 < p.B; b0 += 64) {
-    const PaSeq q = pa_seq(p, min(b0 + lane, p.B - 1));
-    many += pa_lane_value(pa_scan(cost(q, b0 + lane, false)), 63);
-    if (FEW) few += pa_lane_value(pa_scan(cost(q, b0 + lane, true)), 63);
+  // a lane counts a sequence, or, of more than 64, as many that lie one behind the other
+  const int each = (p.B + 63) / 64;
+  PaSeq mine = pa_seq(p, min(lane * each, p.B - 1));
+  int64_t sum_many = cost(mine, lane * each, false), sum_few = FEW ? cost(mine, lane * each, true) : 0;
+#pragma unroll 4
+  for (int i = 1; i < each; ++i) {
+    const int b = lane * each + i;
+    const PaSeq q = pa_seq(p, min(b, p.B - 1));
+    sum_many += cost(q, b, false);
+    if (FEW) sum_few += cost(q, b, true);
   }
+  sum_many = pa_scan(sum_many);
+  if (FEW) sum_few = pa_scan(sum_few);
+  const int64_t many = pa_lane_value(sum_many, 63), few = pa_lane_value(sum_few, 63);
   PaStretch s;
   s.left = 0;
   s.b = s.i = 0;
@@ -155,24 +161,27 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w, PaSeq &seq
   s.left = min(s.line.quota, s.line.all - s.off);
   s.pos = s.off;
   int64_t sum = s.few ? sum_few : sum_many;
-  for (int b0 = 0;; b0 += 64) {
-    if (b0 > 0) {
-      mine = pa_seq(p, min(b0 + lane, p.B - 1));
-      sum = pa_scan(cost(mine, b0 + lane, s.few));
-    }
-    const int64_t here = pa_lane_value(sum, 63);
-    if (s.off >= here && b0 + 64 < p.B) {
+  int at = __ffsll((unsigned long long)__ballot(sum > s.off)) - 1;  // (off is below the line's end)
+  if (at > 0) s.off -= pa_lane_value(sum, at - 1);
+  int first = at * each;
+  if (each == 1) {
+    first = 0;
+  } else {
+    for (const int end = min(first + each, p.B);; first += 64) {
+      const int b = first + lane;
+      mine = pa_seq(p, min(b, p.B - 1));
+      sum = pa_scan(b < end ? cost(mine, b, s.few) : 0);
+      const int64_t here = pa_lane_value(sum, 63);
+      if (s.off < here || first + 64 >= end) break;
       s.off -= here;
-      continue;
     }
-    const int at = __ffsll((unsigned long long)__ballot(sum > s.off)) - 1;  // (off is below the line's end)
-    s.b = __builtin_amdgcn_readfirstlane(b0 + at);
+    at = __ffsll((unsigned long long)__ballot(sum > s.off)) - 1;
     if (at > 0) s.off -= pa_lane_value(sum, at - 1);
-    seq.lq = __builtin_amdgcn_readlane(mine.lq, at);
-    seq.lk = __builtin_amdgcn_readlane(mine.lk, at);
-    seq.q0 = pa_lane_value(mine.q0, at);
-    break;
   }
+  s.b = __builtin_amdgcn_readfirstlane(first + at);
+  seq.lq = __builtin_amdgcn_readlane(mine.lq, at);
+  seq.lk = __builtin_amdgcn_readlane(mine.lk, at);
+  seq.q0 = pa_lane_value(mine.q0, at);
   tiles = pa_tiles<R, FEW>(p, seq, s.few);
   if (tiles.n > 1) {
     // upto(i) <= off < upto(i + 1): the quadratic's root, and what its rounding may have missed

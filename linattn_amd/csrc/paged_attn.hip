@@ -167,15 +167,6 @@ __device__ __forceinline__ const PaKP &pa_args() {
   return *(const PaKP *)x;
 }
 
-template <int R, bool FEW>
-__device__ __forceinline__ void pa_load(const PaKP &p, PaWalk &w) {
-  w.seq = pa_seq(p, w.s.b);
-  const PaTiles t = pa_tiles<R, FEW>(p, w.seq, w.s.few);
-  w.a = t.a;
-  w.step = t.step;
-  w.n = t.n;
-}
-
 // The stretch's beginning, by every wave; false: there is none.
 template <int R, bool FEW>
 __device__ __forceinline__ bool pa_begin(PaWalk *walk) {
@@ -206,23 +197,34 @@ __device__ __forceinline__ bool pa_next(PaWalk *walk) {
   const int64_t cost = w.a + w.step * (w.s.i + 1), upto = min(cost, w.s.off + w.s.left);
   w.s.left -= upto - w.s.off;
   const bool more = __builtin_amdgcn_readfirstlane(w.s.left > 0);
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 64) {
     const int64_t own = blockIdx.x / (uint32_t)p.Hkv - w.s.line.first;
     if (!more) {
       const int parts = w.s.off == 0 && upto < cost ? (int)(pa_div(w.s.pos + cost - 1, w.s.line.quota) - own) + 1 : 0;
-      p.ws_join[blockIdx.x] = int4{w.s.b, w.s.i, parts, w.s.few ? 1 + (int)own : 0};
+      if (threadIdx.x == 0) p.ws_join[blockIdx.x] = int4{w.s.b, w.s.i, parts, w.s.few ? 1 + (int)own : 0};
     } else {
       w.s.off = 0;
       w.s.pos += cost;
       w.since = w.s.pos - own * w.s.line.quota;
-      if (++w.s.i >= w.n) {
+      if (++w.s.i >= w.n) {  // the next sequence that has tiles in the line (of a padded batch most may have none)
         w.s.i = 0;
-        do {
-          ++w.s.b;
-          pa_load<R, FEW>(p, w);
-        } while (w.n == 0 && w.s.b + 1 < p.B);
+        for (int b0 = w.s.b + 1; b0 < p.B; b0 += 64) {
+          const int b = b0 + (int)threadIdx.x;
+          const PaSeq seq = pa_seq(p, min(b, p.B - 1));
+          const PaTiles t = pa_tiles<R, FEW>(p, seq, w.s.few);
+          const uint64_t there = __ballot(b < p.B && t.n > 0);
+          if (there == 0) continue;
+          const int at = __ffsll((unsigned long long)there) - 1;
+          w.s.b = b0 + at;
+          w.seq.lq = __builtin_amdgcn_readlane(seq.lq, at);
+          w.seq.lk = __builtin_amdgcn_readlane(seq.lk, at);
+          w.seq.q0 = pa_lane_value(seq.q0, at);
+          w.a = pa_lane_value(t.a, at);
+          w.n = __builtin_amdgcn_readlane(t.n, at);
+          break;
+        }
       }
-      *walk = w;
+      if (threadIdx.x == 0) *walk = w;
     }
   }
   __syncthreads();
@@ -612,9 +614,8 @@ __device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x
 //
 // Bound by matrix and vector unit in turn: 8192 tokens behind 24576 3.33 to 3.47 ms, 1.11 to 1.16 PFLOP/s
 // (a large product has 1.36), the matrix unit busy for 57 to 64 % of the cycles
-// at 1.75 to 1.55 GHz.  Products of the next block
-// beside a block's weights (32 keys at a time, for the registers) take 3.77 to 3.90 ms, two workgroups
-// a CU with them 4.16.
+// at 1.75 to 1.55 GHz.  Products of the next block beside a block's weights (32 keys at a time, for the
+// registers) take 3.77 to 3.90 ms, two workgroups a CU with them 4.16.
 template <class T, int D, bool KV8, bool EVEN>
 __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_scale) {
   typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V

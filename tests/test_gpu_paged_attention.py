@@ -325,3 +325,39 @@ def test_streams_and_graphs(dev):
         torch.cuda.synchronize()
         for e, o in zip(eager, outs):
             assert torch.equal(e, o), lens
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,G", [(64, 2), (128, 4)])
+def test_one_token_of_many_parts(dev, dtype, D, G):
+    """A row of more parts than are joined one behind the other, finite and not."""
+    lq, lk = [1, 1, 1], [13000, 700, 9001]
+    q, k, v = _case(24, lq, lk, G, 1, D, dtype)
+    vb = [x.clone() for x in v]
+    vb[2][0, 8000, 7], vb[2][0, 3, 9] = math.inf, math.nan
+    for values, clean in ((v, [0, 1, 2]), (vb, [0, 1])):
+        kp, vp, table = (x.to(dev) for x in _paged(25, k, values, 16))
+        out, lse = (x.cpu() for x in paged_attention(q.to(dev), kp, vp, table, _i32(lk, dev), _cu(lq, dev), return_lse=True))
+        for b in range(3):
+            for h in range(G):
+                o, ls, tol, tol_l = attention(q[b:b + 1, h], k[b][0], v[b][0], True, None, HALF_STEP[dtype])
+                close(lse[h, b:b + 1], ls, tol_l)
+                keep = torch.ones(D, dtype=torch.bool)
+                if b not in clean:
+                    keep[[7, 9]] = False
+                    assert out[b, h, 7] == math.inf and torch.isnan(out[b, h, 9])
+                close(out[b:b + 1, h][:, keep], o[:, keep], tol[:, keep])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B", [700, 9000])
+def test_batches_of_mostly_empty_sequences(dev, dtype, B):
+    """Slots of a server of which few are in use: what lies between two of them is passed over."""
+    used = {0: (1, 300), 1: (40, 40), 130: (1, 17), 131: (0, 50), 400: (70, 900), 401: (1, 1), 640: (2, 64), 690: (1, 70),
+            B - 1: (33, 2000)}
+    lq, lk = ([used.get(b, (0, 0))[i] for b in range(B)] for i in (0, 1))
+    q, k, v = _case(26, lq, lk, 4, 2, 64, dtype)
+    kp, vp, table = _paged(27, k, v, 16)
+    args = (q.to(dev), kp.to(dev), vp.to(dev), table.to(dev), _i32(lk, dev), _cu(lq, dev))
+    out, lse = paged_attention(*args, return_lse=True)
+    _check(out.cpu(), lse.cpu(), q, k, v, lq, lk)
