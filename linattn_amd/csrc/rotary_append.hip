@@ -142,11 +142,18 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_kernel(RaKP p) {
     for (int i = 0; i < AHEAD; ++i)
       if (r0 + i * p.hs < R) unit.load(ra_source<E, V>(p, xb_, xt, r0 + i * p.hs), xa[i], xb[i]);
   if (p.cu) {
-    // a wave a token: its sequence is the last that begins at or before it
+    // a wave a token: its sequence is the last that begins at or before it, looked for among every
+    // `each`th, then from there on
+    const int B = (int)p.B, each = (B + 63) / 64;
     for (int i = w; i < count; i += RO_NT / 64) {
       const int64_t x = tok0 + i;
-      int b = -1;
-      for (int b0 = 0; b0 < p.B; b0 += 64) b += __popcll(__ballot(b0 + lane < p.B && ra_cu(p, min(b0 + lane, (int)p.B)) <= x));
+      int b = __popcll(__ballot(lane * each < B && ra_cu(p, min(lane * each, B)) <= x)) - 1;
+      if (each > 1 && b >= 0) {
+        const int end = min((b + 1) * each, B);
+        int n = 0;
+        for (int b0 = b * each; b0 < end; b0 += 64) n += __popcll(__ballot(b0 + lane < end && ra_cu(p, min(b0 + lane, B)) <= x));
+        b = b * each + max(n, 1) - 1;
+      }
       const bool in = b >= 0 && x < ra_cu(p, b + 1) && x >= ra_cu(p, b);
       if (lane == 0) s_tok[i] = ra_token(p, in ? b : -1, in ? x - ra_cu(p, b) : 0, 0, (int)x);
     }
@@ -200,7 +207,8 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_bounds_kernel(RaKP p) {
   extern __shared__ float2 cs[];
   __shared__ RaToken s_tok[TOK];
   __shared__ float s_red[RO_NT * 2 * V];
-  __shared__ int s_any;
+  __shared__ int s_any, s_sum[RO_NT / 64];
+  __shared__ int2 s_at;  // the sequence that is looked for (or the first of some that hold it), the pages before it
   const int tid = threadIdx.x, lane = tid & 63, n = p.an.n, mp = p.meta_page;
   const int kvh = (int)(blockIdx.x % (uint32_t)p.Hkv), G = p.Hq / p.Hkv;
   int64_t blk = blockIdx.x / (uint32_t)p.Hkv;
@@ -208,27 +216,49 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_bounds_kernel(RaKP p) {
   int b = -1;
   int64_t pos0 = 0, first = 0, new_tokens = 0;  // its position, its first row (packed), its tokens
   if (p.cu) {
-    for (int b0 = 0; b0 < p.B && b < 0; b0 += 64) {
-      const int x = b0 + lane;
-      int c = 0;
-      if (x < p.B) {
-        const int64_t m = ra_cu(p, x + 1) - ra_cu(p, x), at = p.positions[x];
-        if (m > 0) c = (int)(floor_div(at + m - 1, mp) - floor_div(at, mp) + 1);
-      }
-      int sum = c;
+    // pages that sequence x touches; a thread counts a sequence, or, of more than there are threads, as
+    // many that lie one behind the other
+    const int B = (int)p.B, each = (B + RO_NT - 1) / RO_NT;
+    auto pages = [&](int x, int end) -> int {
+      const int y = min(x, B - 1);
+      const int64_t m = ra_cu(p, y + 1) - ra_cu(p, y), at = p.positions[y];
+      return x < end && m > 0 ? (int)(floor_div(at + m - 1, mp) - floor_div(at, mp) + 1) : 0;
+    };
+    auto scan = [&](int sum) -> int {
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int y = __shfl_up(sum, o, 64);
         if (lane >= o) sum += y;
       }
-      const int all = __shfl(sum, 63, 64);
-      if (blk < all) {
-        const int at = __ffsll((unsigned long long)__ballot(sum > blk)) - 1;
-        b = b0 + at;
-        blk -= __shfl(sum - c, at, 64);
-      } else {
-        blk -= all;
+      return sum;
+    };
+    int c = 0;
+#pragma unroll 4
+    for (int i = 0; i < each; ++i) c += pages(tid * each + i, B);
+    int sum = scan(c), before = 0, all = 0;
+    if (lane == 63) s_sum[tid >> 6] = sum;
+    if (tid == 0) s_at = int2{-1, 0};
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < RO_NT / 64; ++w) {
+      if (w < tid >> 6) before += s_sum[w];
+      all += s_sum[w];
+    }
+    if (before + sum - c <= blk && blk < before + sum) s_at = int2{tid * each, before + sum - c};
+    __syncthreads();
+    b = s_at.x;
+    blk -= b < 0 ? all : s_at.y;
+    if (b >= 0 && each > 1) {
+      for (const int end = min(b + each, B);; b += 64) {
+        c = pages(b + lane, end);
+        sum = scan(c);
+        const int here = __shfl(sum, 63, 64);
+        if (blk < here || b + 64 >= end) break;
+        blk -= here;
       }
+      const int at = max(__ffsll((unsigned long long)__ballot(sum > blk)) - 1, 0);
+      blk -= __shfl(sum - c, at, 64);
+      b = min(b + at, B - 1);
     }
     if (b >= 0) {
       first = ra_cu(p, b);
@@ -339,8 +369,9 @@ static int ra_launch(RaKP p, hipStream_t st) {
   }
   const size_t turns = (size_t)p.an.n * sizeof(float2);
   if (p.mn) {
-    // (packed: a page more than the tokens fill at either end of each sequence, and one for the rest)
-    p.blocks = p.cu ? p.T / p.meta_page + 2 * p.B + 1 : p.B * (ceil_div(p.T - 1, p.meta_page) + 1);
+    // (packed: no more than a token each, or than the tokens fill and one at either end of each sequence;
+    // and one for the rest)
+    p.blocks = p.cu ? std::min(p.T, p.T / p.meta_page + 2 * p.B) + 1 : p.B * (ceil_div(p.T - 1, p.meta_page) + 1);
     LA_REQUIRE(grid_fits(p.blocks * p.Hkv, RO_NT), "la_rotary_append: too many tokens");
     rotary_append_bounds_kernel<E, V><<<dim3((uint32_t)(p.blocks * p.Hkv)), RO_NT, 32 * turns, st>>>(p);
     LA_LAUNCHED();

@@ -399,3 +399,28 @@ def test_append_bounds_of_the_widest_heads(dev, dtype):
     assert torch.equal(gv[phys, :, slot].cpu(), v)
     emn, emx = bounds(mn, mx, stored, b, t, ok, before, page)
     assert torch.equal(gmn.cpu(), emn) and torch.equal(gmx.cpu(), emx)
+
+
+@pytest.mark.parametrize("with_bounds", [False, True])
+@pytest.mark.parametrize("B", [65, 700, 9000])
+def test_batches_of_mostly_empty_sequences(dev, with_bounds, B):
+    """Slots of a server of which few are in use, the first and last among them."""
+    dtype, page, Hq, Hkv, D = torch.bfloat16, 16, 4, 2, 64
+    used = {0: (1, 30), 1: (40, 0), 3: (1, 17), 31: (0, 50), 32: (20, 9), 63: (1, 1), 64: (2, 14), B - 2: (1, 15), B - 1: (33, 20)}
+    lq, before = ([used.get(b, (0, 5))[i] for b in range(B)] for i in (0, 1))
+    q, k, v, kp, vp, table = _case(41, lq, before, page, Hq, Hkv, D, dtype)
+    freq, kp, vp = _freq(32), kp.to(dtype), vp.to(dtype)
+    b, t, ok, phys, slot, (wq, tq), (wk, tk) = _expect(q, k, v, kp, vp, table, before, lq, freq)
+    mn, mx = (_rand(s, B, Hkv, 4, D, dtype=dtype) for s in (42, 43))
+    gk, gv, gmn, gmx = (x.to(dev) for x in (kp, vp, mn, mx))
+    more = dict(page_min=gmn, page_max=gmx, page_size=page) if with_bounds else {}
+    cu = _i32([sum(lq[:i]) for i in range(B + 1)], dev)
+    gq = rotary_kv_append(q.to(dev), k.to(dev), v.to(dev), gk, gv, table.to(dev), _i32(before, dev), freq.to(dev),
+                          cu_seqlens=cu, **more)
+    close(gq, wq, rounded(wq, tq, dtype), "q")
+    stored = gk[phys, :, slot].cpu()
+    close(stored, wk, rounded(wk, tk, dtype), "k")
+    assert torch.equal(gv[phys, :, slot].cpu(), v)
+    if with_bounds:
+        emn, emx = bounds(mn, mx, stored, b, t, ok, before, page)
+        assert torch.equal(gmn.cpu(), emn) and torch.equal(gmx.cpu(), emx)
