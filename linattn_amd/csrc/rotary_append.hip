@@ -199,7 +199,9 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_kernel(RaKP p) {
 }
 
 // With page bounds: a workgroup takes the new tokens of one page of bounds of one sequence, and one KV
-// head with its group of q, so that a page's least and largest keys are found without atomics.
+// head with its group of q, so that a page's least and largest keys are found without atomics.  Which
+// page that is every workgroup finds by itself: in a batch of 4096 slots with 64 tokens in all that takes
+// no time beside the rest (14 us, as without the empty slots), with 4096 tokens 189 us.
 template <class E, int V>
 __global__ __launch_bounds__(RO_NT) void rotary_append_bounds_kernel(RaKP p) {
   typedef RoUnit<E, V> U;
