@@ -121,7 +121,7 @@ struct PaLine {
 struct PaStretch {
   PaLine line;
   int64_t off, left, pos;
-  int32_t b, i, few;
+  int32_t b, i, few, mixed;  // mixed: there are both lines
 };
 template <int R, bool FEW>
 __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w, PaSeq &seq, PaTiles &tiles) {
@@ -152,6 +152,7 @@ __device__ __forceinline__ PaStretch pa_stretch(const PaKP &p, int w, PaSeq &seq
   // 0.65, 0.8, 1 and 1.3)
   const int wm = few == 0 ? p.W : many == 0 ? 0 : max(1, min(p.W - 1, (int)((double)p.W * (double)many / ((double)many + 0.7 * (double)few) + 0.5)));
   s.few = w >= wm && few > 0;
+  s.mixed = few > 0 && many > 0;
   s.line.all = s.few ? few : many;
   s.line.first = s.few ? wm : 0;
   const int places = s.few ? p.W - wm : max(wm, 1);

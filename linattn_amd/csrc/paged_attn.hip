@@ -235,7 +235,7 @@ __device__ __forceinline__ bool pa_next(PaWalk *walk) {
 // blocks of BS keys.
 struct PaPiece {
   PaSeq sq;
-  int32_t b, r0, kvh;
+  int32_t b, r0, kvh, mixed;
   PaBlocks blocks;
   int64_t part;  // (-1: the whole tile)
 };
@@ -250,6 +250,7 @@ __device__ __forceinline__ PaPiece pa_piece(const PaKP &p, const PaWalk *walk) {
   x.b = __builtin_amdgcn_readfirstlane(w.s.b);
   x.r0 = __builtin_amdgcn_readfirstlane(w.s.i) * R;
   x.kvh = (int)(blockIdx.x % (uint32_t)p.Hkv);
+  x.mixed = __builtin_amdgcn_readfirstlane(w.s.mixed);
   const int last = (min(x.r0 + R, x.sq.lq * p.G) - 1) / p.G;  // its last query
   const int lim = p.causal ? x.sq.lk - x.sq.lq + last : x.sq.lk - 1;
   const int n_all = lim < 0 ? 0 : lim / BS + 1;
@@ -347,13 +348,27 @@ __device__ __forceinline__ f32x4 pa_mfma16(s16x4 a, s16x4 b, f32x4 c) {
 
 // Of a CU's three workgroups each is preferred for a block in turn: else the one that came first is, and
 // they end one after the other (8192 tokens behind 24576, equal stretches: after 2.87, 3.23 and
-// 3.81 ms; in turn 3.50, 3.59, 3.65).
-__device__ __forceinline__ void pa_prefer(int turn) {
-  turn %= 3;
-  if (turn == 0) __builtin_amdgcn_s_setprio(0);
-  else if (turn == 1) __builtin_amdgcn_s_setprio(1);
-  else __builtin_amdgcn_s_setprio(2);
-}
+// 3.81 ms).  In six blocks the first is preferred to both others once, the second twice and the third
+// three times, for which all three end at the same time (3.32, 3.33 and 3.33 ms on the mean, as often as one
+// another 3.24, 3.33, 3.43): that call 3.34 ms (3.37), chunks of four prompts 225 us (227), tokens over fp8
+// caches 136 (139).  Where single tokens lie beside chunks the third holds the tokens, which would come
+// first: as often as one another there (243 us, 250 otherwise).
+struct PaTurns {
+  uint32_t order;  // two bits a block
+  __device__ __forceinline__ PaTurns(int third, bool mixed, int i) {
+    constexpr uint32_t A = 0x112, B = 0x648, C = 0x8a5, X = 0x924, Y = 0x249, Z = 0x492;
+    order = third == 0 ? (mixed ? X : A) : third == 1 ? (mixed ? Y : B) : (mixed ? Z : C);
+    i %= 6;
+    order = (order >> 2 * i | order << (12 - 2 * i)) & 0xfff;
+  }
+  __device__ __forceinline__ void next() {
+    const uint32_t now = order & 3;
+    order = order >> 2 | now << 10;
+    if (now == 0) __builtin_amdgcn_s_setprio(0);
+    else if (now == 1) __builtin_amdgcn_s_setprio(1);
+    else __builtin_amdgcn_s_setprio(2);
+  }
+};
 
 constexpr int PA_WAVE_LDS = 12288;  // of a wave, where the waves of a workgroup go their own ways
 
@@ -429,10 +444,10 @@ __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale,
     }
 #pragma unroll
     for (int s = 0; s < NK; ++s) settle(qf[s]);
-    const int third = (int)(blockIdx.x / (uint32_t)(p.W * p.Hkv / 3 + 1));
+    PaTurns turns((int)(blockIdx.x / (uint32_t)(p.W * p.Hkv / 3 + 1)), x.mixed, 0);
     for (int i = 0; i < n; ++i) {
       const int j = x.blocks.j0 + i;
-      pa_prefer(i + third);
+      turns.next();
       // newer pieces on their way: V of this block, and K (fp8: and V) of the next
       if (i + 1 < n) wait_vmcnt<(NU - 1) * NX + (KV8 ? 1 : 0)>();
       else wait_vmcnt<NX>();
@@ -807,11 +822,11 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
     };
 
     const int jw = r_first < nrow && lim_hi >= 0 ? lim_hi / DA_BS : -1;  // this wave's last block
-    const int third = (int)(blockIdx.x / (uint32_t)(p.W * p.Hkv / 3 + 1));
+    PaTurns turns((int)(blockIdx.x / (uint32_t)(p.W * p.Hkv / 3 + 1)), x.mixed, j0);
     int sk = 0, sv = 1;  // this block's slots
     for (int i = j0; i < j1; ++i) {
       const int next = j + 1 < blocks.n_all ? j + 1 : 0, free = 3 - sk - sv;
-      pa_prefer(i + third);
+      turns.next();
       f32x16 st[2];
       px8 pw[2];
       if constexpr (KV8) {
