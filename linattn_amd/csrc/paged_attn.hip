@@ -377,9 +377,9 @@ constexpr int PA_WAVE_LDS = 12288;  // of a wave, where the waves of a workgroup
 // sixteen rows of K or V on their way into LDS of its own (fp8: four), of which one is used.
 // S^T = K Q^T by 16x16x32 products, O^T += V^T P^T by 16x16x16, P as the sum of two
 // terms of the type (16 bits of each weight), which the matrix cores have room for here.
-// One token each behind 48 caches of up to 16384 keys 309 us, 5.6 TB/s of the 6.0 that plain reads have;
-// behind 8 fp8 caches of up to 65537 140 us, 4.9 TB/s: widening codes takes registers and time, so that
-// fewer bytes are on their way.
+// One token each behind 48 caches of up to 16384 keys 307 us, 5.6 TB/s of the 6.0 that plain reads have;
+// behind 8 fp8 caches of up to 65537 136 us, 5.1 TB/s, the beginning and end of one wave of workgroups
+// among them.
 template <class T, int D, bool KV8, bool EVEN>
 __device__ __forceinline__ void pa_few(PaWalk *walk, char *smem, float *s_scale, uint32_t *s_bad) {
   typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V
@@ -627,9 +627,9 @@ __device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x
 // (KV8): codes of K and V go into LDS a block ahead, and are widened there once a workgroup (e4m3 is exact
 // in bf16 and fp16); the scale of a key multiplies its scores, that of its value its weights, both in fp32.
 //
-// Bound by matrix and vector unit in turn: 8192 tokens behind 24576 3.33 to 3.47 ms, 1.11 to 1.16 PFLOP/s
-// (a large product has 1.36), the matrix unit busy for 57 to 64 % of the cycles
-// at 1.75 to 1.55 GHz.  Products of the next block beside a block's weights (32 keys at a time, for the
+// Bound by matrix and vector unit in turn: 8192 tokens behind 24576 3.34 to 3.39 ms, 1.14 to 1.15 PFLOP/s
+// (a large product has 1.36), the matrix unit busy for 57 to 65 % of the cycles
+// at 1.75 to 1.53 GHz.  Products of the next block beside a block's weights (32 keys at a time, for the
 // registers) take 3.77 to 3.90 ms, two workgroups a CU with them 4.16.
 template <class T, int D, bool KV8, bool EVEN>
 __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_scale) {
