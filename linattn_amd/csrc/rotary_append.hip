@@ -8,7 +8,7 @@
 // taken by as many lanes as it has units, four rows of a lane on their way at a time.  Bound by the
 // rows' reads and writes: 14567 tokens of 32 + 8 + 8 heads of 128 bf16 values 76 us, 4.7 TB/s (a large
 // copy has 4.9); 2048 into an fp8 cache 14 us (bytes 9.5, then the chain from a token's sequence to its
-// page, its angles and its rows); 96 single tokens with page bounds 8 us, that chain alone.
+// page, its angles and its rows); 64 single tokens with page bounds 8 us, that chain alone.
 #include <algorithm>
 
 #include "rotary.h"

@@ -163,3 +163,35 @@ def test_a_captured_decode_step(dev, fp8):
         k.copy_(torch.randn(k.shape, generator=s.g))
         pos.add_(1)
         n.add_(1)
+
+
+@pytest.mark.parametrize("kind,D,page", [("bf16", 128, 64), ("bf16", 128, 24), ("fp32", 64, 64), ("fp8", 128, 64)])
+def test_pools_past_4_gib(dev, kind, D, page):
+    """Pages more than 2^32 bytes into their pools: the bits are those of small pools."""
+    Hq, Hkv, lq, before = 16, 8, [40, 1, 7], [100, 900, 0]
+    dtype = torch.float32 if kind == "fp32" else torch.bfloat16
+    held = torch.float8_e4m3fn if kind == "fp8" else dtype
+    size = Hkv * page * D * torch.empty((), dtype=held).element_size()
+    P = 1000 // page + 1
+    table = torch.arange(3 * P, dtype=torch.int32).view(3, P)
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (torch.randn(sum(lq), h, D, generator=g).to(dtype).to(dev) for h in (Hq, Hkv, Hkv))
+    old = [torch.randn(3 * P, Hkv, page, D, generator=g).to(held).to(dev) for _ in "kv"]
+    olds = torch.rand(2, 3 * P, Hkv, page, generator=g).to(dev)
+    cu, pos, freq = _i32([0, 40, 41, 48], dev), _i32(before, dev), torch.rand(D // 2, generator=g).to(dev)
+    lengths = _i32([a + b for a, b in zip(before, lq)], dev)
+    got = []
+    for first in (0, (1 << 32) // size + 1):
+        n = first + 3 * P
+        pools = [torch.empty(n, Hkv, page, D, dtype=held, device=dev) for _ in "kv"]
+        scales = list(fp8_scale_pairs(n, Hkv, page, dev)) if kind == "fp8" else []
+        for x, y in zip(pools + scales, old + list(olds)):
+            x[first:] = y
+        named = dict(zip(("k_scale", "v_scale"), scales))
+        t = (table + first).to(dev)
+        gq = rotary_kv_append(q, k, v, *pools, t, pos, freq, cu_seqlens=cu, **named)
+        out = paged_attention(gq, *pools, t, lengths, cu, **named)
+        one = paged_attention(gq[:3, :, None].contiguous(), *pools, t, lengths, **named)  # (single tokens, batched)
+        got.append([gq, out, one, *(x[first:].contiguous().view(torch.uint8) for x in pools), *(x[first:].clone() for x in scales)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
