@@ -198,10 +198,95 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_kernel(RaKP p) {
   }
 }
 
+__device__ __forceinline__ int64_t ra_floor(int64_t x, int64_t y) { return x / y - (x % y < 0); }
+
+// Packed: which sequence the page of bounds is of that number blk of all that new tokens touch is (-1: of none),
+// by all threads; blk becomes its place among the sequence's, or among those behind the last.
+__device__ __forceinline__ int ra_page(const RaKP &p, int64_t &blk) {
+  __shared__ int s_sum[RO_NT / 64];
+  __shared__ int2 s_at;  // the sequence (or the first of some that hold it), the pages before it
+  const int tid = threadIdx.x, lane = tid & 63, mp = p.meta_page;
+  // pages that sequence x touches; a thread counts a sequence, or, of more than there are threads, as
+  // many that lie one behind the other
+  const int B = (int)p.B, each = (B + RO_NT - 1) / RO_NT;
+  auto pages = [&](int x, int end) -> int {
+    const int y = min(x, B - 1);
+    const int64_t m = ra_cu(p, y + 1) - ra_cu(p, y), at = p.positions[y];
+    return x < end && m > 0 ? (int)(ra_floor(at + m - 1, mp) - ra_floor(at, mp) + 1) : 0;
+  };
+  auto scan = [&](int sum) -> int {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += y;
+    }
+    return sum;
+  };
+  int c = 0;
+#pragma unroll 4
+  for (int i = 0; i < each; ++i) c += pages(tid * each + i, B);
+  int sum = scan(c), before = 0, all = 0;
+  if (lane == 63) s_sum[tid >> 6] = sum;
+  if (tid == 0) s_at = int2{-1, 0};
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < RO_NT / 64; ++w) {
+    if (w < tid >> 6) before += s_sum[w];
+    all += s_sum[w];
+  }
+  if (before + sum - c <= blk && blk < before + sum) s_at = int2{tid * each, before + sum - c};
+  __syncthreads();
+  int b = s_at.x;
+  blk -= b < 0 ? all : s_at.y;
+  if (b >= 0 && each > 1) {
+    for (const int end = min(b + each, B);; b += 64) {
+      c = pages(b + lane, end);
+      sum = scan(c);
+      const int here = __shfl(sum, 63, 64);
+      if (blk < here || b + 64 >= end) break;
+      blk -= here;
+    }
+    const int at = max(__ffsll((unsigned long long)__ballot(sum > blk)) - 1, 0);
+    blk -= __shfl(sum - c, at, 64);
+    b = min(b + at, B - 1);
+  }
+  return b;
+}
+
+// The least and largest of the slots' (V-value pairs `least`, `most` of each thread) into bounds of a page.
+template <class E, int V>
+__device__ __forceinline__ void ra_bounds(const RaKP &p, const float (&least)[2 * V],
+                                          const float (&most)[2 * V], float *s_red, int b, int kvh, int64_t page, int64_t pos0,
+                                          int64_t tokens) {
+  typedef RoUnit<E, V> U;
+  const int tid = threadIdx.x, n = p.an.n, mp = p.meta_page, slots = RO_NT / p.units, slot = tid / p.units, u = tid - slot * p.units;
+  // a page that starts among the new tokens holds only them; else its old bounds cover the others
+  const bool fresh = page * mp >= pos0;
+  const int used = (int)min((int64_t)slots, tokens), cols = p.units * 2 * V;
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    if (slot < used)
+#pragma unroll
+      for (int j = 0; j < 2 * V; ++j) s_red[slot * cols + j * p.units + u] = side ? most[j] : least[j];
+    __syncthreads();
+    for (int e = tid; e < cols; e += RO_NT) {
+      const int j = e / p.units;
+      const U at(e - j * p.units, p.D, n, p.an.interleaved);
+      if (j >= V && at.ob < 0) continue;
+      float x = s_red[e];
+      for (int s = 1; s < used; ++s) x = side ? fmaxf(x, s_red[s * cols + e]) : fminf(x, s_red[s * cols + e]);
+      E *to = (E *)(side ? p.mx : p.mn) + b * p.m_sb + kvh * p.m_sh + page * p.m_sp + (j < V ? at.oa + j : at.ob + j - V) * p.m_sd;
+      if (!fresh) x = side ? fmaxf(x, (float)*to) : fminf(x, (float)*to);
+      *to = (E)x;
+    }
+    __syncthreads();
+  }
+}
+
 // With page bounds: a workgroup takes the new tokens of one page of bounds of one sequence, and one KV
 // head with its group of q, so that a page's least and largest keys are found without atomics.  Which
 // page that is every workgroup finds by itself: in a batch of 4096 slots with 64 tokens in all that takes
-// no time beside the rest (14 us, as without the empty slots), with 4096 tokens 189 us.
+// no time beside the rest (14 us, as without the empty slots).
 template <class E, int V>
 __global__ __launch_bounds__(RO_NT) void rotary_append_bounds_kernel(RaKP p) {
   typedef RoUnit<E, V> U;
@@ -209,59 +294,14 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_bounds_kernel(RaKP p) {
   extern __shared__ float2 cs[];
   __shared__ RaToken s_tok[TOK];
   __shared__ float s_red[RO_NT * 2 * V];
-  __shared__ int s_any, s_sum[RO_NT / 64];
-  __shared__ int2 s_at;  // the sequence that is looked for (or the first of some that hold it), the pages before it
-  const int tid = threadIdx.x, lane = tid & 63, n = p.an.n, mp = p.meta_page;
+  __shared__ int s_any;
+  const int tid = threadIdx.x, n = p.an.n, mp = p.meta_page;
   const int kvh = (int)(blockIdx.x % (uint32_t)p.Hkv), G = p.Hq / p.Hkv;
   int64_t blk = blockIdx.x / (uint32_t)p.Hkv;
-  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
   int b = -1;
   int64_t pos0 = 0, first = 0, new_tokens = 0;  // its position, its first row (packed), its tokens
   if (p.cu) {
-    // pages that sequence x touches; a thread counts a sequence, or, of more than there are threads, as
-    // many that lie one behind the other
-    const int B = (int)p.B, each = (B + RO_NT - 1) / RO_NT;
-    auto pages = [&](int x, int end) -> int {
-      const int y = min(x, B - 1);
-      const int64_t m = ra_cu(p, y + 1) - ra_cu(p, y), at = p.positions[y];
-      return x < end && m > 0 ? (int)(floor_div(at + m - 1, mp) - floor_div(at, mp) + 1) : 0;
-    };
-    auto scan = [&](int sum) -> int {
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += y;
-      }
-      return sum;
-    };
-    int c = 0;
-#pragma unroll 4
-    for (int i = 0; i < each; ++i) c += pages(tid * each + i, B);
-    int sum = scan(c), before = 0, all = 0;
-    if (lane == 63) s_sum[tid >> 6] = sum;
-    if (tid == 0) s_at = int2{-1, 0};
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < RO_NT / 64; ++w) {
-      if (w < tid >> 6) before += s_sum[w];
-      all += s_sum[w];
-    }
-    if (before + sum - c <= blk && blk < before + sum) s_at = int2{tid * each, before + sum - c};
-    __syncthreads();
-    b = s_at.x;
-    blk -= b < 0 ? all : s_at.y;
-    if (b >= 0 && each > 1) {
-      for (const int end = min(b + each, B);; b += 64) {
-        c = pages(b + lane, end);
-        sum = scan(c);
-        const int here = __shfl(sum, 63, 64);
-        if (blk < here || b + 64 >= end) break;
-        blk -= here;
-      }
-      const int at = max(__ffsll((unsigned long long)__ballot(sum > blk)) - 1, 0);
-      blk -= __shfl(sum - c, at, 64);
-      b = min(b + at, B - 1);
-    }
+    b = ra_page(p, blk);
     if (b >= 0) {
       first = ra_cu(p, b);
       new_tokens = max(ra_cu(p, b + 1) - first, (int64_t)0);
@@ -282,7 +322,7 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_bounds_kernel(RaKP p) {
     return;
   }
   pos0 = p.positions[b];
-  const int64_t page = floor_div(pos0, mp) + blk;
+  const int64_t page = ra_floor(pos0, mp) + blk;
   const int64_t lo = max(page * mp, pos0), hi = min((page + 1) * mp, pos0 + new_tokens);
   if (lo >= hi) return;  // (batched: fewer pages than there could be)
   const int xb = p.cu ? 0 : b;
@@ -338,26 +378,74 @@ __global__ __launch_bounds__(RO_NT) void rotary_append_bounds_kernel(RaKP p) {
   }
   __syncthreads();
   if (!s_any || page < 0 || page >= p.n_pages) return;  // (a token on no page counts in no bounds)
-  // a page that starts among the new tokens holds only them; else its old bounds cover the others
-  const bool fresh = page * mp >= pos0;
-  const int used = (int)min((int64_t)slots, hi - lo), cols = p.units * 2 * V;
+  ra_bounds<E, V>(p, least, most, s_red, b, kvh, page, pos0, hi - lo);
+}
+
+// The bounds alone, of the keys as rotary_append_kernel has stored them: a workgroup takes a page of bounds and
+// `hs` KV heads, as many as leave four workgroups a CU (1024 single tokens 36 us, with a head each 66).
+// Bound by the chain from the page's sequence to its keys, and by LDS, where the slots come together.
+template <class E, int V>
+__global__ __launch_bounds__(RO_NT) void rotary_bounds_kernel(RaKP p) {
+  typedef RoUnit<E, V> U;
+  __shared__ int64_t s_row[RO_NT];
+  __shared__ float s_red[RO_NT * 2 * V];
+  __shared__ int s_any;
+  const int tid = threadIdx.x, mp = p.meta_page, groups = p.Hkv / p.hs;
+  const int h0 = (int)(blockIdx.x % (uint32_t)groups) * p.hs;
+  int64_t blk = blockIdx.x / (uint32_t)groups, new_tokens = p.T;
+  int b = 0;
+  if (p.cu) {
+    b = ra_page(p, blk);
+    if (b < 0) return;  // (fewer pages than there could be)
+    new_tokens = max(ra_cu(p, b + 1) - ra_cu(p, b), 0);
+  } else {
+    const int64_t per = p.blocks / p.B;
+    b = (int)(blk / per);
+    blk -= b * per;
+  }
+  const int64_t pos0 = p.positions[b], page = ra_floor(pos0, mp) + blk;
+  const int64_t lo = max(page * mp, pos0), hi = min((page + 1) * mp, pos0 + new_tokens);
+  if (lo >= hi || page < 0 || page >= p.n_pages) return;
+  const int slots = RO_NT / p.units, slot = tid / p.units, u = tid - slot * p.units;
+  const U unit(u, p.D, p.an.n, p.an.interleaved);
+  if (tid == 0) s_any = 0;
+  for (int kvh = h0; kvh < h0 + p.hs; ++kvh) {
+    float least[2 * V], most[2 * V];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    if (slot < used)
+    for (int i = 0; i < 2 * V; ++i) {
+      least[i] = __int_as_float(0x7f800000);
+      most[i] = __int_as_float(0xff800000);
+    }
+    for (int64_t base = lo; base < hi; base += RO_NT) {
+      const int count = (int)min((int64_t)RO_NT, hi - base);
+      if (kvh == h0 || hi - lo > RO_NT) {  // (else they are there)
+        __syncthreads();
+        if (tid < count) {
+          const int64_t row = ra_token(p, b, base + tid - pos0, 0, 0).row;
+          s_row[tid] = row;
+          if (row >= 0) s_any = 1;
+        }
+        __syncthreads();
+      }
+      if (slot < slots)
+#pragma unroll 4
+        for (int i = slot; i < count; i += slots) {
+          const int64_t row = s_row[i];
+          if (row < 0) continue;
+          typename U::vec a, c;
+          unit.load((const E *)p.k_pool + (row + (int64_t)kvh * p.pool_page) * p.D, a, c);
+          float y[2 * V];
+          U::widen(a, c, y);
 #pragma unroll
-      for (int j = 0; j < 2 * V; ++j) s_red[slot * cols + j * p.units + u] = side ? most[j] : least[j];
-    __syncthreads();
-    for (int e = tid; e < cols; e += RO_NT) {
-      const int j = e / p.units;
-      const U at(e - j * p.units, p.D, n, p.an.interleaved);
-      if (j >= V && at.ob < 0) continue;
-      float x = s_red[e];
-      for (int s = 1; s < used; ++s) x = side ? fmaxf(x, s_red[s * cols + e]) : fminf(x, s_red[s * cols + e]);
-      E *to = (E *)(side ? p.mx : p.mn) + b * p.m_sb + kvh * p.m_sh + page * p.m_sp + (j < V ? at.oa + j : at.ob + j - V) * p.m_sd;
-      if (!fresh) x = side ? fmaxf(x, (float)*to) : fminf(x, (float)*to);
-      *to = (E)x;
+          for (int j = 0; j < 2 * V; ++j) {
+            least[j] = fminf(least[j], y[j]);
+            most[j] = fmaxf(most[j], y[j]);
+          }
+        }
     }
     __syncthreads();
+    if (!s_any) return;  // (a token on no page counts in no bounds)
+    ra_bounds<E, V>(p, least, most, s_red, b, kvh, page, pos0, hi - lo);
   }
 }
 
@@ -370,16 +458,21 @@ static int ra_launch(RaKP p, hipStream_t st) {
     if (p.lanes > 64) return fail(LA_ERR_UNSUPPORTED, "la_rotary_append: fp8 rows of %d values need aligned chunks", p.D);
   }
   const size_t turns = (size_t)p.an.n * sizeof(float2);
+  const int64_t tokens = p.cu ? p.T : p.B * p.T;
   if (p.mn) {
     // (packed: no more than a token each, or than the tokens fill and one at either end of each sequence;
     // and one for the rest)
     p.blocks = p.cu ? std::min(p.T, p.T / p.meta_page + 2 * p.B) + 1 : p.B * (ceil_div(p.T - 1, p.meta_page) + 1);
     LA_REQUIRE(grid_fits(p.blocks * p.Hkv, RO_NT), "la_rotary_append: too many tokens");
-    rotary_append_bounds_kernel<E, V><<<dim3((uint32_t)(p.blocks * p.Hkv)), RO_NT, 32 * turns, st>>>(p);
-    LA_LAUNCHED();
-    return LA_OK;
+    // few tokens in one launch; of more its angles, once a KV head, cost more than a launch (64 tokens 14.0 us,
+    // in two 14.7; 128 of four sequences 17.6 and 14.9, 2048 31 and 23, twelve prompts into pages of 16
+    // 141 and 110, 256 single ones 20.5 and 15.5)
+    if (tokens < 128) {
+      rotary_append_bounds_kernel<E, V><<<dim3((uint32_t)(p.blocks * p.Hkv)), RO_NT, 32 * turns, st>>>(p);
+      LA_LAUNCHED();
+      return LA_OK;
+    }
   }
-  const int64_t tokens = p.cu ? p.T : p.B * p.T;
   const int slots = RO_NT / p.lanes, R = p.Hq + 2 * p.Hkv;
   // tokens of a workgroup: about eight rows a lane, where there are tokens for every CU (twelve prompts
   // into pages of 16 76 us, with four rows a lane 81, sixteen 77; into fp8 72, 82 and 70)
@@ -390,6 +483,12 @@ static int ra_launch(RaKP p, hipStream_t st) {
   LA_REQUIRE(grid_fits(wgs, RO_NT), "la_rotary_append: too many tokens");
   rotary_append_kernel<E, V><<<dim3((uint32_t)wgs), RO_NT, p.ts * turns, st>>>(p);
   LA_LAUNCHED();
+  if (p.mn) {
+    p.hs = (int32_t)std::min<int64_t>(p.Hkv, std::max<int64_t>(1, p.blocks * p.Hkv / (4 * num_cus())));
+    while (p.Hkv % p.hs) --p.hs;
+    rotary_bounds_kernel<E, V><<<dim3((uint32_t)(p.blocks * (p.Hkv / p.hs))), RO_NT, 0, st>>>(p);
+    LA_LAUNCHED();
+  }
   return LA_OK;
 }
 

@@ -424,3 +424,47 @@ def test_batches_of_mostly_empty_sequences(dev, with_bounds, B):
     if with_bounds:
         emn, emx = bounds(mn, mx, stored, b, t, ok, before, page)
         assert torch.equal(gmn.cpu(), emn) and torch.equal(gmx.cpu(), emx)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float32, 80), (torch.float16, 30)])
+@pytest.mark.parametrize("page,mp", [(16, 16), (24, 300), (64, 48)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_many_tokens_as_few_at_a_time(dev, dtype, D, page, mp, packed):
+    """What a call turns and stores is what calls of a few tokens each do, bit for bit, and its bounds are of
+    the keys as stored: pages of more tokens than a workgroup has threads, places outside of the table and
+    pages outside of the pool among them.  (The bounds of both need not be the same: where a page's first
+    tokens are stored nowhere, a later call that brings its others keeps its old bounds.)"""
+    Hq, Hkv, T, before = 8, 4, 410, [-9, 37, 700, 0]
+    B, P = len(before), 1100 // page
+    g = torch.Generator().manual_seed(44)
+    table = torch.randperm(B * P, generator=g).int().view(B, P)
+    table[1, 100 // page], table[3, 0] = -1, 10 ** 6
+    table = table.to(dev)
+    q, k, v = (torch.randn(B, T, h, D, generator=g).to(dtype).to(dev) for h in (Hq, Hkv, Hkv))
+    old = [torch.randn(B * P, Hkv, page, D, generator=g).to(dtype).to(dev) for _ in "kv"]
+    M = P * page // mp + 1
+    low = (torch.randn(B, Hkv, M, D, generator=g) - 1).to(dtype).to(dev)
+    freq, results = _freq(D // 2).to(dev), []
+    for step in (T, 30 if packed else 31):
+        pools, mn, mx = [x.clone() for x in old], low.clone(), -low
+        out, want = [], (low.cpu(), -low.cpu())
+        for t in range(0, T, step):
+            n = min(step, T - t)
+            part = [x[:, t:t + n] for x in (q, k, v)]
+            pos = _i32([b + t for b in before], dev)
+            more = dict(page_min=mn, page_max=mx, page_size=mp)
+            if packed:
+                o = rotary_kv_append(*[x.reshape(B * n, -1, D) for x in part], *pools, table, pos, freq,
+                                     cu_seqlens=_i32([n * b for b in range(B + 1)], dev), **more).view(B, n, Hq, D)
+            else:
+                o = rotary_kv_append(*[x.transpose(1, 2) for x in part], *pools, table, pos, freq, **more).transpose(1, 2)
+            out.append(o)
+            at = [b + t for b in before]
+            seq, place = places(at, [n] * B)
+            ok, phys, slot = slots(table.cpu(), seq, place, page, B * P)
+            want = bounds(*want, pools[0].cpu()[phys, :, slot], seq, place, ok, at, mp)
+            for got, x in zip((mn, mx), want):
+                assert torch.equal(got.cpu(), x), (step, t)
+        results.append([torch.cat(out, 1), *pools])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
