@@ -350,17 +350,19 @@ def by_bytes(cls: type, *names: str) -> Tuple[Callable[..., bytes], Callable[[],
     null pointer is 0) as ``cls`` lays them out, 1.7 us faster than the struct of the larger
     ones, and what returns the library's functions ``names`` taking those bytes (and a stream)."""
     pack = struct.Struct("@" + "".join(_FORMAT[t] for _, t in cls._fields_)).pack
-    found: list = []
+    found: Optional[Tuple] = None
 
     def functions() -> Tuple:
-        if not found:
-            lib = load()
+        nonlocal found
+        if found is None:
+            lib, made = load(), []
             for name in names:
                 fn = lib[name]
                 plain = getattr(lib, name)
                 fn.restype = plain.restype
                 fn.argtypes = [ctypes.c_char_p, *plain.argtypes[1:]]
-                found.append(fn)
+                made.append(fn)
+            found = tuple(made)  # (whole at once: threads whose first calls meet make one each)
         return found
 
     return pack, functions
