@@ -49,9 +49,9 @@ struct Cover {
     int64_t stride, count;
   };
   int64_t p, run, end;  // (run 0: nothing; p is its lowest byte, end is behind its last)
-  Dim dim[3];
-  Cover(const void *at, int64_t bytes, Dim x = {0, 1}, Dim y = {0, 1}, Dim z = {0, 1})
-      : p((int64_t)(uintptr_t)at), run(at ? bytes : 0), dim{x, y, z} {
+  Dim dim[4];
+  Cover(const void *at, int64_t bytes, Dim x = {0, 1}, Dim y = {0, 1}, Dim z = {0, 1}, Dim w = {0, 1})
+      : p((int64_t)(uintptr_t)at), run(at ? bytes : 0), dim{x, y, z, w} {
     int64_t up = run;
     for (Dim &d : dim) {
       if (d.count <= 0) run = 0;
@@ -70,6 +70,20 @@ struct Cover {
 bool overlap_runs(const Cover &a, const Cover &b);
 inline bool overlap(const Cover &a, const Cover &b) {
   return a.run > 0 && b.run > 0 && a.p < b.end && b.p < a.end && overlap_runs(a, b);
+}
+// Whether one of them holds some of its bytes twice: its strides do not nest.
+bool overlap_self(const Cover &a);
+// Whether what a call writes holds bytes twice, or shares some with what else it writes or reads.
+template <size_t W, size_t R>
+inline bool overlap_any(const Cover (&written)[W], const Cover (&read)[R]) {
+  for (size_t i = 0; i < W; ++i) {
+    if (overlap_self(written[i])) return true;
+    for (size_t j = i + 1; j < W; ++j)
+      if (overlap(written[i], written[j])) return true;
+    for (const Cover &r : read)
+      if (overlap(written[i], r)) return true;
+  }
+  return false;
 }
 
 // Whether a launch may have that many workgroups (2^32 threads are too many).

@@ -63,7 +63,7 @@ static bool overlap_from(const OverlapTerm *t, int n, int64_t at, int64_t low, i
 }
 
 bool overlap_runs(const Cover &a, const Cover &b) {
-  OverlapTerm t[6];
+  OverlapTerm t[8];
   int n = 0;
   for (const Cover *x : {&a, &b})
     for (const Cover::Dim &d : x->dim) {
@@ -77,6 +77,21 @@ bool overlap_runs(const Cover &a, const Cover &b) {
   std::sort(t, t + n, [](const OverlapTerm &x, const OverlapTerm &y) { return x.s > y.s; });
   int left = 4096;
   return overlap_from(t, n, a.p - b.p, -a.run, b.run, &left);
+}
+
+bool overlap_self(const Cover &a) {
+  if (a.run == 0) return false;
+  Cover::Dim d[4];
+  int n = 0;
+  for (const Cover::Dim &x : a.dim)
+    if (x.count > 1) d[n++] = x;
+  std::sort(d, d + n, [](const Cover::Dim &x, const Cover::Dim &y) { return x.stride < y.stride; });
+  int64_t extent = a.run;
+  for (int i = 0; i < n; ++i) {
+    if (d[i].stride < extent) return true;
+    extent += d[i].stride * (d[i].count - 1);
+  }
+  return false;
 }
 
 }  // namespace la

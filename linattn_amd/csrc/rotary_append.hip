@@ -537,20 +537,31 @@ extern "C" int la_rotary_append(const la_rotary_append_args *args, void *stream)
   auto cover = [&](const void *y, int64_t b, int64_t h, int64_t t, int64_t heads) {
     return Cover(y, a->D * esz, {b * esz, nb}, {h * esz, heads}, {t * esz, a->T});
   };
-  const Cover q = cover(a->Hq ? a->q : nullptr, a->q_sb, a->q_sh, a->q_st, a->Hq);
-  const Cover out = cover(a->Hq ? a->q_out : nullptr, a->o_sb, a->o_sh, a->o_st, a->Hq);
-  const Cover kn = cover(a->k_new, a->kn_sb, a->kn_sh, a->kn_st, a->Hkv), vn = cover(a->v_new, a->vn_sb, a->vn_sh, a->vn_st, a->Hkv);
-  const int64_t pool = a->n_phys * a->Hkv * a->pool_page;
-  const Cover kp(a->k_pool, pool * a->D * psz), vp(a->v_pool, pool * a->D * psz);
+  const int64_t pool = a->n_phys * a->Hkv * a->pool_page, m_run = a->m_sd == 1 ? a->D : 1;
+  auto page_bounds = [&](const void *y) {
+    return Cover(meta ? y : nullptr, m_run * esz, {a->m_sb * esz, a->B}, {a->m_sh * esz, a->Hkv}, {a->m_sp * esz, a->n_pages},
+                 {a->m_sd * esz, a->D / m_run});
+  };
   const Cover::Dim each{a->s_stride * 4, pool};
-  const Cover ks(fp8 ? a->k_scale : nullptr, 4, each), vs(fp8 ? a->v_scale : nullptr, 4, each);
+  const Cover written[] = {cover(a->Hq ? a->q_out : nullptr, a->o_sb, a->o_sh, a->o_st, a->Hq),
+                           Cover(a->k_pool, pool * a->D * psz),
+                           Cover(a->v_pool, pool * a->D * psz),
+                           Cover(fp8 ? a->k_scale : nullptr, 4, each),
+                           Cover(fp8 ? a->v_scale : nullptr, 4, each),
+                           page_bounds(a->page_min),
+                           page_bounds(a->page_max)};
+  // (in place: the same rows, each of which the lanes that write it have read)
   const bool in = a->q_out == a->q && a->o_sb == a->q_sb && a->o_sh == a->q_sh && a->o_st == a->q_st;
-  LA_REQUIRE((in || !overlap(out, q)) && !overlap(out, kn) && !overlap(out, vn) && !overlap(out, kp) && !overlap(out, vp) &&
-                 !overlap(kp, vp) && !overlap(kp, q) && !overlap(kp, kn) && !overlap(kp, vn) && !overlap(vp, q) &&
-                 !overlap(vp, kn) && !overlap(vp, vn) && !overlap(ks, vs) && !overlap(ks, kp) && !overlap(ks, vp) &&
-                 !overlap(vs, kp) && !overlap(vs, vp) && !overlap(ks, out) && !overlap(vs, out) && !overlap(ks, q) &&
-                 !overlap(vs, q) && !overlap(ks, kn) && !overlap(vs, kn) && !overlap(ks, vn) && !overlap(vs, vn),
-             "la_rotary_append: what is written shares memory with another argument");
+  const Cover read[] = {cover(a->Hq && !in ? a->q : nullptr, a->q_sb, a->q_sh, a->q_st, a->Hq),
+                        cover(a->k_new, a->kn_sb, a->kn_sh, a->kn_st, a->Hkv),
+                        cover(a->v_new, a->vn_sb, a->vn_sh, a->vn_st, a->Hkv),
+                        Cover(a->page_table, a->pt_pages * 4, {a->pt_sb * 4, a->B}),
+                        Cover(a->positions, a->B * 4),
+                        Cover(a->cu, (a->B + 1) * 4),
+                        Cover(a->rot_positions, 4, {a->p_sa * 4, a->A}, {a->p_sb * 4, nb}, {a->p_st * 4, a->T}),
+                        Cover(a->inv_freq, a->n * 4),
+                        Cover(a->axes, a->n * 4)};
+  LA_REQUIRE(!overlap_any(written, read), "la_rotary_append: what is written shares memory with another argument");
   RaKP p{};
   p.an = RoAngles{a->rot_positions, a->axes, a->inv_freq, a->p_sa, a->p_sb, a->p_st, (int32_t)a->n, (int32_t)a->A,
                   a->interleaved != 0, 0};

@@ -1,0 +1,110 @@
+"""What ``la_rotary``, ``la_rotary_append`` and ``la_paged_attention`` write shares no memory with itself or
+with anything else that they read or write: refused before anything is launched.  The addresses
+are made up; calls whose memory is apart end at something else that they lack."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from linattn_amd import _native as N
+
+BASE, FAR = 1 << 40, 1 << 32
+
+
+def _said(fn, a):
+    lib = N.load()
+    rc = getattr(lib, fn)(ctypes.byref(a), None)
+    assert rc in (N.LA_ERR_INVALID, N.LA_ERR_UNSUPPORTED, N.LA_ERR_WORKSPACE), (rc, lib.la_last_error())
+    return lib.la_last_error().decode()
+
+
+# ------------------------------------------------------------- page bounds ----
+B, HKV, P, D, PAGES = 2, 2, 5, 64, 6 * 2 * 16  # PAGES: rows of the pools
+
+
+def _append(minor=False):
+    """An fp32 call with page bounds, pages (or dims) side by side, whose k_new is not aligned: what
+    is refused for nothing else is refused for that."""
+    a = N.LaRotaryAppendArgs()
+    names = ("q", "k_new", "v_new", "q_out", "k_pool", "v_pool", "page_table", "positions", "inv_freq", "page_min", "page_max")
+    at = {name: BASE + i * FAR for i, name in enumerate(names)}
+    for name, x in at.items():
+        setattr(a, name, x)
+    a.k_new += 2
+    a.B, a.T, a.Hq, a.Hkv, a.D, a.n, a.A = B, 8, 4, HKV, D, 32, 1
+    a.q_sb, a.q_sh, a.q_st = a.o_sb, a.o_sh, a.o_st = 2048, 512, 64
+    a.kn_sb, a.kn_sh, a.kn_st = a.vn_sb, a.vn_sh, a.vn_st = 1024, 512, 64
+    a.n_phys, a.pool_page, a.pt_sb, a.pt_pages, a.s_stride = 6, 16, 4, 4, 1
+    a.meta_page, a.n_pages = 16, P
+    a.m_sb, a.m_sh, a.m_sp, a.m_sd = (HKV * P * D, P * D, 1, P) if minor else (HKV * P * D, P * D, D, 1)
+    return a, at
+
+
+@pytest.mark.parametrize("minor", [False, True])
+def test_page_bounds_apart(minor):
+    a, at = _append(minor)
+    assert "unaligned" in _said("la_rotary_append", a)
+    # halves of one buffer, value by value, page by page, and one behind the other
+    size = 4 * B * HKV * P * D
+    a.page_max = a.page_min + size
+    assert "unaligned" in _said("la_rotary_append", a)
+    a, at = _append(minor)
+    a.m_sb, a.m_sh, a.m_sp, a.m_sd = (2 * x for x in (a.m_sb, a.m_sh, a.m_sp, a.m_sd))
+    a.page_max = a.page_min + 4
+    assert "unaligned" in _said("la_rotary_append", a)
+    a, at = _append()
+    a.m_sb, a.m_sh, a.m_sp = 2 * a.m_sb, 2 * a.m_sh, 2 * a.m_sp
+    a.page_max = a.page_min + 4 * D
+    assert "unaligned" in _said("la_rotary_append", a)
+
+
+@pytest.mark.parametrize("minor", [False, True])
+@pytest.mark.parametrize("change", [
+    lambda a, at: dict(page_max=at["page_min"]),
+    lambda a, at: dict(page_max=at["page_min"] + 4 * B * HKV * P * D - 4),
+    lambda a, at: dict(page_max=at["page_min"] - 4),
+    lambda a, at: dict(page_min=at["k_pool"] + PAGES * D * 4 - 4),
+    lambda a, at: dict(page_max=at["v_pool"]),
+    lambda a, at: dict(page_min=at["q_out"] + 256),
+    lambda a, at: dict(page_max=at["q"]),
+    lambda a, at: dict(page_min=at["k_new"] + 4096),
+    lambda a, at: dict(page_max=at["v_new"]),
+    lambda a, at: dict(page_min=at["page_table"]),
+    lambda a, at: dict(page_max=at["positions"]),
+    lambda a, at: dict(page_max=at["inv_freq"] + 31 * 4),
+    lambda a, at: dict(m_sb=0),                     # rows held twice
+    lambda a, at: dict(m_sh=0),
+    lambda a, at: dict(m_sp=0),
+    lambda a, at: dict(m_sd=0),
+    lambda a, at: dict(m_sb=a.m_sh),
+])
+def test_page_bounds_over_others(minor, change):
+    a, at = _append(minor)
+    for name, x in change(a, at).items():
+        setattr(a, name, x)
+    assert "shares memory" in _said("la_rotary_append", a)
+
+
+def test_what_else_an_append_writes():
+    for change in (dict(k_pool="page_table"), dict(v_pool="positions"), dict(q_out="inv_freq"), dict(v_pool="k_pool")):
+        a, at = _append()
+        for name, of in change.items():
+            setattr(a, name, at[of])
+        assert "shares memory" in _said("la_rotary_append", a), change
+    for extra in ("cu", "axes", "rot_positions"):
+        a, at = _append()
+        a.p_sb, a.p_st = 8, 1
+        setattr(a, extra, at["k_pool"] + 64)
+        assert "shares memory" in _said("la_rotary_append", a), extra
+    for name in ("o_sb", "o_sh", "o_st"):  # rows of q_out held twice, in place too
+        for place in ("q_out", "q"):
+            a, at = _append()
+            a.q_out = at[place]
+            setattr(a, name, 0)
+            setattr(a, name.replace("o_", "q_"), 0)
+            assert "shares memory" in _said("la_rotary_append", a), (name, place)
+    a, at = _append()
+    a.q_out = a.q  # (in place)
+    assert "unaligned" in _said("la_rotary_append", a)
