@@ -942,7 +942,8 @@ int la_rotary_append(const la_rotary_append_args *a, void *stream);
  * LA_F16), or, with 16-bit dtype, e4m3 codes with fp32 scales of K and V per token (n_phys,
  * Hkv, page) at stride s_stride.  out_dtype is dtype or LA_F32; D 64 or 128; rows of q and out
  * 16-byte aligned; lse (optional, fp32) has strides l_sb, l_sh and 1.  The cache has less than
- * 2^32 rows.  scale must be positive; out shares no memory with q and the cache.  Workspace:
+ * 2^32 rows.  scale must be positive; out, lse and the workspace share no memory with
+ * anything else, and hold their rows once.  Workspace:
  * la_paged_attention_workspace() bytes, 256-byte aligned (the parts of tiles that several
  * workgroups share).  The same call gives the same bits.
  */

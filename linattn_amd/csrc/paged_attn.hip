@@ -1353,10 +1353,20 @@ extern "C" int la_paged_attention(const la_paged_attn_args *args, void *stream) 
   LA_REQUIRE(a->page_table && a->lengths, "la_paged_attention: null page_table or lengths");
   LA_REQUIRE(!kv8 || (a->k_scale && a->v_scale && a->s_stride > 0), "la_paged_attention: fp8 cache needs scales");
   const int64_t pool = a->n_phys * a->Hkv * a->page * a->D * (kv8 ? 1 : esz);
-  const Cover out(a->out, a->D * osz, {a->o_sb * osz, nb}, {a->o_sh * osz, a->Hq}, {a->o_st * osz, a->Tq});
-  LA_REQUIRE(!overlap(out, Cover(a->q, a->D * esz, {a->q_sb * esz, nb}, {a->q_sh * esz, a->Hq}, {a->q_st * esz, a->Tq})) &&
-                 !overlap(out, Cover(a->k_pool, pool)) && !overlap(out, Cover(a->v_pool, pool)),
-             "la_paged_attention: out shares memory with an input");
+  const Cover::Dim each{a->s_stride * 4, a->n_phys * a->Hkv * a->page};
+  const Cover written[] = {Cover(a->out, a->D * osz, {a->o_sb * osz, nb}, {a->o_sh * osz, a->Hq}, {a->o_st * osz, a->Tq}),
+                           Cover(a->lse, a->Tq * 4, {a->l_sb * 4, nb}, {a->l_sh * 4, a->Hq}),
+                           Cover(a->workspace, a->ws_bytes)};
+  const Cover read[] = {Cover(a->q, a->D * esz, {a->q_sb * esz, nb}, {a->q_sh * esz, a->Hq}, {a->q_st * esz, a->Tq}),
+                        Cover(a->k_pool, pool),
+                        Cover(a->v_pool, pool),
+                        Cover(kv8 ? a->k_scale : nullptr, 4, each),
+                        Cover(kv8 ? a->v_scale : nullptr, 4, each),
+                        Cover(a->page_table, a->pt_pages * 4, {a->pt_sb * 4, a->B}),
+                        Cover(a->lengths, a->B * 4),
+                        Cover(a->cu_q, (a->B + 1) * 4),
+                        Cover(a->q_len, a->B * 4)};
+  LA_REQUIRE(!overlap_any(written, read), "la_paged_attention: out, lse or the workspace shares memory with another argument");
   const PaPlan pl = pa_plan(a);
   if (!a->workspace || a->ws_bytes < (int64_t)pl.bytes)
     return fail(LA_ERR_WORKSPACE, "la_paged_attention: workspace %lld < %lld bytes", (long long)a->ws_bytes, (long long)pl.bytes);

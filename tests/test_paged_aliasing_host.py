@@ -108,3 +108,73 @@ def test_what_else_an_append_writes():
     a, at = _append()
     a.q_out = a.q  # (in place)
     assert "unaligned" in _said("la_rotary_append", a)
+
+
+# --------------------------------------------------------------- attention ----
+def _attend(fp8=False):
+    """An fp16 call over a cache of 6 pages, which ends at its workspace."""
+    a = N.LaPagedAttnArgs()
+    names = ("q", "k_pool", "v_pool", "out", "lse", "page_table", "lengths", "workspace", "k_scale", "v_scale")
+    at = {name: BASE + i * FAR for i, name in enumerate(names)}
+    for name, x in at.items():
+        if fp8 or not name.endswith("scale"):
+            setattr(a, name, x)
+    a.B, a.Hq, a.Hkv, a.Tq, a.D = 2, 4, 2, 8, 64
+    a.q_sb, a.q_sh, a.q_st = a.o_sb, a.o_sh, a.o_st = 2048, 512, 64
+    a.l_sb, a.l_sh = 32, 8
+    a.n_phys, a.page, a.pt_sb, a.pt_pages, a.s_stride = 6, 16, 4, 4, 1
+    a.scale, a.causal, a.dtype, a.kv_dtype, a.out_dtype = 0.125, 1, N.LA_F16, N.LA_FP8_E4M3 if fp8 else N.LA_F16, N.LA_F16
+    return a, at
+
+
+@pytest.mark.parametrize("change", [
+    lambda a, at: dict(out=at["k_scale"] + PAGES * 4 - 16),
+    lambda a, at: dict(out=at["v_scale"]),
+    lambda a, at: dict(out=at["lse"]),
+    lambda a, at: dict(out=at["lengths"]),
+    lambda a, at: dict(out=at["page_table"] + 16),
+    lambda a, at: dict(lse=at["out"] + 4096),
+    lambda a, at: dict(lse=at["q"]),
+    lambda a, at: dict(lse=at["k_pool"] + 64),
+    lambda a, at: dict(lse=at["v_pool"] + PAGES * 64 - 4),
+    lambda a, at: dict(lse=at["k_scale"]),
+    lambda a, at: dict(lse=at["v_scale"] + 8),
+    lambda a, at: dict(lse=at["page_table"]),
+    lambda a, at: dict(lse=at["lengths"]),
+    lambda a, at: dict(cu_q=at["lse"], Tq=16),
+    lambda a, at: dict(q_len=at["out"]),
+    lambda a, at: dict(lse=at["workspace"], ws_bytes=256),
+    lambda a, at: dict(workspace=at["q"], ws_bytes=256),
+    lambda a, at: dict(workspace=at["out"] + 256, ws_bytes=256),
+    lambda a, at: dict(o_sb=0),                     # rows held twice
+    lambda a, at: dict(o_sh=0),
+    lambda a, at: dict(o_st=0),
+    lambda a, at: dict(l_sb=0),
+    lambda a, at: dict(l_sh=0),
+    lambda a, at: dict(l_sh=7),
+])
+def test_attention_over_others(change):
+    a, at = _attend(True)
+    for name, x in change(a, at).items():
+        setattr(a, name, x)
+    assert "shares memory" in _said("la_paged_attention", a)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_attention_apart(fp8):
+    a, at = _attend(fp8)
+    assert "workspace" in _said("la_paged_attention", a)
+    a.lse = None
+    a.l_sb = a.l_sh = 0
+    assert "workspace" in _said("la_paged_attention", a)
+    # out beside q, row by row; the halves of the scales' pairs
+    a, at = _attend(fp8)
+    a.out = a.q + 128
+    a.q_sb, a.q_sh, a.q_st = a.o_sb, a.o_sh, a.o_st = 4096, 1024, 128
+    if fp8:
+        a.s_stride, a.v_scale = 2, a.k_scale + 4
+    assert "workspace" in _said("la_paged_attention", a)
+    # packed: one row of lse a head
+    a, at = _attend(fp8)
+    a.cu_q, a.l_sb, a.q_sb, a.o_sb = BASE + 20 * FAR, 0, 0, 0
+    assert "workspace" in _said("la_paged_attention", a)
