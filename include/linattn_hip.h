@@ -852,7 +852,8 @@ int la_evict_decode(const la_evict_decode_args *a, void *stream);
  * q, q_out (B, Hq, T, D), k, k_out (B, Hkv, T, D) (Hkv 0: none) at strides *_sb, *_sh, *_st,
  * unit stride over D; positions (int32) of axis a, token (b, t) at a p_sa + b p_sb + t p_st;
  * inv_freq fp32 [n]; axes (int32 [n], clamped to 0 .. A - 1; null with A = 1).  D at most
- * 512.  q_out may be q and k_out may be k, else outputs share no memory with anything.
+ * 512.  q_out may be q and k_out may be k, else outputs share no memory with anything; they
+ * hold their rows once.
  */
 typedef struct {
   const void *q;

@@ -131,10 +131,14 @@ extern "C" int la_rotary(const la_rotary_args *args, void *stream) {
   // in place: the same rows, each of which one lane reads before it writes
   const bool q_in = a->q_out == a->q && a->qo_sb == a->q_sb && a->qo_sh == a->q_sh && a->qo_st == a->q_st;
   const bool k_in = a->k_out == a->k && a->ko_sb == a->k_sb && a->ko_sh == a->k_sh && a->ko_st == a->k_st;
-  const Cover q = cover(a->q, a->q_sb, a->q_sh, a->q_st, a->Hq), qo = cover(a->q_out, a->qo_sb, a->qo_sh, a->qo_st, a->Hq);
-  const Cover k = cover(a->k, a->k_sb, a->k_sh, a->k_st, a->Hkv), ko = cover(a->k_out, a->ko_sb, a->ko_sh, a->ko_st, a->Hkv);
-  LA_REQUIRE((q_in || !overlap(qo, q)) && !overlap(qo, k) && (k_in || !overlap(ko, k)) && !overlap(ko, q) && !overlap(qo, ko),
-             "la_rotary: an output shares memory with another argument");
+  const void *k = a->Hkv > 0 ? a->k : nullptr, *k_out = a->Hkv > 0 ? a->k_out : nullptr;
+  const Cover written[] = {cover(a->q_out, a->qo_sb, a->qo_sh, a->qo_st, a->Hq), cover(k_out, a->ko_sb, a->ko_sh, a->ko_st, a->Hkv)};
+  const Cover read[] = {cover(q_in ? nullptr : a->q, a->q_sb, a->q_sh, a->q_st, a->Hq),
+                        cover(k_in ? nullptr : k, a->k_sb, a->k_sh, a->k_st, a->Hkv),
+                        Cover(a->positions, 4, {a->p_sa * 4, a->A}, {a->p_sb * 4, a->B}, {a->p_st * 4, a->T}),
+                        Cover(a->inv_freq, a->n * 4),
+                        Cover(a->axes, a->n * 4)};
+  LA_REQUIRE(!overlap_any(written, read), "la_rotary: an output shares memory with another argument");
   RoKP p{};
   p.an = RoAngles{a->positions, a->axes, a->inv_freq, a->p_sa, a->p_sb, a->p_st, (int32_t)a->n, (int32_t)a->A,
                   a->interleaved != 0, a->inverse != 0};

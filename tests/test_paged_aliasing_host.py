@@ -178,3 +178,41 @@ def test_attention_apart(fp8):
     a, at = _attend(fp8)
     a.cu_q, a.l_sb, a.q_sb, a.o_sb = BASE + 20 * FAR, 0, 0, 0
     assert "workspace" in _said("la_paged_attention", a)
+
+
+# ------------------------------------------------------------------ rotary ----
+def _rotary():
+    a = N.LaRotaryArgs()
+    names = ("q", "k", "q_out", "k_out", "positions", "inv_freq", "axes")
+    at = {name: BASE + i * FAR for i, name in enumerate(names)}
+    for name, x in at.items():
+        setattr(a, name, x)
+    a.B, a.T, a.Hq, a.Hkv, a.D, a.n, a.A = 2, 8, 4, 2, 64, 32, 3
+    a.q_sb, a.q_sh, a.q_st = a.qo_sb, a.qo_sh, a.qo_st = 2048, 512, 64
+    a.k_sb, a.k_sh, a.k_st = a.ko_sb, a.ko_sh, a.ko_st = 1024, 512, 64
+    a.p_sa, a.p_sb, a.p_st = 16, 8, 1
+    a.dtype = N.LA_F32
+    return a, at
+
+
+@pytest.mark.parametrize("change", [
+    lambda at: dict(q_out=at["positions"] + 188),
+    lambda at: dict(k_out=at["positions"] - 256),
+    lambda at: dict(q_out=at["inv_freq"]),
+    lambda at: dict(k_out=at["axes"] + 124),
+    lambda at: dict(q_out=at["k_out"]),
+    lambda at: dict(k_out=at["q"] + 4),
+    lambda at: dict(qo_sb=0),
+    lambda at: dict(qo_sh=0),
+    lambda at: dict(qo_st=32),
+    lambda at: dict(ko_sb=0),
+    lambda at: dict(ko_sh=0),
+    lambda at: dict(ko_st=0),
+    lambda at: dict(q_out=at["q"], qo_sh=0, q_sh=0),  # (in place)
+    lambda at: dict(k_out=at["k"], ko_st=0, k_st=0),
+])
+def test_rotary_over_others(change):
+    a, at = _rotary()
+    for name, x in change(at).items():
+        setattr(a, name, x)
+    assert "shares memory" in _said("la_rotary", a)
