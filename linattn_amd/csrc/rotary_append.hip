@@ -587,10 +587,11 @@ extern "C" int la_rotary_append(const la_rotary_append_args *args, void *stream)
     at |= (uint64_t)(uintptr_t)a->q | (uint64_t)(uintptr_t)a->q_out;
     by |= (uint64_t)(a->q_sb | a->q_sh | a->q_st | a->o_sb | a->o_sh | a->o_st);
   }
-  // codes of a chunk are written four at a time: half or a quarter of the input's alignment
-  at |= ((uint64_t)(uintptr_t)a->k_pool | (uint64_t)(uintptr_t)a->v_pool) * (fp8 ? 4 : 1);
+  const uint64_t pools = (uint64_t)(uintptr_t)a->k_pool | (uint64_t)(uintptr_t)a->v_pool;
+  if (!fp8) at |= pools;
   hipStream_t st = (hipStream_t)stream;
-  const int v = ro_vector((int)esz, a->D, a->n, at, by);
+  // codes are written four at a time, of chunks of any size but one
+  const int v = fp8 && pools % 4 != 0 ? 1 : ro_vector((int)esz, a->D, a->n, at, by);
   LA_REQUIRE(at % esz == 0, "la_rotary_append: unaligned tensors");
   if (a->dtype == LA_F32) return v == 4 ? ra_launch<float, 4>(p, st) : ra_launch<float, 1>(p, st);
   if (a->dtype == LA_BF16)

@@ -216,3 +216,20 @@ def test_rotary_over_others(change):
     for name, x in change(at).items():
         setattr(a, name, x)
     assert "shares memory" in _said("la_rotary", a)
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_codes_of_unaligned_pools_are_not_written_four_at_a_time(off):
+    """Chunks of four 16-bit values (n = 36: rows of 256 have 64 of them) need pools at whole fours."""
+    a, at = _append()
+    a.page_min = a.page_max = None
+    a.k_new -= 2
+    a.dtype, a.pool_dtype, a.D, a.n = N.LA_BF16, N.LA_FP8_E4M3, 256, 36
+    a.k_scale, a.v_scale = BASE + 20 * FAR, BASE + 21 * FAR
+    for s in ("q_s", "o_s", "kn_s", "vn_s"):
+        for d in "bht":
+            setattr(a, s + d, 4 * getattr(a, s + d))
+    for name in ("k_pool", "v_pool"):
+        setattr(a, name, at[name] + off)
+        assert "aligned chunks" in _said("la_rotary_append", a)
+        setattr(a, name, at[name])
