@@ -619,8 +619,10 @@ __device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x
 
 // bf16 / fp16 rows: four waves of 32 rows, three workgroups a CU, and the products and registers of
 // dense_attn_kernel (S^T by 32x32x16 products leaves a lane 16 scores of one row; P goes into its
-// product with V from the same registers, rounded to the inputs' type (bf16 with an fp8 cache);
-// l is of the fp32 weights).
+// product with V from the same registers, rounded to the inputs' type; l is of the fp32 weights).
+// With an fp8 cache weights take the values' scales, whose range is fp32's, and are rounded to bf16; of
+// fp16 queries, whose bits that would lose, to two terms of bf16 (16 bits): chunks of four prompts
+// 325 us, with one term 271, and 2.1e-4 of the norm off in place of 1.7e-3.
 //
 // A wave stages 16 keys of each block of 64 (PaRows).  K and V of the blocks take three slots in turn,
 // so that each is on its way while the block before is scored and weighed.  fp8 caches
@@ -634,6 +636,7 @@ __device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x
 template <class T, int D, bool KV8, bool EVEN>
 __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_scale) {
   typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V
+  constexpr bool TWO = KV8 && !std::is_same<T, TP>::value;     // P in two terms
   constexpr int NW = 4, R = 32 * NW, BLK = DA_BS * D, NX = D / 32;
   constexpr int NS = D / 16, ND = D / 32;
   constexpr int SLOT = 2 * BLK;  // bytes; KV8: K, V, then codes of K and of V
@@ -790,7 +793,7 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
       }
     };
     // weights of half kt of a block, added among themselves first
-    auto weigh = [&](int kt, f32x16 &st, px8 (&pw)[2]) __attribute__((always_inline)) {
+    auto weigh = [&](int kt, f32x16 &st, px8 (&pw)[TWO ? 4 : 2]) __attribute__((always_inline)) {
       float sum[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -804,11 +807,16 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
         for (int g = 0; g < 4; ++g) {
           const f32x4 sc = *(const f32x4 *)(s_scale + DA_BS + 32 * kt + 8 * g + 4 * hf);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) pw[g >> 1][4 * (g & 1) + i] = (pelem)(st[4 * g + i] * sc[i]);
+          for (int i = 0; i < 4; ++i) {
+            const float x = st[4 * g + i] * sc[i];
+            const pelem hi = (pelem)x;
+            pw[g >> 1][4 * (g & 1) + i] = hi;
+            if constexpr (TWO) pw[2 + (g >> 1)][4 * (g & 1) + i] = (pelem)(x - (float)hi);
+          }
         }
       }
     };
-    auto values = [&](int slot, int kt, const px8 (&pw)[2]) __attribute__((always_inline)) {
+    auto values = [&](int slot, int kt, const px8 (&pw)[TWO ? 4 : 2]) __attribute__((always_inline)) {
       const uint32_t at = v_at + slot * SLOT;
 #pragma unroll
       for (int y = 0; y < 2; ++y)
@@ -817,7 +825,9 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
           const char *v = lds + (at ^ (64 * dt)) + 2 * (32 * kt + 16 * y) * D;
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)v);
           const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(v + 16 * D));
-          acc[dt] = TP::mfma(__builtin_bit_cast(px8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), pw[y], acc[dt]);
+          const px8 vt = __builtin_bit_cast(px8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          acc[dt] = TP::mfma(vt, pw[y], acc[dt]);
+          if constexpr (TWO) acc[dt] = TP::mfma(vt, pw[2 + y], acc[dt]);
         }
     };
 
@@ -828,7 +838,7 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
       const int next = j + 1 < blocks.n_all ? j + 1 : 0, free = 3 - sk - sv;
       turns.next();
       f32x16 st[2];
-      px8 pw[2];
+      px8 pw[TWO ? 4 : 2];
       if constexpr (KV8) {
         wait_vmcnt<0>();
         lds_barrier();  // the block before is read
@@ -900,7 +910,8 @@ __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_s
   }
   if (bad != 0) {
     const int lim_hi = p.causal ? x.sq.lk - x.sq.lq + min(r_first + 31, nrow - 1) / G : x.sq.lk - 1;
-    pa_again<elem, D, DA_BS, 32, KV8, false, (!KV8 && T::BIAS > 0.f), true>(p, x.b, x.sq, x.kvh, x.part, x.r0, r_first,
+    // (in two terms: as in pa_few)
+    pa_again<elem, D, DA_BS, 32, KV8, TWO, (!KV8 && T::BIAS > 0.f), true>(p, x.b, x.sq, x.kvh, x.part, x.r0, r_first,
                                                                      (uint32_t)(bad | (bad >> 32)) & (uint32_t)__ballot(live),
                                                                      x.blocks, lim_hi / DA_BS);
   }
