@@ -890,7 +890,8 @@ int la_rotary(const la_rotary_args *a, void *stream);
  * Angles go by rot_positions (as in la_rotary, packed: axis a, row t), or, null, by the
  * tokens' places.  The pool holds the inputs' dtype (LA_F32, LA_BF16, LA_F16), or e4m3 codes
  * with fp32 scales (n_phys, Hkv, pool_page) at stride s_stride: scale = max(largest, 1e-8) /
- * 448 of the row as turned in fp32, codes = e4m3(x / scale).
+ * 448 of the row as turned in fp32, codes = e4m3(x / scale); D above 128 then needs D, n,
+ * strides and addresses of whole fours of values (pools: of codes), else LA_ERR_UNSUPPORTED.
  * page_min, page_max (optional, not with fp8; the dtype of k_new): the least and largest keys
  * of pages of meta_page tokens, (B, Hkv, n_pages, D) at m_sb, m_sh, m_sp, m_sd; those that the
  * new tokens touch are brought up to date (a page that starts among them holds only them).

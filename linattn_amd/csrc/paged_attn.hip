@@ -629,9 +629,10 @@ __device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x
 // (KV8): codes of K and V go into LDS a block ahead, and are widened there once a workgroup (e4m3 is exact
 // in bf16 and fp16); the scale of a key multiplies its scores, that of its value its weights, both in fp32.
 //
-// Bound by matrix and vector unit in turn: 8192 tokens behind 24576 3.34 to 3.39 ms, 1.14 to 1.15 PFLOP/s
+// Bound by matrix and vector unit in turn: 8192 tokens behind 24576 3.34 to 3.49 ms, 1.15 to 1.10 PFLOP/s
 // (a large product has 1.36), the matrix unit busy for 57 to 65 % of the cycles
-// at 1.75 to 1.53 GHz.  Products of the next block beside a block's weights (32 keys at a time, for the
+// at 1.75 to 1.53 GHz.  Over fp8 caches the widening stands between two barriers, beside which nothing else of
+// the workgroup goes on: chunks of four prompts 255 us, over bf16 205.  Products of the next block beside a block's weights (32 keys at a time, for the
 // registers) take 3.77 to 3.90 ms, two workgroups a CU with them 4.16.
 template <class T, int D, bool KV8, bool EVEN>
 __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_scale) {
@@ -935,9 +936,11 @@ __global__ __launch_bounds__(256, 3) void paged_attn_kernel(PaKP) {
 }
 
 // fp32 rows: four waves of 16 rows on 16x16x4 products, blocks of 32 keys (dense_attn_f32_kernel's),
-// over pages of any size, a lane a key, two blocks ahead.  Bound by the fp32 products (two chunks of 256
-// tokens behind 4096, 16 heads on 8, 177 us) or, for single tokens, the reads (32 behind up to 8192
-// 290 us).
+// over pages of any size, a lane a key, pages two blocks ahead and keys one.  Bound by the fp32 products (two
+// chunks of 256 tokens behind 4096, 16 heads on 8, 177 us, of which the products alone would take 110; the matrix
+// unit is busy for 62 % of the cycles).  Of single tokens the rows fill one wave, which does all products while
+// the other three only stage, and a block's keys are on their way for as long as one block's products take:
+// 32 tokens behind up to 8192 290 us, 4.5 TB/s of the 6.0 that plain reads have, waves waiting 75 % of the time.
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_attn_f32_kernel(PaKP p) {
   constexpr int NW = 4, R = 16 * NW, BS = 32, BLK = BS * D, CH = D / 4, RP = 64 / CH, NX = BS / RP / NW;

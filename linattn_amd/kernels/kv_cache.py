@@ -130,7 +130,8 @@ def rotary_kv_append(q: Optional[torch.Tensor], k_new: torch.Tensor, v_new: torc
     place % pool_page of page ``page_table[b, place // pool_page]`` of the pools (n_phys, Hkv,
     pool_page, D); a token whose place lies outside of the table, or whose page outside of the
     pool, is not stored.  The pools hold k_new's dtype, or float8_e4m3fn codes with ``k_scale`` /
-    ``v_scale`` (as ``paged_kv_append``; codes are of the row as it was turned in fp32).
+    ``v_scale`` (as ``paged_kv_append``; codes are of the row as it was turned in fp32; of D above
+    128 only where D, n and all rows are whole fours of values, and pools begin at whole fours).
     Angles: ``inv_freq``, ``axes`` and ``interleaved`` as in ``rotary``, by the tokens' places, or by
     ``rotary_positions`` (int32, (B, Tn) or (N,); with ``axes`` (A, B, Tn) or (A, N)).
     ``page_min`` / ``page_max`` (B, Hkv, n_pages, D) in k_new's dtype, with ``page_size``: Quest's
