@@ -631,9 +631,10 @@ __device__ __forceinline__ void pa_rows_out(const PaKP &p, int64_t o, const f32x
 //
 // Bound by matrix and vector unit in turn: 8192 tokens behind 24576 3.34 to 3.49 ms, 1.15 to 1.10 PFLOP/s
 // (a large product has 1.36), the matrix unit busy for 57 to 65 % of the cycles
-// at 1.75 to 1.53 GHz.  Over fp8 caches the widening stands between two barriers, beside which nothing else of
-// the workgroup goes on: chunks of four prompts 255 us, over bf16 205.  Products of the next block beside a block's weights (32 keys at a time, for the
+// at 1.75 to 1.53 GHz.  Products of the next block beside a block's weights (32 keys at a time, for the
 // registers) take 3.77 to 3.90 ms, two workgroups a CU with them 4.16.
+// Over fp8 caches a block is widened between two barriers, and nothing else of the workgroup goes on
+// meanwhile: chunks of four prompts 255 us, over bf16 205.
 template <class T, int D, bool KV8, bool EVEN>
 __device__ __forceinline__ void pa_many(PaWalk *walk, uint16_t *smem, float *s_scale) {
   typedef typename std::conditional<KV8, DaBf16, T>::type TP;  // of P and V
